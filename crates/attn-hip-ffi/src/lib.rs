@@ -184,6 +184,21 @@ pub mod sys {
                                g: *const f32, beta: *const f32, state: *mut f32, y: *mut c_void, batch: i32,
                                n_tokens: i32, hk: i32, hv: i32, dk: i32, dv: i32, dtype: i32,
                                workspace: *mut c_void, workspace_bytes: u64) -> i32;
+        pub fn ema_paged_append(stream: EmaStream, qkv: *const c_void, q_norm_w: *const c_void,
+            k_norm_w: *const c_void, eps: f32, theta: f32, q_starts: *const i32, offsets: *const i32,
+            prefix_len: *const i32, batch: i32, n_rows: i32, n_heads: i32, flags: u32, q_out: *mut c_void, pages: *const EmaKvCacheDesc,
+            table: *const i32, table_cols: i32) -> i32;
+        pub fn ema_paged_workspace_size(batch: i32, n_rows: i32, n_heads: i32, n_kv_heads: i32, head_dim: i32,
+            max_q: i32, max_len: i32, max_prefix: i32, bytes: *mut u64) -> i32;
+        pub fn ema_paged_attention(stream: EmaStream, q: *const c_void, pages: *const EmaKvCacheDesc,
+            table: *const i32, table_cols: i32, q_starts: *const i32, lengths: *const i32, batch: i32, n_rows: i32,
+            max_q: i32, max_len: i32, n_heads: i32, scale: f32, flags: u32, out: *mut c_void,
+            workspace: *mut c_void, workspace_bytes: u64) -> i32;
+        pub fn ema_prefix_attention(stream: EmaStream, q: *const c_void, pages: *const EmaKvCacheDesc,
+            prefix_table: *const i32, prefix_cols: i32, prefix_len: *const i32, max_prefix: i32,
+            table: *const i32, table_cols: i32, q_starts: *const i32, lengths: *const i32, batch: i32, n_rows: i32,
+            max_q: i32, max_len: i32, n_heads: i32, scale: f32, out: *mut c_void, workspace: *mut c_void,
+            workspace_bytes: u64) -> i32;
         pub fn ema_quantized_matmul(stream: EmaStream, x: *const c_void, ldx: i64, w: *const u32,
                                     scales: *const c_void, biases: *const c_void, y: *mut c_void, ldy: i64,
                                     m: i32, n: i32, k: i32, group_size: i32, bits: i32, dtype: i32) -> i32;

@@ -12,6 +12,7 @@
 #include <mutex>
 
 #include "ema_common.hpp"
+#include "paged.hpp"
 
 namespace ema {
 
@@ -659,6 +660,151 @@ int32_t ema_prefill_attention(ema_stream_t stream, const void* q, const ema_kvca
 }
 
 }  // extern "C"
+
+// What the calls over a page pool share: a bf16 or plain FP8 descriptor whose rows are the pages.
+static int32_t check_pages(const char* op, const ema_kvcache_desc* c) {
+  const int32_t rc = check_cache(op, c);
+  if (rc) return rc;
+  if (c->dtype == EMA_DTYPE_INT4_AFFINE || c->n_rot)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: pages are bf16 or fp8 without a RoPE tail", op);
+  if (c->flags) return set_error(EMA_ERR_INVALID_ARG, "%s: a page pool takes no cache flags (0x%x)", op, c->flags);
+  if (c->capacity < kPagedMinPage || (c->capacity & (c->capacity - 1)))
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: page size %d is not a power of two of at least %d", op, c->capacity,
+                     kPagedMinPage);
+  if (c->dtype == EMA_DTYPE_FP8_E4M3 && (((uintptr_t)c->k_exp | (uintptr_t)c->v_exp) & 1u))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: fp8 exponents must be 2-byte aligned", op);
+  if (c->stride_pos >= ((int64_t)1 << 26))  // 16 rows of a page within a 32-bit buffer range
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: stride_pos %lld exceeds 2^26", op, (long long)c->stride_pos);
+  return EMA_OK;
+}
+
+static int32_t check_page_table(const char* op, const ema_kvcache_desc* c, const int32_t* table, int32_t cols) {
+  if (!table) return set_error(EMA_ERR_INVALID_ARG, "%s: null page table", op);
+  if (cols <= 0) return set_error(EMA_ERR_SHAPE, "%s: a page table row of %d entries", op, cols);
+  if ((int64_t)cols * c->capacity > INT32_MAX)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %d pages of %d positions exceed 2^31 - 1 positions", op, cols, c->capacity);
+  return EMA_OK;
+}
+
+static int32_t check_paged_rows(const char* op, int32_t batch, int32_t n_rows, int32_t n_heads, bool uniform) {
+  if (batch <= 0 || n_rows < 0) return set_error(EMA_ERR_SHAPE, "%s: batch=%d n_rows=%d", op, batch, n_rows);
+  if (batch > kPagedMaxB) return set_error(EMA_ERR_UNSUPPORTED, "%s: batch %d exceeds %d", op, batch, kPagedMaxB);
+  if (uniform && n_rows % batch)
+    return set_error(EMA_ERR_SHAPE, "%s: %d rows are not the same number for each of %d sequences (pass q_starts)", op,
+                     n_rows, batch);
+  if ((int64_t)n_rows * n_heads > INT32_MAX / 256)
+    return set_error(EMA_ERR_SHAPE, "%s: %d rows of %d heads are too many", op, n_rows, n_heads);
+  return EMA_OK;
+}
+
+extern "C" int32_t ema_paged_append(ema_stream_t stream, const void* qkv, const void* q_norm_w, const void* k_norm_w,
+                                    float eps, float theta, const int32_t* q_starts, const int32_t* offsets,
+                                    const int32_t* prefix_len, int32_t batch, int32_t n_rows, int32_t n_heads,
+                                    uint32_t flags, void* q_out, const ema_kvcache_desc* pages, const int32_t* table,
+                                    int32_t table_cols) {
+  const char* op = "ema_paged_append";
+  int32_t rc = check_pages(op, pages);
+  if (rc) return rc;
+  if ((rc = check_page_table(op, pages, table, table_cols))) return rc;
+  if (!qkv || !q_out || !offsets) return set_error(EMA_ERR_INVALID_ARG, "%s: null qkv/q_out/offsets", op);
+  if (flags & ~(EMA_PRE_NO_NORM | EMA_PRE_NO_ROPE | EMA_PRE_NO_Q_NORM | EMA_PRE_NO_K_NORM))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
+  if ((rc = check_norm_weights(op, q_norm_w, k_norm_w, flags))) return rc;
+  if ((rc = check_heads(op, n_heads, pages->n_kv_heads))) return rc;
+  if ((rc = check_paged_rows(op, batch, n_rows, n_heads, !q_starts))) return rc;
+  if (pages->head_dim != 64 && pages->head_dim != 128 && pages->head_dim != 256)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: head_dim %d not supported (64/128/256)", op, pages->head_dim);
+  if (!(eps >= 0.f) || !(theta > 0.f)) return set_error(EMA_ERR_INVALID_ARG, "%s: eps must be >= 0 and theta > 0", op);
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(q_norm_w) || !aligned16(k_norm_w))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: qkv, q_out and the norm weights must be 16-byte aligned", op);
+  if (n_rows == 0) return EMA_OK;
+  const PagedAppend p{qkv,        q_norm_w, k_norm_w, eps,    theta,   q_starts, offsets, prefix_len,
+                      table, table_cols, batch,    n_rows, n_heads, flags,    q_out};
+  return launch_paged_append((hipStream_t)stream, p, *pages);
+}
+
+extern "C" int32_t ema_paged_workspace_size(int32_t batch, int32_t n_rows, int32_t n_heads, int32_t n_kv_heads,
+                                            int32_t head_dim, int32_t max_q, int32_t max_len, int32_t max_prefix,
+                                            uint64_t* bytes) {
+  const char* op = "ema_paged_workspace_size";
+  if (!bytes) return set_error(EMA_ERR_INVALID_ARG, "%s: output is null", op);
+  int32_t rc = check_heads(op, n_heads, n_kv_heads);
+  if (rc) return rc;
+  if ((rc = check_paged_rows(op, batch, n_rows, n_heads, false))) return rc;
+  if (head_dim != 128) return set_error(EMA_ERR_UNSUPPORTED, "%s: head_dim %d not supported (128)", op, head_dim);
+  if (max_q < 0 || max_len < 0 || max_prefix < 0)
+    return set_error(EMA_ERR_SHAPE, "%s: negative bound (max_q=%d max_len=%d max_prefix=%d)", op, max_q, max_len, max_prefix);
+  *bytes = plan_paged(batch, n_rows, n_heads, n_kv_heads, max_q, max_len, max_prefix).bytes;
+  return EMA_OK;
+}
+
+static int32_t paged_attention(const char* op, ema_stream_t stream, const PagedAttention& p, int32_t max_len,
+                               int32_t max_prefix, const ema_kvcache_desc* pages, void* workspace,
+                               uint64_t workspace_bytes) {
+  int32_t rc = check_page_table(op, pages, p.table, p.table_cols);
+  if (rc) return rc;
+  if (!p.q || !p.out || !p.lengths) return set_error(EMA_ERR_INVALID_ARG, "%s: null q/out/lengths", op);
+  if ((rc = check_heads(op, p.n_heads, pages->n_kv_heads))) return rc;
+  if ((rc = check_paged_rows(op, p.batch, p.n_rows, p.n_heads, !p.q_starts))) return rc;
+  if (pages->head_dim != 128)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: head_dim %d not supported (128)", op, pages->head_dim);
+  if (p.max_q < 0) return set_error(EMA_ERR_SHAPE, "%s: max_q %d is negative", op, p.max_q);
+  const int64_t cap = (int64_t)p.table_cols * pages->capacity;
+  if (max_len < 0 || max_len > cap)
+    return set_error(EMA_ERR_CAPACITY, "%s: max_len %d outside [0, %lld], what %d pages hold", op, max_len,
+                     (long long)cap, p.table_cols);
+  if (!(p.scale > 0.f)) return set_error(EMA_ERR_INVALID_ARG, "%s: scale must be > 0", op);
+  if (!aligned16(p.q) || !aligned16(p.out)) return set_error(EMA_ERR_INVALID_ARG, "%s: q/out must be 16-byte aligned", op);
+  // the kernels count key tiles of all segments in 32 bits; lengths are clamped to what the
+  // tables hold
+  const int G = p.n_heads / pages->n_kv_heads;
+  const int64_t tiles = paged_row_blocks(p.batch, p.n_rows, p.n_rows, G) * pages->n_kv_heads * ((cap + 31) / 32);
+  const int64_t shared = p.prefix_table ? paged_row_blocks(1, p.n_rows, p.n_rows, G) * pages->n_kv_heads *
+                                              (((int64_t)p.prefix_cols * pages->capacity + 31) / 32) : 0;
+  if (tiles >= INT32_MAX || shared >= INT32_MAX)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %lld key tiles over all row blocks exceed 2^31 - 1", op,
+                     (long long)(tiles > shared ? tiles : shared));
+  const PagedPlan plan = plan_paged(p.batch, p.n_rows, p.n_heads, pages->n_kv_heads, p.max_q, max_len, max_prefix);
+  if (!workspace || workspace_bytes < plan.bytes)
+    return set_error(EMA_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", op,
+                     (unsigned long long)plan.bytes, (unsigned long long)(workspace ? workspace_bytes : 0));
+  if (!aligned16(workspace)) return set_error(EMA_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", op);
+  if (p.n_rows == 0) return EMA_OK;
+  return launch_paged_attention((hipStream_t)stream, p, *pages, plan, workspace);
+}
+
+extern "C" int32_t ema_paged_attention(ema_stream_t stream, const void* q, const ema_kvcache_desc* pages,
+                                       const int32_t* table, int32_t table_cols, const int32_t* q_starts,
+                                       const int32_t* lengths, int32_t batch, int32_t n_rows, int32_t max_q,
+                                       int32_t max_len, int32_t n_heads, float scale, uint32_t flags, void* out,
+                                       void* workspace, uint64_t workspace_bytes) {
+  const char* op = "ema_paged_attention";
+  const int32_t rc = check_pages(op, pages);
+  if (rc) return rc;
+  if (flags & ~EMA_PREFILL_CAUSAL) return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
+  const PagedAttention p{q,          table, nullptr, nullptr, q_starts, lengths,
+                         table_cols, 0,     batch,   n_rows,  n_heads,  max_q, (int)(flags & EMA_PREFILL_CAUSAL), scale, out};
+  return paged_attention(op, stream, p, max_len, 0, pages, workspace, workspace_bytes);
+}
+
+extern "C" int32_t ema_prefix_attention(ema_stream_t stream, const void* q, const ema_kvcache_desc* pages,
+                                        const int32_t* prefix_table, int32_t prefix_cols, const int32_t* prefix_len,
+                                        int32_t max_prefix, const int32_t* table, int32_t table_cols,
+                                        const int32_t* q_starts, const int32_t* lengths, int32_t batch, int32_t n_rows,
+                                        int32_t max_q, int32_t max_len, int32_t n_heads, float scale, void* out,
+                                        void* workspace, uint64_t workspace_bytes) {
+  const char* op = "ema_prefix_attention";
+  int32_t rc = check_pages(op, pages);
+  if (rc) return rc;
+  if ((rc = check_page_table(op, pages, prefix_table, prefix_cols))) return rc;
+  if (!prefix_len) return set_error(EMA_ERR_INVALID_ARG, "%s: null prefix_len", op);
+  if (max_prefix <= 0 || max_prefix > (int64_t)prefix_cols * pages->capacity)
+    return set_error(EMA_ERR_CAPACITY, "%s: max_prefix %d outside [1, %lld], what %d pages hold", op, max_prefix,
+                     (long long)prefix_cols * pages->capacity, prefix_cols);
+  const PagedAttention p{q,          table,       prefix_table, prefix_len, q_starts, lengths,
+                         table_cols, prefix_cols, batch,        n_rows,     n_heads,  max_q, 1, scale, out};
+  return paged_attention(op, stream, p, max_len, max_prefix, pages, workspace, workspace_bytes);
+}
 
 static int32_t check_gdn_args(const char* op, const void* q, const void* k, const void* v, const float* g,
                               const float* beta, const float* state, const void* y, int32_t batch, int32_t n_tokens,

@@ -223,6 +223,43 @@ int32_t launch_decode(hipStream_t s, const void* q, const ema_kvcache_desc& c, c
 int32_t launch_prefill(hipStream_t s, const void* q, const ema_kvcache_desc& c,
                        const int32_t* q_off, int T, int Hq, float scale, uint32_t flags,
                        void* out);
+// Paged cache (arguments validated by the caller): a call's inputs, and its workspace plan.
+struct PagedAppend {
+  const void* qkv;
+  const void* q_norm_w;
+  const void* k_norm_w;
+  float eps;
+  float theta;
+  const int32_t* q_starts;  // null: n_rows / batch rows per sequence
+  const int32_t* offsets;
+  const int32_t* prefix_len;  // null: no shared prefix before the sequences' positions
+  const int32_t* table;
+  int table_cols, batch, n_rows, n_heads;
+  uint32_t flags;
+  void* q_out;
+};
+int32_t launch_paged_append(hipStream_t s, const PagedAppend& p, const ema_kvcache_desc& c);
+struct PagedAttention {
+  const void* q;
+  const int32_t* table;
+  const int32_t* prefix_table;  // null: no shared prefix
+  const int32_t* prefix_len;
+  const int32_t* q_starts;
+  const int32_t* lengths;
+  int table_cols, prefix_cols, batch, n_rows, n_heads, max_q, causal;
+  float scale;
+  void* out;
+};
+struct PagedPlan {
+  int workers;          // workgroups over the sequences' own pages
+  int prefix_workers;   // workgroups over the shared prefix
+  uint64_t part_bytes;  // partial states of shared segments
+  uint64_t carry_bytes; // states of the rows over the prefix
+  uint64_t bytes;       // the whole workspace
+};
+PagedPlan plan_paged(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len, int max_prefix);
+int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema_kvcache_desc& c, const PagedPlan& plan,
+                               void* ws);
 // Gated DeltaNet recurrent scan (arguments validated by the caller).
 int32_t launch_gdn_scan(hipStream_t s, const void* q, const void* k, const void* v, const float* g,
                         const float* beta, float* state, void* y, int B, int T, int hk, int hv, int dk,

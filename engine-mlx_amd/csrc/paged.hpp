@@ -1,0 +1,63 @@
+// Shared pieces of the paged-cache kernels: how packed rows, pages and work are addressed.
+//
+// A page pool is a ema_kvcache_desc of n_pages "sequences" of page_size "positions"; row b of
+// the block table names the pages of sequence b. The integer parts are host/device functions,
+// checked on the CPU (tests/cpp/test_paged.cpp).
+#pragma once
+
+#include "ema_schedule.hpp"
+
+namespace ema {
+
+constexpr int kPagedMaxB = 1024;    // sequences of one call (the kernels' tables in LDS)
+constexpr int kPagedRows = 32;      // query rows of a segment: (token, head of the kv group) pairs
+constexpr int kPagedTile = 32;      // keys per tile
+constexpr int kPagedWaves = 4;      // waves per workgroup, each with tiles of its own
+constexpr int kPagedMaxWorkers = 512;
+constexpr int kPagedMinPage = 16;   // a wave's 1 KB loads (4 rows) never straddle two pages
+
+// Query rows of sequence b: packed rows [begin, begin + n). Row starts from the device are
+// taken as given only inside [0, n_rows].
+struct PagedRows {
+  int begin, n;
+};
+EMA_HD PagedRows paged_rows(int s0, int s1, int n_rows) {
+  s0 = s0 < 0 ? 0 : (s0 > n_rows ? n_rows : s0);
+  s1 = s1 < s0 ? s0 : (s1 > n_rows ? n_rows : s1);
+  return PagedRows{s0, s1 - s0};
+}
+
+// The tiles of all segments, laid end to end, cut into W slices that differ by at most one
+// tile; 32-bit arithmetic without products of the two (total < 2^31).
+struct PagedSplit {
+  uint32_t base, rem;  // every slice has base tiles, the first rem of them one more
+};
+EMA_HD int paged_active_workers(int total, int W) {
+  const int want = (int)(((int64_t)total + kPagedWaves - 1) / kPagedWaves);
+  return want < W ? (want < 1 ? 1 : want) : W;
+}
+EMA_HD PagedSplit paged_split(int total, int W) { return PagedSplit{(uint32_t)total / (uint32_t)W, (uint32_t)total % (uint32_t)W}; }
+EMA_HD int paged_begin(PagedSplit s, int w) { return (int)((uint32_t)w * s.base + ((uint32_t)w < s.rem ? (uint32_t)w : s.rem)); }
+EMA_HD int paged_worker_of(PagedSplit s, int t) {
+  const uint32_t cut = s.rem * (s.base + 1);
+  return (int)((uint32_t)t < cut ? (uint32_t)t / (s.base + 1) : s.rem + ((uint32_t)t - cut) / s.base);
+}
+// Partial-state slot of worker w's piece of a segment that several workers share. A slice
+// shares at most two segments: the one it begins inside (slot 2 w) and the one that begins
+// inside it and runs on (slot 2 w + 1, w then being the segment's first worker w0).
+EMA_HD int paged_slot(int w, int w0) { return 2 * w + (w == w0 ? 1 : 0); }
+
+// Workers the plan sizes the workspace for, from the host's bounds: nrb row blocks per kv head
+// (all sequences), max_tiles key tiles each.
+EMA_HD int paged_plan_workers(int64_t nrb, int Hkv, int64_t max_tiles) {
+  const int64_t want = (nrb * Hkv * max_tiles + kPagedWaves - 1) / kPagedWaves;
+  return (int)(want < 1 ? 1 : (want < kPagedMaxWorkers ? want : kPagedMaxWorkers));
+}
+// Row blocks of a batch whose sequences have at most max_q rows and n_rows together.
+EMA_HD int64_t paged_row_blocks(int B, int64_t n_rows, int64_t max_q, int G) {
+  const int64_t each = (int64_t)B * ((max_q * G + kPagedRows - 1) / kPagedRows);
+  const int64_t all = n_rows * G / kPagedRows + B;
+  return each < all ? each : all;
+}
+
+}  // namespace ema

@@ -49,7 +49,8 @@ EXPORTED = (
     "ema_kvcache_memory_bytes", "ema_pre_attention", "ema_pre_attention_ws", "ema_decode_workspace_size",
     "ema_decode_attention", "ema_decode_step", "ema_decode_step_noalloc", "ema_prefill_attention", "ema_prefill_workspace_size",
     "ema_prefill_attention_ws", "ema_gdn_scan", "ema_gdn_scan_workspace_size", "ema_gdn_scan_ws",
-    "ema_quantized_matmul",
+    "ema_quantized_matmul", "ema_paged_append", "ema_paged_workspace_size", "ema_paged_attention",
+    "ema_prefix_attention",
 )
 
 
@@ -114,6 +115,11 @@ def lib() -> ctypes.CDLL:
             "ema_gdn_scan": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32]),
             "ema_gdn_scan_workspace_size": (i32, [i32, i32, i32, i32, i32, i32, ctypes.POINTER(u64)]),
             "ema_gdn_scan_ws": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, u64]),
+            "ema_paged_append": (i32, [vp, vp, vp, vp, f32, f32, vp, vp, vp, i32, i32, i32, u32, vp, D, vp, i32]),
+            "ema_paged_workspace_size": (i32, [i32] * 8 + [ctypes.POINTER(u64)]),
+            "ema_paged_attention": (i32, [vp, vp, D, vp, i32, vp, vp, i32, i32, i32, i32, i32, f32, u32, vp, vp, u64]),
+            "ema_prefix_attention": (i32, [vp, vp, D, vp, i32, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, f32,
+                                           vp, vp, u64]),
             "ema_quantized_matmul": (i32, [vp, vp, i64, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32]),
         }
         for name, (res, args) in sig.items():
@@ -464,3 +470,220 @@ def quantized_matmul(x, w, scales, biases, group_size=64, bits=4, out=None, stre
                                       _ptr(y2), y2.stride(0), M, N, K, group_size, bits, dtypes[x.dtype]),
            "ema_quantized_matmul")
     return y2.reshape(x.shape[:-1] + (N,)) if out is None else y2
+
+
+class PagedCache:
+    """Pool of K/V pages shared by many sequences: [n_pages, Hkv, page_size, D], bf16 or FP8
+    (E4M3 codes with ``k_exp``/``v_exp`` int8 [n_pages, Hkv, page_size, D/64] exponents, as
+    StaticCache's), page_size a power of two of at least 16.
+
+    A page table int32 [B, cols] names each sequence's pages in order: position p lies in slot
+    p % page_size of page table[b, p // page_size]. Entries outside [0, n_pages) are never
+    followed: nothing is written there and their positions read as zero rows.
+
+    bf16 ``k``/``v`` may be views with any page, head and position strides (multiples of 8
+    elements, D contiguous, both alike), e.g. ``pool.transpose(1, 2)`` of a
+    [n_pages, page_size, Hkv, D] tensor.
+    """
+
+    def __init__(self, n_pages: int, n_kv_heads: int, page_size: int, head_dim: int, device="cuda", k=None, v=None,
+                 dtype="bf16", k_exp=None, v_exp=None):
+        import torch
+
+        op = "PagedCache"
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        if dtype not in ("bf16", "fp8"):
+            raise ValueError(f"unknown page dtype {dtype!r} (bf16 or fp8)")
+        want = torch.bfloat16 if dtype == "bf16" else torch.uint8
+        self.k = k if k is not None else torch.zeros(shape, dtype=want, device=device)
+        self.v = v if v is not None else torch.zeros(shape, dtype=want, device=device)
+        for name, t in (("k", self.k), ("v", self.v)):
+            if t.dtype != want or tuple(t.shape) != shape or t.stride(3) != 1:
+                raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be {want} {shape}, its last axis contiguous")
+        if self.k.stride() != self.v.stride() or self.k.device != self.v.device:
+            raise EmaError(EMA_ERR_SHAPE, op, "k and v differ in strides or device")
+        self.desc = KvCacheDesc()
+        self.dtype = dtype
+        self.k_exp = self.v_exp = None
+        if dtype == "bf16":
+            _check(lib().ema_kvcache_init(ctypes.byref(self.desc), _ptr(self.k), _ptr(self.v), *shape),
+                   "ema_kvcache_init")
+        else:
+            eshape = shape[:3] + (head_dim // 64,)
+            self.k_exp = k_exp if k_exp is not None else torch.zeros(eshape, dtype=torch.int8, device=device)
+            self.v_exp = v_exp if v_exp is not None else torch.zeros(eshape, dtype=torch.int8, device=device)
+            for name, t in (("k_exp", self.k_exp), ("v_exp", self.v_exp)):
+                if t.dtype != torch.int8 or tuple(t.shape) != eshape or not t.is_contiguous():
+                    raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be contiguous int8 {eshape}")
+            _check(lib().ema_kvcache_init_fp8(ctypes.byref(self.desc), _ptr(self.k), _ptr(self.v), _ptr(self.k_exp),
+                                              _ptr(self.v_exp), *shape, 0), "ema_kvcache_init_fp8")
+        self.desc.stride_batch, self.desc.stride_head, self.desc.stride_pos = self.k.stride()[:3]
+
+    @property
+    def n_pages(self) -> int:
+        return self.desc.batch
+
+    @property
+    def page_size(self) -> int:
+        return self.desc.capacity
+
+    def memory_bytes(self) -> int:
+        out = ctypes.c_uint64()
+        _check(lib().ema_kvcache_memory_bytes(ctypes.byref(self.desc), ctypes.byref(out)), "ema_kvcache_memory_bytes")
+        return out.value
+
+
+def _want(op: str, name: str, t, dtype, shape, device) -> None:
+    """A contiguous device tensor of the given dtype and shape on the pool's device (None in
+    ``shape``: any size)."""
+    if (t.dtype != dtype or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape))
+            or not t.is_contiguous()):
+        raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be a contiguous {dtype} tensor {tuple(shape)}, not "
+                                          f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+    if t.device != device:
+        raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} is on {t.device}, the pages on {device}")
+
+
+def _paged_batch(op: str, cache, table, q_starts, per_seq, name: str):
+    import torch
+
+    dev = cache.k.device
+    _want(op, "table", table, torch.int32, (None, None), dev)
+    B = table.shape[0]
+    _want(op, name, per_seq, torch.int32, (B,), dev)
+    if q_starts is not None:
+        _want(op, "q_starts", q_starts, torch.int32, (B + 1,), dev)
+    return B
+
+
+class _on_device:
+    """Makes the pool's device current around a call, when it is not."""
+
+    def __init__(self, device):
+        import torch
+
+        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+def paged_append(qkv, q_norm_w, k_norm_w, eps, theta, offsets, n_heads, cache: PagedCache, table, q_starts=None,
+                 flags=0, q_out=None, prefix_len=None, stream=None):
+    """Norm, rotation and append of a ragged batch (ema_paged_append): qkv [n, (Hq+2Hkv)*D] bf16,
+    offsets int32 [B] (position of each sequence's first row), table int32 [B, cols], q_starts
+    int32 [B+1] (None: n / B rows each); prefix_len int32 [1]: a shared prefix's positions, which
+    the rotation counts before the sequences' own. Returns q_out [n, Hq, D]."""
+    import torch
+
+    op = "ema_paged_append"
+    dev, D, Hkv = cache.k.device, cache.desc.head_dim, cache.desc.n_kv_heads
+    B = _paged_batch(op, cache, table, q_starts, offsets, "offsets")
+    _want(op, "qkv", qkv, torch.bfloat16, (None, (n_heads + 2 * Hkv) * D), dev)
+    n = qkv.shape[0]
+    for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
+        if w is not None:
+            _want(op, name, w, torch.bfloat16, (D,), dev)
+    if prefix_len is not None:
+        _want(op, "prefix_len", prefix_len, torch.int32, (1,), dev)
+    if q_out is None:
+        q_out = torch.empty((n, n_heads, D), dtype=torch.bfloat16, device=dev)
+    else:
+        _want(op, "q_out", q_out, torch.bfloat16, (n, n_heads, D), dev)
+    with _on_device(dev):
+        _check(lib().ema_paged_append(_stream(stream), _ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), eps, theta,
+                                      _ptr(q_starts), _ptr(offsets), _ptr(prefix_len), B, n, n_heads, flags,
+                                      _ptr(q_out), ctypes.byref(cache.desc), _ptr(table), table.shape[1]), op)
+    return q_out
+
+
+def paged_workspace_size(batch, n_rows, n_heads, n_kv_heads, head_dim, max_q, max_len, max_prefix=0) -> int:
+    out = ctypes.c_uint64()
+    _check(lib().ema_paged_workspace_size(batch, n_rows, n_heads, n_kv_heads, head_dim, max_q, max_len, max_prefix,
+                                          ctypes.byref(out)), "ema_paged_workspace_size")
+    return out.value
+
+
+def paged_workspace(batch, n_rows, n_heads, n_kv_heads, head_dim, max_q, max_len, max_prefix=0, device="cuda"):
+    """A workspace for paged_attention and (with max_prefix) prefix_attention: zero-filled, as the
+    arrival counters at its start must be before the first call; reusable on one stream."""
+    import torch
+
+    n = paged_workspace_size(batch, n_rows, n_heads, n_kv_heads, head_dim, max_q, max_len, max_prefix)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def _paged_out(op, q, cache, out):
+    import torch
+
+    dev, D = cache.k.device, cache.desc.head_dim
+    _want(op, "q", q, torch.bfloat16, (None, None, D), dev)
+    n, Hq = q.shape[:2]
+    if out is None:
+        return torch.empty((n, Hq * D), dtype=torch.bfloat16, device=dev)
+    _want(op, "out", out, torch.bfloat16, (n, Hq * D), dev)
+    return out
+
+
+def _rows_bound(op, q, B, q_starts, max_q):
+    if q_starts is None:
+        return -(-q.shape[0] // B) if B else 0
+    return q.shape[0] if max_q is None else max_q
+
+
+def paged_attention(q, cache: PagedCache, table, lengths, max_len, q_starts=None, max_q=None, causal=True, scale=None,
+                    out=None, workspace=None, stream=None):
+    """Attention of a ragged batch over its pages (ema_paged_attention): q [n, Hq, D] bf16, lengths
+    int32 [B] (positions held, the call's rows included), table int32 [B, cols]; max_len and
+    max_q are host bounds of the lengths and of a sequence's rows. Returns out [n, Hq * D]."""
+    import torch
+
+    op = "ema_paged_attention"
+    B = _paged_batch(op, cache, table, q_starts, lengths, "lengths")
+    out = _paged_out(op, q, cache, out)
+    n, Hq, D = q.shape
+    max_q = _rows_bound(op, q, B, q_starts, max_q)
+    if workspace is None:
+        workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, device=q.device)
+    else:
+        _want(op, "workspace", workspace, torch.uint8, (None,), q.device)
+    with _on_device(q.device):
+        _check(lib().ema_paged_attention(_stream(stream), _ptr(q), ctypes.byref(cache.desc), _ptr(table),
+                                         table.shape[1], _ptr(q_starts), _ptr(lengths), B, n, max_q, max_len, Hq,
+                                         1.0 / math.sqrt(D) if scale is None else scale,
+                                         EMA_PREFILL_CAUSAL if causal else 0, _ptr(out), _ptr(workspace),
+                                         workspace.numel()), op)
+    return out
+
+
+def prefix_attention(q, cache: PagedCache, prefix_table, prefix_len, max_prefix, table, lengths, max_len,
+                     q_starts=None, max_q=None, scale=None, out=None, workspace=None, stream=None):
+    """Causal attention where every sequence's own pages continue one shared prefix
+    (ema_prefix_attention): prefix_table int32 [cols], prefix_len int32 [1] (its positions,
+    max_prefix a host bound); table and lengths are of the sequences' own positions, the rest as
+    in paged_attention. The prefix is read once for the batch. Returns out [n, Hq * D]."""
+    import torch
+
+    op = "ema_prefix_attention"
+    B = _paged_batch(op, cache, table, q_starts, lengths, "lengths")
+    _want(op, "prefix_table", prefix_table, torch.int32, (None,), cache.k.device)
+    _want(op, "prefix_len", prefix_len, torch.int32, (1,), cache.k.device)
+    out = _paged_out(op, q, cache, out)
+    n, Hq, D = q.shape
+    max_q = _rows_bound(op, q, B, q_starts, max_q)
+    if workspace is None:
+        workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, max_prefix, device=q.device)
+    else:
+        _want(op, "workspace", workspace, torch.uint8, (None,), q.device)
+    with _on_device(q.device):
+        _check(lib().ema_prefix_attention(_stream(stream), _ptr(q), ctypes.byref(cache.desc), _ptr(prefix_table),
+                                          prefix_table.shape[0], _ptr(prefix_len), max_prefix, _ptr(table),
+                                          table.shape[1], _ptr(q_starts), _ptr(lengths), B, n, max_q, max_len, Hq,
+                                          1.0 / math.sqrt(D) if scale is None else scale, _ptr(out), _ptr(workspace),
+                                          workspace.numel()), op)
+    return out

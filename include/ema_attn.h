@@ -379,6 +379,83 @@ EMA_API int32_t ema_prefill_attention_ws(ema_stream_t stream, const void* q, con
                                          float scale, uint32_t flags, void* out, int32_t max_kv_len,
                                          void* workspace, uint64_t workspace_bytes);
 
+/* ---- Paged cache -------------------------------------------------------------------
+ * K and V of many sequences in pages of one pool. The pool is a descriptor whose rows are the
+ * pages: batch = the number of pages, capacity = the positions per page (a power of two, at
+ * least 16), bf16 or FP8 E4M3 without a RoPE tail; ema_kvcache_init, _init_fp8, the _alloc
+ * calls, ema_kvcache_convert and ema_kvcache_memory_bytes apply to it as to any other. Strides
+ * may be set for other orders of a page (positions before heads: stride_head = head_dim,
+ * stride_pos = n_kv_heads * head_dim).
+ *   table       device int32 [batch, table_cols]: row b names the pages of sequence b in order;
+ *               its position p lies in slot p % capacity of page table[b][p / capacity]. An entry
+ *               outside [0, number of pages) is never followed: nothing is written there, and
+ *               its positions read as zero rows (k = v = 0, finite scores).
+ *   q_starts    device int32 [batch + 1], ascending: sequence b's rows of the packed tensors
+ *               are [q_starts[b], q_starts[b + 1]); rows from q_starts[batch] on are neither
+ *               read nor written. NULL: n_rows / batch rows for every sequence.
+ * At most 1024 sequences a call; n_rows * n_heads at most 2^23 - 1; table_cols * capacity below
+ * 2^31. The reference has no paged cache; the calls are the paged forms of ema_pre_attention,
+ * ema_decode_attention and ema_prefill_attention. */
+
+/* Norm, rotation and append for a ragged batch: ema_pre_attention over pages.
+ *   qkv      [n_rows, (n_heads + 2*n_kv_heads) * head_dim] bf16, order q|k|v
+ *   offsets  device int32 [batch]: position of each sequence's first row; its other rows follow
+ *   prefix_len  device int32 [1], or NULL (0): positions of a shared prefix that the sequences
+ *            continue (ema_prefix_attention). It is added to the positions in the rotation, not
+ *            to the slots: offsets and table are of the sequences' own positions
+ *   q_out    [n_rows, n_heads, head_dim] bf16
+ * Per head of q and k: x / sqrt(mean x^2 + eps) * w, then the split-half rotation by the angles
+ * pos * theta^(-2i/head_dim) (formed in 64 bits, so far positions keep bf16's accuracy); 32-bit
+ * arithmetic, one rounding. K and V go to their slots (FP8: the bf16 row, quantised as
+ * ema_pre_attention does); a row whose position is negative, past the table or on an entry
+ * outside the pool still gets its q and is not stored. flags as for ema_pre_attention;
+ * head_dim 64, 128 or 256 (FP8: 128). No two rows of a call may share a slot. */
+EMA_API int32_t ema_paged_append(ema_stream_t stream, const void* qkv, const void* q_norm_w, const void* k_norm_w,
+                                 float eps, float theta, const int32_t* q_starts, const int32_t* offsets,
+                                 const int32_t* prefix_len, int32_t batch, int32_t n_rows, int32_t n_heads,
+                                 uint32_t flags, void* q_out, const ema_kvcache_desc* pages, const int32_t* table,
+                                 int32_t table_cols);
+
+/* Workspace (bytes) of ema_paged_attention (max_prefix 0) and ema_prefix_attention for these
+ * bounds. Like a decode workspace it begins with EMA_DECODE_COUNTER_BYTES of arrival counters
+ * that must be zero before its first use and are zero again after every call; it may be shared
+ * with decode calls, and calls that overlap (two streams, two graphs replayed at once) need one
+ * each. */
+EMA_API int32_t ema_paged_workspace_size(int32_t batch, int32_t n_rows, int32_t n_heads, int32_t n_kv_heads,
+                                         int32_t head_dim, int32_t max_q, int32_t max_len, int32_t max_prefix,
+                                         uint64_t* bytes);
+
+/* Attention of a ragged batch over its pages: single tokens, a few drafted tokens, prompts and
+ * chunks, mixed as they come.
+ *   q        [n_rows, n_heads, head_dim] bf16 (as ema_paged_append leaves it); head_dim 128
+ *   lengths  device int32 [batch]: positions held, the call's own rows included; clamped to
+ *            [0, table_cols * capacity]. Sequence b's n rows are its last n positions.
+ *   max_q, max_len  host bounds of a sequence's rows and of the lengths; they size the grid and
+ *            the workspace, and true values beyond them still give the exact result.
+ *   flags    EMA_PREFILL_CAUSAL: row i of n sees positions up to length - n + i; 0: all of them
+ *            (an encoder's states). A row that sees nothing yields zeros.
+ *   out      [n_rows, n_heads * head_dim] bf16; must not overlap q */
+EMA_API int32_t ema_paged_attention(ema_stream_t stream, const void* q, const ema_kvcache_desc* pages,
+                                    const int32_t* table, int32_t table_cols, const int32_t* q_starts,
+                                    const int32_t* lengths, int32_t batch, int32_t n_rows, int32_t max_q,
+                                    int32_t max_len, int32_t n_heads, float scale, uint32_t flags, void* out,
+                                    void* workspace, uint64_t workspace_bytes);
+
+/* ema_paged_attention (causal) for sequences that continue one shared prefix, held once in the
+ * same pool: every row sees all prefix positions, then causally its sequence's own. The prefix
+ * is read once for the whole batch.
+ *   prefix_table  device int32 [prefix_cols]: the prefix's pages
+ *   prefix_len    device int32 [1]: its positions, clamped to [0, prefix_cols * capacity]
+ *   max_prefix    host bound of it, as max_len is of the lengths
+ *   table, lengths  of the sequences' own positions, the prefix not counted (append with the
+ *            same prefix_len) */
+EMA_API int32_t ema_prefix_attention(ema_stream_t stream, const void* q, const ema_kvcache_desc* pages,
+                                     const int32_t* prefix_table, int32_t prefix_cols, const int32_t* prefix_len,
+                                     int32_t max_prefix, const int32_t* table, int32_t table_cols,
+                                     const int32_t* q_starts, const int32_t* lengths, int32_t batch, int32_t n_rows,
+                                     int32_t max_q, int32_t max_len, int32_t n_heads, float scale, void* out,
+                                     void* workspace, uint64_t workspace_bytes);
+
 /* Gated DeltaNet recurrent scan over n_tokens tokens (n_tokens = 1: the decode step of
  * gdn_step / gdn_step_metal, crates/ops/src/gdn.rs:83-150 and gdn_metal.rs:56-88; n_tokens
  * > 1: the token loop of gdn_forward, crates/ops/src/gdn_forward.rs:173-192). For each
