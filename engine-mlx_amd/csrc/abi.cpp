@@ -755,7 +755,7 @@ static int32_t paged_attention(const char* op, ema_stream_t stream, const PagedA
                      (long long)cap, p.table_cols);
   if (!(p.scale > 0.f)) return set_error(EMA_ERR_INVALID_ARG, "%s: scale must be > 0", op);
   if (!aligned16(p.q) || !aligned16(p.out)) return set_error(EMA_ERR_INVALID_ARG, "%s: q/out must be 16-byte aligned", op);
-  // the kernels count key tiles of all segments in 32 bits; lengths are clamped to what the
+  // the kernels count rounds of key tiles of all segments in 32 bits; lengths are clamped to what the
   // tables hold
   const int G = p.n_heads / pages->n_kv_heads;
   const int64_t tiles = paged_row_blocks(p.batch, p.n_rows, p.n_rows, G) * pages->n_kv_heads * ((cap + 31) / 32);

@@ -193,10 +193,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 // ------------------------------------------------------------------ attention, rows in blocks of 32
 // A segment is 32 query rows of one (sequence, kv head): row i is token i / G, head i % G of
 // the kv head's group, so a decode step's G heads and a few drafted tokens' share one pass over
-// K and V. The keys of a segment are tiles of 32; the tiles of all segments, laid end to end,
-// are cut into equal slices, one per workgroup, whatever the lengths. The four waves of a
-// workgroup take a piece's tiles in turn, each with its own softmax state and its own LDS slot
-// for the tile, and no barrier until their states meet at the piece's end. A segment cut over
+// K and V. The keys of a segment are tiles of 32, four tiles a round; the rounds of all
+// segments, laid end to end, are cut into equal slices, one per workgroup, whatever the lengths.
+// The four waves of a workgroup take a round's tiles, each with its own softmax state and its own
+// LDS slot for the tile, and no barrier until their states meet at the piece's end. A segment cut over
 // several workgroups leaves partial states in the workspace; the last of them to arrive joins
 // them.
 //
@@ -302,7 +302,6 @@ __device__ __forceinline__ int clamp_len(const PagedArgs& a, int L) {
   const int64_t cap = (int64_t)a.cols << a.shift;
   return L < 0 ? 0 : (L > cap ? (int)cap : L);
 }
-__device__ __forceinline__ int tiles_of(int L) { return (int)(((uint32_t)L + kPagedTile - 1) / kPagedTile); }
 __device__ __forceinline__ int blocks_of(const PagedArgs& a, int T) {
   return (int)(((uint32_t)T * (uint32_t)a.G + kPagedRows - 1) / kPagedRows);
 }
@@ -316,7 +315,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  // Tiles before each sequence, by every wave for itself (all write the same values): lane l
+  // Rounds before each sequence, by every wave for itself (all write the same values): lane l
   // takes sequences l step .. +step-1, and the lanes' sums are scanned.
   const int step = (a.B + 63) >> 6;
   int sum = 0;
@@ -324,7 +323,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     const int b = lane * step + i;
     if (b < a.B) {
       const int T = a.starts ? paged_rows(a.starts[b], a.starts[b + 1], a.n_rows).n : a.T;
-      sum += tiles_of(clamp_len(a, a.len[b])) * blocks_of(a, T) * a.Hkv;
+      sum += paged_rounds(clamp_len(a, a.len[b])) * blocks_of(a, T) * a.Hkv;
     }
   }
   int lane_pre = sum;
@@ -340,7 +339,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     if (b < a.B) {
       pre[b] = run;
       const int T = a.starts ? paged_rows(a.starts[b], a.starts[b + 1], a.n_rows).n : a.T;
-      run += tiles_of(clamp_len(a, a.len[b])) * blocks_of(a, T) * a.Hkv;
+      run += paged_rounds(clamp_len(a, a.len[b])) * blocks_of(a, T) * a.Hkv;
     }
   }
   if (lane == 0) pre[a.B] = total;
@@ -348,7 +347,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 
-  // rows of sequences that hold nothing: no tile visits them
+  // rows of sequences that hold nothing: no round visits them
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
     if (pre[b + 1] != pre[b]) continue;
     const PagedRows rw = rows_of(a, b);
@@ -387,7 +386,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
   for (int dt = 0; dt < 4; ++dt) v_col[dt] = tr_row * kD + 16 * (grp & 1) + 4 * (s16 & 3) + 32 * (dt ^ (s16 >> 2));
 
   while (t < t_end) {
-    // the segment of tile t: the last b whose tiles begin at or before it
+    // the segment of round t: the last b whose rounds begin at or before it
     uint64_t le = __ballot(lane * step < a.B && lane_pre <= t);
     int b = (63 - __builtin_clzll(le)) * step;
     if (step > 1) {
@@ -398,13 +397,15 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     const int pre_b = __builtin_amdgcn_readfirstlane(pre[b]);
     const PagedRows rw = rows_of(a, b);
     const int L = clamp_len(a, ld_uniform(a.len, b));
-    const int nt = tiles_of(L), nrb = blocks_of(a, rw.n);
-    const uint32_t seg = (uint32_t)(t - pre_b) / (uint32_t)nt;
-    const int tile0 = (int)((uint32_t)(t - pre_b) - seg * (uint32_t)nt);
+    const int nr = paged_rounds(L), nrb = blocks_of(a, rw.n);
+    const uint32_t seg = (uint32_t)(t - pre_b) / (uint32_t)nr;
+    const int round0 = (int)((uint32_t)(t - pre_b) - seg * (uint32_t)nr);
     const int kh = (int)(seg / (uint32_t)nrb), rb = (int)(seg - (uint32_t)kh * (uint32_t)nrb);
-    const int seg_begin = t - tile0, seg_end = seg_begin + nt;
+    const int seg_begin = t - round0, seg_end = seg_begin + nr;
     const int piece_end = t_end < seg_end ? t_end : seg_end;
-    const int tile1 = tile0 + (piece_end - t);
+    const int tile0 = round0 * kPagedWaves;
+    const int tile_end = (int)(((uint32_t)L + kPagedTile - 1) / kPagedTile);
+    const int tile1 = min(tile0 + (piece_end - t) * kPagedWaves, tile_end);
     const int row0 = rb * kPagedRows;                     // the segment's first row (token * G + head)
     const int n_seg = rw.n * a.G - row0 < kPagedRows ? rw.n * a.G - row0 : kPagedRows;
 
@@ -728,11 +729,11 @@ int32_t launch_paged_append(hipStream_t s, const PagedAppend& p, const ema_kvcac
 PagedPlan plan_paged(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len, int max_prefix) {
   PagedPlan p;
   const int G = Hq / Hkv;
-  p.workers = paged_plan_workers(paged_row_blocks(B, n_rows, max_q, G), Hkv, ((int64_t)max_len + kPagedTile - 1) / kPagedTile);
+  p.workers = paged_plan_workers(paged_row_blocks(B, n_rows, max_q, G), Hkv, max_len);
   p.prefix_workers = 0;
   p.carry_bytes = 0;
   if (max_prefix > 0) {
-    p.prefix_workers = paged_plan_workers(paged_row_blocks(1, n_rows, n_rows, G), Hkv, ((int64_t)max_prefix + kPagedTile - 1) / kPagedTile);
+    p.prefix_workers = paged_plan_workers(paged_row_blocks(1, n_rows, n_rows, G), Hkv, max_prefix);
     p.carry_bytes = (uint64_t)n_rows * Hq * kStateStride * sizeof(float);
   }
   const int w = p.workers > p.prefix_workers ? p.workers : p.prefix_workers;

@@ -27,15 +27,17 @@ EMA_HD PagedRows paged_rows(int s0, int s1, int n_rows) {
   return PagedRows{s0, s1 - s0};
 }
 
-// The tiles of all segments, laid end to end, cut into W slices that differ by at most one
-// tile; 32-bit arithmetic without products of the two (total < 2^31).
+// Rounds of a segment of L keys: a round is one tile for each wave of a workgroup.
+constexpr int kPagedRound = kPagedTile * kPagedWaves;
+EMA_HD int paged_rounds(int L) { return (int)(((uint32_t)L + kPagedRound - 1) / kPagedRound); }
+
+// The rounds of all segments, laid end to end, cut into W slices that differ by at most one
+// round; 32-bit arithmetic without products of the two (total < 2^31). Whole rounds, so that a
+// short segment (a few own tokens behind a prefix) is one workgroup's alone.
 struct PagedSplit {
-  uint32_t base, rem;  // every slice has base tiles, the first rem of them one more
+  uint32_t base, rem;  // every slice has base rounds, the first rem of them one more
 };
-EMA_HD int paged_active_workers(int total, int W) {
-  const int want = (int)(((int64_t)total + kPagedWaves - 1) / kPagedWaves);
-  return want < W ? (want < 1 ? 1 : want) : W;
-}
+EMA_HD int paged_active_workers(int total, int W) { return total < W ? (total < 1 ? 1 : total) : W; }
 EMA_HD PagedSplit paged_split(int total, int W) { return PagedSplit{(uint32_t)total / (uint32_t)W, (uint32_t)total % (uint32_t)W}; }
 EMA_HD int paged_begin(PagedSplit s, int w) { return (int)((uint32_t)w * s.base + ((uint32_t)w < s.rem ? (uint32_t)w : s.rem)); }
 EMA_HD int paged_worker_of(PagedSplit s, int t) {
@@ -48,9 +50,9 @@ EMA_HD int paged_worker_of(PagedSplit s, int t) {
 EMA_HD int paged_slot(int w, int w0) { return 2 * w + (w == w0 ? 1 : 0); }
 
 // Workers the plan sizes the workspace for, from the host's bounds: nrb row blocks per kv head
-// (all sequences), max_tiles key tiles each.
-EMA_HD int paged_plan_workers(int64_t nrb, int Hkv, int64_t max_tiles) {
-  const int64_t want = (nrb * Hkv * max_tiles + kPagedWaves - 1) / kPagedWaves;
+// (all sequences), max_len keys each.
+EMA_HD int paged_plan_workers(int64_t nrb, int Hkv, int max_len) {
+  const int64_t want = nrb * Hkv * paged_rounds(max_len);
   return (int)(want < 1 ? 1 : (want < kPagedMaxWorkers ? want : kPagedMaxWorkers));
 }
 // Row blocks of a batch whose sequences have at most max_q rows and n_rows together.

@@ -518,6 +518,8 @@ class PagedCache:
             _check(lib().ema_kvcache_init_fp8(ctypes.byref(self.desc), _ptr(self.k), _ptr(self.v), _ptr(self.k_exp),
                                               _ptr(self.v_exp), *shape, 0), "ema_kvcache_init_fp8")
         self.desc.stride_batch, self.desc.stride_head, self.desc.stride_pos = self.k.stride()[:3]
+        self.desc_ref = ctypes.byref(self.desc)
+        self.device_index = self.k.get_device()
 
     @property
     def n_pages(self) -> int:
@@ -533,44 +535,41 @@ class PagedCache:
         return out.value
 
 
-def _want(op: str, name: str, t, dtype, shape, device) -> None:
-    """A contiguous device tensor of the given dtype and shape on the pool's device (None in
-    ``shape``: any size)."""
-    if (t.dtype != dtype or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape))
-            or not t.is_contiguous()):
+def _want(op: str, name: str, t, dtype, shape, device: int) -> None:
+    """A contiguous tensor of the given dtype and shape on the pool's device (an index; -1: CPU)."""
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
         raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be a contiguous {dtype} tensor {tuple(shape)}, not "
                                           f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}")
-    if t.device != device:
-        raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} is on {t.device}, the pages on {device}")
+    if t.get_device() != device:
+        raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} is on {t.device}, the pages on device {device}")
 
 
-def _paged_batch(op: str, cache, table, q_starts, per_seq, name: str):
+def _paged_batch(op: str, cache, table, q_starts, per_seq, name: str, device: int):
+    """The checks of a call's table and per-sequence tensors; returns (B, table columns)."""
     import torch
 
-    dev = cache.k.device
-    _want(op, "table", table, torch.int32, (None, None), dev)
-    B = table.shape[0]
-    _want(op, name, per_seq, torch.int32, (B,), dev)
+    i32 = torch.int32
+    B, cols = table.shape if table.dim() == 2 else (None, None)
+    _want(op, "table", table, i32, (B, cols), device)
+    _want(op, name, per_seq, i32, (B,), device)
     if q_starts is not None:
-        _want(op, "q_starts", q_starts, torch.int32, (B + 1,), dev)
-    return B
+        _want(op, "q_starts", q_starts, i32, (B + 1,), device)
+    return B, cols
 
 
-class _on_device:
-    """Makes the pool's device current around a call, when it is not."""
+def _launch(device: int, stream, call, *args) -> int:
+    """call(stream, *args) with the pool's device current, on that device's current torch stream
+    when no stream is given. (torch._C's accessors: what torch.cuda.current_stream() and
+    current_device() wrap, without the objects they build, 2 us a call.)"""
+    import torch
 
-    def __init__(self, device):
-        import torch
-
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+    if device < 0:
+        raise EmaError(EMA_ERR_INVALID_ARG, call.__name__, "the pages are not on a GPU")
+    raw = torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
+    if torch._C._cuda_getDevice() == device:
+        return call(raw, *args)
+    with torch.cuda.device(device):
+        return call(raw, *args)
 
 
 def paged_append(qkv, q_norm_w, k_norm_w, eps, theta, offsets, n_heads, cache: PagedCache, table, q_starts=None,
@@ -581,24 +580,24 @@ def paged_append(qkv, q_norm_w, k_norm_w, eps, theta, offsets, n_heads, cache: P
     the rotation counts before the sequences' own. Returns q_out [n, Hq, D]."""
     import torch
 
-    op = "ema_paged_append"
-    dev, D, Hkv = cache.k.device, cache.desc.head_dim, cache.desc.n_kv_heads
-    B = _paged_batch(op, cache, table, q_starts, offsets, "offsets")
-    _want(op, "qkv", qkv, torch.bfloat16, (None, (n_heads + 2 * Hkv) * D), dev)
-    n = qkv.shape[0]
+    op, bf = "ema_paged_append", torch.bfloat16
+    desc, dev = cache.desc, cache.device_index
+    D = desc.head_dim
+    B, cols = _paged_batch(op, cache, table, q_starts, offsets, "offsets", dev)
+    n = qkv.shape[0] if qkv.dim() else 0
+    _want(op, "qkv", qkv, bf, (n, (n_heads + 2 * desc.n_kv_heads) * D), dev)
     for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
         if w is not None:
-            _want(op, name, w, torch.bfloat16, (D,), dev)
+            _want(op, name, w, bf, (D,), dev)
     if prefix_len is not None:
         _want(op, "prefix_len", prefix_len, torch.int32, (1,), dev)
     if q_out is None:
-        q_out = torch.empty((n, n_heads, D), dtype=torch.bfloat16, device=dev)
+        q_out = torch.empty((n, n_heads, D), dtype=bf, device=qkv.device)
     else:
-        _want(op, "q_out", q_out, torch.bfloat16, (n, n_heads, D), dev)
-    with _on_device(dev):
-        _check(lib().ema_paged_append(_stream(stream), _ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), eps, theta,
-                                      _ptr(q_starts), _ptr(offsets), _ptr(prefix_len), B, n, n_heads, flags,
-                                      _ptr(q_out), ctypes.byref(cache.desc), _ptr(table), table.shape[1]), op)
+        _want(op, "q_out", q_out, bf, (n, n_heads, D), dev)
+    _check(_launch(dev, stream, lib().ema_paged_append, qkv.data_ptr(), _ptr(q_norm_w), _ptr(k_norm_w), eps, theta,
+                   _ptr(q_starts), offsets.data_ptr(), _ptr(prefix_len), B, n, n_heads, flags, q_out.data_ptr(),
+                   cache.desc_ref, table.data_ptr(), cols), op)
     return q_out
 
 
@@ -621,12 +620,12 @@ def paged_workspace(batch, n_rows, n_heads, n_kv_heads, head_dim, max_q, max_len
 def _paged_out(op, q, cache, out):
     import torch
 
-    dev, D = cache.k.device, cache.desc.head_dim
-    _want(op, "q", q, torch.bfloat16, (None, None, D), dev)
-    n, Hq = q.shape[:2]
+    bf, dev, D = torch.bfloat16, cache.device_index, cache.desc.head_dim
+    n, Hq = q.shape[:2] if q.dim() == 3 else (None, None)
+    _want(op, "q", q, bf, (n, Hq, D), dev)
     if out is None:
-        return torch.empty((n, Hq * D), dtype=torch.bfloat16, device=dev)
-    _want(op, "out", out, torch.bfloat16, (n, Hq * D), dev)
+        return torch.empty((n, Hq * D), dtype=bf, device=q.device)
+    _want(op, "out", out, bf, (n, Hq * D), dev)
     return out
 
 
@@ -644,20 +643,19 @@ def paged_attention(q, cache: PagedCache, table, lengths, max_len, q_starts=None
     import torch
 
     op = "ema_paged_attention"
-    B = _paged_batch(op, cache, table, q_starts, lengths, "lengths")
+    dev = cache.device_index
+    B, cols = _paged_batch(op, cache, table, q_starts, lengths, "lengths", dev)
     out = _paged_out(op, q, cache, out)
     n, Hq, D = q.shape
     max_q = _rows_bound(op, q, B, q_starts, max_q)
     if workspace is None:
         workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, device=q.device)
     else:
-        _want(op, "workspace", workspace, torch.uint8, (None,), q.device)
-    with _on_device(q.device):
-        _check(lib().ema_paged_attention(_stream(stream), _ptr(q), ctypes.byref(cache.desc), _ptr(table),
-                                         table.shape[1], _ptr(q_starts), _ptr(lengths), B, n, max_q, max_len, Hq,
-                                         1.0 / math.sqrt(D) if scale is None else scale,
-                                         EMA_PREFILL_CAUSAL if causal else 0, _ptr(out), _ptr(workspace),
-                                         workspace.numel()), op)
+        _want(op, "workspace", workspace, torch.uint8, (workspace.numel(),), dev)
+    _check(_launch(dev, stream, lib().ema_paged_attention, q.data_ptr(), cache.desc_ref, table.data_ptr(), cols,
+                   _ptr(q_starts), lengths.data_ptr(), B, n, max_q, max_len, Hq,
+                   1.0 / math.sqrt(D) if scale is None else scale, EMA_PREFILL_CAUSAL if causal else 0,
+                   out.data_ptr(), workspace.data_ptr(), workspace.numel()), op)
     return out
 
 
@@ -670,20 +668,20 @@ def prefix_attention(q, cache: PagedCache, prefix_table, prefix_len, max_prefix,
     import torch
 
     op = "ema_prefix_attention"
-    B = _paged_batch(op, cache, table, q_starts, lengths, "lengths")
-    _want(op, "prefix_table", prefix_table, torch.int32, (None,), cache.k.device)
-    _want(op, "prefix_len", prefix_len, torch.int32, (1,), cache.k.device)
+    dev = cache.device_index
+    B, cols = _paged_batch(op, cache, table, q_starts, lengths, "lengths", dev)
+    pcols = prefix_table.numel()
+    _want(op, "prefix_table", prefix_table, torch.int32, (pcols,), dev)
+    _want(op, "prefix_len", prefix_len, torch.int32, (1,), dev)
     out = _paged_out(op, q, cache, out)
     n, Hq, D = q.shape
     max_q = _rows_bound(op, q, B, q_starts, max_q)
     if workspace is None:
         workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, max_prefix, device=q.device)
     else:
-        _want(op, "workspace", workspace, torch.uint8, (None,), q.device)
-    with _on_device(q.device):
-        _check(lib().ema_prefix_attention(_stream(stream), _ptr(q), ctypes.byref(cache.desc), _ptr(prefix_table),
-                                          prefix_table.shape[0], _ptr(prefix_len), max_prefix, _ptr(table),
-                                          table.shape[1], _ptr(q_starts), _ptr(lengths), B, n, max_q, max_len, Hq,
-                                          1.0 / math.sqrt(D) if scale is None else scale, _ptr(out), _ptr(workspace),
-                                          workspace.numel()), op)
+        _want(op, "workspace", workspace, torch.uint8, (workspace.numel(),), dev)
+    _check(_launch(dev, stream, lib().ema_prefix_attention, q.data_ptr(), cache.desc_ref, prefix_table.data_ptr(),
+                   pcols, prefix_len.data_ptr(), max_prefix, table.data_ptr(), cols, _ptr(q_starts),
+                   lengths.data_ptr(), B, n, max_q, max_len, Hq, 1.0 / math.sqrt(D) if scale is None else scale,
+                   out.data_ptr(), workspace.data_ptr(), workspace.numel()), op)
     return out
