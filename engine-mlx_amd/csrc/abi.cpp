@@ -738,7 +738,7 @@ extern "C" int32_t ema_paged_workspace_size(int32_t batch, int32_t n_rows, int32
   return EMA_OK;
 }
 
-static int32_t paged_attention(const char* op, ema_stream_t stream, const PagedAttention& p, int32_t max_len,
+static int32_t paged_attention(const char* op, ema_stream_t stream, PagedAttention p, int32_t max_len,
                                int32_t max_prefix, const ema_kvcache_desc* pages, void* workspace,
                                uint64_t workspace_bytes) {
   int32_t rc = check_page_table(op, pages, p.table, p.table_cols);
@@ -764,6 +764,9 @@ static int32_t paged_attention(const char* op, ema_stream_t stream, const PagedA
   if (tiles >= INT32_MAX || shared >= INT32_MAX)
     return set_error(EMA_ERR_UNSUPPORTED, "%s: %lld key tiles over all row blocks exceed 2^31 - 1", op,
                      (long long)(tiles > shared ? tiles : shared));
+  // a bound of the rows of one sequence beyond the call's own, or none where all have the same
+  if (!p.q_starts) p.max_q = p.n_rows / p.batch;
+  if (p.max_q > p.n_rows) p.max_q = p.n_rows;
   const PagedPlan plan = plan_paged(p.batch, p.n_rows, p.n_heads, pages->n_kv_heads, p.max_q, max_len, max_prefix);
   if (!workspace || workspace_bytes < plan.bytes)
     return set_error(EMA_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", op,

@@ -252,12 +252,19 @@ struct PagedAttention {
 };
 struct PagedPlan {
   int workers;          // workgroups over the sequences' own pages
-  int prefix_workers;   // workgroups over the shared prefix
+  int prefix_workers;   // workgroups over the shared prefix (few rows)
+  int chunks;           // chunks of the shared prefix (more rows), and their 64-key blocks
+  int chunk_blocks;
   uint64_t part_bytes;  // partial states of shared segments
   uint64_t carry_bytes; // states of the rows over the prefix
   uint64_t bytes;       // the whole workspace
 };
 PagedPlan plan_paged(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len, int max_prefix);
+// Prompts and chunks in prefill_kernel's 128-row blocks: the sequences of few < n <= p.max_q rows.
+int32_t launch_paged_prefill(hipStream_t s, const PagedAttention& p, const ema_kvcache_desc& c, int few);
+// All rows over chunks of the shared prefix, their states into part.
+int32_t launch_prefix_rows(hipStream_t s, const PagedAttention& p, const ema_kvcache_desc& c, int chunks,
+                           int chunk_blocks, float* part);
 int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema_kvcache_desc& c, const PagedPlan& plan,
                                void* ws);
 // Gated DeltaNet recurrent scan (arguments validated by the caller).

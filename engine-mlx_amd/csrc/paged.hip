@@ -11,11 +11,6 @@
 namespace ema {
 namespace {
 
-// Constant-address-space loads: table entries, lengths and row starts are uniform over a wave
-// and not written by the kernels, so they come as scalar loads.
-typedef const __attribute__((address_space(4))) int32_t cint;
-__device__ __forceinline__ int ld_uniform(const int32_t* p, int64_t i) { return ((cint*)p)[i]; }
-
 // ------------------------------------------------------------------ append
 // One workgroup per packed row, its groups of 8 lanes over the row's heads, as in the static
 // cache's pre-attention kernel (8 lanes hold a head: lane j elements jE.. of both halves, so a
@@ -214,7 +209,6 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kD = 128;
 constexpr int kSlot = kPagedTile * kD * 2;     // one K or V tile as bf16: 8 KB
-constexpr int kStateStride = kD + 4;           // floats of a partial state's row: m, l, pad, pad, o[D]
 
 struct PagedArgs {
   const uint16_t* q;
@@ -224,16 +218,21 @@ struct PagedArgs {
   const uint16_t* vexp;
   const int32_t* table;
   const int32_t* starts;  // null: T rows per sequence
+  const int32_t* rows_end;  // starts null, B 1: the rows end there, or null
   const int32_t* len;
   uint16_t* out;
   int32_t* cnt;     // arrival counters, one per worker
-  float* part;      // partial states, slots of [32][kStateStride]
-  const float* carry_in;  // states of the rows over a shared prefix [n_rows, Hq][kStateStride], or null
+  float* part;      // partial states, slots of [32][kPagedState]
+  const float* carry_in;  // states of the rows over a shared prefix [chunk][n_rows, Hq][kPagedState], or null
   float* carry_out;       // leave the rows' states there instead of their output, or null
+  const int32_t* prefix_len;
+  int carry_blocks;       // 64-key blocks of a chunk of the prefix (0: one state, always there)
+  int prefix_cap;         // positions that the prefix's table holds
   int64_t sb, sh;   // bytes
   uint32_t row_bytes;
   float qk_scale;   // scale * log2(e): scores live in the log2 domain
   int B, T, n_rows, Hq, Hkv, G, cols, shift, n_pages, W, causal;
+  int few, max_q;   // sequences of few < n <= max_q rows are prefill_kernel's
 };
 
 __device__ __forceinline__ u32x4 rsrc_words(const void* base, uint32_t bytes) {
@@ -270,33 +269,56 @@ struct State4 {  // four dims of a row: running max, row sum, unnormalised outpu
 };
 __device__ __forceinline__ float weight(float m, float M) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); }
 
-// A row's final state: joined with the carried one, then stored as output or carried on.
-__device__ __forceinline__ void finish4(const PagedArgs& a, int64_t row, int h, int d, State4 s) {
+// A row's final state: joined with those over the prefix's chunks, then stored as output or
+// carried on.
+__device__ __forceinline__ void finish4(const PagedArgs& a, int n_carry, bool keys, int64_t row, int h, int d, State4 s) {
   const int64_t rh = row * a.Hq + h;
   if (a.carry_in) {
-    const float* const c = a.carry_in + rh * kStateStride;
-    const float cm = c[0], cl = c[1];
-    const f32x4 co = *(const f32x4*)(c + 4 + d);
-    const float M = fmaxf(s.m, cm);
-    const float ws = weight(s.m, M), wc = weight(cm, M);
-    s.l = s.l * ws + (wc > 0.f ? cl * wc : 0.f);
-    s.o = s.o * ws;
-    if (wc > 0.f) s.o += co * wc;
-    s.m = M;
+    constexpr int kChunk = 8;  // states whose loads are in flight together
+    for (int c0 = 0; c0 < n_carry; c0 += kChunk) {
+      float2 cm[kChunk];
+      f32x4 co[kChunk];
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        const int c = c0 + i < n_carry ? c0 + i : n_carry - 1;
+        const float* const p = a.carry_in + ((int64_t)c * a.n_rows * a.Hq + rh) * kPagedState;
+        cm[i] = *(const float2*)p;
+        co[i] = *(const f32x4*)(p + 4 + d);
+      }
+      float M = s.m;
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) M = fmaxf(M, cm[i].x);
+      const float f = weight(s.m, M);
+      s.l *= f;
+      s.o *= f;
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        const float g = weight(cm[i].x, M);
+        if (c0 + i < n_carry && (g > 0.f || cm[i].y != cm[i].y)) {  // (a row that is not finite stays so)
+          s.l += cm[i].y * g;
+          s.o += co[i] * g;
+        }
+      }
+      s.m = M;
+    }
   }
   if (a.carry_out) {
-    float* const c = a.carry_out + rh * kStateStride;
+    float* const c = a.carry_out + rh * kPagedState;
     if (d == 0) *(float2*)c = make_float2(s.m, s.l);
     *(f32x4*)(c + 4 + d) = s.o;
     return;
   }
-  const float inv = s.l > 0.f ? 1.0f / s.l : 0.f;  // no key: zeros
+  const float inv = keys ? 1.0f / s.l : 0.f;  // no key: zeros; keys and no finite score: NaN, as the softmax is
   *(u32x2*)(a.out + rh * kD + d) = u32x2{pack_bf16x2(s.o[0] * inv, s.o[1] * inv), pack_bf16x2(s.o[2] * inv, s.o[3] * inv)};
 }
 
+__device__ __forceinline__ PagedRows own_rows(const PagedArgs& a, PagedRows r) {
+  if (r.n > a.few && r.n <= a.max_q) r.n = 0;
+  return r;
+}
 __device__ __forceinline__ PagedRows rows_of(const PagedArgs& a, int b) {
-  if (!a.starts) return PagedRows{b * a.T, a.T};
-  return paged_rows(ld_uniform(a.starts, b), ld_uniform(a.starts, b + 1), a.n_rows);
+  if (!a.starts) return a.rows_end ? paged_rows(0, ld_uniform(a.rows_end, 0), a.T) : PagedRows{b * a.T, a.T};
+  return own_rows(a, paged_rows(ld_uniform(a.starts, b), ld_uniform(a.starts, b + 1), a.n_rows));
 }
 __device__ __forceinline__ int clamp_len(const PagedArgs& a, int L) {
   const int64_t cap = (int64_t)a.cols << a.shift;
@@ -315,14 +337,28 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
+  // states of the rows over the prefix: one per chunk that holds keys
+  int n_carry = 1;
+  bool shared_keys = false;
+  if (a.carry_in) {
+    int n = ld_uniform(a.prefix_len, 0);
+    n = n < 0 ? 0 : (n > a.prefix_cap ? a.prefix_cap : n);
+    shared_keys = n > 0;
+    if (a.carry_blocks) n_carry = ((n + 63) / 64 + a.carry_blocks - 1) / a.carry_blocks;
+  }
+
   // Rounds before each sequence, by every wave for itself (all write the same values): lane l
   // takes sequences l step .. +step-1, and the lanes' sums are scanned.
   const int step = (a.B + 63) >> 6;
+  auto rows_n = [&](int b) __attribute__((always_inline)) {
+    if (a.starts) return own_rows(a, paged_rows(a.starts[b], a.starts[b + 1], a.n_rows)).n;
+    return rows_of(a, 0).n;
+  };
   int sum = 0;
   for (int i = 0; i < step; ++i) {
     const int b = lane * step + i;
     if (b < a.B) {
-      const int T = a.starts ? paged_rows(a.starts[b], a.starts[b + 1], a.n_rows).n : a.T;
+      const int T = rows_n(b);
       sum += paged_rounds(clamp_len(a, a.len[b])) * blocks_of(a, T) * a.Hkv;
     }
   }
@@ -338,7 +374,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     const int b = lane * step + i;
     if (b < a.B) {
       pre[b] = run;
-      const int T = a.starts ? paged_rows(a.starts[b], a.starts[b + 1], a.n_rows).n : a.T;
+      const int T = rows_n(b);
       run += paged_rounds(clamp_len(a, a.len[b])) * blocks_of(a, T) * a.Hkv;
     }
   }
@@ -353,7 +389,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     const PagedRows rw = rows_of(a, b);
     const State4 none = {-INFINITY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
     for (int64_t e = tid; e < (int64_t)rw.n * a.Hq * 32; e += 64 * kPagedWaves)
-      finish4(a, rw.begin + e / (a.Hq * 32), (int)(e / 32 % a.Hq), (int)(e % 32) * 4, none);
+      finish4(a, n_carry, shared_keys, rw.begin + e / (a.Hq * 32), (int)(e / 32 % a.Hq), (int)(e % 32) * 4, none);
   }
 
   const int W = paged_active_workers(total, a.W);
@@ -617,9 +653,9 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       }
       if (w0 == w1) {
         const int ir = row0 + r, tk = (int)((uint32_t)ir / (uint32_t)a.G);
-        finish4(a, (int64_t)rw.begin + tk, kh * a.G + ir - tk * a.G, 4 * d4, s);
+        finish4(a, n_carry, shared_keys || !a.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk, kh * a.G + ir - tk * a.G, 4 * d4, s);
       } else {
-        float* const p = a.part + ((int64_t)paged_slot(w, w0) * kPagedRows + r) * kStateStride;
+        float* const p = a.part + ((int64_t)paged_slot(w, w0) * kPagedRows + r) * kPagedState;
         if (d4 == 0) put2(p, s.m, s.l);
         put2(p + 4 + 4 * d4, s.o[0], s.o[1]);
         put2(p + 6 + 4 * d4, s.o[2], s.o[3]);
@@ -650,7 +686,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
             for (int i = 0; i < kChunk; ++i) {
               const int ww = c0 + i <= w1 ? c0 + i : w1;
-              const float* const p = a.part + ((int64_t)paged_slot(ww, w0) * kPagedRows + r) * kStateStride;
+              const float* const p = a.part + ((int64_t)paged_slot(ww, w0) * kPagedRows + r) * kPagedState;
               pm[i] = get2(p);
               pa[i] = get2(p + 4 + 4 * d4);
               pb[i] = get2(p + 6 + 4 * d4);
@@ -671,19 +707,13 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
             s.m = M;
           }
           const int ir = row0 + r, tk = (int)((uint32_t)ir / (uint32_t)a.G);
-          finish4(a, (int64_t)rw.begin + tk, kh * a.G + ir - tk * a.G, 4 * d4, s);
+          finish4(a, n_carry, shared_keys || !a.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk, kh * a.G + ir - tk * a.G, 4 * d4, s);
         }
       }
     }
     __syncthreads();  // the slots and ml are reused by the next piece
     t = piece_end;
   }
-}
-
-int page_shift(int page) {
-  int s = 0;
-  while ((1 << s) < page) ++s;
-  return s;
 }
 
 }  // namespace
@@ -713,7 +743,7 @@ int32_t launch_paged_append(hipStream_t s, const PagedAppend& p, const ema_kvcac
   a.Hq = p.n_heads;
   a.Hkv = c.n_kv_heads;
   a.cols = p.table_cols;
-  a.shift = page_shift(c.capacity);
+  a.shift = paged_shift(c.capacity);
   a.n_pages = c.batch;
   a.flags = p.flags;
   const dim3 grid((unsigned)p.n_rows), block(256);
@@ -724,6 +754,12 @@ int32_t launch_paged_append(hipStream_t s, const PagedAppend& p, const ema_kvcac
   return check_hip(hipGetLastError(), "ema_paged_append launch");
 }
 
+// More query rows than this per (sequence, kv head) run in prefill_kernel's 128-row blocks (bf16
+// pages), fewer in paged_kernel's 32-row segments.
+constexpr int kFewRows = 128;
+// A shared prefix: more rows than this per kv head in 128-row blocks over chunks of it.
+constexpr int kFewPrefixRows = 32;
+
 // Workspace: the arrival counters, the partial states of the workers' shared segments, then
 // the rows' states over a shared prefix.
 PagedPlan plan_paged(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len, int max_prefix) {
@@ -731,13 +767,17 @@ PagedPlan plan_paged(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len,
   const int G = Hq / Hkv;
   p.workers = paged_plan_workers(paged_row_blocks(B, n_rows, max_q, G), Hkv, max_len);
   p.prefix_workers = 0;
+  p.chunks = p.chunk_blocks = 0;
   p.carry_bytes = 0;
   if (max_prefix > 0) {
     p.prefix_workers = paged_plan_workers(paged_row_blocks(1, n_rows, n_rows, G), Hkv, max_prefix);
-    p.carry_bytes = (uint64_t)n_rows * Hq * kStateStride * sizeof(float);
+    const PagedChunks c = paged_chunks((int64_t)n_rows * G, Hkv, max_prefix, device_cus());
+    p.chunks = c.n;
+    p.chunk_blocks = c.blocks;
+    p.carry_bytes = (uint64_t)c.n * n_rows * Hq * kPagedState * sizeof(float);
   }
   const int w = p.workers > p.prefix_workers ? p.workers : p.prefix_workers;
-  p.part_bytes = (uint64_t)2 * w * kPagedRows * kStateStride * sizeof(float);
+  p.part_bytes = (uint64_t)2 * w * kPagedRows * kPagedState * sizeof(float);
   p.bytes = kDecodeCounterBytes + p.part_bytes + p.carry_bytes;
   return p;
 }
@@ -754,12 +794,16 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
   a.vexp = (const uint16_t*)c.v_exp;
   a.table = p.table;
   a.starts = p.q_starts;
+  a.rows_end = nullptr;
   a.len = p.lengths;
   a.out = (uint16_t*)p.out;
   a.cnt = (int32_t*)ws;
   a.part = (float*)((char*)ws + kDecodeCounterBytes);
   a.carry_in = nullptr;
   a.carry_out = nullptr;
+  a.prefix_len = p.prefix_len;
+  a.carry_blocks = 0;
+  a.prefix_cap = p.prefix_cols << paged_shift(c.capacity);
   a.sb = c.stride_batch * es;
   a.sh = c.stride_head * es;
   a.row_bytes = (uint32_t)(c.stride_pos * es);
@@ -771,27 +815,42 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
   a.Hkv = c.n_kv_heads;
   a.G = p.n_heads / c.n_kv_heads;
   a.cols = p.table_cols;
-  a.shift = page_shift(c.capacity);
+  a.shift = paged_shift(c.capacity);
   a.n_pages = c.batch;
   a.causal = p.causal;
+  a.few = INT32_MAX;
+  a.max_q = 0;
   const dim3 block(64 * kPagedWaves);
   if (p.prefix_table) {
     float* const carry = (float*)((char*)ws + kDecodeCounterBytes + plan.part_bytes);
-    PagedArgs x = a;  // all rows of the batch as one sequence over the shared pages
-    x.table = p.prefix_table;
-    x.cols = p.prefix_cols;
-    x.len = p.prefix_len;
-    x.starts = nullptr;
-    x.B = 1;
-    x.T = p.n_rows;
-    x.causal = 0;
-    x.carry_out = carry;
-    x.W = plan.prefix_workers;
-    if (fp8) hipLaunchKernelGGL(paged_kernel<true>, dim3(x.W), block, 0, s, x);
-    else hipLaunchKernelGGL(paged_kernel<false>, dim3(x.W), block, 0, s, x);
-    const int32_t rc = check_hip(hipGetLastError(), "ema_prefix_attention prefix launch");
-    if (rc) return rc;
+    if (!fp8 && (int64_t)p.n_rows * a.G > kFewPrefixRows) {
+      const int32_t rc = launch_prefix_rows(s, p, c, plan.chunks, plan.chunk_blocks, carry);
+      if (rc) return rc;
+      a.carry_blocks = plan.chunk_blocks;
+    } else {
+      PagedArgs x = a;  // all rows of the batch as one sequence over the shared pages
+      x.table = p.prefix_table;
+      x.cols = p.prefix_cols;
+      x.len = p.prefix_len;
+      x.starts = nullptr;
+      x.rows_end = p.q_starts ? p.q_starts + p.batch : nullptr;
+      x.B = 1;
+      x.T = p.n_rows;
+      x.causal = 0;
+      x.carry_out = carry;
+      x.W = plan.prefix_workers;
+      if (fp8) hipLaunchKernelGGL(paged_kernel<true>, dim3(x.W), block, 0, s, x);
+      else hipLaunchKernelGGL(paged_kernel<false>, dim3(x.W), block, 0, s, x);
+      const int32_t rc = check_hip(hipGetLastError(), "ema_prefix_attention prefix launch");
+      if (rc) return rc;
+    }
     a.carry_in = carry;
+  } else if (!fp8 && (int64_t)p.max_q * a.G > kFewRows) {
+    const int few = kFewRows / a.G;
+    const int32_t rc = launch_paged_prefill(s, p, c, few);
+    if (rc || !p.q_starts) return rc;  // (the same rows for all: every sequence is done)
+    a.few = few;  // the sequences of few rows, and of more than the bound says, are left
+    a.max_q = p.max_q;
   }
   a.W = plan.workers;
   if (fp8) hipLaunchKernelGGL(paged_kernel<true>, dim3(a.W), block, 0, s, a);

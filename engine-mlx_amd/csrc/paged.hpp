@@ -14,6 +14,7 @@ constexpr int kPagedRows = 32;      // query rows of a segment: (token, head of 
 constexpr int kPagedTile = 32;      // keys per tile
 constexpr int kPagedWaves = 4;      // waves per workgroup, each with tiles of its own
 constexpr int kPagedMaxWorkers = 512;
+constexpr int kPagedState = 128 + 4;  // floats of a row's partial state: m, l, pad, pad, o[128]
 constexpr int kPagedMinPage = 16;   // a wave's 1 KB loads (4 rows) never straddle two pages
 
 // Query rows of sequence b: packed rows [begin, begin + n). Row starts from the device are
@@ -56,10 +57,40 @@ EMA_HD int paged_plan_workers(int64_t nrb, int Hkv, int max_len) {
   return (int)(want < 1 ? 1 : (want < kPagedMaxWorkers ? want : kPagedMaxWorkers));
 }
 // Row blocks of a batch whose sequences have at most max_q rows and n_rows together.
+EMA_HD int paged_shift(int page) {
+  int s = 0;
+  while ((1 << s) < page) ++s;
+  return s;
+}
 EMA_HD int64_t paged_row_blocks(int B, int64_t n_rows, int64_t max_q, int G) {
   const int64_t each = (int64_t)B * ((max_q * G + kPagedRows - 1) / kPagedRows);
   const int64_t all = n_rows * G / kPagedRows + B;
   return each < all ? each : all;
 }
+
+// A shared prefix cut into chunks of 64-key blocks for its row blocks of 128 over all kv heads:
+// as many chunks as give the chip one workgroup per CU, of two blocks at least (one for each
+// half of a workgroup).
+struct PagedChunks {
+  int n, blocks;  // chunks, and 64-key blocks of each
+};
+EMA_HD PagedChunks paged_chunks(int64_t rows, int Hkv, int max_prefix, int cus) {
+  const int64_t wgs = (rows > 0 ? (rows + 127) / 128 : 1) * Hkv;
+  const int total = (int)(((int64_t)max_prefix + 63) / 64);
+  int64_t n = cus / wgs;
+  if (n > (total + 1) / 2) n = (total + 1) / 2;
+  if (n < 1) n = 1;
+  PagedChunks c;
+  c.blocks = (int)((total + n - 1) / n);
+  c.n = (total + c.blocks - 1) / c.blocks;
+  return c;
+}
+
+#if defined(__HIPCC__)
+// Constant-address-space loads: table entries, lengths and row starts are uniform over a wave
+// and not written by the kernels, so they come as scalar loads.
+typedef const __attribute__((address_space(4))) int32_t paged_cint;
+__device__ __forceinline__ int ld_uniform(const int32_t* p, int64_t i) { return ((paged_cint*)p)[i]; }
+#endif
 
 }  // namespace ema

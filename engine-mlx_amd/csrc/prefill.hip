@@ -32,8 +32,11 @@
 // softmax of its block (VALU, exp) and issues the global-to-LDS loads of its next tiles;
 // in the next phase the roles swap. The matrix pipe and the vector pipe of a SIMD are fed
 // by different waves throughout.
+#include <type_traits>
+
 #include "ema_common.hpp"
 #include "ema_schedule.hpp"
+#include "paged.hpp"
 
 namespace ema {
 namespace {
@@ -66,6 +69,21 @@ struct PrefillArgs {
   uint32_t flags;
 };
 
+// Where a kernel's keys and query rows come from.
+constexpr int kStaticCache = 0;  // a cache plane per (sequence, kv head), q [B, Hq, T, D]
+constexpr int kPages = 1;        // pages of a pool, packed ragged rows
+constexpr int kSharedPages = 2;  // pages that every packed row of the batch sees
+struct PagedPrefillArgs : PrefillArgs {
+  const int32_t* table;
+  const int32_t* starts;  // null: T rows per sequence
+  const int32_t* len;
+  float* part;  // kSharedPages: the rows' states [chunk][n_rows, Hq][kPagedState]
+  int64_t page_bytes, head_bytes;
+  int n_rows, cols, shift, n_pages;
+  int few, max_q;       // kPages: sequences of few < n <= max_q rows are this kernel's
+  int chunk_blocks;     // kSharedPages: 64-key blocks per chunk of the keys
+};
+
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // compile-time choice of the softmax step's masking code
 struct MaskOn { static constexpr bool value = true; };
@@ -94,15 +112,16 @@ __device__ __forceinline__ u32x4 buffer_rsrc(const void* base, uint32_t bytes) {
 // compiler does not track it: the caller orders it with explicit vmcnt waits before the
 // barrier that publishes the tile, instead of the compiler draining every load in flight
 // at each barrier and before each LDS read.
-template <int I>
+// kNops: wait states after the write of M0, less one.
+template <int I, int kNops = 0>
 __device__ __forceinline__ void dma16(u32x4 rsrc, uint32_t voff, uint32_t lds_addr) {
   // lds_addr is wave-uniform; readfirstlane keeps it in a scalar register for M0
   // s_nop 0: the DMA reads M0 no earlier than one wait state after the SALU write, a wait
   // the compiler inserts only for the LDS-DMAs it emits itself. (Its SGPR operands need five
   // after a VALU write; check_hazards.py fails the build if the compiler places one closer.)
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen offset:%3 lds"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop %4\n\tbuffer_load_dwordx4 %0, %1, 0 offen offset:%3 lds"
                :
-               : "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "i"(1024 * I)
+               : "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "i"(1024 * I), "i"(kNops)
                : "memory", "m0");
 }
 // Block offset that no buffer range reaches (ranges stay below 2^31 bytes, and a per-lane
@@ -114,6 +133,45 @@ __device__ __forceinline__ uint32_t pk_max3_f16(uint32_t a, uint32_t b, uint32_t
   uint32_t r;
   asm("v_pk_maximum3_f16 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
+}
+
+// Item x of a ragged batch's (one kv head): its sequence, and its place p among the sequence's
+// blocks of 128 rows, heaviest first (kPair: among its pairs). Lane l of every wave counts the
+// items of sequences l step .. +step-1; the counts are scanned over the lanes, and where a lane
+// has several sequences, over those of the lane found. False past the last item.
+template <bool kPair>
+__device__ __forceinline__ bool ragged_item(const PagedPrefillArgs& a, int x, int& b, int& p) {
+  const int lane = threadIdx.x & 63;
+  const int step = (a.B + 63) >> 6;
+  auto items = [&](int i) __attribute__((always_inline)) {
+    if (i >= a.B) return 0;
+    const int n = paged_rows(a.starts[i], a.starts[i + 1], a.n_rows).n;
+    if (n <= a.few || n > a.max_q) return 0;  // paged_kernel's
+    const int nqb = (n * a.G + kBM - 1) / kBM;
+    return kPair ? (nqb + 1) / 2 : nqb;
+  };
+  auto before = [&](int v) __attribute__((always_inline)) {
+    int s = v;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(s, d, 64);
+      if (lane >= d) s += y;
+    }
+    return s - v;
+  };
+  int sum = 0;
+  for (int i = 0; i < step; ++i) sum += items(lane * step + i);
+  int pre = before(sum);
+  if (x >= __builtin_amdgcn_readlane(pre + sum, 63)) return false;
+  int at = 63 - __builtin_clzll(__ballot(pre <= x));  // the last lane that begins at or before x
+  p = x - __builtin_amdgcn_readlane(pre, at);
+  b = at * step;
+  if (step > 1) {
+    pre = before(lane < step ? items(b + lane) : 0);
+    at = 63 - __builtin_clzll(__ballot(lane < step && pre <= p));
+    p -= __builtin_amdgcn_readlane(pre, at);
+    b += at;
+  }
+  return true;
 }
 
 // kRot: rotating cache (EMA_KV_ROTATING). The keys of a sequence are the positions
@@ -130,11 +188,23 @@ __device__ __forceinline__ uint32_t pk_max3_f16(uint32_t a, uint32_t b, uint32_t
 // rows are complete when group 0 leaves them; group 0 stores them on its own. A middle
 // block paired with itself (odd block count) runs as a heavy block with no light rows.
 // kWindow (with kPair): chunk-only calls, whose window may begin inside a key block.
+//
+// kMode kPages: the keys lie in pages (at least 16 positions: the 16 rows of a tile that a wave
+// loads are one page's, whose table entry is read two blocks ahead), and the query rows are the
+// (token, head of the kv group) pairs of the sequence's packed rows, row i being token i / G,
+// head i % G: a block of 128 rows spans 128 / G tokens, so the causal edge costs less than a
+// block of one head does. kSharedPages: the rows of the whole batch over a chunk of the pages
+// that all of them see; the rows' states (o not normalised, running max, row sum) are left for
+// paged_kernel to join with the sequences' own. In both the Q operand is q as it came, and the
+// scores are scaled in 32 bits (a multiply per score, which the other group's matrix step
+// hides), where the static kernels round the scaled q to bf16.
 // Aligned, since the time of a kernel this long depends on where its code lies (T 2048, 32q/8kv
 // with its pre-attention: 51.6 us from a 4 KB boundary, 51.8 to 52.3 at other multiples of 256).
-template <bool kRot, bool kPair, bool kWindow = false>
+template <bool kRot, bool kPair, bool kWindow = false, int kMode = kStaticCache>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2), aligned(4096))) void prefill_kernel(
-    PrefillArgs a) {
+    std::conditional_t<kMode == kStaticCache, PrefillArgs, PagedPrefillArgs> a) {
+  constexpr bool kPaged = kMode != kStaticCache;
+  static_assert(!kPaged || (!kRot && !kWindow), "a pool of pages is no ring and has no chunk window");
   extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
 
   const int tid = threadIdx.x;
@@ -146,14 +216,52 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   // blocks first, and with two workgroups' worth of query blocks or more per CU a pair
   // per workgroup -- the heavy block nqb-1-p, then the light one p of the same head --
   // which balances the causal work per workgroup and pays one launch per pair.
-  const PrefillItem item = prefill_item(blockIdx.x, gridDim.x, a.B, a.Hkv, a.G, a.nqb, kPair ? 1 : 0);
+  PrefillItem item;
+  PagedRows prow = {0, 0};  // kPaged: the sequence's packed rows
+  int chunk = 0;            // kSharedPages: the workgroup's chunk of the keys
+  if constexpr (kMode == kSharedPages) {
+    // row blocks innermost, so that those of one chunk meet on one XCD
+    const int rank = xcd_rank((int)blockIdx.x, (int)gridDim.x), rest = rank / a.nqb;
+    item.b = 0;
+    item.kh = item.h = rest % a.Hkv;
+    item.qb_first = item.qb_second = rank % a.nqb;
+    chunk = rest / a.Hkv;
+    prow.n = a.starts ? paged_rows(0, ld_uniform(a.starts, a.B), a.n_rows).n : a.n_rows;
+    // paged_kernel reads the states of the chunks that hold keys (and no load is in flight yet)
+    const int64_t keys = min((int64_t)ld_uniform(a.len, 0), (int64_t)a.cols << a.shift);
+    if ((int64_t)chunk * a.chunk_blocks * kBN >= keys) return;
+  } else if constexpr (kMode == kPages) {
+    if (a.starts) {
+      item.kh = item.h = (int)(blockIdx.x % (uint32_t)a.Hkv);
+      int p;
+      if (!ragged_item<kPair>(a, (int)(blockIdx.x / (uint32_t)a.Hkv), item.b, p)) return;  // (past the batch's items)
+      prow = paged_rows(ld_uniform(a.starts, item.b), ld_uniform(a.starts, item.b + 1), a.n_rows);
+      item.qb_first = (prow.n * a.G + kBM - 1) / kBM - 1 - p;
+      item.qb_second = kPair ? p : item.qb_first;
+    } else {
+      item = prefill_item(blockIdx.x, gridDim.x, a.B, a.Hkv, 1, a.nqb, kPair ? 1 : 0);
+      prow = PagedRows{item.b * a.T, a.T};
+    }
+  } else {
+    item = prefill_item(blockIdx.x, gridDim.x, a.B, a.Hkv, a.G, a.nqb, kPair ? 1 : 0);
+  }
   const int b = item.b;
   const int h = item.h;
   const int kh = item.kh;
-  const int q_off_arg = a.q_off[b];  // (a scalar load, waited for after the Q loads are issued)
+  int q_off_arg;
+  if constexpr (kPaged) q_off_arg = ld_uniform(a.len, b);
+  else q_off_arg = a.q_off[b];  // (a scalar load, waited for after the Q loads are issued)
   const int qb_h = item.qb_first;
   const bool has_light = kPair && item.qb_second != qb_h;
   const int qb_l = has_light ? item.qb_second : qb_h;
+  const int n_rows = kPaged ? prow.n * a.G : a.T;  // query rows of the item's (sequence, head or kv head)
+  // token of query row r, relative to the sequence's first, and the row of q and out that it is
+  auto token_of = [&](int r) __attribute__((always_inline)) { return kPaged ? (int)((uint32_t)r / (uint32_t)a.G) : r; };
+  auto out_row = [&](int r0, int r) __attribute__((always_inline)) {
+    if (!kPaged) return ((int64_t)b * a.T + r0 + r) * a.Hq + h;
+    const int t = token_of(r0 + r);
+    return ((int64_t)prow.begin + t) * a.Hq + kh * a.G + (r0 + r - t * a.G);
+  };
   const int row0 = qb_h * kBM;                    // first query row of the heavy block
   const int row0A = qb_l * kBM;                   // and of the light block
 
@@ -164,6 +272,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   // T arrive as zeros.
   const int r4 = lane >> 4, p16 = lane & 15;  // row within the 4, chunk position in the row
   auto load_q = [&](int qrow0, uint32_t dst) __attribute__((always_inline)) {
+    if constexpr (kPaged) {  // rows of the kv head's group, a token's Hq rows apart; offsets below 2^31 (host)
+      const u32x4 r = buffer_rsrc(a.q + ((int64_t)prow.begin * a.Hq + kh * a.G) * kD, (uint32_t)prow.n * a.Hq * kD * 2);
+      for (int i = 0; i < 4; ++i) {
+        const int row = qrow0 + 16 * wave + 4 * i + r4;
+        const int t = token_of(row);
+        const uint32_t off = (uint32_t)(t * a.Hq + row - t * a.G) * kD * 2 + (uint32_t)((p16 ^ (4 * i + r4)) * 16);
+        dma16<0, 4>(r, row < n_rows ? off : kNoRow, dst + 4 * i * kD * 2);
+      }
+      return;
+    }
     const int qrows = a.T - qrow0 < kBM ? a.T - qrow0 : kBM;
     const u32x4 r = buffer_rsrc(a.q + (((int64_t)b * a.Hq + h) * a.T + qrow0) * kD, (uint32_t)qrows * kD * 2);
     for (int i = 0; i < 4; ++i) {
@@ -181,6 +299,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   if (has_light) load_q(row0A, (uint32_t)(uintptr_t)(lds_void*)light_q(16 * wave));
 
   int q_off = q_off_arg < 0 ? 0 : q_off_arg;
+  int kv_held = 0;  // kPaged: keys of the sequence
+  if constexpr (kPaged) {
+    const int64_t cap = (int64_t)a.cols << a.shift;
+    kv_held = q_off > cap ? (int)cap : q_off;
+    q_off = kv_held - prow.n;  // (negative: the first rows see nothing)
+  }
   int key_base = 0;  // absolute position of key index 0 (rotating cache; n_tokens <= cap)
   if (kRot) {
     key_base = q_off + a.T - a.cap;
@@ -189,15 +313,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   }
   int kv_len = q_off + a.T;
   kv_len = kv_len > a.cap ? a.cap : kv_len;
-  const bool causal = a.flags & EMA_PREFILL_CAUSAL;
-  int kv_begin = (a.flags & EMA_PREFILL_CHUNK_ONLY) ? q_off : 0;
+  if constexpr (kPaged) kv_len = kv_held;
+  const bool causal = kMode != kSharedPages && (a.flags & EMA_PREFILL_CAUSAL);
+  int kv_begin = !kPaged && (a.flags & EMA_PREFILL_CHUNK_ONLY) ? q_off : 0;
+  if constexpr (kMode == kSharedPages) {
+    kv_begin = chunk * a.chunk_blocks * kBN;
+    kv_len = kv_len < kv_begin + a.chunk_blocks * kBN ? kv_len : kv_begin + a.chunk_blocks * kBN;
+  }
   kv_begin = kv_begin > kv_len ? kv_len : kv_begin;
   const int blk_begin = kv_begin / kBN;
   // 64-key blocks attended by query block qb: [blk_begin, blk_begin + blocks_of(qb))
   auto blocks_of = [&](int qb) __attribute__((always_inline)) {
     int wg_end = kv_len;
     if (causal) {
-      const int lim = q_off + qb * kBM + kBM;     // its last row sees keys < lim
+      const int lim = kPaged ? q_off + token_of(qb * kBM + kBM - 1) + 1 : q_off + qb * kBM + kBM;  // its last row sees keys < lim
       wg_end = lim < wg_end ? lim : wg_end;
     }
     const int blk_end = (wg_end + kBN - 1) / kBN;
@@ -228,8 +357,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   const int hh = lane >> 5;                       // which half of the k slots
   // the wave's first query row in either segment; lane row: + (lane & 31), causal limit
   // key <= that
-  const int wfaB = q_off + row0 + 32 * wq, wfaA = q_off + row0A + 32 * wq;
+  const int wfaB = kPaged ? q_off + token_of(row0 + 32 * wq) : q_off + row0 + 32 * wq;
+  const int wfaA = kPaged ? q_off + token_of(row0A + 32 * wq) : q_off + row0A + 32 * wq;
   auto wfa_of = [&](int j, auto seg) __attribute__((always_inline)) { return in_a(j, seg) ? wfaA : wfaB; };
+  // limits of the wave's last row and of the lane's own
+  const int wlaB = kPaged ? q_off + token_of(row0 + 32 * wq + 31) : wfaB + 31;
+  const int wlaA = kPaged ? q_off + token_of(row0A + 32 * wq + 31) : wfaA + 31;
+  const int laneB = kPaged ? q_off + token_of(row0 + 32 * wq + (lane & 31)) : 0;
+  const int laneA = kPaged && kPair ? q_off + token_of(row0A + 32 * wq + (lane & 31)) : 0;
+
+  // (a row that sees keys and no finite score is NaN, as its softmax is; one that sees none, zeros)
+  auto row_has_keys = [&](int last) __attribute__((always_inline)) { return causal ? last >= 0 : kv_len > 0; };
 
   uint16_t* const Ks = lds + g * kGroupElems;     // this group's K tiles: buffer i at Ks + i * kTile
   uint16_t* const Vs = Ks + 2 * kTile;            // and V tiles
@@ -261,7 +399,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   // non-negative) and stay the same for every block.
   uint32_t koff[4], voff[4];
   for (int i = 0; i < 4; ++i) {
-    const uint32_t row = (uint32_t)(16 * wq + 4 * i + r4);
+    const uint32_t row = (uint32_t)((kPaged ? 0 : 16 * wq) + 4 * i + r4);  // (paged: of the wave's 16 rows)
     koff[i] = row * row_bytes + (uint32_t)((p16 ^ (4 * i + r4)) * 16) - 1024u * i;
     voff[i] = row * row_bytes + (uint32_t)((p16 ^ (4 * r4)) * 16) - 1024u * i;
   }
@@ -278,6 +416,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
     return kRot && j < ng ? a.cap - (key_base + blk_of(j) * kBN) % a.cap : kBN;
   };
   const uint32_t ring_bytes = (uint32_t)a.cap * row_bytes;
+  // kPaged: the table entry of the 16 keys of block j that this wave loads (any entry past the
+  // keys), and their rows: none past the stream, past the keys or on an entry outside the pool
+  auto entry = [&](int j) __attribute__((always_inline)) {
+    if constexpr (kPaged) {
+      const int c = (blk_of(j < ng ? j : 0) * kBN + 16 * wq) >> a.shift;
+      return ld_uniform(a.table + (int64_t)b * a.cols, c < a.cols ? c : a.cols - 1);
+    }
+    return 0;
+  };
+  auto page_rsrc = [&](const uint16_t* pool, int j, int page) __attribute__((always_inline)) {
+    if constexpr (kPaged) {
+      const int pos = blk_of(j) * kBN + 16 * wq;
+      const bool in = (uint32_t)page < (uint32_t)a.n_pages;
+      int n = kv_len - pos;
+      n = j < ng && in && n > 0 ? (n < 16 ? n : 16) : 0;
+      return buffer_rsrc((const char*)pool + (in ? (int64_t)page * a.page_bytes : 0) + (int64_t)kh * a.head_bytes +
+                             (int64_t)(pos & ((1 << a.shift) - 1)) * row_bytes,
+                         (uint32_t)n * row_bytes);
+    }
+    return u32x4{0u, 0u, 0u, 0u};
+  };
+  int ent_v = 0, ent_k = 0;  // entries of blocks j + 1 and j + 2 in softmax step j
   auto tile_dst = [&](const uint16_t* tile) __attribute__((always_inline)) {
     return (uint32_t)(uintptr_t)(lds_void*)(tile + 16 * wq * kD);
   };
@@ -296,6 +456,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       return;
     }
     const uint32_t o = lane_rows && off_blk == kNoRow ? kNoRow : off[i];
+    if constexpr (kPaged) {
+      switch (i) {
+        case 0: dma16<0, 4>(r, o, dst); break;
+        case 1: dma16<1, 4>(r, o, dst); break;
+        case 2: dma16<2, 4>(r, o, dst); break;
+        default: dma16<3, 4>(r, o, dst); break;
+      }
+      return;
+    }
     switch (i) {
       case 0: dma16<0>(r, o, dst); break;
       case 1: dma16<1>(r, o, dst); break;
@@ -321,8 +490,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       for (int i = 0; i < 4; ++i) dma_part(r, ob, off, dst, i, wrap);
     }
   };
-  auto load_k = [&](int j) __attribute__((always_inline)) { dma(Kg, k_rsrc, j, koff, Ks + (j & 1) * kTile); };
-  auto load_v = [&](int j) __attribute__((always_inline)) { dma(Vg, v_rsrc, j, voff, Vs + (j & 1) * kTile); };
+  auto load_k = [&](int j, int ent) __attribute__((always_inline)) {
+    if constexpr (kPaged) {
+      const u32x4 r = page_rsrc(a.k, j, ent);
+      for (int i = 0; i < 4; ++i) dma_part(r, 0u, koff, tile_dst(Ks + (j & 1) * kTile), i, kBN);
+    } else {
+      dma(Kg, k_rsrc, j, koff, Ks + (j & 1) * kTile);
+    }
+  };
+  auto load_v = [&](int j, int ent) __attribute__((always_inline)) {
+    if constexpr (kPaged) {
+      const u32x4 r = page_rsrc(a.v, j, ent);
+      for (int i = 0; i < 4; ++i) dma_part(r, 0u, voff, tile_dst(Vs + (j & 1) * kTile), i, kBN);
+    } else {
+      dma(Vg, v_rsrc, j, voff, Vs + (j & 1) * kTile);
+    }
+  };
 
   // Online softmax state of this lane's row, in the log2 domain. The accumulators hold
   // o and l relative to the base m_use (p = 2^(s - m_use)); the score MFMA chains start
@@ -332,6 +515,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   float m_use = 0.f;
   bool seen = false;      // m_use is this row's running max (some score was finite)
   bool all_seen = false;  // wave-uniform: every row of the wave is seen
+  // kPaged: the row's scores are not finite; it takes no part in the products (the row sums' MFMA
+  // would spread its NaN to the row 16 away, which may be another sequence's) and ends as NaN
+  bool broken = false, broken_a = false;  // (of the rows in hand, and of segment A's until they leave)
   bool rescale = false;   // wave-uniform: o and the row sums are to be scaled before the next PV
   float o_scale = 1.f;    // factor of this lane's row
   f32x16 o[4], sc[2];
@@ -366,7 +552,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
 
   // Some row of the wave attends to a key of block j (the last row's limit is the first's + 31).
   auto active = [&](int j, auto seg) __attribute__((always_inline)) {
-    return !causal || (j + (in_a(j, seg) ? gbA : offB)) * kBN <= wfa_of(j, seg) + 31;
+    return !causal || (j + (in_a(j, seg) ? gbA : offB)) * kBN <= (kPaged ? (in_a(j, seg) ? wlaA : wlaB) : wfa_of(j, seg) + 31);
   };
   // Block j holds keys outside [kv_begin, kv_len) or above the causal limit of some row
   // of this wave. Inside a segment, for its blocks after the first, this holds exactly
@@ -385,9 +571,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
     }
     return jm < 1 ? 1 : jm;
   };
-  auto seg_act = [&](int gb, int wave_first, int n) __attribute__((always_inline)) {
+  auto seg_act = [&](int gb, int wave_last, int n) __attribute__((always_inline)) {
     if (!causal) return n;
-    const int last = (wave_first + 31) / kBN - gb + 1;
+    const int last = wave_last / kBN - gb + 1;
     return last < 0 ? 0 : (last < n ? last : n);
   };
 
@@ -475,6 +661,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   // buffer held K of block j, last read by the matrix step just before) and of V for
   // block j+1 (its buffer held V of block j-1, last read by that same matrix step).
   // With kMask false the block is known to need no mask (the steady-state loop).
+  // exp2 of a score difference, which is in the log2 domain already unless Q came unscaled
+  auto prob = [&](float s) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f(kPaged ? s * a.qk_scale : s); };
   auto vstep = [&](int j, auto mask_tag, auto seg) __attribute__((always_inline)) {
     constexpr bool kMask = decltype(mask_tag)::value;
     if (j < 0 || j >= ng) return;
@@ -482,7 +670,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       const int kbase = blk_of(j) * kBN;
       // key of slot i in sub-tile kt: kbase + 32kt + (i%4) + 8(i/4) + 4hh
       if (kMask && need_mask(j, seg)) {
-        const int q_abs = wfa_of(j, seg) + (lane & 31);
+        const int q_abs = kPaged ? (in_a(j, seg) ? laneA : laneB) : wfa_of(j, seg) + (lane & 31);
         int hi = causal && q_abs < kv_len - 1 ? q_abs : kv_len - 1;
         hi -= kbase + 4 * hh;
         const int lo = kv_begin - kbase - 4 * hh;
@@ -505,14 +693,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       if (fast) {
         const uint32_t kob = blk_off(j + 2), vob = blk_off(j + 1);
         const int kwrap = wrap_rows(j + 2), vwrap = wrap_rows(j + 1);
-        const u32x4 kr = kRot ? k_rsrc : tile_rsrc(Kg, kob), vr = kRot ? v_rsrc : tile_rsrc(Vg, vob);
+        const u32x4 kr = kPaged ? page_rsrc(a.k, j + 2, ent_k) : kRot ? k_rsrc : tile_rsrc(Kg, kob);
+        const u32x4 vr = kPaged ? page_rsrc(a.v, j + 1, ent_v) : kRot ? v_rsrc : tile_rsrc(Vg, vob);
         const uint32_t kdst = tile_dst(Ks + (j & 1) * kTile), vdst = tile_dst(Vs + ((j + 1) & 1) * kTile);
         for (int st = 0; st < 4; ++st) {
           dma_part(kr, kob, koff, kdst, st, kwrap);
           dma_part(vr, vob, voff, vdst, st, vwrap);
           for (int e = 0; e < 4; ++e) {
             const int kt = st >> 1, i = 8 * (st & 1) + 2 * e;
-            pw[st][e] = pack_bf16x2(__builtin_amdgcn_exp2f(sc[kt][i]), __builtin_amdgcn_exp2f(sc[kt][i + 1]));
+            pw[st][e] = pack_bf16x2(prob(sc[kt][i]), prob(sc[kt][i + 1]));
           }
         }
         uint32_t pm = pk_max3_f16(pw[0][0], pw[0][1], pw[0][2]);
@@ -525,8 +714,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
         pm = pk_max3_f16(pm, pw[3][3], pw[3][3]);
         fast = !__any((pm & 0xffffu) > 0x4380u || pm > 0x4380ffffu);  // some p > 256
       } else {
-        load_k(j + 2);
-        load_v(j + 1);
+        load_k(j + 2, ent_k);
+        load_v(j + 1, ent_v);
       }
       if (!fast) {
         // Slow path (first block of a row, or a row max that grew): move the base to
@@ -534,24 +723,38 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
         float mx = sc[0][0];
         for (int kt = 0; kt < 2; ++kt)
           for (int i = kt ? 0 : 1; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
+        if constexpr (kPaged) {
+          float sum = 0.f;  // finite or -inf exactly when no score is NaN or +inf
+          for (int kt = 0; kt < 2; ++kt)
+            for (int i = 0; i < 16; ++i) sum = sc[kt][i] < INFINITY ? sum : NAN;
+          broken = broken || __shfl_xor((int)(sum != sum), 32, 64) || sum != sum;
+          if (broken) {
+            mx = -INFINITY;
+            for (int kt = 0; kt < 2; ++kt)
+              for (int i = 0; i < 16; ++i) sc[kt][i] = -INFINITY;
+          }
+        }
         const float bm = wave_max_xor(mx, 32);
         const float delta = seen ? fmaxf(bm, 0.f) : (bm == -INFINITY ? 0.f : bm);
         seen = seen || bm != -INFINITY;
-        const float alpha = __builtin_amdgcn_exp2f(-delta);
+        const float alpha = prob(-delta);
         o_scale = alpha;
         rescale = true;
         m_use += delta;
         for (int st = 0; st < 4; ++st)
           for (int e = 0; e < 4; ++e) {
             const int kt = st >> 1, i = 8 * (st & 1) + 2 * e;
-            pw[st][e] = pack_bf16x2(__builtin_amdgcn_exp2f(sc[kt][i] - delta),
-                                    __builtin_amdgcn_exp2f(sc[kt][i + 1] - delta));
+            pw[st][e] = pack_bf16x2(prob(sc[kt][i] - delta), prob(sc[kt][i + 1] - delta));
           }
-        all_seen = __all(seen);
+        all_seen = __all(kPaged ? seen || broken : seen);
       }
     } else {
-      load_k(j + 2);
-      load_v(j + 1);
+      load_k(j + 2, ent_k);
+      load_v(j + 1, ent_v);
+    }
+    if constexpr (kPaged) {  // read here for the next step's loads
+      ent_v = ent_k;
+      ent_k = entry(j + 3);
     }
     // the score chains of the next matrix step start from -m_use
     for (int kt = 0; kt < 2; ++kt)
@@ -566,9 +769,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   // fills past the stream, so the count is fixed). The first matrix step reads Q and K of
   // block 0 only: the wait leaves the last 8 loads in flight, and the first softmax step's
   // wait (before the barrier that precedes the second matrix step) covers them.
-  load_k(0);
-  load_v(0);
-  load_k(1);
+  {
+    const int e0 = entry(0);
+    ent_v = entry(1);
+    ent_k = entry(2);
+    load_k(0, e0);
+    load_v(0, e0);
+    load_k(1, ent_v);
+  }
   __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8)
   __syncthreads();
 
@@ -576,6 +784,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   // scaled by scale*log2(e) and rounded to bf16 here, so the scores come out of the
   // MFMA in the log2 domain and the softmax needs no multiply per score.
   auto scale_q = [&](const u32x4 raw) __attribute__((always_inline)) {
+    if (kPaged) return as_bf16x8(raw);
     u32x4 w;
     for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(bf16_lo(raw[e]) * a.qk_scale, bf16_hi(raw[e]) * a.qk_scale);
     return as_bf16x8(w);
@@ -588,6 +797,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
     m_use = 0.f;
     seen = false;
     all_seen = false;
+    broken_a = broken;
+    broken = false;
     for (int kt = 0; kt < 2; ++kt)
       for (int i = 0; i < 16; ++i) sc[kt][i] = 0.f;
   };
@@ -597,7 +808,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   auto finish_a = [&]() __attribute__((always_inline)) {
     const float l_lo = __shfl(lsum[0], lane & 15, 64), l_hi = __shfl(lsum[1], lane & 15, 64);
     const float l_run = (lane & 16) ? l_hi : l_lo;
-    const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+    const float inv = kPaged ? (broken_a ? NAN : row_has_keys(laneA) ? 1.0f / l_run : 0.f)
+                             : l_run > 0.f ? 1.0f / l_run : 0.f;
     const int rr = 32 * wq + (lane & 31);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     for (int dt = 0; dt < 4; ++dt)
@@ -614,7 +826,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       const int n = it * 64 + lane;
       const int r = 32 * wq + (n >> 4), c = n & 15;
       const u32x4 v = *(const u32x4*)(Qs + r * kD + 8 * (c ^ (r & 15)));
-      if (row0A + r < a.T) *(u32x4*)(a.out + (((int64_t)b * a.T + row0A + r) * a.Hq + h) * kD + 8 * c) = v;
+      if (row0A + r < n_rows) *(u32x4*)(a.out + out_row(row0A, r) * kD + 8 * c) = v;
     }
     for (int dt = 0; dt < 4; ++dt)
       for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
@@ -629,7 +841,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   // no mask, so their softmax step carries no masking code.
   const MaskOn mask_on;
   const MaskOff mask_off;
-  const int actB = seg_act(gbB, wfaB, nB), maskB = seg_mask(gbB, wfaB);
+  const int actB = seg_act(gbB, wlaB, nB), maskB = seg_mask(gbB, wfaB);
   if (g == 0) {
     auto half0 = [&](int t, bool full, auto mask_tag, auto seg, bool switch_rows) __attribute__((always_inline)) {
       if (full) mstep_full(t);
@@ -644,7 +856,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       // segment A: blocks 0 .. n1-1, the last one followed by the switch of the Q operand
       const uint16_t* qp = light_q(32 * wq) + k_lane;
       for (int s = 0; s < 8; ++s) qop[s] = scale_q(*(const u32x4*)(qp + (k_x ^ (16 * s))));
-      const int actA = seg_act(gbA, wfaA, n1), maskA = seg_mask(gbA, wfaA);
+      const int actA = seg_act(gbA, wlaA, n1), maskA = seg_mask(gbA, wfaA);
       int tfA = actA < maskA ? actA : maskA;
       if (kWindow && tfA > n1_edge) tfA = n1_edge;
       for (; t < n1 - 1 && t < 1; ++t) half0(t, false, mask_on, SegA{}, false);
@@ -714,19 +926,37 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
     if (g == 0) publish(2);
     else publish(0);
     xm[(g * 4 + wq) * 64 + lane] = seen ? m_use : -INFINITY;
-    xl[(g * 4 + wq) * 64 + lane] = l_run;
+    xl[(g * 4 + wq) * 64 + lane] = kPaged && broken ? NAN : l_run;
   }
   __syncthreads();
   {
     const float m0 = xm[wq * 64 + lane], m1 = xm[(4 + wq) * 64 + lane];
     const float l0 = xl[wq * 64 + lane], l1 = xl[(4 + wq) * 64 + lane];
     const float m = fmaxf(m0, m1);
-    const float a0 = m0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m0 - m);
-    const float a1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
-    const float l_tot = l0 * a0 + l1 * a1;
-    const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;
+    const float a0 = m0 == -INFINITY ? 0.f : prob(m0 - m);
+    const float a1 = m1 == -INFINITY ? 0.f : prob(m1 - m);
+    const float l_tot = kPaged ? (l0 != l0 || l1 != l1 ? NAN : l0 * a0 + l1 * a1) : l0 * a0 + l1 * a1;
+    const float inv = kPaged ? (row_has_keys(laneB) ? 1.0f / l_tot : 0.f) : l_tot > 0.f ? 1.0f / l_tot : 0.f;
     const float a_mine = g ? a1 : a0, a_other = g ? a0 : a1;
     const float* const ox = xo + (1 - g) * (2 * 4 * 4 * 64 * 4);
+    if constexpr (kMode == kSharedPages) {  // the state itself, in 32 bits
+      if (row0 + rr < n_rows) {
+        float* const P = a.part + ((int64_t)chunk * a.n_rows * a.Hq + out_row(row0, rr)) * kPagedState;
+        if (g == 0 && hh == 0) *(float2*)P = make_float2(m == -INFINITY ? m : m * a.qk_scale, l_tot);
+        auto leave = [&](const int dt0) __attribute__((always_inline)) {
+          for (int d = 0; d < 2; ++d)
+            for (int i4 = 0; i4 < 4; ++i4) {
+              const f32x4 v = *(const f32x4*)(ox + (((d * 4 + i4) * 4 + wq) * 64 + lane) * 4);
+              f32x4 r;
+              for (int e = 0; e < 4; ++e) r[e] = o[dt0 + d][4 * i4 + e] * a_mine + v[e] * a_other;
+              *(f32x4*)(P + 4 + 32 * (dt0 + d) + 8 * i4 + 4 * hh) = r;
+            }
+        };
+        if (g == 0) leave(0);
+        else leave(2);
+      }
+      return;
+    }
     uint16_t* const St = Qs;  // bf16 [128 rows][128 dims], 16-byte chunk c of row r at c ^ (r & 15)
     auto finish = [&](const int dt0) __attribute__((always_inline)) {
       for (int d = 0; d < 2; ++d)
@@ -752,7 +982,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       const int n = it * kThreads + tid;
       const int r = n >> 4, c = n & 15;
       const u32x4 v = *(const u32x4*)(Qs + r * kD + 8 * (c ^ (r & 15)));
-      if (row0 + r < a.T) *(u32x4*)(a.out + (((int64_t)b * a.T + row0 + r) * a.Hq + h) * kD + 8 * c) = v;
+      if (row0 + r < n_rows) *(u32x4*)(a.out + out_row(row0, r) * kD + 8 * c) = v;
     }
   }
 }
@@ -1033,6 +1263,91 @@ int32_t launch_prefill(hipStream_t s, const void* q, const ema_kvcache_desc& c,
   else
     hipLaunchKernelGGL((prefill_kernel<false, false>), dim3((unsigned)blocks), dim3(kThreads), kLdsBytes, s, a);
   return check_hip(hipGetLastError(), "ema_prefill_attention launch");
+}
+
+namespace {
+// What the two launches over a pool share.
+PagedPrefillArgs paged_prefill_args(const PagedAttention& p, const ema_kvcache_desc& c) {
+  PagedPrefillArgs a;
+  a.q = (const uint16_t*)p.q;
+  a.k = (const uint16_t*)c.k;
+  a.v = (const uint16_t*)c.v;
+  a.q_off = nullptr;
+  a.out = (uint16_t*)p.out;
+  a.sb = c.stride_batch;
+  a.sh = c.stride_head;
+  a.sp = c.stride_pos;
+  a.page_bytes = c.stride_batch * 2;
+  a.head_bytes = c.stride_head * 2;
+  a.qk_scale = p.scale * kLog2e;
+  a.B = p.batch;
+  a.Hq = p.n_heads;
+  a.Hkv = c.n_kv_heads;
+  a.G = p.n_heads / c.n_kv_heads;
+  a.T = p.q_starts ? 1 : p.n_rows / p.batch;
+  a.cap = 0;
+  a.paired = 0;
+  a.flags = p.causal ? EMA_PREFILL_CAUSAL : 0u;
+  a.table = p.table;
+  a.starts = p.q_starts;
+  a.len = p.lengths;
+  a.part = nullptr;
+  a.n_rows = p.n_rows;
+  a.cols = p.table_cols;
+  a.shift = paged_shift(c.capacity);
+  a.n_pages = c.batch;
+  a.few = 0;
+  a.max_q = p.max_q;
+  a.chunk_blocks = 0;
+  return a;
+}
+int32_t allow_paged_lds(const char* what) {
+  static std::atomic<uint64_t> lds_set;
+  const void* const kernels[3] = {(const void*)prefill_kernel<false, false, false, kPages>,
+                                  (const void*)prefill_kernel<false, true, false, kPages>,
+                                  (const void*)prefill_kernel<false, false, false, kSharedPages>};
+  return allow_lds_once(kernels, 3, kLdsBytes, &lds_set, what);
+}
+}  // namespace
+
+int32_t launch_paged_prefill(hipStream_t s, const PagedAttention& p, const ema_kvcache_desc& c, int few) {
+  const int32_t rc = allow_paged_lds("ema_paged_attention: LDS attribute");
+  if (rc) return rc;
+  PagedPrefillArgs a = paged_prefill_args(p, c);
+  a.few = few;
+  a.nqb = (int)(((int64_t)p.max_q * a.G + kBM - 1) / kBM);
+  // blocks per kv head: exact for equal rows, else at most the rows' and one for each sequence of
+  // more than `few` rows (half that many pairs and one for each)
+  const int64_t large = p.q_starts ? (a.B < p.n_rows / (few + 1) ? a.B : p.n_rows / (few + 1)) : a.B;
+  const int64_t whole = (int64_t)p.n_rows * a.G / kBM;
+  const int64_t each = p.q_starts ? whole + large : (int64_t)a.nqb * a.B;
+  a.paired = a.nqb >= 2 && each * a.Hkv >= 2 * (int64_t)device_cus();
+  const int64_t pairs = p.q_starts ? whole / 2 + 1 + large : (int64_t)((a.nqb + 1) / 2) * a.B;
+  const int64_t blocks = (a.paired ? pairs : each) * a.Hkv;
+  if (blocks == 0) return EMA_OK;
+  if (blocks > 0x7fffffff) return set_error(EMA_ERR_SHAPE, "ema_paged_attention: grid too large");
+  const dim3 grid((unsigned)blocks), block(kThreads);
+  if (a.paired) hipLaunchKernelGGL((prefill_kernel<false, true, false, kPages>), grid, block, kLdsBytes, s, a);
+  else hipLaunchKernelGGL((prefill_kernel<false, false, false, kPages>), grid, block, kLdsBytes, s, a);
+  return check_hip(hipGetLastError(), "ema_paged_attention launch");
+}
+
+int32_t launch_prefix_rows(hipStream_t s, const PagedAttention& p, const ema_kvcache_desc& c, int chunks, int chunk_blocks,
+                           float* part) {
+  const int32_t rc = allow_paged_lds("ema_prefix_attention: LDS attribute");
+  if (rc) return rc;
+  PagedPrefillArgs a = paged_prefill_args(p, c);
+  a.table = p.prefix_table;
+  a.cols = p.prefix_cols;
+  a.len = p.prefix_len;
+  a.part = part;
+  a.chunk_blocks = chunk_blocks;
+  a.nqb = (int)(((int64_t)p.n_rows * a.G + kBM - 1) / kBM);
+  const int64_t blocks = (int64_t)a.nqb * a.Hkv * chunks;
+  if (blocks > 0x7fffffff) return set_error(EMA_ERR_SHAPE, "ema_prefix_attention: grid too large");
+  hipLaunchKernelGGL((prefill_kernel<false, false, false, kSharedPages>), dim3((unsigned)blocks), dim3(kThreads),
+                     kLdsBytes, s, a);
+  return check_hip(hipGetLastError(), "ema_prefix_attention prefix launch");
 }
 
 }  // namespace ema

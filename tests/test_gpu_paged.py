@@ -191,6 +191,64 @@ def test_rows_behind_the_last_sequence(ema):
     ref.check_attention(down(out[:3]), *b.attention(), "padded batch")
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("new,kv,prefix", [
+    ([1] * 6, [50, 1, 33, 200, 64, 5], 0), ([40, 17, 90], [40, 200, 90], 0), ([260, 3], [300, 30], 0),
+    ([1] * 6, [9] * 6, 70), ([1] * 40, [9] * 40, 300), ([2] * 130, [9] * 130, 130),
+])
+def test_rows_that_are_not_finite(ema, new, kv, prefix, bad):
+    """A query row that is not finite gives a row that is not finite, and no other row changes:
+    neither its neighbours nor the other sequences'."""
+    import torch
+
+    b = ref.Batch(new, kv, 16, 8, 2, seed=31, prefix=prefix)
+    g = OnGpu(ema, b)
+    want = g.attention().clone()
+    rows = [0, b.rows // 2, b.rows - 1]
+    g.q[rows, 3, 17] = bad
+    got = g.attention()
+    torch.cuda.synchronize()
+    hit = torch.zeros(b.rows, 8, dtype=torch.bool, device="cuda")
+    hit[rows, 3] = True
+    got, want = got.view(-1, 8, 128), want.view(-1, 8, 128)
+    assert not torch.isfinite(got[hit]).all(-1).any()
+    assert torch.isfinite(got[~hit]).all()
+    ref.check_attention(down(got[~hit]), down(want[~hit]), down(want[~hit].abs()) + 1.0, "the other rows")
+
+
+def test_prompt_sized_rows(ema):
+    """Sequences of more rows than a segment, beside short ones, with and without row starts, and
+    bounds below the truth (the sequences past them take another way)."""
+    for new, kv in (([300, 1, 128, 0, 700], [300, 90, 1000, 0, 701]), ([129], [129]), ([400], [60]), ([2, 515], [2, 3000])):
+        for heads in ((8, 2), (12, 1), (4, 4)):
+            b = ref.Batch(new, kv, 16, *heads, seed=sum(new))
+            run(ema, b, "prompts")
+            run(ema, b, "prompts, not causal", causal=False)
+            run(ema, b, "a low bound", max_q=200)
+    for heads in ((16, 4), (5, 1)):
+        run(ema, ref.Batch([250] * 5, [250, 400, 251, 1000, 333], 64, *heads, seed=3), "equal prompts", q_starts=None, max_q=None)
+
+
+def test_prompts_of_many_sequences(ema):
+    rng = np.random.default_rng(8)
+    for B in (65, 200):
+        new = rng.choice([0, 1, 2, 70, 150], B).tolist()
+        kv = [n + int(rng.integers(0, 90)) for n in new]
+        run(ema, ref.Batch(new, kv, 16, 4, 2, seed=B), f"{B} mixed sequences")
+    # enough blocks for pairs of them
+    new = rng.integers(300, 500, 70).tolist()
+    run(ema, ref.Batch(new, new, 32, 16, 2, seed=5), "pairs of blocks")
+    new[3], new[40], new[41] = 0, 1, 129
+    run(ema, ref.Batch(new, [n + 60 for n in new], 16, 16, 2, seed=6), "pairs of blocks, ragged")
+    run(ema, ref.Batch([600] * 24, [600] * 24, 16, 16, 2, seed=7), "equal pairs", q_starts=None, max_q=None)
+
+
+def test_prompts_over_bad_pages_and_orders(ema):
+    run(ema, ref.Batch([200, 3], [230, 50], 16, 8, 2, seed=9, holes=[(0, 0), (0, 7), (0, 14), (1, 1)]), "bad pages")
+    for page in (32, 256):
+        run(ema, ref.Batch([200, 310], [230, 400], page, 8, 2, seed=page), f"page {page}, nphd", order="nphd")
+
+
 def test_uniform_rows(ema):
     """Without q_starts every sequence has n / B rows."""
     b = ref.Batch([4] * 3, [4, 90, 33], 16, 8, 2, seed=17)
