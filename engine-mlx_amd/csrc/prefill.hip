@@ -78,7 +78,7 @@ struct PagedPrefillArgs : PrefillArgs {
   const int32_t* starts;  // null: T rows per sequence
   const int32_t* len;
   float* part;  // kSharedPages: the rows' states [chunk][n_rows, Hq][kPagedState]
-  int64_t page_bytes, head_bytes;
+  uint32_t page_bytes, head_bytes;  // (page_bytes below 2^32: host)
   int n_rows, cols, shift, n_pages;
   int few, max_q;       // kPages: sequences of few < n <= max_q rows are this kernel's
   int chunk_blocks;     // kSharedPages: 64-key blocks per chunk of the keys
@@ -425,19 +425,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
     }
     return 0;
   };
-  auto page_rsrc = [&](const uint16_t* pool, int j, int page) __attribute__((always_inline)) {
+  uint32_t head_bytes = 0;
+  if constexpr (kPaged) head_bytes = a.head_bytes;
+  struct Rows {
+    int64_t at;      // byte offset in the K pool, and in the V pool
+    uint32_t bytes;  // of the rows that are held, whole rows
+  };
+  const int64_t head_at = kPaged ? (int64_t)kh * head_bytes : 0;
+  auto rows_at = [&](int j, int page) __attribute__((always_inline)) {
+    Rows r = {head_at, 0u};
     if constexpr (kPaged) {
       const int pos = blk_of(j) * kBN + 16 * wq;
-      const bool in = (uint32_t)page < (uint32_t)a.n_pages;
-      int n = kv_len - pos;
-      n = j < ng && in && n > 0 ? (n < 16 ? n : 16) : 0;
-      return buffer_rsrc((const char*)pool + (in ? (int64_t)page * a.page_bytes : 0) + (int64_t)kh * a.head_bytes +
-                             (int64_t)(pos & ((1 << a.shift) - 1)) * row_bytes,
-                         (uint32_t)n * row_bytes);
+      const bool in = j < ng && (uint32_t)page < (uint32_t)a.n_pages;
+      const int left = kv_len - pos;
+      const uint32_t n = in && left > 0 ? (left < 16 ? left : 16) : 0;
+      r.bytes = n * row_bytes;
+      r.at += (int64_t)((uint64_t)(uint32_t)(in ? page : 0) * a.page_bytes) +
+              (uint32_t)(pos & ((1 << a.shift) - 1)) * row_bytes;
     }
-    return u32x4{0u, 0u, 0u, 0u};
+    return r;
   };
-  int ent_v = 0, ent_k = 0;  // entries of blocks j + 1 and j + 2 in softmax step j
+  int ent = 0;          // softmax step j: the entry of block j + 2,
+  Rows next = {0, 0u};  // and the rows of block j + 1 (whose K was requested in step j - 1)
   auto tile_dst = [&](const uint16_t* tile) __attribute__((always_inline)) {
     return (uint32_t)(uintptr_t)(lds_void*)(tile + 16 * wq * kD);
   };
@@ -459,9 +468,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
     if constexpr (kPaged) {
       switch (i) {
         case 0: dma16<0, 4>(r, o, dst); break;
-        case 1: dma16<1, 4>(r, o, dst); break;
-        case 2: dma16<2, 4>(r, o, dst); break;
-        default: dma16<3, 4>(r, o, dst); break;
+        case 1: dma16<1>(r, o, dst); break;
+        case 2: dma16<2>(r, o, dst); break;
+        default: dma16<3>(r, o, dst); break;
       }
       return;
     }
@@ -490,17 +499,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       for (int i = 0; i < 4; ++i) dma_part(r, ob, off, dst, i, wrap);
     }
   };
-  auto load_k = [&](int j, int ent) __attribute__((always_inline)) {
+  const char* const Kp = (const char*)a.k;
+  const char* const Vp = (const char*)a.v;
+  auto load_k = [&](int j, Rows rows) __attribute__((always_inline)) {
     if constexpr (kPaged) {
-      const u32x4 r = page_rsrc(a.k, j, ent);
+      const u32x4 r = buffer_rsrc(Kp + rows.at, rows.bytes);
       for (int i = 0; i < 4; ++i) dma_part(r, 0u, koff, tile_dst(Ks + (j & 1) * kTile), i, kBN);
     } else {
       dma(Kg, k_rsrc, j, koff, Ks + (j & 1) * kTile);
     }
   };
-  auto load_v = [&](int j, int ent) __attribute__((always_inline)) {
+  auto load_v = [&](int j, Rows rows) __attribute__((always_inline)) {
     if constexpr (kPaged) {
-      const u32x4 r = page_rsrc(a.v, j, ent);
+      const u32x4 r = buffer_rsrc(Vp + rows.at, rows.bytes);
       for (int i = 0; i < 4; ++i) dma_part(r, 0u, voff, tile_dst(Vs + (j & 1) * kTile), i, kBN);
     } else {
       dma(Vg, v_rsrc, j, voff, Vs + (j & 1) * kTile);
@@ -666,6 +677,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   auto vstep = [&](int j, auto mask_tag, auto seg) __attribute__((always_inline)) {
     constexpr bool kMask = decltype(mask_tag)::value;
     if (j < 0 || j >= ng) return;
+    const Rows rows_k = rows_at(j + 2, ent);
     if (active(j, seg)) {
       const int kbase = blk_of(j) * kBN;
       // key of slot i in sub-tile kt: kbase + 32kt + (i%4) + 8(i/4) + 4hh
@@ -693,8 +705,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       if (fast) {
         const uint32_t kob = blk_off(j + 2), vob = blk_off(j + 1);
         const int kwrap = wrap_rows(j + 2), vwrap = wrap_rows(j + 1);
-        const u32x4 kr = kPaged ? page_rsrc(a.k, j + 2, ent_k) : kRot ? k_rsrc : tile_rsrc(Kg, kob);
-        const u32x4 vr = kPaged ? page_rsrc(a.v, j + 1, ent_v) : kRot ? v_rsrc : tile_rsrc(Vg, vob);
+        const u32x4 kr = kPaged ? buffer_rsrc(Kp + rows_k.at, rows_k.bytes) : kRot ? k_rsrc : tile_rsrc(Kg, kob);
+        const u32x4 vr = kPaged ? buffer_rsrc(Vp + next.at, next.bytes) : kRot ? v_rsrc : tile_rsrc(Vg, vob);
         const uint32_t kdst = tile_dst(Ks + (j & 1) * kTile), vdst = tile_dst(Vs + ((j + 1) & 1) * kTile);
         for (int st = 0; st < 4; ++st) {
           dma_part(kr, kob, koff, kdst, st, kwrap);
@@ -714,8 +726,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
         pm = pk_max3_f16(pm, pw[3][3], pw[3][3]);
         fast = !__any((pm & 0xffffu) > 0x4380u || pm > 0x4380ffffu);  // some p > 256
       } else {
-        load_k(j + 2, ent_k);
-        load_v(j + 1, ent_v);
+        load_k(j + 2, rows_k);
+        load_v(j + 1, next);
       }
       if (!fast) {
         // Slow path (first block of a row, or a row max that grew): move the base to
@@ -749,12 +761,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
         all_seen = __all(kPaged ? seen || broken : seen);
       }
     } else {
-      load_k(j + 2, ent_k);
-      load_v(j + 1, ent_v);
+      load_k(j + 2, rows_k);
+      load_v(j + 1, next);
     }
     if constexpr (kPaged) {  // read here for the next step's loads
-      ent_v = ent_k;
-      ent_k = entry(j + 3);
+      next = rows_k;
+      ent = entry(j + 3);
     }
     // the score chains of the next matrix step start from -m_use
     for (int kt = 0; kt < 2; ++kt)
@@ -770,12 +782,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   // block 0 only: the wait leaves the last 8 loads in flight, and the first softmax step's
   // wait (before the barrier that precedes the second matrix step) covers them.
   {
-    const int e0 = entry(0);
-    ent_v = entry(1);
-    ent_k = entry(2);
-    load_k(0, e0);
-    load_v(0, e0);
-    load_k(1, ent_v);
+    const int e0 = entry(0), e1 = entry(1);
+    ent = entry(2);
+    const Rows r0 = rows_at(0, e0);
+    next = rows_at(1, e1);
+    load_k(0, r0);
+    load_v(0, r0);
+    load_k(1, next);
   }
   __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8)
   __syncthreads();
@@ -1277,8 +1290,8 @@ PagedPrefillArgs paged_prefill_args(const PagedAttention& p, const ema_kvcache_d
   a.sb = c.stride_batch;
   a.sh = c.stride_head;
   a.sp = c.stride_pos;
-  a.page_bytes = c.stride_batch * 2;
-  a.head_bytes = c.stride_head * 2;
+  a.page_bytes = (uint32_t)(c.stride_batch * 2);
+  a.head_bytes = (uint32_t)(c.stride_head * 2);
   a.qk_scale = p.scale * kLog2e;
   a.B = p.batch;
   a.Hq = p.n_heads;

@@ -74,6 +74,8 @@ def test_pools_that_are_refused(ema):
         assert call(ema, pool(ema, fp8=True, k_exp=P + 1)) == ema.EMA_ERR_INVALID_ARG
         assert call(ema, pool(ema, stride_pos=64)) == ema.EMA_ERR_SHAPE
         assert call(ema, pool(ema, stride_pos=1 << 26)) == ema.EMA_ERR_UNSUPPORTED
+        assert call(ema, pool(ema, stride_batch=1 << 31)) == ema.EMA_ERR_UNSUPPORTED
+        assert call(ema, pool(ema, stride_head=1 << 31)) == ema.EMA_ERR_UNSUPPORTED
         d = ema.KvCacheDesc()
         assert ema.lib().ema_kvcache_init_int4(ctypes.byref(d), P, P, P, P, P, P, 10, 8, 32, 128) == ema.EMA_OK
         assert call(ema, d) == ema.EMA_ERR_UNSUPPORTED
