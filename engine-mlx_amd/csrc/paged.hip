@@ -5,6 +5,8 @@
 // table[b][p / P]. A table entry outside [0, n_pages) is never followed: nothing is written
 // there, and its positions read as zero rows. A batch is ragged: sequence b's query rows are
 // packed rows [starts[b], starts[b + 1]).
+#include <type_traits>
+
 #include "ema_common.hpp"
 #include "paged.hpp"
 
@@ -188,8 +190,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 // ------------------------------------------------------------------ attention, rows in blocks of 32
 // A segment is 32 query rows of one (sequence, kv head): row i is token i / G, head i % G of
 // the kv head's group, so a decode step's G heads and a few drafted tokens' share one pass over
-// K and V. The keys of a segment are tiles of 32, four tiles a round; the rounds of all
-// segments, laid end to end, are cut into equal slices, one per workgroup, whatever the lengths.
+// K and V. The keys of a segment are tiles of 32, four tiles a round, one or four rounds a unit;
+// the units of all segments, laid end to end, are cut into equal slices, one per workgroup,
+// whatever the lengths.
 // The four waves of a workgroup take a round's tiles, each with its own softmax state and its own
 // LDS slot for the tile, and no barrier until their states meet at the piece's end. A segment cut over
 // several workgroups leaves partial states in the workspace; the last of them to arrive joins
@@ -245,12 +248,19 @@ __device__ __forceinline__ u32x4 rsrc_words(const void* base, uint32_t bytes) {
 // resource's range). Asm, so that the compiler does not track it; the s_nop gives the wait
 // states that the DMA needs after the write of M0 (one) and, in the first load over a resource,
 // after a vector instruction (a spill's reload) wrote the resource's scalar registers (five).
-template <bool kFirst>
+// kOnce: the bytes are read once in the call (non-temporal).
+template <bool kFirst, bool kOnce>
 __device__ __forceinline__ void dma16(u32x4 rs, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop %3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-               :
-               : "v"(voff), "s"(rs), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(kFirst ? 4 : 0)
-               : "memory", "m0");
+  if constexpr (kOnce)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop %3\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
+                 :
+                 : "v"(voff), "s"(rs), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(kFirst ? 4 : 0)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop %3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :
+                 : "v"(voff), "s"(rs), "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(kFirst ? 4 : 0)
+                 : "memory", "m0");
 }
 
 // Partial states cross XCDs as device-coherent stores and loads (past the XCDs' own L2s).
@@ -328,7 +338,7 @@ __device__ __forceinline__ int blocks_of(const PagedArgs& a, int T) {
   return (int)(((uint32_t)T * (uint32_t)a.G + kPagedRows - 1) / kPagedRows);
 }
 
-template <bool kFp8>
+template <bool kFp8, bool kOnce>
 __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_kernel(PagedArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t slots[kPagedWaves][2 * kSlot];
   __shared__ float2 ml[kPagedWaves][kPagedRows];
@@ -347,49 +357,61 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     if (a.carry_blocks) n_carry = ((n + 63) / 64 + a.carry_blocks - 1) / a.carry_blocks;
   }
 
-  // Rounds before each sequence, by every wave for itself (all write the same values): lane l
-  // takes sequences l step .. +step-1, and the lanes' sums are scanned.
+  // Units of work before each sequence, by every wave for itself: lane l takes sequences
+  // l step .. +step-1 (up to 64 sequences: one each, kept in the lane's registers; more: their
+  // starts go to LDS, where all waves write the same values), and the lanes' sums are scanned.
   const int step = (a.B + 63) >> 6;
-  auto rows_n = [&](int b) __attribute__((always_inline)) {
-    if (a.starts) return own_rows(a, paged_rows(a.starts[b], a.starts[b + 1], a.n_rows)).n;
-    return rows_of(a, 0).n;
+  const PagedRows all_rows = a.starts ? PagedRows{0, 0} : rows_of(a, 0);
+  auto rows_at = [&](int b) __attribute__((always_inline)) {
+    if (a.starts) return own_rows(a, paged_rows(a.starts[b], a.starts[b + 1], a.n_rows));
+    return PagedRows{b * all_rows.n, all_rows.n};
   };
-  int sum = 0;
+  PagedRows lane_rows = {0, 0};
+  int lane_len = 0, sum1 = 0, sum_long = 0;
   for (int i = 0; i < step; ++i) {
     const int b = lane * step + i;
     if (b < a.B) {
-      const int T = rows_n(b);
-      sum += paged_rounds(clamp_len(a, a.len[b])) * blocks_of(a, T) * a.Hkv;
+      lane_rows = rows_at(b);
+      lane_len = clamp_len(a, a.len[b]);
+      const int nr = paged_rounds(lane_len), segs = blocks_of(a, lane_rows.n) * a.Hkv;
+      sum1 += segs * paged_units(nr, 1);
+      sum_long += segs * paged_units(nr, kPagedLongUnit);
     }
   }
-  int lane_pre = sum;
+  int pre1 = sum1, pre_long = sum_long;
   for (int d = 1; d < 64; d <<= 1) {
-    const int x = __shfl_up(lane_pre, d, 64);
-    if (lane >= d) lane_pre += x;
+    const int x = __shfl_up(pre1, d, 64), y = __shfl_up(pre_long, d, 64);
+    if (lane >= d) pre1 += x, pre_long += y;
   }
-  const int total = __builtin_amdgcn_readlane(lane_pre, 63);
-  lane_pre -= sum;
-  int run = lane_pre;
-  for (int i = 0; i < step; ++i) {
-    const int b = lane * step + i;
-    if (b < a.B) {
-      pre[b] = run;
-      const int T = rows_n(b);
-      run += paged_rounds(clamp_len(a, a.len[b])) * blocks_of(a, T) * a.Hkv;
+  const int unit = paged_unit(__builtin_amdgcn_readlane(pre1, 63), a.W);
+  const int total = __builtin_amdgcn_readlane(unit == 1 ? pre1 : pre_long, 63);
+  const int lane_pre = unit == 1 ? pre1 - sum1 : pre_long - sum_long;
+  if (step > 1) {
+    int run = lane_pre;
+    for (int i = 0; i < step; ++i) {
+      const int b = lane * step + i;
+      if (b < a.B) {
+        pre[b] = run;
+        run += blocks_of(a, rows_at(b).n) * a.Hkv * paged_units(paged_rounds(clamp_len(a, a.len[b])), unit);
+      }
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
-  if (lane == 0) pre[a.B] = total;
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 
-  // rows of sequences that hold nothing: no round visits them
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    if (pre[b + 1] != pre[b]) continue;
-    const PagedRows rw = rows_of(a, b);
-    const State4 none = {-INFINITY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
-    for (int64_t e = tid; e < (int64_t)rw.n * a.Hq * 32; e += 64 * kPagedWaves)
-      finish4(a, n_carry, shared_keys, rw.begin + e / (a.Hq * 32), (int)(e / 32 % a.Hq), (int)(e % 32) * 4, none);
+  // rows of sequences that hold nothing: no unit visits them
+  for (int i = 0; i < step; ++i) {
+    const int bl = lane * step + i;
+    uint64_t none = __ballot(bl < a.B && a.len[bl < a.B ? bl : 0] <= 0);
+    for (; none; none &= none - 1) {
+      const int b = __builtin_ctzll(none) * step + i;
+      if (b % (int)gridDim.x != (int)blockIdx.x) continue;
+      const PagedRows rw = rows_of(a, b);
+      const State4 empty = {-INFINITY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+      for (int64_t e = tid; e < (int64_t)rw.n * a.Hq * 32; e += 64 * kPagedWaves)
+        finish4(a, n_carry, shared_keys, rw.begin + e / (a.Hq * 32), (int)(e / 32 % a.Hq), (int)(e % 32) * 4, empty);
+    }
   }
 
   const int W = paged_active_workers(total, a.W);
@@ -422,26 +444,31 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
   for (int dt = 0; dt < 4; ++dt) v_col[dt] = tr_row * kD + 16 * (grp & 1) + 4 * (s16 & 3) + 32 * (dt ^ (s16 >> 2));
 
   while (t < t_end) {
-    // the segment of round t: the last b whose rounds begin at or before it
-    uint64_t le = __ballot(lane * step < a.B && lane_pre <= t);
-    int b = (63 - __builtin_clzll(le)) * step;
-    if (step > 1) {
-      const int bi = b + lane;
-      le = __ballot(lane < step && bi < a.B && pre[bi < a.B ? bi : 0] <= t);
-      b += 63 - __builtin_clzll(le);
+    // the segment of unit t: the last b whose units begin at or before it
+    const uint64_t le = __ballot(lane * step < a.B && lane_pre <= t);
+    const int at = 63 - __builtin_clzll(le);
+    int b = at, L, pre_b;
+    PagedRows rw;
+    if (step == 1) {
+      rw = PagedRows{__builtin_amdgcn_readlane(lane_rows.begin, at), __builtin_amdgcn_readlane(lane_rows.n, at)};
+      L = __builtin_amdgcn_readlane(lane_len, at);
+      pre_b = __builtin_amdgcn_readlane(lane_pre, at);
+    } else {
+      const int bi = at * step + lane;
+      b = at * step + 63 - __builtin_clzll(__ballot(lane < step && bi < a.B && pre[bi < a.B ? bi : 0] <= t));
+      rw = rows_of(a, b);
+      L = clamp_len(a, ld_uniform(a.len, b));
+      pre_b = __builtin_amdgcn_readfirstlane(pre[b]);
     }
-    const int pre_b = __builtin_amdgcn_readfirstlane(pre[b]);
-    const PagedRows rw = rows_of(a, b);
-    const int L = clamp_len(a, ld_uniform(a.len, b));
-    const int nr = paged_rounds(L), nrb = blocks_of(a, rw.n);
-    const uint32_t seg = (uint32_t)(t - pre_b) / (uint32_t)nr;
-    const int round0 = (int)((uint32_t)(t - pre_b) - seg * (uint32_t)nr);
-    const int kh = (int)(seg / (uint32_t)nrb), rb = (int)(seg - (uint32_t)kh * (uint32_t)nrb);
-    const int seg_begin = t - round0, seg_end = seg_begin + nr;
+    const int nu = paged_units(paged_rounds(L), unit), nrb = blocks_of(a, rw.n);
+    const uint32_t seg = (uint32_t)(t - pre_b) / (uint32_t)nu;
+    const int unit0 = (int)((uint32_t)(t - pre_b) - seg * (uint32_t)nu);
+    const int kh = nrb == 1 ? (int)seg : (int)(seg / (uint32_t)nrb), rb = (int)(seg - (uint32_t)kh * (uint32_t)nrb);
+    const int seg_begin = t - unit0, seg_end = seg_begin + nu;
     const int piece_end = t_end < seg_end ? t_end : seg_end;
-    const int tile0 = round0 * kPagedWaves;
+    const int tile0 = unit0 * unit * kPagedWaves;
     const int tile_end = (int)(((uint32_t)L + kPagedTile - 1) / kPagedTile);
-    const int tile1 = min(tile0 + (piece_end - t) * kPagedWaves, tile_end);
+    const int tile1 = min(tile0 + (piece_end - t) * unit * kPagedWaves, tile_end);
     const int row0 = rb * kPagedRows;                     // the segment's first row (token * G + head)
     const int n_seg = rw.n * a.G - row0 < kPagedRows ? rw.n * a.G - row0 : kPagedRows;
 
@@ -475,9 +502,9 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         const int e = half ? e1 : e0;
         const u32x4 r = rsrc_words(half_base(k ? a.k : a.v, tile, half, e), (uint32_t)valid_rows(tile, half, e) * a.row_bytes);
         const uint32_t dst = (k ? kdst : vdst) + 4096 * half;
-        dma16<true>(r, k ? koff[0] : voff[0], dst);
+        dma16<true, kOnce>(r, k ? koff[0] : voff[0], dst);
 #pragma unroll
-        for (int i = 1; i < 4; ++i) dma16<false>(r, k ? koff[i] : voff[i], dst + 1024 * i);
+        for (int i = 1; i < 4; ++i) dma16<false, kOnce>(r, k ? koff[i] : voff[i], dst + 1024 * i);
       }
     };
     // fp8: a tile's codes into registers (row 8 i + lane / 8, codes 16 (lane % 8) .. +15), with
@@ -503,7 +530,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t row = 8 * i + (lane >> 3);
-          c.w[2 * half + i] = __builtin_amdgcn_raw_buffer_load_b128(r, row * a.row_bytes + 16 * (lane & 7), 0, 0);
+          c.w[2 * half + i] = __builtin_amdgcn_raw_buffer_load_b128(r, row * a.row_bytes + 16 * (lane & 7), 0, kOnce ? 2 : 0);
           c.e[2 * half + i] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(re, 2 * row + ((lane >> 2) & 1), 0, 0);
         }
       }
@@ -677,43 +704,59 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       }
       __syncthreads();
       if (arrived) {
-        for (int u = tid; u < units; u += 64 * kPagedWaves) {
-          const int r = u >> 5, d4 = u & 31;
-          State4 s = {-INFINITY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
-          constexpr int kChunk = 8;  // pieces whose loads are in flight together
-          for (int c0 = w0; c0 <= w1; c0 += kChunk) {
-            float2 pm[kChunk], pa[kChunk], pb[kChunk];
+        auto join = [&](auto chunk_tag) __attribute__((always_inline)) {
+          constexpr int kChunk = decltype(chunk_tag)::value;  // pieces whose loads are in flight together
+          for (int u = tid; u < units; u += 64 * kPagedWaves) {
+            const int r = u >> 5, d4 = u & 31;
+            State4 s = {-INFINITY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+            for (int c0 = w0; c0 <= w1; c0 += kChunk) {
+              float2 pm[kChunk], pa[kChunk], pb[kChunk];
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-              const int ww = c0 + i <= w1 ? c0 + i : w1;
-              const float* const p = a.part + ((int64_t)paged_slot(ww, w0) * kPagedRows + r) * kPagedState;
-              pm[i] = get2(p);
-              pa[i] = get2(p + 4 + 4 * d4);
-              pb[i] = get2(p + 6 + 4 * d4);
-            }
-            float M = s.m;
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) M = fmaxf(M, pm[i].x);
-            const float f = weight(s.m, M);
-            s.l *= f;
-            s.o *= f;
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i)
-              if (c0 + i <= w1) {
-                const float g = weight(pm[i].x, M);
-                s.l += pm[i].y * g;
-                s.o += f32x4{pa[i].x, pa[i].y, pb[i].x, pb[i].y} * g;
+              for (int i = 0; i < kChunk; ++i) {
+                const int ww = c0 + i <= w1 ? c0 + i : w1;
+                const float* const p = a.part + ((int64_t)paged_slot(ww, w0) * kPagedRows + r) * kPagedState;
+                pm[i] = get2(p);
+                pa[i] = get2(p + 4 + 4 * d4);
+                pb[i] = get2(p + 6 + 4 * d4);
               }
-            s.m = M;
+              float M = s.m;
+#pragma unroll
+              for (int i = 0; i < kChunk; ++i) M = fmaxf(M, pm[i].x);
+              const float f = weight(s.m, M);
+              s.l *= f;
+              s.o *= f;
+#pragma unroll
+              for (int i = 0; i < kChunk; ++i)
+                if (c0 + i <= w1) {
+                  const float g = weight(pm[i].x, M);
+                  s.l += pm[i].y * g;
+                  s.o += f32x4{pa[i].x, pa[i].y, pb[i].x, pb[i].y} * g;
+                }
+              s.m = M;
+            }
+            const int ir = row0 + r, tk = (int)((uint32_t)ir / (uint32_t)a.G);
+            finish4(a, n_carry, shared_keys || !a.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk,
+                    kh * a.G + ir - tk * a.G, 4 * d4, s);
           }
-          const int ir = row0 + r, tk = (int)((uint32_t)ir / (uint32_t)a.G);
-          finish4(a, n_carry, shared_keys || !a.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk, kh * a.G + ir - tk * a.G, 4 * d4, s);
-        }
+        };
+        if (w1 - w0 < 3) join(std::integral_constant<int, 3>{});
+        else join(std::integral_constant<int, 8>{});
       }
     }
     __syncthreads();  // the slots and ml are reused by the next piece
     t = piece_end;
   }
+}
+
+// max_q: most rows of a sequence. Where all are one segment, K and V are read once.
+int32_t launch_rows(hipStream_t s, const PagedArgs& a, bool fp8, int max_q, const char* what) {
+  const bool once = (int64_t)max_q * a.G <= kPagedRows;
+  const dim3 grid(a.W), block(64 * kPagedWaves);
+  if (fp8 && once) hipLaunchKernelGGL((paged_kernel<true, true>), grid, block, 0, s, a);
+  else if (fp8) hipLaunchKernelGGL((paged_kernel<true, false>), grid, block, 0, s, a);
+  else if (once) hipLaunchKernelGGL((paged_kernel<false, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((paged_kernel<false, false>), grid, block, 0, s, a);
+  return check_hip(hipGetLastError(), what);
 }
 
 }  // namespace
@@ -820,7 +863,6 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
   a.causal = p.causal;
   a.few = INT32_MAX;
   a.max_q = 0;
-  const dim3 block(64 * kPagedWaves);
   if (p.prefix_table) {
     float* const carry = (float*)((char*)ws + kDecodeCounterBytes + plan.part_bytes);
     if (!fp8 && (int64_t)p.n_rows * a.G > kFewPrefixRows) {
@@ -839,9 +881,7 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
       x.causal = 0;
       x.carry_out = carry;
       x.W = plan.prefix_workers;
-      if (fp8) hipLaunchKernelGGL(paged_kernel<true>, dim3(x.W), block, 0, s, x);
-      else hipLaunchKernelGGL(paged_kernel<false>, dim3(x.W), block, 0, s, x);
-      const int32_t rc = check_hip(hipGetLastError(), "ema_prefix_attention prefix launch");
+      const int32_t rc = launch_rows(s, x, fp8, p.n_rows, "ema_prefix_attention prefix launch");
       if (rc) return rc;
     }
     a.carry_in = carry;
@@ -853,9 +893,7 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
     a.max_q = p.max_q;
   }
   a.W = plan.workers;
-  if (fp8) hipLaunchKernelGGL(paged_kernel<true>, dim3(a.W), block, 0, s, a);
-  else hipLaunchKernelGGL(paged_kernel<false>, dim3(a.W), block, 0, s, a);
-  return check_hip(hipGetLastError(), "ema_paged_attention launch");
+  return launch_rows(s, a, fp8, p.max_q, "ema_paged_attention launch");
 }
 
 }  // namespace ema

@@ -32,11 +32,18 @@ EMA_HD PagedRows paged_rows(int s0, int s1, int n_rows) {
 constexpr int kPagedRound = kPagedTile * kPagedWaves;
 EMA_HD int paged_rounds(int L) { return (int)(((uint32_t)L + kPagedRound - 1) / kPagedRound); }
 
-// The rounds of all segments, laid end to end, cut into W slices that differ by at most one
-// round; 32-bit arithmetic without products of the two (total < 2^31). Whole rounds, so that a
-// short segment (a few own tokens behind a prefix) is one workgroup's alone.
+// Units of a segment: one round each, or kPagedLongUnit rounds where there are more rounds than
+// workgroups but no more than kPagedLongUnit for each. A piece costs a workgroup about as much as
+// three rounds before and after its tiles, so short segments (own tokens behind a prefix) are
+// better whole than in pieces of a round.
+constexpr int kPagedLongUnit = 4;
+EMA_HD int paged_units(int rounds, int unit) { return (rounds + unit - 1) / unit; }
+EMA_HD int paged_unit(int rounds, int W) { return rounds > W && rounds <= kPagedLongUnit * W ? kPagedLongUnit : 1; }
+
+// The units of all segments, laid end to end, cut into W slices that differ by at most one
+// unit; 32-bit arithmetic without products of the two (total < 2^31).
 struct PagedSplit {
-  uint32_t base, rem;  // every slice has base rounds, the first rem of them one more
+  uint32_t base, rem;  // every slice has base units, the first rem of them one more
 };
 EMA_HD int paged_active_workers(int total, int W) { return total < W ? (total < 1 ? 1 : total) : W; }
 EMA_HD PagedSplit paged_split(int total, int W) { return PagedSplit{(uint32_t)total / (uint32_t)W, (uint32_t)total % (uint32_t)W}; }

@@ -1,5 +1,5 @@
 // CPU checks of the paged kernels' integer parts (engine-mlx_amd/csrc/paged.hpp): the split's
-// slices cover every round once, worker_of inverts them, and the partial-state slots and arrival
+// slices cover every unit once, worker_of inverts them, and the partial-state slots and arrival
 // counters of pieces that are alive together are distinct.
 #include <cstdio>
 #include <cstdlib>
