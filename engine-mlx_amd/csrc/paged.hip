@@ -284,7 +284,7 @@ __device__ __forceinline__ float weight(float m, float M) { return m == -INFINIT
 __device__ __forceinline__ void finish4(const PagedArgs& a, int n_carry, bool keys, int64_t row, int h, int d, State4 s) {
   const int64_t rh = row * a.Hq + h;
   if (a.carry_in) {
-    constexpr int kChunk = 8;  // states whose loads are in flight together
+    constexpr int kChunk = 16;  // states whose loads are in flight together
     for (int c0 = 0; c0 < n_carry; c0 += kChunk) {
       float2 cm[kChunk];
       f32x4 co[kChunk];
@@ -378,11 +378,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       sum_long += segs * paged_units(nr, kPagedLongUnit);
     }
   }
-  int pre1 = sum1, pre_long = sum_long;
-  for (int d = 1; d < 64; d <<= 1) {
-    const int x = __shfl_up(pre1, d, 64), y = __shfl_up(pre_long, d, 64);
-    if (lane >= d) pre1 += x, pre_long += y;
-  }
+  const int pre1 = sum_up_to_lane(sum1), pre_long = sum_up_to_lane(sum_long);
   const int unit = paged_unit(__builtin_amdgcn_readlane(pre1, 63), a.W);
   const int total = __builtin_amdgcn_readlane(unit == 1 ? pre1 : pre_long, 63);
   const int lane_pre = unit == 1 ? pre1 - sum1 : pre_long - sum_long;
@@ -403,7 +399,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
   // rows of sequences that hold nothing: no unit visits them
   for (int i = 0; i < step; ++i) {
     const int bl = lane * step + i;
-    uint64_t none = __ballot(bl < a.B && a.len[bl < a.B ? bl : 0] <= 0);
+    uint64_t none = __ballot(bl < a.B && (step == 1 ? lane_len : a.len[bl < a.B ? bl : 0]) <= 0);
     for (; none; none &= none - 1) {
       const int b = __builtin_ctzll(none) * step + i;
       if (b % (int)gridDim.x != (int)blockIdx.x) continue;
@@ -560,7 +556,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     if constexpr (kFp8) {
       kc = load_codes(true, first, e0, e1);
       vc = load_codes(false, first, e0, e1);
-    } else {
+    } else if (first < tile1) {
       dma_tile(true, first, e0, e1);
       dma_tile(false, first, e0, e1);
     }
@@ -584,12 +580,17 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       } else {
         asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // K of this tile
       }
-      f32x16 sc;
+      f32x16 sc, sc2;  // two chains of products
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+      for (int i = 0; i < 16; ++i) sc[i] = sc2[i] = 0.f;
 #pragma unroll
-      for (int s = 0; s < 8; ++s) sc = mfma32(as_bf16x8(*(const u32x4*)(kp + (k_x ^ (16 * s)))), qop[s], sc);
-      if constexpr (!kFp8) {
+      for (int s = 0; s < 8; s += 2) {
+        sc = mfma32(as_bf16x8(*(const u32x4*)(kp + (k_x ^ (16 * s)))), qop[s], sc);
+        sc2 = mfma32(as_bf16x8(*(const u32x4*)(kp + (k_x ^ (16 * s + 16)))), qop[s + 1], sc2);
+      }
+      sc += sc2;
+      const bool more = tile + kPagedWaves < tile1;
+      if (!kFp8 && more) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
         dma_tile(true, tile + kPagedWaves, e0, e1);
       }
@@ -628,7 +629,8 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       } else {
-        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // V of this tile
+        if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // V of this tile, and not K of the next
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       }
 #pragma unroll
       for (int st = 0; st < 2; ++st)
@@ -643,15 +645,13 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         }
       if constexpr (!kFp8) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        dma_tile(false, tile + kPagedWaves, e0, e1);
+        if (more) dma_tile(false, tile + kPagedWaves, e0, e1);
       } else {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the loads past the last tile: nothing read)
-
     // the waves' states meet: o of wave w in its own slots, [row][d / 4] with unit d4 of row r
     // at d4 ^ r
     f32x4* const os = (f32x4*)Kt;

@@ -46,9 +46,14 @@ struct PagedSplit {
   uint32_t base, rem;  // every slice has base units, the first rem of them one more
 };
 EMA_HD int paged_active_workers(int total, int W) { return total < W ? (total < 1 ? 1 : total) : W; }
-EMA_HD PagedSplit paged_split(int total, int W) { return PagedSplit{(uint32_t)total / (uint32_t)W, (uint32_t)total % (uint32_t)W}; }
+EMA_HD PagedSplit paged_split(int total, int W) {
+  if (total == W) return PagedSplit{1u, 0u};  // (no division on the small calls' path)
+  const uint32_t base = (uint32_t)total / (uint32_t)W;
+  return PagedSplit{base, (uint32_t)total - base * (uint32_t)W};
+}
 EMA_HD int paged_begin(PagedSplit s, int w) { return (int)((uint32_t)w * s.base + ((uint32_t)w < s.rem ? (uint32_t)w : s.rem)); }
 EMA_HD int paged_worker_of(PagedSplit s, int t) {
+  if (s.base == 1 && s.rem == 0) return t;
   const uint32_t cut = s.rem * (s.base + 1);
   return (int)((uint32_t)t < cut ? (uint32_t)t / (s.base + 1) : s.rem + ((uint32_t)t - cut) / s.base);
 }
@@ -98,6 +103,16 @@ EMA_HD PagedChunks paged_chunks(int64_t rows, int Hkv, int max_prefix, int cus) 
 // and not written by the kernels, so they come as scalar loads.
 typedef const __attribute__((address_space(4))) int32_t paged_cint;
 __device__ __forceinline__ int ld_uniform(const int32_t* p, int64_t i) { return ((paged_cint*)p)[i]; }
+// Sum of v over this lane and those before it, by DPP: within rows of 16, then across them.
+__device__ __forceinline__ int sum_up_to_lane(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
 #endif
 
 }  // namespace ema

@@ -150,14 +150,7 @@ __device__ __forceinline__ bool ragged_item(const PagedPrefillArgs& a, int x, in
     const int nqb = (n * a.G + kBM - 1) / kBM;
     return kPair ? (nqb + 1) / 2 : nqb;
   };
-  auto before = [&](int v) __attribute__((always_inline)) {
-    int s = v;
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(s, d, 64);
-      if (lane >= d) s += y;
-    }
-    return s - v;
-  };
+  auto before = [&](int v) __attribute__((always_inline)) { return sum_up_to_lane(v) - v; };
   int sum = 0;
   for (int i = 0; i < step; ++i) sum += items(lane * step + i);
   int pre = before(sum);
