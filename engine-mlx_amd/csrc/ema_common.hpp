@@ -253,6 +253,7 @@ struct PagedAttention {
 struct PagedPlan {
   int workers;          // workgroups over the sequences' own pages
   int prefix_workers;   // workgroups over the shared prefix (few rows)
+  bool direct;          // the segments take the prefix's tiles themselves
   int chunks;           // chunks of the shared prefix (more rows), and their 64-key blocks
   int chunk_blocks;
   uint64_t part_bytes;  // partial states of shared segments

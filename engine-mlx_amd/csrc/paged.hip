@@ -228,7 +228,9 @@ struct PagedArgs {
   float* part;      // partial states, slots of [32][kPagedState]
   const float* carry_in;  // states of the rows over a shared prefix [chunk][n_rows, Hq][kPagedState], or null
   float* carry_out;       // leave the rows' states there instead of their output, or null
-  const int32_t* prefix_len;
+  const int32_t* prefix_len;      // null: no shared prefix
+  const int32_t* prefix_table;    // its pages, where the segments take them themselves (else null)
+  int prefix_cols;
   int carry_blocks;       // 64-key blocks of a chunk of the prefix (0: one state, always there)
   int prefix_cap;         // positions that the prefix's table holds
   int64_t sb, sh;   // bytes
@@ -338,7 +340,8 @@ __device__ __forceinline__ int blocks_of(const PagedArgs& a, int T) {
   return (int)(((uint32_t)T * (uint32_t)a.G + kPagedRows - 1) / kPagedRows);
 }
 
-template <bool kFp8, bool kOnce>
+// kDirect: the segments take a shared prefix's tiles before their own.
+template <bool kFp8, bool kOnce, bool kDirect>
 __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_kernel(PagedArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t slots[kPagedWaves][2 * kSlot];
   __shared__ float2 ml[kPagedWaves][kPagedRows];
@@ -347,15 +350,16 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  // states of the rows over the prefix: one per chunk that holds keys
-  int n_carry = 1;
-  bool shared_keys = false;
-  if (a.carry_in) {
-    int n = ld_uniform(a.prefix_len, 0);
-    n = n < 0 ? 0 : (n > a.prefix_cap ? a.prefix_cap : n);
-    shared_keys = n > 0;
-    if (a.carry_blocks) n_carry = ((n + 63) / 64 + a.carry_blocks - 1) / a.carry_blocks;
+  // a shared prefix: its keys, the states of the rows over it (one per chunk that holds keys), or
+  // its tiles, which then come before each segment's own
+  int n_carry = 1, prefix = 0, prefix_tiles = 0;
+  if (a.prefix_len) {
+    prefix = ld_uniform(a.prefix_len, 0);
+    prefix = prefix < 0 ? 0 : (prefix > a.prefix_cap ? a.prefix_cap : prefix);
+    if (a.carry_blocks) n_carry = ((prefix + 63) / 64 + a.carry_blocks - 1) / a.carry_blocks;
+    if (kDirect) prefix_tiles = paged_tiles(prefix);
   }
+  const bool shared_keys = prefix > 0;
 
   // Units of work before each sequence, by every wave for itself: lane l takes sequences
   // l step .. +step-1 (up to 64 sequences: one each, kept in the lane's registers; more: their
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     if (b < a.B) {
       lane_rows = rows_at(b);
       lane_len = clamp_len(a, a.len[b]);
-      const int nr = paged_rounds(lane_len), segs = blocks_of(a, lane_rows.n) * a.Hkv;
+      const int nr = paged_rounds(prefix_tiles + paged_tiles(lane_len)), segs = blocks_of(a, lane_rows.n) * a.Hkv;
       sum1 += segs * paged_units(nr, 1);
       sum_long += segs * paged_units(nr, kPagedLongUnit);
     }
@@ -388,7 +392,8 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       const int b = lane * step + i;
       if (b < a.B) {
         pre[b] = run;
-        run += blocks_of(a, rows_at(b).n) * a.Hkv * paged_units(paged_rounds(clamp_len(a, a.len[b])), unit);
+        const int nr = paged_rounds(prefix_tiles + paged_tiles(clamp_len(a, a.len[b])));
+        run += blocks_of(a, rows_at(b).n) * a.Hkv * paged_units(nr, unit);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -396,8 +401,8 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 
-  // rows of sequences that hold nothing: no unit visits them
-  for (int i = 0; i < step; ++i) {
+  // rows of sequences that see nothing: no unit visits them
+  for (int i = 0; i < step && prefix_tiles == 0; ++i) {
     const int bl = lane * step + i;
     uint64_t none = __ballot(bl < a.B && (step == 1 ? lane_len : a.len[bl < a.B ? bl : 0]) <= 0);
     for (; none; none &= none - 1) {
@@ -456,14 +461,14 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       L = clamp_len(a, ld_uniform(a.len, b));
       pre_b = __builtin_amdgcn_readfirstlane(pre[b]);
     }
-    const int nu = paged_units(paged_rounds(L), unit), nrb = blocks_of(a, rw.n);
+    const int tile_end = prefix_tiles + paged_tiles(L);
+    const int nu = paged_units(paged_rounds(tile_end), unit), nrb = blocks_of(a, rw.n);
     const uint32_t seg = (uint32_t)(t - pre_b) / (uint32_t)nu;
     const int unit0 = (int)((uint32_t)(t - pre_b) - seg * (uint32_t)nu);
     const int kh = nrb == 1 ? (int)seg : (int)(seg / (uint32_t)nrb), rb = (int)(seg - (uint32_t)kh * (uint32_t)nrb);
     const int seg_begin = t - unit0, seg_end = seg_begin + nu;
     const int piece_end = t_end < seg_end ? t_end : seg_end;
     const int tile0 = unit0 * unit * kPagedWaves;
-    const int tile_end = (int)(((uint32_t)L + kPagedTile - 1) / kPagedTile);
     const int tile1 = min(tile0 + (piece_end - t) * unit * kPagedWaves, tile_end);
     const int row0 = rb * kPagedRows;                     // the segment's first row (token * G + head)
     const int n_seg = rw.n * a.G - row0 < kPagedRows ? rw.n * a.G - row0 : kPagedRows;
@@ -474,20 +479,24 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     const int last_key = a.causal ? L - rw.n + tok : L - 1;
     const int first_limit = a.causal ? L - rw.n + (int)((uint32_t)row0 / (uint32_t)a.G) : L - 1;
 
-    const int32_t* const tab = a.table + (int64_t)b * a.cols;
-    // table entry of the page that holds position 32 tile + 16 half (any entry past the tiles)
+    // tile of the segment's list: the prefix's first, then its own
+    const int32_t* const own_table = a.table + (int64_t)b * a.cols;
+    auto is_own = [&](int tile) __attribute__((always_inline)) { return !kDirect || tile >= prefix_tiles; };
+    auto place = [&](int tile) __attribute__((always_inline)) { return kDirect && is_own(tile) ? tile - prefix_tiles : tile; };
+    // table entry of the page that holds position 16 half of the tile (any entry past the tiles)
     auto entry = [&](int tile, int half) __attribute__((always_inline)) {
-      const int c = (int)(((uint32_t)tile * kPagedTile + 16u * half) >> a.shift);
-      return ld_uniform(tab, c < a.cols ? c : a.cols - 1);
+      const int c = (int)(((uint32_t)place(tile) * kPagedTile + 16u * half) >> a.shift);
+      const int cols = is_own(tile) ? a.cols : a.prefix_cols;
+      return ld_uniform(is_own(tile) ? own_table : a.prefix_table, c < cols ? c : cols - 1);
     };
     // 16 rows of a page: where they begin and how many of them are held (0: none are read)
     auto valid_rows = [&](int tile, int half, int page) __attribute__((always_inline)) {
-      const int left = L - tile * kPagedTile - 16 * half;
+      const int left = (is_own(tile) ? L : prefix) - place(tile) * kPagedTile - 16 * half;
       const int n = left < 0 ? 0 : (left > 16 ? 16 : left);
       return tile < tile1 && (uint32_t)page < (uint32_t)a.n_pages ? n : 0;
     };
     auto half_base = [&](const uint8_t* pool, int tile, int half, int page) __attribute__((always_inline)) {
-      const uint32_t slot = ((uint32_t)tile * kPagedTile + 16u * half) & ((1u << a.shift) - 1u);
+      const uint32_t slot = ((uint32_t)place(tile) * kPagedTile + 16u * half) & ((1u << a.shift) - 1u);
       return pool + ((uint32_t)page < (uint32_t)a.n_pages ? (int64_t)page * a.sb : 0) + (int64_t)kh * a.sh +
              (int64_t)slot * a.row_bytes;
     };
@@ -516,7 +525,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         const int page = half ? e1 : e0;
         const int n = valid_rows(tile, half, page);
         const uint8_t* const base = half_base(k ? a.k : a.v, tile, half, page);
-        const uint32_t slot = ((uint32_t)tile * kPagedTile + 16u * half) & ((1u << a.shift) - 1u);
+        const uint32_t slot = ((uint32_t)place(tile) * kPagedTile + 16u * half) & ((1u << a.shift) - 1u);
         const uint16_t* const eb = (k ? a.kexp : a.vexp) +
             (n ? (((int64_t)page * a.Hkv + kh) << a.shift) + slot : 0);
         const __amdgpu_buffer_rsrc_t r =
@@ -594,9 +603,10 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
         dma_tile(true, tile + kPagedWaves, e0, e1);
       }
-      // key of score i: 32 tile + (i % 4) + 8 (i / 4) + 4 hh
-      if (tile * kPagedTile + kPagedTile - 1 > first_limit) {
-        const int room = last_key - tile * kPagedTile - 4 * hh;
+      // key of score i: 32 place + (i % 4) + 8 (i / 4) + 4 hh
+      const int key0 = place(tile) * kPagedTile;
+      if (key0 + kPagedTile - 1 > (is_own(tile) ? first_limit : prefix - 1)) {
+        const int room = (is_own(tile) ? last_key : prefix - 1) - key0 - 4 * hh;
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[i] = (i & 3) + 8 * (i >> 2) <= room ? sc[i] : -INFINITY;
       }
@@ -752,10 +762,18 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
 int32_t launch_rows(hipStream_t s, const PagedArgs& a, bool fp8, int max_q, const char* what) {
   const bool once = (int64_t)max_q * a.G <= kPagedRows;
   const dim3 grid(a.W), block(64 * kPagedWaves);
-  if (fp8 && once) hipLaunchKernelGGL((paged_kernel<true, true>), grid, block, 0, s, a);
-  else if (fp8) hipLaunchKernelGGL((paged_kernel<true, false>), grid, block, 0, s, a);
-  else if (once) hipLaunchKernelGGL((paged_kernel<false, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((paged_kernel<false, false>), grid, block, 0, s, a);
+  if (a.prefix_table) {  // (several sequences' segments read the prefix)
+    if (fp8) hipLaunchKernelGGL((paged_kernel<true, false, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((paged_kernel<false, false, true>), grid, block, 0, s, a);
+  } else if (fp8 && once) {
+    hipLaunchKernelGGL((paged_kernel<true, true, false>), grid, block, 0, s, a);
+  } else if (fp8) {
+    hipLaunchKernelGGL((paged_kernel<true, false, false>), grid, block, 0, s, a);
+  } else if (once) {
+    hipLaunchKernelGGL((paged_kernel<false, true, false>), grid, block, 0, s, a);
+  } else {
+    hipLaunchKernelGGL((paged_kernel<false, false, false>), grid, block, 0, s, a);
+  }
   return check_hip(hipGetLastError(), what);
 }
 
@@ -802,18 +820,25 @@ int32_t launch_paged_append(hipStream_t s, const PagedAppend& p, const ema_kvcac
 constexpr int kFewRows = 128;
 // A shared prefix: more rows than this per kv head in 128-row blocks over chunks of it.
 constexpr int kFewPrefixRows = 32;
+// A shared prefix whose tiles are no more rounds than this when every segment takes them itself:
+// one launch over the prefix's and the own tiles together, K and V of the prefix from the L2s.
+constexpr int kDirectRounds = 4 * kPagedMaxWorkers;
 
 // Workspace: the arrival counters, the partial states of the workers' shared segments, then
 // the rows' states over a shared prefix.
 PagedPlan plan_paged(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len, int max_prefix) {
   PagedPlan p;
   const int G = Hq / Hkv;
-  p.workers = paged_plan_workers(paged_row_blocks(B, n_rows, max_q, G), Hkv, max_len);
+  const int64_t nrb = paged_row_blocks(B, n_rows, max_q, G);
+  p.workers = paged_plan_workers(nrb, Hkv, paged_tiles(max_len));
   p.prefix_workers = 0;
   p.chunks = p.chunk_blocks = 0;
   p.carry_bytes = 0;
-  if (max_prefix > 0) {
-    p.prefix_workers = paged_plan_workers(paged_row_blocks(1, n_rows, n_rows, G), Hkv, max_prefix);
+  p.direct = max_prefix > 0 && nrb * Hkv * paged_rounds(paged_tiles(max_prefix) + paged_tiles(max_len)) <= kDirectRounds;
+  if (p.direct) {
+    p.workers = paged_plan_workers(nrb, Hkv, paged_tiles(max_prefix) + paged_tiles(max_len));
+  } else if (max_prefix > 0) {
+    p.prefix_workers = paged_plan_workers(paged_row_blocks(1, n_rows, n_rows, G), Hkv, paged_tiles(max_prefix));
     const PagedChunks c = paged_chunks((int64_t)n_rows * G, Hkv, max_prefix, device_cus());
     p.chunks = c.n;
     p.chunk_blocks = c.blocks;
@@ -845,6 +870,8 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
   a.carry_in = nullptr;
   a.carry_out = nullptr;
   a.prefix_len = p.prefix_len;
+  a.prefix_table = nullptr;
+  a.prefix_cols = p.prefix_cols;
   a.carry_blocks = 0;
   a.prefix_cap = p.prefix_cols << paged_shift(c.capacity);
   a.sb = c.stride_batch * es;
@@ -863,7 +890,9 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
   a.causal = p.causal;
   a.few = INT32_MAX;
   a.max_q = 0;
-  if (p.prefix_table) {
+  if (p.prefix_table && plan.direct) {
+    a.prefix_table = p.prefix_table;
+  } else if (p.prefix_table) {
     float* const carry = (float*)((char*)ws + kDecodeCounterBytes + plan.part_bytes);
     if (!fp8 && (int64_t)p.n_rows * a.G > kFewPrefixRows) {
       const int32_t rc = launch_prefix_rows(s, p, c, plan.chunks, plan.chunk_blocks, carry);
@@ -874,6 +903,7 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
       x.table = p.prefix_table;
       x.cols = p.prefix_cols;
       x.len = p.prefix_len;
+      x.prefix_len = nullptr;
       x.starts = nullptr;
       x.rows_end = p.q_starts ? p.q_starts + p.batch : nullptr;
       x.B = 1;

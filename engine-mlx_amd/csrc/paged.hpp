@@ -28,9 +28,9 @@ EMA_HD PagedRows paged_rows(int s0, int s1, int n_rows) {
   return PagedRows{s0, s1 - s0};
 }
 
-// Rounds of a segment of L keys: a round is one tile for each wave of a workgroup.
-constexpr int kPagedRound = kPagedTile * kPagedWaves;
-EMA_HD int paged_rounds(int L) { return (int)(((uint32_t)L + kPagedRound - 1) / kPagedRound); }
+// Key tiles of L positions, and rounds of n tiles: a round is one tile for each wave of a workgroup.
+EMA_HD int paged_tiles(int L) { return (int)(((uint32_t)L + kPagedTile - 1) / kPagedTile); }
+EMA_HD int paged_rounds(int tiles) { return (tiles + kPagedWaves - 1) / kPagedWaves; }
 
 // Units of a segment: one round each, or kPagedLongUnit rounds where there are more rounds than
 // workgroups but no more than kPagedLongUnit for each. A piece costs a workgroup about as much as
@@ -63,9 +63,9 @@ EMA_HD int paged_worker_of(PagedSplit s, int t) {
 EMA_HD int paged_slot(int w, int w0) { return 2 * w + (w == w0 ? 1 : 0); }
 
 // Workers the plan sizes the workspace for, from the host's bounds: nrb row blocks per kv head
-// (all sequences), max_len keys each.
-EMA_HD int paged_plan_workers(int64_t nrb, int Hkv, int max_len) {
-  const int64_t want = nrb * Hkv * paged_rounds(max_len);
+// (all sequences), max_tiles key tiles each.
+EMA_HD int paged_plan_workers(int64_t nrb, int Hkv, int max_tiles) {
+  const int64_t want = nrb * Hkv * paged_rounds(max_tiles);
   return (int)(want < 1 ? 1 : (want < kPagedMaxWorkers ? want : kPagedMaxWorkers));
 }
 // Row blocks of a batch whose sequences have at most max_q rows and n_rows together.
