@@ -752,6 +752,9 @@ static int32_t paged_attention(const char* op, ema_stream_t stream, PagedAttenti
   if ((rc = check_paged_rows(op, p.batch, p.n_rows, p.n_heads, !p.q_starts))) return rc;
   if (pages->head_dim != 128)
     return set_error(EMA_ERR_UNSUPPORTED, "%s: head_dim %d not supported (128)", op, pages->head_dim);
+  if (p.n_heads / pages->n_kv_heads > kPagedMaxGroup)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %d query heads per kv head exceed %d", op, p.n_heads / pages->n_kv_heads,
+                     kPagedMaxGroup);
   if (p.max_q < 0) return set_error(EMA_ERR_SHAPE, "%s: max_q %d is negative", op, p.max_q);
   const int64_t cap = (int64_t)p.table_cols * pages->capacity;
   if (max_len < 0 || max_len > cap)

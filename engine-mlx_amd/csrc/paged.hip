@@ -235,6 +235,7 @@ struct PagedArgs {
   int prefix_cap;         // positions that the prefix's table holds
   int64_t sb, sh;   // bytes
   uint32_t row_bytes;
+  uint32_t magic;   // paged_magic(G)
   float qk_scale;   // scale * log2(e): scores live in the log2 domain
   int B, T, n_rows, Hq, Hkv, G, cols, shift, n_pages, W, causal;
   int few, max_q;   // sequences of few < n <= max_q rows are prefill_kernel's
@@ -475,9 +476,9 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
 
     // this lane's query row, and the last key it sees
     const int i_row = row0 + ((lane & 31) < n_seg ? (lane & 31) : n_seg - 1);
-    const int tok = (int)((uint32_t)i_row / (uint32_t)a.G), head = i_row - tok * a.G;
+    const int tok = paged_div(i_row, a.magic), head = i_row - tok * a.G;
     const int last_key = a.causal ? L - rw.n + tok : L - 1;
-    const int first_limit = a.causal ? L - rw.n + (int)((uint32_t)row0 / (uint32_t)a.G) : L - 1;
+    const int first_limit = a.causal ? L - rw.n + paged_div(row0, a.magic) : L - 1;
 
     // tile of the segment's list: the prefix's first, then its own
     const int32_t* const own_table = a.table + (int64_t)b * a.cols;
@@ -689,7 +690,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         s.o += ((const f32x4*)slots[v])[r * 32 + (d4 ^ r)] * f;
       }
       if (w0 == w1) {
-        const int ir = row0 + r, tk = (int)((uint32_t)ir / (uint32_t)a.G);
+        const int ir = row0 + r, tk = paged_div(ir, a.magic);
         finish4(a, n_carry, shared_keys || !a.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk, kh * a.G + ir - tk * a.G, 4 * d4, s);
       } else {
         float* const p = a.part + ((int64_t)paged_slot(w, w0) * kPagedRows + r) * kPagedState;
@@ -744,7 +745,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
                 }
               s.m = M;
             }
-            const int ir = row0 + r, tk = (int)((uint32_t)ir / (uint32_t)a.G);
+            const int ir = row0 + r, tk = paged_div(ir, a.magic);
             finish4(a, n_carry, shared_keys || !a.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk,
                     kh * a.G + ir - tk * a.G, 4 * d4, s);
           }
@@ -884,6 +885,7 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
   a.Hq = p.n_heads;
   a.Hkv = c.n_kv_heads;
   a.G = p.n_heads / c.n_kv_heads;
+  a.magic = paged_magic(a.G);
   a.cols = p.table_cols;
   a.shift = paged_shift(c.capacity);
   a.n_pages = c.batch;

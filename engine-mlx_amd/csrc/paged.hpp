@@ -62,6 +62,11 @@ EMA_HD int paged_worker_of(PagedSplit s, int t) {
 // inside it and runs on (slot 2 w + 1, w then being the segment's first worker w0).
 EMA_HD int paged_slot(int w, int w0) { return 2 * w + (w == w0 ? 1 : 0); }
 
+// r / G for r < 2^23 by a product: magic = ceil(2^32 / G), exact while r * G < 2^32 (G <= 256).
+constexpr int kPagedMaxGroup = 256;
+EMA_HD uint32_t paged_magic(int G) { return G == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + G - 1) / (uint64_t)G); }
+EMA_HD int paged_div(int r, uint32_t magic) { return magic ? (int)(((uint64_t)(uint32_t)r * magic) >> 32) : r; }
+
 // Workers the plan sizes the workspace for, from the host's bounds: nrb row blocks per kv head
 // (all sequences), max_tiles key tiles each.
 EMA_HD int paged_plan_workers(int64_t nrb, int Hkv, int max_tiles) {

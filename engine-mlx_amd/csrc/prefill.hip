@@ -80,6 +80,7 @@ struct PagedPrefillArgs : PrefillArgs {
   float* part;  // kSharedPages: the rows' states [chunk][n_rows, Hq][kPagedState]
   uint32_t page_bytes, head_bytes;  // (page_bytes below 2^32: host)
   int n_rows, cols, shift, n_pages;
+  uint32_t magic;       // paged_magic(G)
   int few, max_q;       // kPages: sequences of few < n <= max_q rows are this kernel's
   int chunk_blocks;     // kSharedPages: 64-key blocks per chunk of the keys
 };
@@ -249,7 +250,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   const int qb_l = has_light ? item.qb_second : qb_h;
   const int n_rows = kPaged ? prow.n * a.G : a.T;  // query rows of the item's (sequence, head or kv head)
   // token of query row r, relative to the sequence's first, and the row of q and out that it is
-  auto token_of = [&](int r) __attribute__((always_inline)) { return kPaged ? (int)((uint32_t)r / (uint32_t)a.G) : r; };
+  auto token_of = [&](int r) __attribute__((always_inline)) {
+    if constexpr (kPaged) return paged_div(r, a.magic);
+    return r;
+  };
   auto out_row = [&](int r0, int r) __attribute__((always_inline)) {
     if (!kPaged) return ((int64_t)b * a.T + r0 + r) * a.Hq + h;
     const int t = token_of(r0 + r);
@@ -945,21 +949,29 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
     const float inv = kPaged ? (row_has_keys(laneB) ? 1.0f / l_tot : 0.f) : l_tot > 0.f ? 1.0f / l_tot : 0.f;
     const float a_mine = g ? a1 : a0, a_other = g ? a0 : a1;
     const float* const ox = xo + (1 - g) * (2 * 4 * 4 * 64 * 4);
-    if constexpr (kMode == kSharedPages) {  // the state itself, in 32 bits
-      if (row0 + rr < n_rows) {
-        float* const P = a.part + ((int64_t)chunk * a.n_rows * a.Hq + out_row(row0, rr)) * kPagedState;
-        if (g == 0 && hh == 0) *(float2*)P = make_float2(m == -INFINITY ? m : m * a.qk_scale, l_tot);
-        auto leave = [&](const int dt0) __attribute__((always_inline)) {
-          for (int d = 0; d < 2; ++d)
-            for (int i4 = 0; i4 < 4; ++i4) {
-              const f32x4 v = *(const f32x4*)(ox + (((d * 4 + i4) * 4 + wq) * 64 + lane) * 4);
-              f32x4 r;
-              for (int e = 0; e < 4; ++e) r[e] = o[dt0 + d][4 * i4 + e] * a_mine + v[e] * a_other;
-              *(f32x4*)(P + 4 + 32 * (dt0 + d) + 8 * i4 + 4 * hh) = r;
-            }
-        };
-        if (g == 0) leave(0);
-        else leave(2);
+    if constexpr (kMode == kSharedPages) {
+      // the state itself, in 32 bits: staged behind the exchange (64 KB + 4 KB) as [row][d / 4]
+      // with unit d4 of row r at d4 ^ (r & 31), then stored as whole rows
+      f32x4* const St = (f32x4*)(lds + 34816);
+      auto leave = [&](const int dt0) __attribute__((always_inline)) {
+        for (int d = 0; d < 2; ++d)
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const f32x4 v = *(const f32x4*)(ox + (((d * 4 + i4) * 4 + wq) * 64 + lane) * 4);
+            f32x4 r;
+            for (int e = 0; e < 4; ++e) r[e] = o[dt0 + d][4 * i4 + e] * a_mine + v[e] * a_other;
+            St[rr * 32 + ((8 * (dt0 + d) + 2 * i4 + hh) ^ (rr & 31))] = r;
+          }
+      };
+      if (g == 0) leave(0);
+      else leave(2);
+      float* const P = a.part + (int64_t)chunk * a.n_rows * a.Hq * kPagedState;
+      if (g == 0 && hh == 0 && row0 + rr < n_rows)
+        *(float2*)(P + out_row(row0, rr) * kPagedState) = make_float2(m == -INFINITY ? m : m * a.qk_scale, l_tot);
+      __syncthreads();
+      for (int it = 0; it < 8; ++it) {
+        const int n = it * kThreads + tid;
+        const int r = n >> 5, d4 = n & 31;
+        if (row0 + r < n_rows) *(f32x4*)(P + out_row(row0, r) * kPagedState + 4 + 4 * d4) = St[r * 32 + (d4 ^ (r & 31))];
       }
       return;
     }
@@ -1302,6 +1314,7 @@ PagedPrefillArgs paged_prefill_args(const PagedAttention& p, const ema_kvcache_d
   a.cols = p.table_cols;
   a.shift = paged_shift(c.capacity);
   a.n_pages = c.batch;
+  a.magic = paged_magic(a.G);
   a.few = 0;
   a.max_q = p.max_q;
   a.chunk_blocks = 0;

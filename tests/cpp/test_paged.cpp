@@ -84,5 +84,18 @@ int main() {
     }
     CHECK(blocks <= paged_row_blocks(B, rows, most, G));
   }
+  for (int G = 1; G <= kPagedMaxGroup; ++G) {  // the product for r / G
+    const uint32_t m = paged_magic(G);
+    for (int i = 0; i < 3000; ++i) {
+      const int r = (int)(rng() & ((1u << 23) - 1));
+      CHECK(paged_div(r, m) == r / G);
+      CHECK(paged_div(r / G * G, m) == r / G && (r < G || paged_div(r / G * G - 1, m) == r / G - 1));
+    }
+    CHECK(paged_div((1 << 23) - 1, m) == ((1 << 23) - 1) / G && paged_div(0, m) == 0);
+  }
+  for (int64_t rows : {0, 1, 33, 128, 129, 5000}) for (int n : {1, 63, 64, 65, 8001, 32768, 2000000000}) for (int hkv : {1, 8, 40}) {
+    const PagedChunks c = paged_chunks(rows, hkv, n, 256);  // the chunks cover the prefix, none empty
+    CHECK(c.n >= 1 && c.blocks >= 1 && (int64_t)c.n * c.blocks * 64 >= n && ((int64_t)c.n - 1) * c.blocks * 64 < n);
+  }
   std::printf("%ld checks passed\n", checks);
 }

@@ -194,7 +194,8 @@ def test_rows_behind_the_last_sequence(ema):
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("new,kv,prefix", [
     ([1] * 6, [50, 1, 33, 200, 64, 5], 0), ([40, 17, 90], [40, 200, 90], 0), ([260, 3], [300, 30], 0),
-    ([1] * 6, [9] * 6, 70), ([1] * 40, [9] * 40, 300), ([2] * 130, [9] * 130, 130),
+    ([1] * 6, [9] * 6, 70), ([1] * 40, [9] * 40, 300), ([2] * 130, [9] * 130, 130), ([1] * 40, [9] * 40, 3500),
+    ([1] * 8, [0, 3] * 4, 17000),
 ])
 def test_rows_that_are_not_finite(ema, new, kv, prefix, bad):
     """A query row that is not finite gives a row that is not finite, and no other row changes:
@@ -400,6 +401,32 @@ def test_prefix(ema, prefix, new, kv, heads):
 def test_prefix_long(ema, page):
     run(ema, ref.Batch([1] * 9, [30] * 9, page, 40, 8, seed=1, prefix=4001), "long prefix")
     run(ema, ref.Batch([1] * 64, [3] * 64, page, 8, 2, seed=2, prefix=2500), "long prefix, 256 rows")
+
+
+def test_prefix_ways(ema):
+    """The three ways a prefix is read: its tiles in every segment (short ones), once in segments of
+    few rows, once in blocks of 128 rows; each with sequences that hold nothing of their own."""
+    for new, kv, heads, prefix in (([1] * 4, [0, 5, 33, 0], (8, 4), 200), ([1] * 6, [0, 5, 33, 1, 0, 90], (16, 8), 8000),
+                                   ([2, 1, 0, 3], [2, 400, 7, 0], (10, 2), 40000), ([1] * 40, list(range(40)), (8, 2), 3300),
+                                   ([3] * 30, [3] * 30, (12, 1), 10000)):
+        run(ema, ref.Batch(new, kv, 64, *heads, seed=prefix, prefix=prefix), f"prefix {prefix}, {heads[0] // heads[1] * sum(new)} rows")
+    run(ema, ref.Batch([1] * 6, [0, 5, 33, 1, 0, 90], 64, 16, 8, seed=1, prefix=8000), "prefix once, fp8", pages="fp8")
+
+
+@pytest.mark.parametrize("held", [0, 1, 64, 129])
+def test_prefix_shorter_than_its_bound(ema, held):
+    """The prefix's length is on the device: what it holds counts, the bound only sizes the call."""
+    import torch
+
+    for n, heads in ((5, (16, 8)), (40, (8, 2))):
+        b = ref.Batch([1] * n, [7] * n, 16, *heads, seed=held, prefix=held)
+        g = OnGpu(ema, b)
+        table = torch.full((600,), -1, dtype=torch.int32, device="cuda")
+        if held:
+            table[:g.prefix_table.numel()] = g.prefix_table
+        out = ema.prefix_attention(g.q, g.cache, table, up(np.asarray([held], np.int32)), 9600, g.table, g.lengths, 7)
+        torch.cuda.synchronize()
+        ref.check_attention(down(out), *b.attention(), f"{held} of 9600")
 
 
 def test_prefix_fp8(ema):

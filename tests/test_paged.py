@@ -114,6 +114,7 @@ def test_attention_that_is_refused(ema, prefix):
     for name in ("q", "out", "ws"):
         assert attend(ema, d, prefix, **{name: P + 4}) == ema.EMA_ERR_INVALID_ARG, name
     assert attend(ema, d, prefix, heads=12) == ema.EMA_ERR_SHAPE
+    assert attend(ema, pool(ema, Hkv=1), prefix, heads=257) == ema.EMA_ERR_UNSUPPORTED
     assert attend(ema, d, prefix, cols=0) == ema.EMA_ERR_SHAPE
     assert attend(ema, d, prefix, starts=None) == ema.EMA_ERR_SHAPE
     assert attend(ema, d, prefix, batch=1025) == ema.EMA_ERR_UNSUPPORTED
