@@ -415,29 +415,29 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   const uint32_t ring_bytes = (uint32_t)a.cap * row_bytes;
   // kPaged: the table entry of the 16 keys of block j that this wave loads (any entry past the
   // keys), and their rows: none past the stream, past the keys or on an entry outside the pool
+  const int32_t* table = nullptr;
+  if constexpr (kPaged) table = a.table + (int64_t)b * a.cols;
   auto entry = [&](int j) __attribute__((always_inline)) {
     if constexpr (kPaged) {
-      const int c = (blk_of(j < ng ? j : 0) * kBN + 16 * wq) >> a.shift;
-      return ld_uniform(a.table + (int64_t)b * a.cols, c < a.cols ? c : a.cols - 1);
+      int pos = blk_of(j) * kBN + 16 * wq;
+      pos = pos < kv_len ? pos : kv_len - 1;
+      return ld_uniform(table, pos > 0 ? pos >> a.shift : 0);
     }
     return 0;
   };
-  uint32_t head_bytes = 0;
-  if constexpr (kPaged) head_bytes = a.head_bytes;
   struct Rows {
-    int64_t at;      // byte offset in the K pool, and in the V pool
+    int64_t at;      // byte offset in the K pool from the head's first row, and in the V pool
     uint32_t bytes;  // of the rows that are held, whole rows
   };
-  const int64_t head_at = kPaged ? (int64_t)kh * head_bytes : 0;
   auto rows_at = [&](int j, int page) __attribute__((always_inline)) {
-    Rows r = {head_at, 0u};
+    Rows r = {0, 0u};
     if constexpr (kPaged) {
       const int pos = blk_of(j) * kBN + 16 * wq;
       const bool in = j < ng && (uint32_t)page < (uint32_t)a.n_pages;
       const int left = kv_len - pos;
       const uint32_t n = in && left > 0 ? (left < 16 ? left : 16) : 0;
       r.bytes = n * row_bytes;
-      r.at += (int64_t)((uint64_t)(uint32_t)(in ? page : 0) * a.page_bytes) +
+      r.at = (int64_t)((uint64_t)(uint32_t)(in ? page : 0) * a.page_bytes) +
               (uint32_t)(pos & ((1 << a.shift) - 1)) * row_bytes;
     }
     return r;
@@ -496,8 +496,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
       for (int i = 0; i < 4; ++i) dma_part(r, ob, off, dst, i, wrap);
     }
   };
-  const char* const Kp = (const char*)a.k;
-  const char* const Vp = (const char*)a.v;
+  const char *Kp = nullptr, *Vp = nullptr;
+  if constexpr (kPaged) {
+    Kp = (const char*)a.k + (int64_t)kh * a.head_bytes;
+    Vp = (const char*)a.v + (int64_t)kh * a.head_bytes;
+  }
   auto load_k = [&](int j, Rows rows) __attribute__((always_inline)) {
     if constexpr (kPaged) {
       const u32x4 r = buffer_rsrc(Kp + rows.at, rows.bytes);
