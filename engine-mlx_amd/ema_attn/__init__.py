@@ -544,32 +544,22 @@ def _want(op: str, name: str, t, dtype, shape, device: int) -> None:
         raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} is on {t.device}, the pages on device {device}")
 
 
-def _paged_batch(op: str, cache, table, q_starts, per_seq, name: str, device: int):
-    """The checks of a call's table and per-sequence tensors; returns (B, table columns)."""
-    import torch
-
-    i32 = torch.int32
-    B, cols = table.shape if table.dim() == 2 else (None, None)
-    _want(op, "table", table, i32, (B, cols), device)
-    _want(op, name, per_seq, i32, (B,), device)
-    if q_starts is not None:
-        _want(op, "q_starts", q_starts, i32, (B + 1,), device)
-    return B, cols
+def _refuse(op: str, device: int, *wanted) -> None:
+    """Raises for the first of (name, tensor, dtype, shape) that is not as wanted."""
+    for name, t, dtype, shape in wanted:
+        if t is not None:
+            _want(op, name, t, dtype, shape, device)
+    raise EmaError(EMA_ERR_SHAPE, op, "arguments that do not belong together")
 
 
-def _launch(device: int, stream, call, *args) -> int:
-    """call(stream, *args) with the pool's device current, on that device's current torch stream
-    when no stream is given. (torch._C's accessors: what torch.cuda.current_stream() and
-    current_device() wrap, without the objects they build, 2 us a call.)"""
+def _elsewhere(device: int, call, *args) -> int:
+    """call(*args) with the pool's device, which is not the current one, made current."""
     import torch
 
     if device < 0:
         raise EmaError(EMA_ERR_INVALID_ARG, call.__name__, "the pages are not on a GPU")
-    raw = torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
-    if torch._C._cuda_getDevice() == device:
-        return call(raw, *args)
     with torch.cuda.device(device):
-        return call(raw, *args)
+        return call(*args)
 
 
 def paged_append(qkv, q_norm_w, k_norm_w, eps, theta, offsets, n_heads, cache: PagedCache, table, q_starts=None,
@@ -580,24 +570,37 @@ def paged_append(qkv, q_norm_w, k_norm_w, eps, theta, offsets, n_heads, cache: P
     the rotation counts before the sequences' own. Returns q_out [n, Hq, D]."""
     import torch
 
-    op, bf = "ema_paged_append", torch.bfloat16
-    desc, dev = cache.desc, cache.device_index
-    D = desc.head_dim
-    B, cols = _paged_batch(op, cache, table, q_starts, offsets, "offsets", dev)
-    n = qkv.shape[0] if qkv.dim() else 0
-    _want(op, "qkv", qkv, bf, (n, (n_heads + 2 * desc.n_kv_heads) * D), dev)
-    for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
-        if w is not None:
-            _want(op, name, w, bf, (D,), dev)
-    if prefix_len is not None:
-        _want(op, "prefix_len", prefix_len, torch.int32, (1,), dev)
-    if q_out is None:
+    # one expression for what is right (2 us for the five to seven tensors of a call: the smallest
+    # calls are bound by the host), the tensor to name looked for only when it is not
+    op, bf, i32, dev = "ema_paged_append", torch.bfloat16, torch.int32, cache.device_index
+    D, F = cache.desc.head_dim, n_heads + 2 * cache.desc.n_kv_heads
+    B, cols = table.shape if table.dim() == 2 else (-1, -1)
+    n = qkv.shape[0] if qkv.dim() else -1
+    if q_out is None and n >= 0:
         q_out = torch.empty((n, n_heads, D), dtype=bf, device=qkv.device)
-    else:
-        _want(op, "q_out", q_out, bf, (n, n_heads, D), dev)
-    _check(_launch(dev, stream, lib().ema_paged_append, qkv.data_ptr(), _ptr(q_norm_w), _ptr(k_norm_w), eps, theta,
-                   _ptr(q_starts), offsets.data_ptr(), _ptr(prefix_len), B, n, n_heads, flags, q_out.data_ptr(),
-                   cache.desc_ref, table.data_ptr(), cols), op)
+    if not (table.dtype is i32 and table.is_contiguous() and table.get_device() == dev
+            and offsets.dtype is i32 and offsets.shape == (B,) and offsets.is_contiguous() and offsets.get_device() == dev
+            and qkv.dtype is bf and qkv.shape == (n, F * D) and qkv.is_contiguous() and qkv.get_device() == dev
+            and q_out.dtype is bf and q_out.shape == (n, n_heads, D) and q_out.is_contiguous() and q_out.get_device() == dev
+            and (q_norm_w is None or (q_norm_w.dtype is bf and q_norm_w.shape == (D,) and q_norm_w.is_contiguous()
+                                      and q_norm_w.get_device() == dev))
+            and (k_norm_w is None or (k_norm_w.dtype is bf and k_norm_w.shape == (D,) and k_norm_w.is_contiguous()
+                                      and k_norm_w.get_device() == dev))
+            and (q_starts is None or (q_starts.dtype is i32 and q_starts.shape == (B + 1,) and q_starts.is_contiguous()
+                                      and q_starts.get_device() == dev))
+            and (prefix_len is None or (prefix_len.dtype is i32 and prefix_len.shape == (1,)
+                                        and prefix_len.get_device() == dev))):
+        _refuse(op, dev, ("table", table, i32, (B, cols)), ("offsets", offsets, i32, (B,)),
+                ("qkv", qkv, bf, (n, F * D)), ("q_out", q_out, bf, (n, n_heads, D)), ("q_norm_w", q_norm_w, bf, (D,)),
+                ("k_norm_w", k_norm_w, bf, (D,)), ("q_starts", q_starts, i32, (B + 1,)),
+                ("prefix_len", prefix_len, i32, (1,)))
+    args = (torch._C._cuda_getCurrentRawStream(dev) if stream is None and dev >= 0 else _stream(stream), qkv.data_ptr(),
+            _ptr(q_norm_w), _ptr(k_norm_w), eps, theta, _ptr(q_starts), offsets.data_ptr(), _ptr(prefix_len), B, n,
+            n_heads, flags, q_out.data_ptr(), cache.desc_ref, table.data_ptr(), cols)
+    call = lib().ema_paged_append
+    rc = call(*args) if torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, *args)
+    if rc:
+        _check(rc, op)
     return q_out
 
 
@@ -617,22 +620,52 @@ def paged_workspace(batch, n_rows, n_heads, n_kv_heads, head_dim, max_q, max_len
     return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
-def _paged_out(op, q, cache, out):
+def _paged_args(op, q, cache, table, lengths, q_starts, max_q, max_len, scale, out, workspace, stream, max_prefix=0,
+                prefix_table=None, prefix_len=None):
+    """Checks the tensors of an attention call (see paged_append) and returns (stream, B, n, Hq, cols,
+    max_q, scale, out, workspace)."""
     import torch
 
-    bf, dev, D = torch.bfloat16, cache.device_index, cache.desc.head_dim
-    n, Hq = q.shape[:2] if q.dim() == 3 else (None, None)
-    _want(op, "q", q, bf, (n, Hq, D), dev)
-    if out is None:
-        return torch.empty((n, Hq * D), dtype=bf, device=q.device)
-    _want(op, "out", out, bf, (n, Hq * D), dev)
-    return out
-
-
-def _rows_bound(op, q, B, q_starts, max_q):
+    bf, i32, dev = torch.bfloat16, torch.int32, cache.device_index
+    D = cache.desc.head_dim
+    B, cols = table.shape if table.dim() == 2 else (-1, -1)
+    n, Hq = q.shape[:2] if q.dim() == 3 else (-1, -1)
     if q_starts is None:
-        return -(-q.shape[0] // B) if B else 0
-    return q.shape[0] if max_q is None else max_q
+        max_q = -(-n // B) if B > 0 else 0
+    elif max_q is None:
+        max_q = n
+    if out is None and n >= 0:
+        out = torch.empty((n, Hq * D), dtype=bf, device=q.device)
+    if not (table.dtype is i32 and table.is_contiguous() and table.get_device() == dev
+            and lengths.dtype is i32 and lengths.shape == (B,) and lengths.is_contiguous() and lengths.get_device() == dev
+            and q.dtype is bf and q.shape == (n, Hq, D) and q.is_contiguous() and q.get_device() == dev
+            and out.dtype is bf and out.shape == (n, Hq * D) and out.is_contiguous() and out.get_device() == dev
+            and (q_starts is None or (q_starts.dtype is i32 and q_starts.shape == (B + 1,) and q_starts.is_contiguous()
+                                      and q_starts.get_device() == dev))
+            and (workspace is None or (workspace.dtype is torch.uint8 and workspace.is_contiguous()
+                                       and workspace.get_device() == dev))
+            and (prefix_table is None or (prefix_table.dtype is i32 and prefix_table.dim() == 1
+                                          and prefix_table.is_contiguous() and prefix_table.get_device() == dev
+                                          and prefix_len.dtype is i32 and prefix_len.shape == (1,)
+                                          and prefix_len.get_device() == dev))):
+        _refuse(op, dev, ("table", table, i32, (B, cols)), ("lengths", lengths, i32, (B,)), ("q", q, bf, (n, Hq, D)),
+                ("out", out, bf, (n, Hq * D)), ("q_starts", q_starts, i32, (B + 1,)),
+                ("workspace", workspace, torch.uint8, workspace.shape if workspace is not None else ()),
+                ("prefix_table", prefix_table, i32, (prefix_table.numel(),) if prefix_table is not None else ()),
+                ("prefix_len", prefix_len, i32, (1,)))
+    if workspace is None:
+        workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, max_prefix, device=q.device)
+    raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None and dev >= 0 else _stream(stream)
+    return raw, B, n, Hq, cols, max_q, 1.0 / math.sqrt(D) if scale is None else scale, out, workspace
+
+
+def _paged_call(op: str, cache, call, *args) -> None:
+    import torch
+
+    dev = cache.device_index
+    rc = call(*args) if torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, *args)
+    if rc:
+        _check(rc, op)
 
 
 def paged_attention(q, cache: PagedCache, table, lengths, max_len, q_starts=None, max_q=None, causal=True, scale=None,
@@ -640,22 +673,12 @@ def paged_attention(q, cache: PagedCache, table, lengths, max_len, q_starts=None
     """Attention of a ragged batch over its pages (ema_paged_attention): q [n, Hq, D] bf16, lengths
     int32 [B] (positions held, the call's rows included), table int32 [B, cols]; max_len and
     max_q are host bounds of the lengths and of a sequence's rows. Returns out [n, Hq * D]."""
-    import torch
-
     op = "ema_paged_attention"
-    dev = cache.device_index
-    B, cols = _paged_batch(op, cache, table, q_starts, lengths, "lengths", dev)
-    out = _paged_out(op, q, cache, out)
-    n, Hq, D = q.shape
-    max_q = _rows_bound(op, q, B, q_starts, max_q)
-    if workspace is None:
-        workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, device=q.device)
-    else:
-        _want(op, "workspace", workspace, torch.uint8, (workspace.numel(),), dev)
-    _check(_launch(dev, stream, lib().ema_paged_attention, q.data_ptr(), cache.desc_ref, table.data_ptr(), cols,
-                   _ptr(q_starts), lengths.data_ptr(), B, n, max_q, max_len, Hq,
-                   1.0 / math.sqrt(D) if scale is None else scale, EMA_PREFILL_CAUSAL if causal else 0,
-                   out.data_ptr(), workspace.data_ptr(), workspace.numel()), op)
+    raw, B, n, Hq, cols, max_q, scale, out, workspace = _paged_args(op, q, cache, table, lengths, q_starts, max_q,
+                                                                    max_len, scale, out, workspace, stream)
+    _paged_call(op, cache, lib().ema_paged_attention, raw, q.data_ptr(), cache.desc_ref, table.data_ptr(), cols,
+                _ptr(q_starts), lengths.data_ptr(), B, n, max_q, max_len, Hq, scale, EMA_PREFILL_CAUSAL if causal else 0,
+                out.data_ptr(), workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -665,23 +688,12 @@ def prefix_attention(q, cache: PagedCache, prefix_table, prefix_len, max_prefix,
     (ema_prefix_attention): prefix_table int32 [cols], prefix_len int32 [1] (its positions,
     max_prefix a host bound); table and lengths are of the sequences' own positions, the rest as
     in paged_attention. The prefix is read once for the batch. Returns out [n, Hq * D]."""
-    import torch
-
     op = "ema_prefix_attention"
-    dev = cache.device_index
-    B, cols = _paged_batch(op, cache, table, q_starts, lengths, "lengths", dev)
-    pcols = prefix_table.numel()
-    _want(op, "prefix_table", prefix_table, torch.int32, (pcols,), dev)
-    _want(op, "prefix_len", prefix_len, torch.int32, (1,), dev)
-    out = _paged_out(op, q, cache, out)
-    n, Hq, D = q.shape
-    max_q = _rows_bound(op, q, B, q_starts, max_q)
-    if workspace is None:
-        workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, max_prefix, device=q.device)
-    else:
-        _want(op, "workspace", workspace, torch.uint8, (workspace.numel(),), dev)
-    _check(_launch(dev, stream, lib().ema_prefix_attention, q.data_ptr(), cache.desc_ref, prefix_table.data_ptr(),
-                   pcols, prefix_len.data_ptr(), max_prefix, table.data_ptr(), cols, _ptr(q_starts),
-                   lengths.data_ptr(), B, n, max_q, max_len, Hq, 1.0 / math.sqrt(D) if scale is None else scale,
-                   out.data_ptr(), workspace.data_ptr(), workspace.numel()), op)
+    raw, B, n, Hq, cols, max_q, scale, out, workspace = _paged_args(op, q, cache, table, lengths, q_starts, max_q,
+                                                                    max_len, scale, out, workspace, stream, max_prefix,
+                                                                    prefix_table, prefix_len)
+    _paged_call(op, cache, lib().ema_prefix_attention, raw, q.data_ptr(), cache.desc_ref, prefix_table.data_ptr(),
+                prefix_table.numel(), prefix_len.data_ptr(), max_prefix, table.data_ptr(), cols, _ptr(q_starts),
+                lengths.data_ptr(), B, n, max_q, max_len, Hq, scale, out.data_ptr(), workspace.data_ptr(),
+                workspace.numel())
     return out
