@@ -276,6 +276,20 @@ __device__ __forceinline__ float2 get2(const float* p) {
   return make_float2(__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32)));
 }
 
+// The kernel's arguments, read again from where they came: through a pointer that the compiler
+// cannot see into, so that what a piece needs before or after its tiles is not held in scalar
+// registers over them (with every argument live the kernels spilled 55 to 79 of them to vector
+// lanes and reloaded some in each tile).
+__device__ __forceinline__ PagedArgs args_again() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  auto p = (const __attribute__((address_space(4))) PagedArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+#else
+  return {};
+#endif
+}
+
 struct State4 {  // four dims of a row: running max, row sum, unnormalised output
   float m, l;
   f32x4 o;
@@ -446,6 +460,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
   for (int dt = 0; dt < 4; ++dt) v_col[dt] = tr_row * kD + 16 * (grp & 1) + 4 * (s16 & 3) + 32 * (dt ^ (s16 >> 2));
 
   while (t < t_end) {
+    const PagedArgs a = args_again();
     // the segment of unit t: the last b whose units begin at or before it
     const uint64_t le = __ballot(lane * step < a.B && lane_pre <= t);
     const int at = 63 - __builtin_clzll(le);
@@ -663,6 +678,8 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       }
     }
+    // (from here on, arguments read again)
+    const PagedArgs z = args_again();
     // the waves' states meet: o of wave w in its own slots, [row][d / 4] with unit d4 of row r
     // at d4 ^ r
     f32x4* const os = (f32x4*)Kt;
@@ -690,10 +707,10 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         s.o += ((const f32x4*)slots[v])[r * 32 + (d4 ^ r)] * f;
       }
       if (w0 == w1) {
-        const int ir = row0 + r, tk = paged_div(ir, a.magic);
-        finish4(a, n_carry, shared_keys || !a.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk, kh * a.G + ir - tk * a.G, 4 * d4, s);
+        const int ir = row0 + r, tk = paged_div(ir, z.magic);
+        finish4(z, n_carry, shared_keys || !z.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk, kh * z.G + ir - tk * z.G, 4 * d4, s);
       } else {
-        float* const p = a.part + ((int64_t)paged_slot(w, w0) * kPagedRows + r) * kPagedState;
+        float* const p = z.part + ((int64_t)paged_slot(w, w0) * kPagedRows + r) * kPagedState;
         if (d4 == 0) put2(p, s.m, s.l);
         put2(p + 4 + 4 * d4, s.o[0], s.o[1]);
         put2(p + 6 + 4 * d4, s.o[2], s.o[3]);
@@ -708,9 +725,9 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       if (tid == 0) {
         int i = w0;
         asm volatile("" : "+v"(i));
-        const int old = __hip_atomic_fetch_add(a.cnt + i, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int old = __hip_atomic_fetch_add(z.cnt + i, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const int last = old == w1 - w0;
-        if (last) __hip_atomic_store(a.cnt + i, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (last) __hip_atomic_store(z.cnt + i, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         arrived = last;
       }
       __syncthreads();
@@ -725,7 +742,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
               for (int i = 0; i < kChunk; ++i) {
                 const int ww = c0 + i <= w1 ? c0 + i : w1;
-                const float* const p = a.part + ((int64_t)paged_slot(ww, w0) * kPagedRows + r) * kPagedState;
+                const float* const p = z.part + ((int64_t)paged_slot(ww, w0) * kPagedRows + r) * kPagedState;
                 pm[i] = get2(p);
                 pa[i] = get2(p + 4 + 4 * d4);
                 pb[i] = get2(p + 6 + 4 * d4);
@@ -745,9 +762,9 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
                 }
               s.m = M;
             }
-            const int ir = row0 + r, tk = paged_div(ir, a.magic);
-            finish4(a, n_carry, shared_keys || !a.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk,
-                    kh * a.G + ir - tk * a.G, 4 * d4, s);
+            const int ir = row0 + r, tk = paged_div(ir, z.magic);
+            finish4(z, n_carry, shared_keys || !z.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk,
+                    kh * z.G + ir - tk * z.G, 4 * d4, s);
           }
         };
         if (w1 - w0 < 3) join(std::integral_constant<int, 3>{});
