@@ -233,8 +233,8 @@ struct PagedArgs {
   int prefix_cols;
   int carry_blocks;       // 64-key blocks of a chunk of the prefix (0: one state, always there)
   int prefix_cap;         // positions that the prefix's table holds
-  int64_t sb, sh;   // bytes
-  uint32_t row_bytes;
+  int64_t sh;       // bytes
+  uint32_t page_bytes, row_bytes;
   uint32_t magic;   // paged_magic(G)
   float qk_scale;   // scale * log2(e): scores live in the log2 domain
   int B, T, n_rows, Hq, Hkv, G, cols, shift, n_pages, W, causal;
@@ -505,23 +505,36 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       const int cols = is_own(tile) ? a.cols : a.prefix_cols;
       return ld_uniform(is_own(tile) ? own_table : a.prefix_table, c < cols ? c : cols - 1);
     };
-    // 16 rows of a page: where they begin and how many of them are held (0: none are read)
-    auto valid_rows = [&](int tile, int half, int page) __attribute__((always_inline)) {
-      const int left = (is_own(tile) ? L : prefix) - place(tile) * kPagedTile - 16 * half;
-      const int n = left < 0 ? 0 : (left > 16 ? 16 : left);
-      return tile < tile1 && (uint32_t)page < (uint32_t)a.n_pages ? n : 0;
+    // The two 16-row halves of a tile: where their rows begin, in bytes from the kv head's first
+    // row in either pool, and how many are held (none past the piece, past the keys or on an entry
+    // outside the pool)
+    struct Halves {
+      int64_t at[2];
+      uint32_t n[2];
     };
-    auto half_base = [&](const uint8_t* pool, int tile, int half, int page) __attribute__((always_inline)) {
-      const uint32_t slot = ((uint32_t)place(tile) * kPagedTile + 16u * half) & ((1u << a.shift) - 1u);
-      return pool + ((uint32_t)page < (uint32_t)a.n_pages ? (int64_t)page * a.sb : 0) + (int64_t)kh * a.sh +
-             (int64_t)slot * a.row_bytes;
-    };
-    // bf16: a tile by eight loads of four whole rows each, straight into the slot
-    auto dma_tile = [&](bool k, int tile, int e0, int e1) __attribute__((always_inline)) {
+    const uint8_t* const kb = a.k + (int64_t)kh * a.sh;
+    const uint8_t* const vb = a.v + (int64_t)kh * a.sh;
+    auto halves = [&](int tile, int e0, int e1) __attribute__((always_inline)) {
+      Halves r;
+      const int left = (is_own(tile) ? L : prefix) - place(tile) * kPagedTile;
+      const uint32_t slot = ((uint32_t)place(tile) * kPagedTile) & ((1u << a.shift) - 1u);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int e = half ? e1 : e0;
-        const u32x4 r = rsrc_words(half_base(k ? a.k : a.v, tile, half, e), (uint32_t)valid_rows(tile, half, e) * a.row_bytes);
+        const uint32_t page = (uint32_t)(half ? e1 : e0);
+        const bool in = tile < tile1 && page < (uint32_t)a.n_pages;
+        const int n = left - 16 * half;
+        r.n[half] = in && n > 0 ? (uint32_t)(n < 16 ? n : 16) : 0u;
+        // (a 16-position page begins anew with the second half)
+        const uint32_t row = half ? (slot + 16u) & ((1u << a.shift) - 1u) : slot;
+        r.at[half] = (int64_t)((uint64_t)(in ? page : 0u) * a.page_bytes + (uint64_t)row * a.row_bytes);
+      }
+      return r;
+    };
+    // bf16: a tile by eight loads of four whole rows each, straight into the slot
+    auto dma_tile = [&](bool k, const Halves& hv) __attribute__((always_inline)) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const u32x4 r = rsrc_words((k ? kb : vb) + hv.at[half], hv.n[half] * a.row_bytes);
         const uint32_t dst = (k ? kdst : vdst) + 4096 * half;
         dma16<true, kOnce>(r, k ? koff[0] : voff[0], dst);
 #pragma unroll
@@ -534,20 +547,18 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       u32x4 w[4];
       int e[4];
     };
-    auto load_codes = [&](bool k, int tile, int e0, int e1) __attribute__((always_inline)) {
+    auto load_codes = [&](bool k, int tile, const Halves& hv, int e0, int e1) __attribute__((always_inline)) {
       Codes c;
+      const uint32_t slot = ((uint32_t)place(tile) * kPagedTile) & ((1u << a.shift) - 1u);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int page = half ? e1 : e0;
-        const int n = valid_rows(tile, half, page);
-        const uint8_t* const base = half_base(k ? a.k : a.v, tile, half, page);
-        const uint32_t slot = ((uint32_t)place(tile) * kPagedTile + 16u * half) & ((1u << a.shift) - 1u);
+        const uint32_t n = hv.n[half], at = half ? (slot + 16u) & ((1u << a.shift) - 1u) : slot;
         const uint16_t* const eb = (k ? a.kexp : a.vexp) +
-            (n ? (((int64_t)page * a.Hkv + kh) << a.shift) + slot : 0);
-        const __amdgpu_buffer_rsrc_t r =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), (short)0, (int)((uint32_t)n * a.row_bytes), 0x00020000);
+            (n ? (((int64_t)(half ? e1 : e0) * a.Hkv + kh) << a.shift) + at : 0);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>((k ? kb : vb) + hv.at[half]), (short)0, (int)(n * a.row_bytes), 0x00020000);
         const __amdgpu_buffer_rsrc_t re =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(eb), (short)0, 2 * n, 0x00020000);
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(eb), (short)0, (int)(2 * n), 0x00020000);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t row = 8 * i + (lane >> 3);
@@ -577,13 +588,14 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
 #pragma unroll
       for (int s = 0; s < 8; ++s) qop[s] = as_bf16x8(qp[2 * s]);
     }
+    Halves hv = halves(first, e0, e1);
     Codes kc, vc;
     if constexpr (kFp8) {
-      kc = load_codes(true, first, e0, e1);
-      vc = load_codes(false, first, e0, e1);
+      kc = load_codes(true, first, hv, e0, e1);
+      vc = load_codes(false, first, hv, e0, e1);
     } else if (first < tile1) {
-      dma_tile(true, first, e0, e1);
-      dma_tile(false, first, e0, e1);
+      dma_tile(true, hv);
+      dma_tile(false, hv);
     }
 
     float m = -INFINITY, l = 0.f;  // of the lane's row; l over this lane's half of the keys
@@ -598,7 +610,8 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       e1 = entry(tile + kPagedWaves, 1);
       if constexpr (kFp8) {
         decode_codes(true, kc);
-        kc = load_codes(true, tile + kPagedWaves, e0, e1);
+        hv = halves(tile + kPagedWaves, e0, e1);
+        kc = load_codes(true, tile + kPagedWaves, hv, e0, e1);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -617,7 +630,8 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       const bool more = tile + kPagedWaves < tile1;
       if (!kFp8 && more) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
-        dma_tile(true, tile + kPagedWaves, e0, e1);
+        hv = halves(tile + kPagedWaves, e0, e1);
+        dma_tile(true, hv);
       }
       // key of score i: 32 place + (i % 4) + 8 (i / 4) + 4 hh
       const int key0 = place(tile) * kPagedTile;
@@ -650,7 +664,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         }
       if constexpr (kFp8) {
         decode_codes(false, vc);
-        vc = load_codes(false, tile + kPagedWaves, e0, e1);
+        vc = load_codes(false, tile + kPagedWaves, hv, e0, e1);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -671,7 +685,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
         }
       if constexpr (!kFp8) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (more) dma_tile(false, tile + kPagedWaves, e0, e1);
+        if (more) dma_tile(false, hv);
       } else {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -892,8 +906,8 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
   a.prefix_cols = p.prefix_cols;
   a.carry_blocks = 0;
   a.prefix_cap = p.prefix_cols << paged_shift(c.capacity);
-  a.sb = c.stride_batch * es;
   a.sh = c.stride_head * es;
+  a.page_bytes = (uint32_t)(c.stride_batch * es);
   a.row_bytes = (uint32_t)(c.stride_pos * es);
   a.qk_scale = p.scale * kLog2e;
   a.B = p.batch;
