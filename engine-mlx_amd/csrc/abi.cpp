@@ -6,6 +6,7 @@
 // is kept in a thread-local string readable through ema_last_error().
 // Validation runs on the host before any HIP call, so every argument error is
 // reported without touching the GPU.
+#include <cfloat>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -685,8 +686,8 @@ static int32_t check_pages(const char* op, const ema_kvcache_desc* c) {
 static int32_t check_page_table(const char* op, const ema_kvcache_desc* c, const int32_t* table, int32_t cols) {
   if (!table) return set_error(EMA_ERR_INVALID_ARG, "%s: null page table", op);
   if (cols <= 0) return set_error(EMA_ERR_SHAPE, "%s: a page table row of %d entries", op, cols);
-  if ((int64_t)cols * c->capacity > INT32_MAX)
-    return set_error(EMA_ERR_UNSUPPORTED, "%s: %d pages of %d positions exceed 2^31 - 1 positions", op, cols, c->capacity);
+  if ((int64_t)cols * c->capacity > ((int64_t)1 << 30))
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %d pages of %d positions exceed 2^30 positions", op, cols, c->capacity);
   return EMA_OK;
 }
 
@@ -710,7 +711,8 @@ extern "C" int32_t ema_paged_append(ema_stream_t stream, const void* qkv, const 
   int32_t rc = check_pages(op, pages);
   if (rc) return rc;
   if ((rc = check_page_table(op, pages, table, table_cols))) return rc;
-  if (!qkv || !q_out || !offsets) return set_error(EMA_ERR_INVALID_ARG, "%s: null qkv/q_out/offsets", op);
+  if (n_rows != 0 && (!qkv || !q_out)) return set_error(EMA_ERR_INVALID_ARG, "%s: null qkv/q_out", op);
+  if (!offsets) return set_error(EMA_ERR_INVALID_ARG, "%s: null offsets", op);
   if (flags & ~(EMA_PRE_NO_NORM | EMA_PRE_NO_ROPE | EMA_PRE_NO_Q_NORM | EMA_PRE_NO_K_NORM))
     return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
   if ((rc = check_norm_weights(op, q_norm_w, k_norm_w, flags))) return rc;
@@ -718,7 +720,8 @@ extern "C" int32_t ema_paged_append(ema_stream_t stream, const void* qkv, const 
   if ((rc = check_paged_rows(op, batch, n_rows, n_heads, !q_starts))) return rc;
   if (pages->head_dim != 64 && pages->head_dim != 128 && pages->head_dim != 256)
     return set_error(EMA_ERR_UNSUPPORTED, "%s: head_dim %d not supported (64/128/256)", op, pages->head_dim);
-  if (!(eps >= 0.f) || !(theta > 0.f)) return set_error(EMA_ERR_INVALID_ARG, "%s: eps must be >= 0 and theta > 0", op);
+  if (!(eps >= 0.f) || !(theta > 0.f && theta <= FLT_MAX))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: eps must be >= 0, theta > 0 and finite", op);
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(q_norm_w) || !aligned16(k_norm_w))
     return set_error(EMA_ERR_INVALID_ARG, "%s: qkv, q_out and the norm weights must be 16-byte aligned", op);
   if (n_rows == 0) return EMA_OK;
@@ -747,7 +750,8 @@ static int32_t paged_attention(const char* op, ema_stream_t stream, PagedAttenti
                                uint64_t workspace_bytes) {
   int32_t rc = check_page_table(op, pages, p.table, p.table_cols);
   if (rc) return rc;
-  if (!p.q || !p.out || !p.lengths) return set_error(EMA_ERR_INVALID_ARG, "%s: null q/out/lengths", op);
+  if (p.n_rows != 0 && (!p.q || !p.out)) return set_error(EMA_ERR_INVALID_ARG, "%s: null q/out", op);
+  if (!p.lengths) return set_error(EMA_ERR_INVALID_ARG, "%s: null lengths", op);
   if ((rc = check_heads(op, p.n_heads, pages->n_kv_heads))) return rc;
   if ((rc = check_paged_rows(op, p.batch, p.n_rows, p.n_heads, !p.q_starts))) return rc;
   if (pages->head_dim != 128)
@@ -793,7 +797,7 @@ extern "C" int32_t ema_paged_attention(ema_stream_t stream, const void* q, const
   if (rc) return rc;
   if (flags & ~EMA_PREFILL_CAUSAL) return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
   const PagedAttention p{q,          table, nullptr, nullptr, q_starts, lengths,
-                         table_cols, 0,     batch,   n_rows,  n_heads,  max_q, (int)(flags & EMA_PREFILL_CAUSAL), scale, out};
+                         table_cols, 0,     0,       batch,   n_rows,   n_heads, max_q, (int)(flags & EMA_PREFILL_CAUSAL), scale, out};
   return paged_attention(op, stream, p, max_len, 0, pages, workspace, workspace_bytes);
 }
 
@@ -812,7 +816,7 @@ extern "C" int32_t ema_prefix_attention(ema_stream_t stream, const void* q, cons
     return set_error(EMA_ERR_CAPACITY, "%s: max_prefix %d outside [1, %lld], what %d pages hold", op, max_prefix,
                      (long long)prefix_cols * pages->capacity, prefix_cols);
   const PagedAttention p{q,          table,       prefix_table, prefix_len, q_starts, lengths,
-                         table_cols, prefix_cols, batch,        n_rows,     n_heads,  max_q, 1, scale, out};
+                         table_cols, prefix_cols, max_prefix,   batch,      n_rows,   n_heads, max_q, 1, scale, out};
   return paged_attention(op, stream, p, max_len, max_prefix, pages, workspace, workspace_bytes);
 }
 

@@ -246,7 +246,7 @@ struct PagedAttention {
   const int32_t* prefix_len;
   const int32_t* q_starts;
   const int32_t* lengths;
-  int table_cols, prefix_cols, batch, n_rows, n_heads, max_q, causal;
+  int table_cols, prefix_cols, max_prefix, batch, n_rows, n_heads, max_q, causal;
   float scale;
   void* out;
 };

@@ -232,12 +232,13 @@ struct PagedArgs {
   const int32_t* prefix_table;    // its pages, where the segments take them themselves (else null)
   int prefix_cols;
   int carry_blocks;       // 64-key blocks of a chunk of the prefix (0: one state, always there)
-  int prefix_cap;         // positions that the prefix's table holds
+  int prefix_cap;         // most positions of the prefix (the call's bound)
   int64_t sh;       // bytes
   uint32_t page_bytes, row_bytes;
   uint32_t magic;   // paged_magic(G)
   float qk_scale;   // scale * log2(e): scores live in the log2 domain
   int B, T, n_rows, Hq, Hkv, G, cols, shift, n_pages, W, causal;
+  int cap;          // most positions of a sequence: what its table row holds
   int few, max_q;   // sequences of few < n <= max_q rows are prefill_kernel's
 };
 
@@ -348,8 +349,7 @@ __device__ __forceinline__ PagedRows rows_of(const PagedArgs& a, int b) {
   return own_rows(a, paged_rows(ld_uniform(a.starts, b), ld_uniform(a.starts, b + 1), a.n_rows));
 }
 __device__ __forceinline__ int clamp_len(const PagedArgs& a, int L) {
-  const int64_t cap = (int64_t)a.cols << a.shift;
-  return L < 0 ? 0 : (L > cap ? (int)cap : L);
+  return L < 0 ? 0 : (L > a.cap ? a.cap : L);
 }
 __device__ __forceinline__ int blocks_of(const PagedArgs& a, int T) {
   return (int)(((uint32_t)T * (uint32_t)a.G + kPagedRows - 1) / kPagedRows);
@@ -482,6 +482,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     const uint32_t seg = (uint32_t)(t - pre_b) / (uint32_t)nu;
     const int unit0 = (int)((uint32_t)(t - pre_b) - seg * (uint32_t)nu);
     const int kh = nrb == 1 ? (int)seg : (int)(seg / (uint32_t)nrb), rb = (int)(seg - (uint32_t)kh * (uint32_t)nrb);
+    if (kh >= a.Hkv) break;  // (row starts that do not ascend can overflow the count of units)
     const int seg_begin = t - unit0, seg_end = seg_begin + nu;
     const int piece_end = t_end < seg_end ? t_end : seg_end;
     const int tile0 = unit0 * unit * kPagedWaves;
@@ -905,7 +906,7 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
   a.prefix_table = nullptr;
   a.prefix_cols = p.prefix_cols;
   a.carry_blocks = 0;
-  a.prefix_cap = p.prefix_cols << paged_shift(c.capacity);
+  a.prefix_cap = p.max_prefix;
   a.sh = c.stride_head * es;
   a.page_bytes = (uint32_t)(c.stride_batch * es);
   a.row_bytes = (uint32_t)(c.stride_pos * es);
@@ -921,6 +922,7 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
   a.shift = paged_shift(c.capacity);
   a.n_pages = c.batch;
   a.causal = p.causal;
+  a.cap = p.table_cols << a.shift;  // (at most 2^30: host)
   a.few = INT32_MAX;
   a.max_q = 0;
   if (p.prefix_table && plan.direct) {
@@ -935,6 +937,7 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
       PagedArgs x = a;  // all rows of the batch as one sequence over the shared pages
       x.table = p.prefix_table;
       x.cols = p.prefix_cols;
+      x.cap = p.max_prefix;
       x.len = p.prefix_len;
       x.prefix_len = nullptr;
       x.starts = nullptr;

@@ -80,6 +80,7 @@ struct PagedPrefillArgs : PrefillArgs {
   float* part;  // kSharedPages: the rows' states [chunk][n_rows, Hq][kPagedState]
   uint32_t page_bytes, head_bytes;  // (page_bytes below 2^32: host)
   int n_rows, cols, shift, n_pages;
+  int cap;              // most positions of a sequence, or of the prefix
   uint32_t magic;       // paged_magic(G)
   int few, max_q;       // kPages: sequences of few < n <= max_q rows are this kernel's
   int chunk_blocks;     // kSharedPages: 64-key blocks per chunk of the keys
@@ -222,8 +223,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
     chunk = rest / a.Hkv;
     prow.n = a.starts ? paged_rows(0, ld_uniform(a.starts, a.B), a.n_rows).n : a.n_rows;
     // paged_kernel reads the states of the chunks that hold keys (and no load is in flight yet)
-    const int64_t keys = min((int64_t)ld_uniform(a.len, 0), (int64_t)a.cols << a.shift);
-    if ((int64_t)chunk * a.chunk_blocks * kBN >= keys) return;
+    if ((int64_t)chunk * a.chunk_blocks * kBN >= min(ld_uniform(a.len, 0), a.cap)) return;
   } else if constexpr (kMode == kPages) {
     if (a.starts) {
       item.kh = item.h = (int)(blockIdx.x % (uint32_t)a.Hkv);
@@ -298,8 +298,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
   int q_off = q_off_arg < 0 ? 0 : q_off_arg;
   int kv_held = 0;  // kPaged: keys of the sequence
   if constexpr (kPaged) {
-    const int64_t cap = (int64_t)a.cols << a.shift;
-    kv_held = q_off > cap ? (int)cap : q_off;
+    kv_held = q_off > a.cap ? a.cap : q_off;
     q_off = kv_held - prow.n;  // (negative: the first rows see nothing)
   }
   int key_base = 0;  // absolute position of key index 0 (rotating cache; n_tokens <= cap)
@@ -1317,6 +1316,7 @@ PagedPrefillArgs paged_prefill_args(const PagedAttention& p, const ema_kvcache_d
   a.cols = p.table_cols;
   a.shift = paged_shift(c.capacity);
   a.n_pages = c.batch;
+  a.cap = p.table_cols << a.shift;  // (at most 2^30: host)
   a.magic = paged_magic(a.G);
   a.few = 0;
   a.max_q = p.max_q;
@@ -1361,6 +1361,7 @@ int32_t launch_prefix_rows(hipStream_t s, const PagedAttention& p, const ema_kvc
   PagedPrefillArgs a = paged_prefill_args(p, c);
   a.table = p.prefix_table;
   a.cols = p.prefix_cols;
+  a.cap = p.max_prefix;
   a.len = p.prefix_len;
   a.part = part;
   a.chunk_blocks = chunk_blocks;

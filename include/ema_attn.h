@@ -393,8 +393,9 @@ EMA_API int32_t ema_prefill_attention_ws(ema_stream_t stream, const void* q, con
  *   q_starts    device int32 [batch + 1], ascending: sequence b's rows of the packed tensors
  *               are [q_starts[b], q_starts[b + 1]); rows from q_starts[batch] on are neither
  *               read nor written. NULL: n_rows / batch rows for every sequence.
- * At most 1024 sequences a call; n_rows * n_heads at most 2^23 - 1; table_cols * capacity below
- * 2^31. The reference has no paged cache; the calls are the paged forms of ema_pre_attention,
+ * At most 1024 sequences a call; n_rows * n_heads at most 2^23 - 1; table_cols * capacity at
+ * most 2^30; at most 256 query heads per kv head in attention. A call of no rows does nothing.
+ * The reference has no paged cache; the calls are the paged forms of ema_pre_attention,
  * ema_decode_attention and ema_prefill_attention. */
 
 /* Norm, rotation and append for a ragged batch: ema_pre_attention over pages.
@@ -445,8 +446,8 @@ EMA_API int32_t ema_paged_attention(ema_stream_t stream, const void* q, const em
  * same pool: every row sees all prefix positions, then causally its sequence's own. The prefix
  * is read once for the whole batch.
  *   prefix_table  device int32 [prefix_cols]: the prefix's pages
- *   prefix_len    device int32 [1]: its positions, clamped to [0, prefix_cols * capacity]
- *   max_prefix    host bound of it, as max_len is of the lengths
+ *   prefix_len    device int32 [1]: its positions, clamped to [0, max_prefix]
+ *   max_prefix    host bound of it, at most prefix_cols * capacity
  *   table, lengths  of the sequences' own positions, the prefix not counted (append with the
  *            same prefix_len) */
 EMA_API int32_t ema_prefix_attention(ema_stream_t stream, const void* q, const ema_kvcache_desc* pages,

@@ -429,6 +429,54 @@ def test_prefix_shorter_than_its_bound(ema, held):
         ref.check_attention(down(out), *b.attention(), f"{held} of 9600")
 
 
+def test_prefix_longer_than_its_bound(ema):
+    """A prefix_len on the device past the call's bound counts as the bound, in every way of reading."""
+    import torch
+
+    for n, heads, bound, pages in ((4, (8, 4), 100, "bf16"), (6, (16, 8), 8000, "bf16"), (40, (8, 2), 3333, "bf16"),
+                                   (6, (16, 8), 8000, "fp8")):
+        b = ref.Batch([1] * n, [5] * n, 16, *heads, seed=bound, prefix=bound)
+        g = OnGpu(ema, b, pages)
+        g.prefix_len.fill_(bound + 3000)
+        table = torch.cat([g.prefix_table, g.prefix_table]).contiguous()  # (pages for what it claims)
+        out = ema.prefix_attention(g.q, g.cache, table, g.prefix_len, bound, g.table, g.lengths, 5)
+        torch.cuda.synchronize()
+        ref.check_attention(down(out), *b.attention(), f"bound {bound}")
+        g.prefix_len.fill_(-5)
+        out = ema.prefix_attention(g.q, g.cache, table, g.prefix_len, bound, g.table, g.lengths, 5)
+        b.prefix, b.shared = 0, [x[:0] for x in b.shared]
+        ref.check_attention(down(out), *b.attention(), "a negative length")
+
+
+def test_wide_groups(ema):
+    """More query heads per kv head than a segment or a block has rows."""
+    for heads in ((40, 1), (144, 1), (256, 1)):
+        run(ema, ref.Batch([1, 3, 2], [40, 3, 300], 16, *heads, seed=heads[0]), f"{heads[0]} heads on one")
+    run(ema, ref.Batch([1, 1], [4, 9], 16, 144, 1, seed=2, prefix=90), "144 heads over a prefix")
+
+
+def test_no_rows(ema):
+    """Empty batches do nothing, whatever the addresses of empty tensors are."""
+    import torch
+
+    b = ref.Batch([1, 1], [5, 9], 16, 8, 2, seed=1)
+    g = OnGpu(ema, b)
+    zero = torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = torch.empty(0, 8, 128, dtype=torch.bfloat16, device="cuda")
+    assert ema.paged_attention(q, g.cache, g.table, g.lengths, 9, q_starts=zero).shape == (0, 1024)
+    qkv, w = torch.empty(0, 12 * 128, dtype=torch.bfloat16, device="cuda"), torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    before = g.cache.k.clone()
+    assert ema.paged_append(qkv, w, w, 1e-6, 1e6, g.lengths, 8, g.cache, g.table, q_starts=zero).shape == (0, 8, 128)
+    torch.cuda.synchronize()
+    assert torch.equal(before.view(torch.int16), g.cache.k.view(torch.int16))
+    # rows, but no sequence has any of them
+    q = torch.randn(4, 8, 128, device="cuda").to(torch.bfloat16)
+    out = torch.full((4, 1024), 7.0, dtype=torch.bfloat16, device="cuda")
+    ema.paged_attention(q, g.cache, g.table, g.lengths, 9, q_starts=zero, max_q=1, out=out)
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+
+
 def test_prefix_fp8(ema):
     run(ema, ref.Batch([1] * 6, [1, 2, 3, 17, 33, 64], 16, 16, 4, seed=3, prefix=333), "fp8 prefix", pages="fp8")
 

@@ -96,13 +96,15 @@ def test_appends_that_are_refused(ema):
     assert append(ema, d, starts=None) == ema.EMA_ERR_SHAPE and "q_starts" in ema.last_error()  # 5 rows of 2 sequences
     assert append(ema, d, batch=1025) == ema.EMA_ERR_UNSUPPORTED
     assert append(ema, d, rows=1 << 20) == ema.EMA_ERR_SHAPE
-    assert append(ema, d, cols=1 << 27) == ema.EMA_ERR_UNSUPPORTED
+    assert append(ema, d, cols=(1 << 26) + 1) == ema.EMA_ERR_UNSUPPORTED
+    assert append(ema, d, theta=float("inf")) == ema.EMA_ERR_INVALID_ARG
     assert append(ema, d, eps=-1.0) == ema.EMA_ERR_INVALID_ARG
     assert append(ema, d, theta=0.0) == ema.EMA_ERR_INVALID_ARG
     assert append(ema, d, theta=float("nan")) == ema.EMA_ERR_INVALID_ARG
     assert append(ema, pool(ema, D=96)) == ema.EMA_ERR_UNSUPPORTED
     # nothing to do: no launch
     assert append(ema, d, rows=0) == ema.EMA_OK
+    assert append(ema, d, rows=0, qkv=None, q=None) == ema.EMA_OK  # what an empty tensor's address is
     assert append(ema, d, rows=0, qw=None, flags=ema.EMA_PRE_NO_Q_NORM) == ema.EMA_OK
 
 
@@ -129,6 +131,7 @@ def test_attention_that_is_refused(ema, prefix):
     # more key tiles over all row blocks than the kernels count
     assert attend(ema, pool(ema, page=4096), prefix, cols=1 << 18, rows=1 << 18) == ema.EMA_ERR_UNSUPPORTED
     assert attend(ema, d, prefix, rows=0) == ema.EMA_OK
+    assert attend(ema, d, prefix, rows=0, q=None, out=None) == ema.EMA_OK
     if prefix:
         assert attend(ema, d, True, ptable=None) == ema.EMA_ERR_INVALID_ARG
         assert attend(ema, d, True, plen=None) == ema.EMA_ERR_INVALID_ARG
