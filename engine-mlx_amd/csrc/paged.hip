@@ -299,6 +299,7 @@ __device__ __forceinline__ float weight(float m, float M) { return m == -INFINIT
 
 // A row's final state: joined with those over the prefix's chunks, then stored as output or
 // carried on.
+template <bool kFp8>
 __device__ __forceinline__ void finish4(const PagedArgs& a, int n_carry, bool keys, int64_t row, int h, int d, State4 s) {
   const int64_t rh = row * a.Hq + h;
   if (a.carry_in) {
@@ -330,7 +331,7 @@ __device__ __forceinline__ void finish4(const PagedArgs& a, int n_carry, bool ke
       s.m = M;
     }
   }
-  if (a.carry_out) {
+  if (kFp8 && a.carry_out) {  // (bf16: prefill_kernel leaves the states)
     float* const c = a.carry_out + rh * kPagedState;
     if (d == 0) *(float2*)c = make_float2(s.m, s.l);
     *(f32x4*)(c + 4 + d) = s.o;
@@ -386,7 +387,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
     return PagedRows{b * all_rows.n, all_rows.n};
   };
   PagedRows lane_rows = {0, 0};
-  int lane_len = 0, sum1 = 0, sum_long = 0;
+  int lane_len = 0, sum1 = 0, sum_long = 0, sum_segs = 0;
   for (int i = 0; i < step; ++i) {
     const int b = lane * step + i;
     if (b < a.B) {
@@ -395,10 +396,11 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       const int nr = paged_rounds(prefix_tiles + paged_tiles(lane_len)), segs = blocks_of(a, lane_rows.n) * a.Hkv;
       sum1 += segs * paged_units(nr, 1);
       sum_long += segs * paged_units(nr, kPagedLongUnit);
+      sum_segs += nr ? segs : 0;
     }
   }
   const int pre1 = sum_up_to_lane(sum1), pre_long = sum_up_to_lane(sum_long);
-  const int unit = paged_unit(__builtin_amdgcn_readlane(pre1, 63), a.W);
+  const int unit = paged_unit(__builtin_amdgcn_readlane(pre1, 63), __builtin_amdgcn_readlane(sum_up_to_lane(sum_segs), 63), a.W);
   const int total = __builtin_amdgcn_readlane(unit == 1 ? pre1 : pre_long, 63);
   const int lane_pre = unit == 1 ? pre1 - sum1 : pre_long - sum_long;
   if (step > 1) {
@@ -426,7 +428,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       const PagedRows rw = rows_of(a, b);
       const State4 empty = {-INFINITY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
       for (int64_t e = tid; e < (int64_t)rw.n * a.Hq * 32; e += 64 * kPagedWaves)
-        finish4(a, n_carry, shared_keys, rw.begin + e / (a.Hq * 32), (int)(e / 32 % a.Hq), (int)(e % 32) * 4, empty);
+        finish4<kFp8>(a, n_carry, shared_keys, rw.begin + e / (a.Hq * 32), (int)(e / 32 % a.Hq), (int)(e % 32) * 4, empty);
     }
   }
 
@@ -723,7 +725,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
       }
       if (w0 == w1) {
         const int ir = row0 + r, tk = paged_div(ir, z.magic);
-        finish4(z, n_carry, shared_keys || !z.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk, kh * z.G + ir - tk * z.G, 4 * d4, s);
+        finish4<kFp8>(z, n_carry, shared_keys || !z.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk, kh * z.G + ir - tk * z.G, 4 * d4, s);
       } else {
         float* const p = z.part + ((int64_t)paged_slot(w, w0) * kPagedRows + r) * kPagedState;
         if (d4 == 0) put2(p, s.m, s.l);
@@ -778,12 +780,13 @@ __global__ __launch_bounds__(64 * kPagedWaves) __attribute__((amdgpu_waves_per_e
               s.m = M;
             }
             const int ir = row0 + r, tk = paged_div(ir, z.magic);
-            finish4(z, n_carry, shared_keys || !z.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk,
+            finish4<kFp8>(z, n_carry, shared_keys || !z.causal || L - rw.n + tk >= 0, (int64_t)rw.begin + tk,
                     kh * z.G + ir - tk * z.G, 4 * d4, s);
           }
         };
         if (w1 - w0 < 3) join(std::integral_constant<int, 3>{});
-        else join(std::integral_constant<int, 8>{});
+        else if (w1 - w0 < 8) join(std::integral_constant<int, 8>{});
+        else join(std::integral_constant<int, 16>{});
       }
     }
     __syncthreads();  // the slots and ml are reused by the next piece
@@ -848,11 +851,13 @@ int32_t launch_paged_append(hipStream_t s, const PagedAppend& p, const ema_kvcac
   return check_hip(hipGetLastError(), "ema_paged_append launch");
 }
 
-// More query rows than this per (sequence, kv head) run in prefill_kernel's 128-row blocks (bf16
-// pages), fewer in paged_kernel's 32-row segments.
+// More query rows than kFewRows per (sequence, kv head) run in prefill_kernel's 128-row blocks
+// (bf16 pages) where these fill a share of the chip, the others in paged_kernel's 32-row segments,
+// whose keys are split.
 constexpr int kFewRows = 128;
-// A shared prefix: more rows than this per kv head in 128-row blocks over chunks of it.
-constexpr int kFewPrefixRows = 32;
+bool paged_blocks(int64_t rows, int B, int Hkv, int cus) {
+  return rows > kFewRows && (rows + 127) / 128 * B * Hkv * 8 >= (int64_t)cus * 3;
+}
 // A shared prefix whose tiles are no more rounds than this when every segment takes them itself:
 // one launch over the prefix's and the own tiles together, K and V of the prefix from the L2s.
 constexpr int kDirectRounds = 4 * kPagedMaxWorkers;
@@ -929,7 +934,7 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
     a.prefix_table = p.prefix_table;
   } else if (p.prefix_table) {
     float* const carry = (float*)((char*)ws + kDecodeCounterBytes + plan.part_bytes);
-    if (!fp8 && (int64_t)p.n_rows * a.G > kFewPrefixRows) {
+    if (!fp8) {  // in blocks of 128 rows over chunks of the prefix
       const int32_t rc = launch_prefix_rows(s, p, c, plan.chunks, plan.chunk_blocks, carry);
       if (rc) return rc;
       a.carry_blocks = plan.chunk_blocks;
@@ -951,7 +956,7 @@ int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema
       if (rc) return rc;
     }
     a.carry_in = carry;
-  } else if (!fp8 && (int64_t)p.max_q * a.G > kFewRows) {
+  } else if (!fp8 && paged_blocks((int64_t)p.max_q * a.G, p.batch, a.Hkv, device_cus())) {
     const int few = kFewRows / a.G;
     const int32_t rc = launch_paged_prefill(s, p, c, few);
     if (rc || !p.q_starts) return rc;  // (the same rows for all: every sequence is done)

@@ -32,13 +32,16 @@ EMA_HD PagedRows paged_rows(int s0, int s1, int n_rows) {
 EMA_HD int paged_tiles(int L) { return (int)(((uint32_t)L + kPagedTile - 1) / kPagedTile); }
 EMA_HD int paged_rounds(int tiles) { return (tiles + kPagedWaves - 1) / kPagedWaves; }
 
-// Units of a segment: one round each, or kPagedLongUnit rounds where there are more rounds than
-// workgroups but no more than kPagedLongUnit for each. A piece costs a workgroup about as much as
-// three rounds before and after its tiles, so short segments (own tokens behind a prefix) are
-// better whole than in pieces of a round.
+// Units of a segment: one round each, or kPagedLongUnit rounds where the rounds are more than the
+// workgroups, or more than 16 for a segment, and no more than kPagedLongUnit for each workgroup.
+// A piece costs a workgroup about as much as three rounds before and after its tiles, and the
+// joining workgroup a load's round trip per 16 pieces, so short segments (own tokens behind a
+// prefix) are better whole and long ones better in fewer pieces than there are rounds.
 constexpr int kPagedLongUnit = 4;
 EMA_HD int paged_units(int rounds, int unit) { return (rounds + unit - 1) / unit; }
-EMA_HD int paged_unit(int rounds, int W) { return rounds > W && rounds <= kPagedLongUnit * W ? kPagedLongUnit : 1; }
+EMA_HD int paged_unit(int rounds, int segments, int W) {
+  return (rounds > W || rounds > 16 * (int64_t)segments) && rounds <= kPagedLongUnit * W ? kPagedLongUnit : 1;
+}
 
 // The units of all segments, laid end to end, cut into W slices that differ by at most one
 // unit; 32-bit arithmetic without products of the two (total < 2^31).
