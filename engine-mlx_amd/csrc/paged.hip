@@ -21,7 +21,8 @@ namespace {
 // the weight as well, as the reference's separate operators do). The angle pos * theta^(-2i/D)
 // is formed and reduced to a fraction of a turn in 64 bits: in 32 bits it is off by 0.004 at
 // position 100000, half a bf16 step of the result.
-// HBM-bound: each byte of qkv is read once, q, k and v written once.
+// HBM-bound: each byte of qkv is read once, q, k and v written once: 11435 rows of 48 heads, 281 MB,
+// in 54 us (5.2 TB/s; a large device copy 4.9). Loads past the caches gain nothing (55.5 us).
 template <int E>
 __device__ __forceinline__ void load_row(const uint16_t* p, float (&x)[E]) {
   if constexpr (E == 4) {
@@ -207,7 +208,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 //
 // Bound by HBM with few rows: at G = 4 a 16 KB tile costs a wave about 500 cycles of MFMA
 // and as many of vector work, an eighth of the time in which HBM delivers a CU's eight tiles,
-// so the 32-row product is used down to one row.
+// so the 32-row product is used down to one row. 32 heads on 8: 8 sequences of about 32k keys
+// (1031 MB) 160 us, 6.4 TB/s; 32 of up to 8k (541 MB) 90 us, FP8 (275 MB) 54; 16 heads on 8, one
+// sequence of 1k keys 7.4 us, a chain of dependent reads. K and V that are read once pass the
+// caches: 183 and 104 us without that.
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kD = 128;
@@ -852,14 +856,18 @@ int32_t launch_paged_append(hipStream_t s, const PagedAppend& p, const ema_kvcac
 }
 
 // More query rows than kFewRows per (sequence, kv head) run in prefill_kernel's 128-row blocks
-// (bf16 pages) where these fill a share of the chip, the others in paged_kernel's 32-row segments,
-// whose keys are split.
+// (bf16 pages) where these are at least 3/8 of the CUs, the others in paged_kernel's 32-row segments,
+// whose keys are split. Segments / blocks, us, 32 heads on 8: 16 sequences after 1000 keys, 128 rows
+// 24.6 / 23.8 and 192 rows 56 / 26; without history 192 rows 13.7 / 9.4; 4 sequences after 8000 keys
+// 512 rows 125 / 114 (128 workgroups of blocks), 256 rows 83 / 107 (64); one sequence, 256 rows 46 / 100.
 constexpr int kFewRows = 128;
 bool paged_blocks(int64_t rows, int B, int Hkv, int cus) {
   return rows > kFewRows && (rows + 127) / 128 * B * Hkv * 8 >= (int64_t)cus * 3;
 }
 // A shared prefix whose tiles are no more rounds than this when every segment takes them itself:
-// one launch over the prefix's and the own tiles together, K and V of the prefix from the L2s.
+// one launch over the prefix's and the own tiles together, K and V of the prefix from the L2s. Against
+// the prefix once in 128-row blocks, us, 32 heads on 8 unless named: 416 rounds 10.5 / 15.9, 832
+// 15.1 / 16.3, 1664 17.7 / 17.2, 2048 26.8 / 20.1 (16 heads on 2 17.4 / 22.7), 4032 46.5 / 27.3.
 constexpr int kDirectRounds = 4 * kPagedMaxWorkers;
 
 // Workspace: the arrival counters, the partial states of the workers' shared segments, then

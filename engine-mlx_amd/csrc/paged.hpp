@@ -36,7 +36,8 @@ EMA_HD int paged_rounds(int tiles) { return (tiles + kPagedWaves - 1) / kPagedWa
 // workgroups, or more than 16 for a segment, and no more than kPagedLongUnit for each workgroup.
 // A piece costs a workgroup about as much as three rounds before and after its tiles, and the
 // joining workgroup a load's round trip per 16 pieces, so short segments (own tokens behind a
-// prefix) are better whole and long ones better in fewer pieces than there are rounds.
+// prefix) are better whole and long ones better in fewer pieces than there are rounds: one
+// sequence's 32 rows after 8000 keys (32 heads on 8) 47 us in pieces of one round, 24 of four.
 constexpr int kPagedLongUnit = 4;
 EMA_HD int paged_units(int rounds, int unit) { return (rounds + unit - 1) / unit; }
 EMA_HD int paged_unit(int rounds, int segments, int W) {
