@@ -741,7 +741,7 @@ extern "C" int32_t ema_paged_workspace_size(int32_t batch, int32_t n_rows, int32
   if (head_dim != 128) return set_error(EMA_ERR_UNSUPPORTED, "%s: head_dim %d not supported (128)", op, head_dim);
   if (max_q < 0 || max_len < 0 || max_prefix < 0)
     return set_error(EMA_ERR_SHAPE, "%s: negative bound (max_q=%d max_len=%d max_prefix=%d)", op, max_q, max_len, max_prefix);
-  *bytes = plan_paged(batch, n_rows, n_heads, n_kv_heads, max_q, max_len, max_prefix).bytes;
+  *bytes = paged_workspace_bytes(batch, n_rows, n_heads, n_kv_heads, max_q, max_len, max_prefix);
   return EMA_OK;
 }
 

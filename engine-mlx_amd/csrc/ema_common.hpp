@@ -261,6 +261,8 @@ struct PagedPlan {
   uint64_t bytes;       // the whole workspace
 };
 PagedPlan plan_paged(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len, int max_prefix);
+// Bytes that every plan of bounds up to these fits in.
+uint64_t paged_workspace_bytes(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len, int max_prefix);
 // Prompts and chunks in prefill_kernel's 128-row blocks: the sequences of few < n <= p.max_q rows.
 int32_t launch_paged_prefill(hipStream_t s, const PagedAttention& p, const ema_kvcache_desc& c, int few);
 // All rows over chunks of the shared prefix, their states into part.

@@ -896,6 +896,23 @@ PagedPlan plan_paged(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len,
   return p;
 }
 
+// The plans' bytes are not monotone (fewer rows are more chunks of a prefix, and the ways to take
+// it differ), so the size told to a caller is a bound of all of them up to the bounds: workgroups
+// over the most tiles of any way, and states of one chunk's rows or of what fills the chip, 128 rows
+// on each CU.
+uint64_t paged_workspace_bytes(int B, int n_rows, int Hq, int Hkv, int max_q, int max_len, int max_prefix) {
+  const int G = Hq / Hkv;
+  const int own = paged_plan_workers(paged_row_blocks(B, n_rows, max_q, G), Hkv,
+                                     paged_tiles(max_prefix) + paged_tiles(max_len));
+  const int all = paged_plan_workers(paged_row_blocks(1, n_rows, n_rows, G), Hkv, paged_tiles(max_prefix));
+  const uint64_t rows = (uint64_t)n_rows * Hq, fill = (uint64_t)device_cus() * 128;
+  const uint64_t most = rows * (((uint64_t)max_prefix + 127) / 128);  // a chunk holds 128 keys at least
+  uint64_t states = most < fill ? most : fill;
+  if (states < rows) states = rows;
+  return kDecodeCounterBytes + (uint64_t)2 * (own > all ? own : all) * kPagedRows * kPagedState * sizeof(float) +
+         (max_prefix > 0 ? states * kPagedState * sizeof(float) : 0);
+}
+
 int32_t launch_paged_attention(hipStream_t s, const PagedAttention& p, const ema_kvcache_desc& c, const PagedPlan& plan,
                                void* ws) {
   const bool fp8 = c.dtype == EMA_DTYPE_FP8_E4M3;

@@ -418,7 +418,7 @@ EMA_API int32_t ema_paged_append(ema_stream_t stream, const void* qkv, const voi
                                  int32_t table_cols);
 
 /* Workspace (bytes) of ema_paged_attention (max_prefix 0) and ema_prefix_attention for these
- * bounds. Like a decode workspace it begins with EMA_DECODE_COUNTER_BYTES of arrival counters
+ * bounds, and for every call of the same heads whose bounds are no larger. Like a decode workspace it begins with EMA_DECODE_COUNTER_BYTES of arrival counters
  * that must be zero before its first use and are zero again after every call; it may be shared
  * with decode calls, and calls that overlap (two streams, two graphs replayed at once) need one
  * each. */

@@ -2,6 +2,8 @@
 that are refused on the host, before any HIP call, with the documented codes."""
 import ctypes
 import os
+import random
+import re
 import subprocess
 
 import pytest
@@ -154,6 +156,29 @@ def test_workspace_sizes(ema):
         with pytest.raises(ema.EmaError) as e:
             ema.paged_workspace_size(**a)
         assert e.value.code == code, bad
+
+
+def needed(ema, **over):
+    """Bytes that a call asks for, from its refusal without a workspace."""
+    assert attend(ema, pool(ema, Hkv=over.pop("hkv"), page=4096), over.pop("prefix"), ws=None, cols=10, pcols=10,
+                  **over) == ema.EMA_ERR_WORKSPACE
+    return int(re.search(r"workspace of (\d+) bytes needed", ema.last_error()).group(1))
+
+
+def test_workspace_is_enough_for_smaller_calls(ema):
+    """A workspace of some bounds holds every call whose bounds are no larger."""
+    rng = random.Random(2)
+    for _ in range(3000):
+        heads, hkv = rng.choice([(32, 8), (16, 2), (12, 1), (8, 8), (64, 8)])
+        B, max_q = rng.randint(1, 200), rng.choice([1, rng.randint(1, 300)])
+        n, max_len = rng.randint(B, B * max_q), rng.randint(1, 40000)
+        prefix = rng.choice([0, 1, 1]) * rng.randint(1, 40000)
+        size = ema.paged_workspace_size(B, n, heads, hkv, 128, max_q, max_len, prefix)
+        b, q = rng.randint(1, B), rng.randint(1, max_q)
+        a = dict(heads=heads, hkv=hkv, batch=b, rows=rng.randint(1, min(n, b * q)), max_q=q, max_len=rng.randint(0, max_len))
+        assert needed(ema, prefix=False, **a) <= size
+        if prefix:
+            assert needed(ema, prefix=True, max_prefix=rng.randint(1, prefix), **a) <= size
 
 
 def test_binding_checks_tensors(ema):
