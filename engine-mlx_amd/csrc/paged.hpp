@@ -77,13 +77,16 @@ EMA_HD int paged_plan_workers(int64_t nrb, int Hkv, int max_tiles) {
   const int64_t want = nrb * Hkv * paged_rounds(max_tiles);
   return (int)(want < 1 ? 1 : (want < kPagedMaxWorkers ? want : kPagedMaxWorkers));
 }
-// Row blocks of a batch whose sequences have at most max_q rows and n_rows together.
+// log2 of a page size.
 EMA_HD int paged_shift(int page) {
   int s = 0;
   while ((1 << s) < page) ++s;
   return s;
 }
+// Row blocks of a batch whose sequences have at most max_q rows and n_rows together (a bound of
+// none, which any row is past, counts as one).
 EMA_HD int64_t paged_row_blocks(int B, int64_t n_rows, int64_t max_q, int G) {
+  if (max_q < 1) max_q = 1;
   const int64_t each = (int64_t)B * ((max_q * G + kPagedRows - 1) / kPagedRows);
   const int64_t all = n_rows * G / kPagedRows + B;
   return each < all ? each : all;

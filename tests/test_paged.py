@@ -181,6 +181,17 @@ def test_workspace_is_enough_for_smaller_calls(ema):
             assert needed(ema, prefix=True, max_prefix=rng.randint(1, prefix), **a) <= size
 
 
+@pytest.mark.parametrize("prefix", [False, True])
+def test_a_bound_of_no_rows_counts_as_one(ema, prefix):
+    """max_q 0 is a bound that any row is past: the call is planned as for max_q 1, so that the
+    choice of a prefix's way, and with it the count of tiles, has the sequences in it."""
+    for B in (1, 40, 1024):
+        a = dict(heads=16, hkv=8, batch=B, rows=B, max_len=4096, prefix=prefix, max_prefix=40000)
+        assert needed(ema, max_q=0, **a) == needed(ema, max_q=1, **a)
+        size = [ema.paged_workspace_size(B, B, 16, 8, 128, q, 4096, 40000 if prefix else 0) for q in (0, 1)]
+        assert size[0] == size[1]
+
+
 def test_binding_checks_tensors(ema):
     """Shapes, types, layouts and devices are checked before the call (CPU tensors here: the call
     itself is never reached)."""
