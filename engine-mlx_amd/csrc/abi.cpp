@@ -674,9 +674,13 @@ static int32_t check_pages(const char* op, const ema_kvcache_desc* c) {
                      kPagedMinPage);
   if (c->dtype == EMA_DTYPE_FP8_E4M3 && (((uintptr_t)c->k_exp | (uintptr_t)c->v_exp) & 1u))
     return set_error(EMA_ERR_INVALID_ARG, "%s: fp8 exponents must be 2-byte aligned", op);
-  // 16 rows of a page within a 32-bit buffer range, a page's and a head's strides in 32 bits
+  // 16 rows of a page within a 32-bit buffer range; a position's offset in its page, a page's and a
+  // head's strides in 32 bits
   if (c->stride_pos >= ((int64_t)1 << 26))
     return set_error(EMA_ERR_UNSUPPORTED, "%s: stride_pos %lld exceeds 2^26", op, (long long)c->stride_pos);
+  if (c->stride_pos * (c->capacity - 1) >= ((int64_t)1 << 31))
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %d positions of stride %lld span more than 2^31 - 1", op, c->capacity,
+                     (long long)c->stride_pos);
   if (c->stride_batch >= ((int64_t)1 << 31) || c->stride_head >= ((int64_t)1 << 31))
     return set_error(EMA_ERR_UNSUPPORTED, "%s: page stride %lld or head stride %lld exceeds 2^31 - 1", op,
                      (long long)c->stride_batch, (long long)c->stride_head);

@@ -385,7 +385,8 @@ EMA_API int32_t ema_prefill_attention_ws(ema_stream_t stream, const void* q, con
  * least 16), bf16 or FP8 E4M3 without a RoPE tail; ema_kvcache_init, _init_fp8, the _alloc
  * calls, ema_kvcache_convert and ema_kvcache_memory_bytes apply to it as to any other. Strides
  * may be set for other orders of a page (positions before heads: stride_head = head_dim,
- * stride_pos = n_kv_heads * head_dim).
+ * stride_pos = n_kv_heads * head_dim); page and head strides, and a page's positions together,
+ * stay below 2^31 elements (FP8: bytes), stride_pos below 2^26.
  *   table       device int32 [batch, table_cols]: row b names the pages of sequence b in order;
  *               its position p lies in slot p % capacity of page table[b][p / capacity]. An entry
  *               outside [0, number of pages) is never followed: nothing is written there, and
@@ -428,7 +429,9 @@ EMA_API int32_t ema_paged_workspace_size(int32_t batch, int32_t n_rows, int32_t 
 
 /* Attention of a ragged batch over its pages: single tokens, a few drafted tokens, prompts and
  * chunks, mixed as they come.
- *   q        [n_rows, n_heads, head_dim] bf16 (as ema_paged_append leaves it); head_dim 128
+ *   q        [n_rows, n_heads, head_dim] bf16 (as ema_paged_append leaves it); head_dim 128. A row
+ *            that is not finite gives a row that is not and changes no other. K and V held must be
+ *            finite: a masked position weighs 0, and 0 times what is not finite is NaN.
  *   lengths  device int32 [batch]: positions held, the call's own rows included; clamped to
  *            [0, table_cols * capacity]. Sequence b's n rows are its last n positions.
  *   max_q, max_len  host bounds of a sequence's rows and of the lengths; they size the grid and

@@ -158,6 +158,17 @@ def test_workspace_sizes(ema):
         assert e.value.code == code, bad
 
 
+def test_pages_whose_positions_span_too_much(ema):
+    """Positions outermost in the pool: the offset of a position within its page is 32 bits of bytes
+    in the prompts' kernel."""
+    for fp8 in (False, True):
+        for call in (append, attend, lambda e, d, **o: attend(e, d, prefix=True, **o)):
+            over = dict(fp8=fp8, page=1024, stride_batch=128, stride_head=1280)
+            d = pool(ema, stride_pos=1 << 22, **over)
+            assert call(ema, d, rows=0) == ema.EMA_ERR_UNSUPPORTED and "span" in ema.last_error()
+            assert call(ema, pool(ema, stride_pos=1 << 21, **over), rows=0) == ema.EMA_OK
+
+
 def needed(ema, **over):
     """Bytes that a call asks for, from its refusal without a workspace."""
     assert attend(ema, pool(ema, Hkv=over.pop("hkv"), page=4096), over.pop("prefix"), ws=None, cols=10, pcols=10,
