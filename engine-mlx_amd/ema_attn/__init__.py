@@ -562,6 +562,16 @@ def _elsewhere(device: int, call, *args) -> int:
         return call(*args)
 
 
+def _on(stream):
+    """What a call allocates for itself belongs to the stream that it is given: filled and reused in
+    that stream's order, not in the current one's."""
+    import contextlib
+
+    import torch
+
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
 def paged_append(qkv, q_norm_w, k_norm_w, eps, theta, offsets, n_heads, cache: PagedCache, table, q_starts=None,
                  flags=0, q_out=None, prefix_len=None, stream=None):
     """Norm, rotation and append of a ragged batch (ema_paged_append): qkv [n, (Hq+2Hkv)*D] bf16,
@@ -577,7 +587,8 @@ def paged_append(qkv, q_norm_w, k_norm_w, eps, theta, offsets, n_heads, cache: P
     B, cols = table.shape if table.dim() == 2 else (-1, -1)
     n = qkv.shape[0] if qkv.dim() else -1
     if q_out is None and n >= 0:
-        q_out = torch.empty((n, n_heads, D), dtype=bf, device=qkv.device)
+        with _on(stream):
+            q_out = torch.empty((n, n_heads, D), dtype=bf, device=qkv.device)
     if not (table.dtype is i32 and table.is_contiguous() and table.get_device() == dev
             and offsets.dtype is i32 and offsets.shape == (B,) and offsets.is_contiguous() and offsets.get_device() == dev
             and qkv.dtype is bf and qkv.shape == (n, F * D) and qkv.is_contiguous() and qkv.get_device() == dev
@@ -635,7 +646,8 @@ def _paged_args(op, q, cache, table, lengths, q_starts, max_q, max_len, scale, o
     elif max_q is None:
         max_q = n
     if out is None and n >= 0:
-        out = torch.empty((n, Hq * D), dtype=bf, device=q.device)
+        with _on(stream):
+            out = torch.empty((n, Hq * D), dtype=bf, device=q.device)
     if not (table.dtype is i32 and table.is_contiguous() and table.get_device() == dev
             and lengths.dtype is i32 and lengths.shape == (B,) and lengths.is_contiguous() and lengths.get_device() == dev
             and q.dtype is bf and q.shape == (n, Hq, D) and q.is_contiguous() and q.get_device() == dev
@@ -654,7 +666,8 @@ def _paged_args(op, q, cache, table, lengths, q_starts, max_q, max_len, scale, o
                 ("prefix_table", prefix_table, i32, (prefix_table.numel(),) if prefix_table is not None else ()),
                 ("prefix_len", prefix_len, i32, (1,)))
     if workspace is None:
-        workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, max_prefix, device=q.device)
+        with _on(stream):
+            workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, max_prefix, device=q.device)
     raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None and dev >= 0 else _stream(stream)
     return raw, B, n, Hq, cols, max_q, 1.0 / math.sqrt(D) if scale is None else scale, out, workspace
 

@@ -326,6 +326,29 @@ def test_streams_and_overlap(ema):
         ref.check_attention(down(o), *b.attention(), "two streams")
 
 
+def test_stream_owns_what_the_call_allocates(ema):
+    """A call on a stream of its own, the current stream busy and its free blocks full of ones: the
+    call's workspace is cleared, and its output used, in the order of the call's stream."""
+    import torch
+
+    b = ref.Batch([1] * 3, [1800, 40, 900], 16, 16, 2, seed=22)
+    g = OnGpu(ema, b)
+    size = ema.paged_workspace_size(3, 3, 16, 2, 128, 1, 1800)
+    s = torch.cuda.Stream()
+    x = torch.ones(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(3):
+        dirty = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        for _ in range(20):
+            x.mul_(1.0)
+        del dirty
+        out = ema.paged_attention(g.q, g.cache, g.table, g.lengths, 1800, q_starts=g.starts, max_q=1, stream=s)
+        s.synchronize()
+        ref.check_attention(down(out), *b.attention(), "a stream's own workspace")
+    torch.cuda.synchronize()
+
+
 def test_captured_and_replayed(ema):
     """Append and attention in a graph, replayed over new inputs, lengths and tables, with eager
     work between; every replay against the eager result."""
