@@ -428,7 +428,7 @@ EMA_API int32_t ema_paged_workspace_size(int32_t batch, int32_t n_rows, int32_t 
                                          uint64_t* bytes);
 
 /* Attention of a ragged batch over its pages: single tokens, a few drafted tokens, prompts and
- * chunks, mixed as they come.
+ * chunks, mixed as they come. (FP8 pages: long prompts run at about 0.3 of the bf16 rate.)
  *   q        [n_rows, n_heads, head_dim] bf16 (as ema_paged_append leaves it); head_dim 128. A row
  *            that is not finite gives a row that is not and changes no other. K and V held must be
  *            finite: a masked position weighs 0, and 0 times what is not finite is NaN.
