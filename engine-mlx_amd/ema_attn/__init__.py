@@ -509,12 +509,15 @@ class PagedCache:
             _check(lib().ema_kvcache_init(ctypes.byref(self.desc), _ptr(self.k), _ptr(self.v), *shape),
                    "ema_kvcache_init")
         else:
-            eshape = shape[:3] + (head_dim // 64,)
-            self.k_exp = k_exp if k_exp is not None else torch.zeros(eshape, dtype=torch.int8, device=device)
-            self.v_exp = v_exp if v_exp is not None else torch.zeros(eshape, dtype=torch.int8, device=device)
+            # (on the codes' device, whose index is all that the calls compare with)
+            eshape, dev = shape[:3] + (head_dim // 64,), self.k.device
+            self.k_exp = k_exp if k_exp is not None else torch.zeros(eshape, dtype=torch.int8, device=dev)
+            self.v_exp = v_exp if v_exp is not None else torch.zeros(eshape, dtype=torch.int8, device=dev)
             for name, t in (("k_exp", self.k_exp), ("v_exp", self.v_exp)):
                 if t.dtype != torch.int8 or tuple(t.shape) != eshape or not t.is_contiguous():
                     raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be contiguous int8 {eshape}")
+                if t.device != dev:
+                    raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} is on {t.device}, the codes on {dev}")
             _check(lib().ema_kvcache_init_fp8(ctypes.byref(self.desc), _ptr(self.k), _ptr(self.v), _ptr(self.k_exp),
                                               _ptr(self.v_exp), *shape, 0), "ema_kvcache_init_fp8")
         self.desc.stride_batch, self.desc.stride_head, self.desc.stride_pos = self.k.stride()[:3]

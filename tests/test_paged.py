@@ -238,3 +238,19 @@ def test_binding_checks_tensors(ema):
     refused(ema.PagedCache, 6, 2, 16, 128, k=torch.zeros(6, 2, 16, 128, dtype=bf), v=torch.zeros(6, 16, 2, 128, dtype=bf).transpose(1, 2))
     with pytest.raises(ValueError):
         ema.PagedCache(6, 2, 16, 128, device="cpu", dtype="int4")
+
+
+def test_exponents_on_another_device_are_refused(ema):
+    """FP8 pages whose exponents lie elsewhere than the codes: refused when the pool is made, since a
+    call checks its tensors against the pool alone. (The meta device stands for any other.)"""
+    import torch
+
+    codes = [torch.zeros(6, 2, 16, 128, dtype=torch.uint8) for _ in range(2)]
+    here, there = (torch.zeros(6, 2, 16, 2, dtype=torch.int8, device=d) for d in ("cpu", "meta"))
+    for k_exp, v_exp, name in ((there, here, "k_exp"), (here, there, "v_exp"), (there, None, "k_exp"), (None, there, "v_exp")):
+        with pytest.raises(ema.EmaError) as e:
+            ema.PagedCache(6, 2, 16, 128, k=codes[0], v=codes[1], dtype="fp8", k_exp=k_exp, v_exp=v_exp, device="cpu")
+        assert e.value.code == ema.EMA_ERR_INVALID_ARG and name in str(e.value)
+    # those that the pool makes for itself lie with the codes, whatever the device of other tensors
+    cache = ema.PagedCache(6, 2, 16, 128, k=codes[0], v=codes[1], dtype="fp8", device="meta")
+    assert cache.k_exp.device == cache.v_exp.device == codes[0].device
