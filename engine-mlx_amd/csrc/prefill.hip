@@ -750,8 +750,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2),
         const float bm = wave_max_xor(mx, 32);
         const float delta = seen ? fmaxf(bm, 0.f) : (bm == -INFINITY ? 0.f : bm);
         seen = seen || bm != -INFINITY;
-        const float alpha = prob(-delta);
-        o_scale = alpha;
+        // (a row's first base may be below -128, where 2^-delta is inf and would make its
+        // accumulators, still zero, NaN: only a base that rises scales them)
+        o_scale = prob(-fmaxf(delta, 0.f));
         rescale = true;
         m_use += delta;
         for (int st = 0; st < 4; ++st)

@@ -217,6 +217,33 @@ def test_rows_that_are_not_finite(ema, new, kv, prefix, bad):
     ref.check_attention(down(got[~hit]), down(want[~hit]), down(want[~hit].abs()) + 1.0, "the other rows")
 
 
+@pytest.mark.parametrize("new,kv,heads,prefix,pages", [
+    ([1, 5, 30], [70, 300, 30], (8, 2), 0, "bf16"),              # segments
+    ([1, 40], [70, 300], (8, 2), 0, "fp8"),
+    ([700] * 6, [700, 701, 900, 760, 764, 3000], (8, 4), 0, "bf16"),  # blocks of 128 rows
+    ([350, 480, 300, 129] * 18, [350, 500, 300, 400] * 18, (16, 2), 0, "bf16"),  # pairs of them
+    ([1] * 6, [0, 5, 33, 1, 0, 90], (16, 8), 700, "bf16"),       # a prefix in every segment
+    ([1] * 40, list(range(40)), (8, 2), 3300, "bf16"),           # once, in blocks
+    ([1] * 6, [0, 5, 33, 1, 0, 90], (16, 8), 8000, "fp8"),       # once, in segments
+])
+def test_scores_far_below_zero(ema, new, kv, heads, prefix, pages):
+    """Keys that share a large component against the queries: every score is near -97 (2^-140 before the
+    row's max is taken off), and the softmax is what it is without the component."""
+    import torch
+
+    b = ref.Batch(new, kv, 16, *heads, seed=41, prefix=prefix)
+    b.q[..., 0] = 10.0
+    for x in [b.k, b.shared[0]] + [h[0] for h in b.held]:
+        x[..., 0] = np.where(np.isnan(x[..., 0]), np.nan, -110.0)
+    g = OnGpu(ema, b, pages)
+    out = g.attention()
+    torch.cuda.synchronize()
+    # a score is at most 129 sums in 32 bits of up to 1100 in size, each off by 2^-14 at most; times
+    # 128^-0.5 and for weight and row sum 2^-9.5 in all, 0.18 of the bound's 2^-7
+    want, mag = b.attention()
+    ref.check_attention(down(out), want, 1.18 * mag, f"scores far below zero {heads} {prefix} {pages}")
+
+
 def test_prompt_sized_rows(ema):
     """Sequences of more rows than a segment, beside short ones, with and without row starts, and
     bounds below the truth (the sequences past them take another way)."""

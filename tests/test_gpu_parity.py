@@ -581,6 +581,36 @@ def test_prefill_ignores_cache_rows_outside_the_window(ema, ora, B, Hq, Hkv, T, 
     assert_close(clean, ref, "prefill window")
 
 
+@pytest.mark.parametrize("rotating", [False, True])
+@pytest.mark.parametrize("B,Hq,Hkv,T,q_off,causal,chunk", [
+    (2, 6, 3, 33, [0, 100], True, False),                  # 32 query rows per workgroup
+    (5, 20, 4, 128, [0, 37, 300, 129, 1], True, False),    # 128, one query block per workgroup
+    (5, 20, 4, 128, [0, 37, 300, 129, 1], False, False),
+    (4, 16, 4, 1000, [0, 37, 300, 129], True, False),      # pairs of blocks
+    (4, 16, 4, 1000, [64, 0, 250, 7], True, True),
+])
+def test_prefill_scores_far_below_zero(ema, ora, B, Hq, Hkv, T, q_off, causal, chunk, rotating):
+    """Keys that share a large component against the queries: every score is near -97, so 2^-max of a
+    row's first block is past 32 bits. The component is the same for all keys, and its rounding with q
+    too, so the softmax and its error are those of ordinary inputs. (A rotating cache that has not
+    wrapped holds the same rows.)"""
+    import torch
+
+    D, cap = 128, 1536
+    say(f"prefill far scores B={B} Hq={Hq} Hkv={Hkv} T={T} causal={causal} chunk={chunk} rotating={rotating}")
+    q = ora.normal_bf16((B, Hq, T, D), seed=365)
+    kc = ora.normal_bf16((B, Hkv, cap, D), seed=366)
+    vc = ora.normal_bf16((B, Hkv, cap, D), seed=367)
+    q[..., 0] = 0x4120   # 10
+    kc[..., 0] = 0xC2DC  # -110
+    qo = np.asarray(q_off, np.int32)
+    cache = ema.StaticCache(B, Hkv, cap, D, k=dev(kc), v=dev(vc), rotating=rotating)
+    out = host(ema.prefill_attention(dev(q), cache, dev(qo), causal=causal, chunk_only=chunk))
+    torch.cuda.synchronize()
+    ref = ora.sdpa(q, kc, vc, qo + T, scale_of(D), causal, kv_begin=qo if chunk else None)
+    assert_close(out, ref, "prefill far scores")
+
+
 def test_prefill_rows_match_decode_on_gpu(ema, ora):
     """Causal prefill row i equals decode with len = off + i + 1 on the same cache."""
     import torch
