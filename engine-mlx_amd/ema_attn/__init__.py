@@ -555,6 +555,15 @@ def _refuse(op: str, device: int, *wanted) -> None:
     raise EmaError(EMA_ERR_SHAPE, op, "arguments that do not belong together")
 
 
+def _no_tensor(op: str, needed: dict, optional: dict) -> None:
+    """Raises for the first argument that is no tensor; an optional one may be None."""
+    import torch
+
+    for name, t in (needed | optional).items():
+        if not isinstance(t, torch.Tensor) and not (t is None and name in optional):
+            raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} must be a tensor, not {type(t).__name__}")
+
+
 def _elsewhere(device: int, call, *args) -> int:
     """call(*args) with the pool's device, which is not the current one, made current."""
     import torch
@@ -587,27 +596,32 @@ def paged_append(qkv, q_norm_w, k_norm_w, eps, theta, offsets, n_heads, cache: P
     # calls are bound by the host), the tensor to name looked for only when it is not
     op, bf, i32, dev = "ema_paged_append", torch.bfloat16, torch.int32, cache.device_index
     D, F = cache.desc.head_dim, n_heads + 2 * cache.desc.n_kv_heads
-    B, cols = table.shape if table.dim() == 2 else (-1, -1)
-    n = qkv.shape[0] if qkv.dim() else -1
-    if q_out is None and n >= 0:
-        with _on(stream):
-            q_out = torch.empty((n, n_heads, D), dtype=bf, device=qkv.device)
-    if not (table.dtype is i32 and table.is_contiguous() and table.get_device() == dev
-            and offsets.dtype is i32 and offsets.shape == (B,) and offsets.is_contiguous() and offsets.get_device() == dev
-            and qkv.dtype is bf and qkv.shape == (n, F * D) and qkv.is_contiguous() and qkv.get_device() == dev
-            and q_out.dtype is bf and q_out.shape == (n, n_heads, D) and q_out.is_contiguous() and q_out.get_device() == dev
-            and (q_norm_w is None or (q_norm_w.dtype is bf and q_norm_w.shape == (D,) and q_norm_w.is_contiguous()
-                                      and q_norm_w.get_device() == dev))
-            and (k_norm_w is None or (k_norm_w.dtype is bf and k_norm_w.shape == (D,) and k_norm_w.is_contiguous()
-                                      and k_norm_w.get_device() == dev))
-            and (q_starts is None or (q_starts.dtype is i32 and q_starts.shape == (B + 1,) and q_starts.is_contiguous()
-                                      and q_starts.get_device() == dev))
-            and (prefix_len is None or (prefix_len.dtype is i32 and prefix_len.shape == (1,)
-                                        and prefix_len.get_device() == dev))):
-        _refuse(op, dev, ("table", table, i32, (B, cols)), ("offsets", offsets, i32, (B,)),
-                ("qkv", qkv, bf, (n, F * D)), ("q_out", q_out, bf, (n, n_heads, D)), ("q_norm_w", q_norm_w, bf, (D,)),
-                ("k_norm_w", k_norm_w, bf, (D,)), ("q_starts", q_starts, i32, (B + 1,)),
-                ("prefix_len", prefix_len, i32, (1,)))
+    try:
+        B, cols = table.shape if table.dim() == 2 else (-1, -1)
+        n = qkv.shape[0] if qkv.dim() else -1
+        if q_out is None and n >= 0:
+            with _on(stream):
+                q_out = torch.empty((n, n_heads, D), dtype=bf, device=qkv.device)
+        if not (table.dtype is i32 and table.is_contiguous() and table.get_device() == dev
+                and offsets.dtype is i32 and offsets.shape == (B,) and offsets.is_contiguous() and offsets.get_device() == dev
+                and qkv.dtype is bf and qkv.shape == (n, F * D) and qkv.is_contiguous() and qkv.get_device() == dev
+                and q_out.dtype is bf and q_out.shape == (n, n_heads, D) and q_out.is_contiguous() and q_out.get_device() == dev
+                and (q_norm_w is None or (q_norm_w.dtype is bf and q_norm_w.shape == (D,) and q_norm_w.is_contiguous()
+                                          and q_norm_w.get_device() == dev))
+                and (k_norm_w is None or (k_norm_w.dtype is bf and k_norm_w.shape == (D,) and k_norm_w.is_contiguous()
+                                          and k_norm_w.get_device() == dev))
+                and (q_starts is None or (q_starts.dtype is i32 and q_starts.shape == (B + 1,) and q_starts.is_contiguous()
+                                          and q_starts.get_device() == dev))
+                and (prefix_len is None or (prefix_len.dtype is i32 and prefix_len.shape == (1,)
+                                            and prefix_len.get_device() == dev))):
+            _refuse(op, dev, ("table", table, i32, (B, cols)), ("offsets", offsets, i32, (B,)),
+                    ("qkv", qkv, bf, (n, F * D)), ("q_out", q_out, bf, (n, n_heads, D)), ("q_norm_w", q_norm_w, bf, (D,)),
+                    ("k_norm_w", k_norm_w, bf, (D,)), ("q_starts", q_starts, i32, (B + 1,)),
+                    ("prefix_len", prefix_len, i32, (1,)))
+    except AttributeError:
+        _no_tensor(op, dict(table=table, qkv=qkv, offsets=offsets),
+                   dict(q_norm_w=q_norm_w, k_norm_w=k_norm_w, q_starts=q_starts, prefix_len=prefix_len, q_out=q_out))
+        raise
     args = (torch._C._cuda_getCurrentRawStream(dev) if stream is None and dev >= 0 else _stream(stream), qkv.data_ptr(),
             _ptr(q_norm_w), _ptr(k_norm_w), eps, theta, _ptr(q_starts), offsets.data_ptr(), _ptr(prefix_len), B, n,
             n_heads, flags, q_out.data_ptr(), cache.desc_ref, table.data_ptr(), cols)
@@ -634,40 +648,46 @@ def paged_workspace(batch, n_rows, n_heads, n_kv_heads, head_dim, max_q, max_len
     return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
-def _paged_args(op, q, cache, table, lengths, q_starts, max_q, max_len, scale, out, workspace, stream, max_prefix=0,
-                prefix_table=None, prefix_len=None):
-    """Checks the tensors of an attention call (see paged_append) and returns (stream, B, n, Hq, cols,
-    max_q, scale, out, workspace)."""
+def _paged_args(op, q, cache, table, lengths, q_starts, max_q, max_len, scale, out, workspace, stream, shared=False,
+                max_prefix=0, prefix_table=None, prefix_len=None):
+    """Checks the tensors of an attention call (see paged_append), with shared those of a prefix too, and
+    returns (stream, B, n, Hq, cols, max_q, scale, out, workspace)."""
     import torch
 
     bf, i32, dev = torch.bfloat16, torch.int32, cache.device_index
     D = cache.desc.head_dim
-    B, cols = table.shape if table.dim() == 2 else (-1, -1)
-    n, Hq = q.shape[:2] if q.dim() == 3 else (-1, -1)
-    if q_starts is None:
-        max_q = -(-n // B) if B > 0 else 0
-    elif max_q is None:
-        max_q = n
-    if out is None and n >= 0:
-        with _on(stream):
-            out = torch.empty((n, Hq * D), dtype=bf, device=q.device)
-    if not (table.dtype is i32 and table.is_contiguous() and table.get_device() == dev
-            and lengths.dtype is i32 and lengths.shape == (B,) and lengths.is_contiguous() and lengths.get_device() == dev
-            and q.dtype is bf and q.shape == (n, Hq, D) and q.is_contiguous() and q.get_device() == dev
-            and out.dtype is bf and out.shape == (n, Hq * D) and out.is_contiguous() and out.get_device() == dev
-            and (q_starts is None or (q_starts.dtype is i32 and q_starts.shape == (B + 1,) and q_starts.is_contiguous()
-                                      and q_starts.get_device() == dev))
-            and (workspace is None or (workspace.dtype is torch.uint8 and workspace.is_contiguous()
-                                       and workspace.get_device() == dev))
-            and (prefix_table is None or (prefix_table.dtype is i32 and prefix_table.dim() == 1
-                                          and prefix_table.is_contiguous() and prefix_table.get_device() == dev
-                                          and prefix_len.dtype is i32 and prefix_len.shape == (1,)
-                                          and prefix_len.get_device() == dev))):
-        _refuse(op, dev, ("table", table, i32, (B, cols)), ("lengths", lengths, i32, (B,)), ("q", q, bf, (n, Hq, D)),
-                ("out", out, bf, (n, Hq * D)), ("q_starts", q_starts, i32, (B + 1,)),
-                ("workspace", workspace, torch.uint8, workspace.shape if workspace is not None else ()),
-                ("prefix_table", prefix_table, i32, (prefix_table.numel(),) if prefix_table is not None else ()),
-                ("prefix_len", prefix_len, i32, (1,)))
+    try:
+        B, cols = table.shape if table.dim() == 2 else (-1, -1)
+        n, Hq = q.shape[:2] if q.dim() == 3 else (-1, -1)
+        if q_starts is None:
+            max_q = -(-n // B) if B > 0 else 0
+        elif max_q is None:
+            max_q = n
+        if out is None and n >= 0:
+            with _on(stream):
+                out = torch.empty((n, Hq * D), dtype=bf, device=q.device)
+        if not (table.dtype is i32 and table.is_contiguous() and table.get_device() == dev
+                and lengths.dtype is i32 and lengths.shape == (B,) and lengths.is_contiguous() and lengths.get_device() == dev
+                and q.dtype is bf and q.shape == (n, Hq, D) and q.is_contiguous() and q.get_device() == dev
+                and out.dtype is bf and out.shape == (n, Hq * D) and out.is_contiguous() and out.get_device() == dev
+                and (q_starts is None or (q_starts.dtype is i32 and q_starts.shape == (B + 1,) and q_starts.is_contiguous()
+                                          and q_starts.get_device() == dev))
+                and (workspace is None or (workspace.dtype is torch.uint8 and workspace.is_contiguous()
+                                           and workspace.get_device() == dev))
+                and (not shared or (prefix_table.dtype is i32 and prefix_table.dim() == 1
+                                    and prefix_table.is_contiguous() and prefix_table.get_device() == dev
+                                    and prefix_len.dtype is i32 and prefix_len.shape == (1,)
+                                    and prefix_len.get_device() == dev))):
+            _refuse(op, dev, ("table", table, i32, (B, cols)), ("lengths", lengths, i32, (B,)), ("q", q, bf, (n, Hq, D)),
+                    ("out", out, bf, (n, Hq * D)), ("q_starts", q_starts, i32, (B + 1,)),
+                    ("workspace", workspace, torch.uint8, workspace.shape if workspace is not None else ()),
+                    ("prefix_table", prefix_table, i32, (prefix_table.numel(),) if shared else ()),
+                    ("prefix_len", prefix_len, i32, (1,)))
+    except AttributeError:
+        _no_tensor(op, dict(table=table, lengths=lengths, q=q,
+                            **(dict(prefix_table=prefix_table, prefix_len=prefix_len) if shared else {})),
+                   dict(q_starts=q_starts, out=out, workspace=workspace))
+        raise
     if workspace is None:
         with _on(stream):
             workspace = paged_workspace(B, n, Hq, cache.desc.n_kv_heads, D, max_q, max_len, max_prefix, device=q.device)
@@ -706,8 +726,8 @@ def prefix_attention(q, cache: PagedCache, prefix_table, prefix_len, max_prefix,
     in paged_attention. The prefix is read once for the batch. Returns out [n, Hq * D]."""
     op = "ema_prefix_attention"
     raw, B, n, Hq, cols, max_q, scale, out, workspace = _paged_args(op, q, cache, table, lengths, q_starts, max_q,
-                                                                    max_len, scale, out, workspace, stream, max_prefix,
-                                                                    prefix_table, prefix_len)
+                                                                    max_len, scale, out, workspace, stream, True,
+                                                                    max_prefix, prefix_table, prefix_len)
     _paged_call(op, cache, lib().ema_prefix_attention, raw, q.data_ptr(), cache.desc_ref, prefix_table.data_ptr(),
                 prefix_table.numel(), prefix_len.data_ptr(), max_prefix, table.data_ptr(), cols, _ptr(q_starts),
                 lengths.data_ptr(), B, n, max_q, max_len, Hq, scale, out.data_ptr(), workspace.data_ptr(),

@@ -254,3 +254,32 @@ def test_exponents_on_another_device_are_refused(ema):
     # those that the pool makes for itself lie with the codes, whatever the device of other tensors
     cache = ema.PagedCache(6, 2, 16, 128, k=codes[0], v=codes[1], dtype="fp8", device="meta")
     assert cache.k_exp.device == cache.v_exp.device == codes[0].device
+
+
+def test_missing_tensors_are_refused(ema):
+    """None (or what is no tensor) in the place of a tensor that a call cannot do without is the
+    documented error, which names it."""
+    import torch
+
+    bf, i32 = torch.bfloat16, torch.int32
+    cache = ema.PagedCache(6, 2, 16, 128, device="cpu")
+    n, one = torch.ones(3, dtype=i32), torch.ones(1, dtype=i32)
+    calls = {
+        ema.paged_append: (dict(qkv=torch.zeros(3, 12 * 128, dtype=bf), offsets=n, table=torch.zeros(3, 2, dtype=i32)),
+                           dict(q_norm_w=None, k_norm_w=None, eps=1e-6, theta=1e6, n_heads=8, cache=cache)),
+        ema.paged_attention: (dict(q=torch.zeros(3, 8, 128, dtype=bf), table=torch.zeros(3, 2, dtype=i32), lengths=n),
+                              dict(cache=cache, max_len=32)),
+        ema.prefix_attention: (dict(q=torch.zeros(3, 8, 128, dtype=bf), table=torch.zeros(3, 2, dtype=i32), lengths=n,
+                                    prefix_table=torch.zeros(2, dtype=i32), prefix_len=one),
+                               dict(cache=cache, max_len=32, max_prefix=16)),
+    }
+    for call, (tensors, rest) in calls.items():
+        for name in tensors:
+            for bad in (None, [1, 2, 3]):
+                with pytest.raises(ema.EmaError) as e:
+                    call(**{**tensors, **rest, name: bad})
+                assert e.value.code == ema.EMA_ERR_INVALID_ARG and name in str(e.value), (call.__name__, name)
+        for name in ("q_starts", "q_out" if "qkv" in tensors else "workspace"):  # optional, but tensors if given
+            with pytest.raises(ema.EmaError) as e:
+                call(**{**tensors, **rest, name: [0, 1, 2, 3]})
+            assert e.value.code == ema.EMA_ERR_INVALID_ARG and name in str(e.value), (call.__name__, name)
