@@ -251,12 +251,12 @@ struct PagedAttention {
   void* out;
 };
 struct PagedPlan {
-  int workers;          // workgroups over the sequences' own pages
-  int prefix_workers;   // workgroups over the shared prefix (few rows)
-  bool direct;          // the segments take the prefix's tiles themselves
-  int chunks;           // chunks of the shared prefix (more rows), and their 64-key blocks
-  int chunk_blocks;
-  uint64_t part_bytes;  // partial states of shared segments
+  int workers;          // workgroups over the sequences' own pages (direct: and the prefix's)
+  bool direct;          // the segments take the prefix's tiles themselves; otherwise a launch of its own:
+  int prefix_workers;   // FP8 pages: workgroups of the segments over the prefix (one state a row)
+  int chunks;           // bf16 pages: chunks of the prefix (a state a row for each), in 128-row blocks,
+  int chunk_blocks;     // and the 64-key blocks of a chunk
+  uint64_t part_bytes;  // partial states of shared segments (the plan serves either type of pages)
   uint64_t carry_bytes; // states of the rows over the prefix
   uint64_t bytes;       // the whole workspace
 };

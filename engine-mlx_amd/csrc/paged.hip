@@ -212,6 +212,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 // (1031 MB) 160 us, 6.4 TB/s; 32 of up to 8k (541 MB) 90 us, FP8 (275 MB) 54; 16 heads on 8, one
 // sequence of 1k keys 7.4 us, a chain of dependent reads. K and V that are read once pass the
 // caches: 183 and 104 us without that.
+//
+// Made for few rows: a segment takes the tiles of all its sequence's keys, also those that only
+// later rows see (masked), so a causal prompt without history costs twice the tiles that it needs,
+// and each segment reads (and, FP8, decodes) K and V again: 4 prompts of 2048 tokens over FP8 pages
+// 574 us against 167 for the blocks over bf16 ones.
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kD = 128;
@@ -856,18 +861,29 @@ int32_t launch_paged_append(hipStream_t s, const PagedAppend& p, const ema_kvcac
 }
 
 // More query rows than kFewRows per (sequence, kv head) run in prefill_kernel's 128-row blocks
-// (bf16 pages) where these are at least 3/8 of the CUs, the others in paged_kernel's 32-row segments,
-// whose keys are split. Segments / blocks, us, 32 heads on 8: 16 sequences after 1000 keys, 128 rows
-// 24.6 / 23.8 and 192 rows 56 / 26; without history 192 rows 13.7 / 9.4; 4 sequences after 8000 keys
-// 512 rows 125 / 114 (128 workgroups of blocks), 256 rows 83 / 107 (64); one sequence, 256 rows 46 / 100.
+// (bf16 pages) where these, were every sequence as long as the longest, are at least 3/8 of the CUs;
+// the others in paged_kernel's 32-row segments, whose keys are split. Segments / blocks, us, 32
+// heads on 8. Blocks taken: 16 sequences of 192 rows 54.7 / 25.7 after 1000 keys and 12.7 / 10.1
+// without history, 4 of 512 rows after 8000 keys 122 / 108, one of 2048 rows 131 / 109. Segments
+// taken: after 8000 keys 4 sequences of 256 rows 82 / 104 (64 workgroups of blocks), one 42 / 100.
+// The rule knows neither the history nor the rows that the sequences really have, and takes the
+// slower way in these: segments, 16 sequences after 8000 keys, 64 rows 121 / 111, 96 rows 293 / 114
+// (their segments read K and V out of phase, each from HBM), 128 rows 147 / 116, after 1000 keys
+// 96 rows 42.9 / 22.5, and 4 of 192 rows after 8000 keys 129 / 103; blocks, a chunk of 64 tokens
+// (256 rows) after 8000 keys beside single tokens after 2000 keys, 7 of them 46.9 / 118, 31
+// 77.7 / 146 (a caller's way out is max_q 1: 55 and 85).
 constexpr int kFewRows = 128;
 bool paged_blocks(int64_t rows, int B, int Hkv, int cus) {
   return rows > kFewRows && (rows + 127) / 128 * B * Hkv * 8 >= (int64_t)cus * 3;
 }
 // A shared prefix whose tiles are no more rounds than this when every segment takes them itself:
 // one launch over the prefix's and the own tiles together, K and V of the prefix from the L2s. Against
-// the prefix once in 128-row blocks, us, 32 heads on 8 unless named: 416 rounds 10.5 / 15.9, 832
-// 15.1 / 16.3, 1664 17.7 / 17.2, 2048 26.8 / 20.1 (16 heads on 2 17.4 / 22.7), 4032 46.5 / 27.3.
+// the prefix in a launch of its own, us, 32 heads on 8 / 16 on 2. bf16 (in 128-row blocks): 416 rounds
+// 10.1 : 16.2 / 11.6 : 17.5, 832 14.6 : 16.9 / 12.0 : 18.2, 1664 17.0 : 17.7 / -, 2048 25.9 : 20.1 /
+// 17.0 : 22.7, 4032 45.8 : 27.3 / 47.1 : 41.6. FP8 (in segments): 1664 16.5 : 26.7, 2048 19.1 : 26.6 /
+// 17.9 : 26.8, 4096 26.4 : 26.6. Near the limit the layouts differ (a prefix on 2 kv heads is read by
+// fewer segments at a time), and rounds alone do not tell them apart: at 2048 rounds the limit is
+// right for 2 kv heads and for FP8 and 6 us too high for bf16 on 8.
 constexpr int kDirectRounds = 4 * kPagedMaxWorkers;
 
 // Workspace: the arrival counters, the partial states of the workers' shared segments, then

@@ -723,7 +723,8 @@ def prefix_attention(q, cache: PagedCache, prefix_table, prefix_len, max_prefix,
     """Causal attention where every sequence's own pages continue one shared prefix
     (ema_prefix_attention): prefix_table int32 [cols], prefix_len int32 [1] (its positions,
     max_prefix a host bound); table and lengths are of the sequences' own positions, the rest as
-    in paged_attention. The prefix is read once for the batch. Returns out [n, Hq * D]."""
+    in paged_attention. The prefix is held once, and a long one read once per 128 packed rows of a kv
+    head (FP8: 32). Returns out [n, Hq * D]."""
     op = "ema_prefix_attention"
     raw, B, n, Hq, cols, max_q, scale, out, workspace = _paged_args(op, q, cache, table, lengths, q_starts, max_q,
                                                                     max_len, scale, out, workspace, stream, True,

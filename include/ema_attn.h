@@ -411,7 +411,9 @@ EMA_API int32_t ema_prefill_attention_ws(ema_stream_t stream, const void* q, con
  * arithmetic, one rounding. K and V go to their slots (FP8: the bf16 row, quantised as
  * ema_pre_attention does); a row whose position is negative, past the table or on an entry
  * outside the pool still gets its q and is not stored. flags as for ema_pre_attention;
- * head_dim 64, 128 or 256 (FP8: 128). No two rows of a call may share a slot. */
+ * head_dim 64, 128 or 256 (FP8: 128; ema_paged_attention and ema_prefix_attention read pages of
+ * head_dim 128 only, the others are for a caller's own reader). No two rows of a call may share a
+ * slot. */
 EMA_API int32_t ema_paged_append(ema_stream_t stream, const void* qkv, const void* q_norm_w, const void* k_norm_w,
                                  float eps, float theta, const int32_t* q_starts, const int32_t* offsets,
                                  const int32_t* prefix_len, int32_t batch, int32_t n_rows, int32_t n_heads,
@@ -419,16 +421,22 @@ EMA_API int32_t ema_paged_append(ema_stream_t stream, const void* qkv, const voi
                                  int32_t table_cols);
 
 /* Workspace (bytes) of ema_paged_attention (max_prefix 0) and ema_prefix_attention for these
- * bounds, and for every call of the same heads whose bounds are no larger. Like a decode workspace it begins with EMA_DECODE_COUNTER_BYTES of arrival counters
- * that must be zero before its first use and are zero again after every call; it may be shared
- * with decode calls, and calls that overlap (two streams, two graphs replayed at once) need one
- * each. */
+ * bounds, and for every call of the same heads whose bounds are no larger. Like a decode workspace
+ * it begins with EMA_DECODE_COUNTER_BYTES of arrival counters that must be zero before its first
+ * use and are zero again after every call; it may be shared with decode calls, and calls that
+ * overlap (two streams, two graphs replayed at once) need one each. */
 EMA_API int32_t ema_paged_workspace_size(int32_t batch, int32_t n_rows, int32_t n_heads, int32_t n_kv_heads,
                                          int32_t head_dim, int32_t max_q, int32_t max_len, int32_t max_prefix,
                                          uint64_t* bytes);
 
 /* Attention of a ragged batch over its pages: single tokens, a few drafted tokens, prompts and
- * chunks, mixed as they come. (FP8 pages: long prompts run at about 0.3 of the bf16 rate.)
+ * chunks, mixed as they come. Prompts over FP8 pages run at about 0.3 of the bf16 rate: they take
+ * the way of few rows, which reads and decodes the keys once per 32 query rows of a kv head and
+ * multiplies a prompt's masked tiles too. bf16 calls whose max_q makes more than 128 rows per kv
+ * head go in blocks of 128 rows, if batch sequences of max_q rows make blocks for 3/8 of the CUs. One
+ * chunk beside many single tokens is counted as many chunks: max_q 1 keeps such a call in the way
+ * of few rows (32 heads on 8, 64 tokens after 8000 keys beside 31 single ones after 2000: 147 us
+ * with max_q 64, 85 with max_q 1).
  *   q        [n_rows, n_heads, head_dim] bf16 (as ema_paged_append leaves it); head_dim 128. A row
  *            that is not finite gives a row that is not and changes no other. K and V held must be
  *            finite: a masked position weighs 0, and 0 times what is not finite is NaN.
@@ -446,8 +454,11 @@ EMA_API int32_t ema_paged_attention(ema_stream_t stream, const void* q, const em
                                     void* workspace, uint64_t workspace_bytes);
 
 /* ema_paged_attention (causal) for sequences that continue one shared prefix, held once in the
- * same pool: every row sees all prefix positions, then causally its sequence's own. The prefix
- * is read once for the whole batch.
+ * same pool: every row sees all prefix positions, then causally its sequence's own. The prefix is
+ * held once and its rows are multiplied with the whole batch's: per kv head it is read once per 128
+ * packed rows (bf16 pages; FP8: per 32), a short one once per 32 rows of each sequence, from the
+ * caches, in one launch with the own pages. The sequences' own pages always go the way of few
+ * rows, however many rows there are.
  *   prefix_table  device int32 [prefix_cols]: the prefix's pages
  *   prefix_len    device int32 [1]: its positions, clamped to [0, max_prefix]
  *   max_prefix    host bound of it, at most prefix_cols * capacity
