@@ -61,6 +61,12 @@ pub mod sys {
     pub const EMA_PREFILL_CAUSAL: u32 = 1;
     pub const EMA_PREFILL_CHUNK_ONLY: u32 = 2;
     pub const EMA_PREFILL_ROWS_DECODED: u32 = 4;
+    pub const EMA_CONV_SILU: u32 = 1;
+    pub const EMA_SSM_SOFTPLUS: u32 = 1;
+    pub const EMA_NORM_GATE_FIRST: u32 = 1;
+    pub const EMA_NORM_GATE_SIGMOID: u32 = 2;
+    pub const EMA_NORM_SHARED_WEIGHT: u32 = 4;
+    pub const EMA_NORM_UNIT_OFFSET: u32 = 8;
 
     /// Arrival counters at the start of every decode workspace: zero before its first use;
     /// every call leaves them at zero.
@@ -199,6 +205,25 @@ pub mod sys {
             table: *const i32, table_cols: i32, q_starts: *const i32, lengths: *const i32, batch: i32, n_rows: i32,
             max_q: i32, max_len: i32, n_heads: i32, scale: f32, out: *mut c_void, workspace: *mut c_void,
             workspace_bytes: u64) -> i32;
+        pub fn ema_causal_conv(stream: EmaStream, x: *const c_void, ldx: i64, w: *const c_void,
+            bias: *const c_void, starts: *const i32, offsets: *const i32, slots: *const i32, batch: i32,
+            n_rows: i32, max_rows: i32, channels: i32, width: i32, flags: u32, state: *mut c_void,
+            n_slots: i32, y: *mut c_void, ldy: i64, dtype: i32) -> i32;
+        pub fn ema_ssm_workspace_size(batch: i32, n_rows: i32, max_rows: i32, n_heads: i32, head_dim: i32,
+            d_state: i32, n_groups: i32, dtype: i32, bytes: *mut u64) -> i32;
+        pub fn ema_ssm_scan(stream: EmaStream, x: *const c_void, ldx: i64, dt: *const c_void, ld_dt: i64,
+            b: *const c_void, ldb: i64, c: *const c_void, ldc: i64, a: *const f32, d: *const f32,
+            dt_bias: *const f32, dt_min: f32, dt_max: f32, starts: *const i32, offsets: *const i32,
+            slots: *const i32, batch: i32, n_rows: i32, max_rows: i32, n_heads: i32, head_dim: i32,
+            n_groups: i32, d_state: i32, flags: u32, state: *mut f32, n_slots: i32, y: *mut c_void, ldy: i64,
+            dtype: i32, workspace: *mut c_void, workspace_bytes: u64) -> i32;
+        pub fn ema_gated_norm(stream: EmaStream, x: *const c_void, ldx: i64, gate: *const c_void, ldg: i64,
+            w: *const c_void, eps: f32, n_rows: i32, dim: i32, group: i32, flags: u32, y: *mut c_void,
+            ldy: i64, dtype: i32) -> i32;
+        pub fn ema_residual_norm(stream: EmaStream, branch: *const c_void, ldx: i64, post_w: *const c_void,
+            gate: *const c_void, ldg: i64, scale: f32, residual: *mut c_void, ldr: i64, residual_dtype: i32,
+            pre_w: *const c_void, eps: f32, n_rows: i32, dim: i32, flags: u32, out: *mut c_void, ldo: i64,
+            dtype: i32) -> i32;
         pub fn ema_quantized_matmul(stream: EmaStream, x: *const c_void, ldx: i64, w: *const u32,
                                     scales: *const c_void, biases: *const c_void, y: *mut c_void, ldy: i64,
                                     m: i32, n: i32, k: i32, group_size: i32, bits: i32, dtype: i32) -> i32;

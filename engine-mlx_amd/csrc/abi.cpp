@@ -13,6 +13,7 @@
 #include <mutex>
 
 #include "ema_common.hpp"
+#include "packed.hpp"
 #include "paged.hpp"
 
 namespace ema {
@@ -886,6 +887,221 @@ int32_t ema_gdn_scan_ws(ema_stream_t stream, const void* q, const void* k, const
                      (unsigned long long)gdn_wy_chunk_bytes(batch, hk, hv, dk, dv));
   return launch_gdn_wy((hipStream_t)stream, q, k, v, g, beta, state, y, batch, n_tokens, hk, hv, dk, dv, workspace,
                        workspace_bytes);
+}
+
+// What the mixer calls share.
+static int32_t check_mixer_dtype(const char* op, int32_t dtype) {
+  if (dtype != EMA_DTYPE_BF16 && dtype != EMA_DTYPE_F16 && dtype != EMA_DTYPE_F32)
+    return set_error(EMA_ERR_INVALID_ARG, "%s: dtype %d is not bf16, f16 or f32", op, dtype);
+  return EMA_OK;
+}
+static uintptr_t el_mask(int32_t dtype) { return dtype == EMA_DTYPE_F32 ? 3u : 1u; }
+static int32_t check_packed(const char* op, int32_t batch, int32_t n_rows, int32_t max_rows, bool uniform) {
+  if (batch <= 0 || n_rows < 0 || max_rows < 0)
+    return set_error(EMA_ERR_SHAPE, "%s: batch=%d n_rows=%d max_rows=%d", op, batch, n_rows, max_rows);
+  if (batch > kPackedMaxB) return set_error(EMA_ERR_UNSUPPORTED, "%s: batch %d exceeds %d", op, batch, kPackedMaxB);
+  if (n_rows > (1 << 30)) return set_error(EMA_ERR_UNSUPPORTED, "%s: %d rows exceed 2^30", op, n_rows);
+  if (uniform && n_rows % batch)
+    return set_error(EMA_ERR_SHAPE, "%s: %d rows are not the same number for each of %d sequences (pass starts)", op,
+                     n_rows, batch);
+  return EMA_OK;
+}
+static int32_t check_slots(const char* op, const int32_t* slots, int32_t n_slots, int32_t batch) {
+  if (n_slots <= 0) return set_error(EMA_ERR_SHAPE, "%s: %d state slots", op, n_slots);
+  if (!slots && n_slots < batch)
+    return set_error(EMA_ERR_CAPACITY, "%s: %d sequences without slots need as many states, not %d", op, batch, n_slots);
+  return EMA_OK;
+}
+
+extern "C" int32_t ema_causal_conv(ema_stream_t stream, const void* x, int64_t ldx, const void* w, const void* bias,
+                                   const int32_t* starts, const int32_t* offsets, const int32_t* slots, int32_t batch,
+                                   int32_t n_rows, int32_t max_rows, int32_t channels, int32_t width, uint32_t flags,
+                                   void* state, int32_t n_slots, void* y, int64_t ldy, int32_t dtype) {
+  const char* op = "ema_causal_conv";
+  int32_t rc = check_mixer_dtype(op, dtype);
+  if (rc) return rc;
+  if ((rc = check_packed(op, batch, n_rows, max_rows, !starts))) return rc;
+  if (channels <= 0) return set_error(EMA_ERR_SHAPE, "%s: %d channels", op, channels);
+  if (width < 2 || width > 4) return set_error(EMA_ERR_UNSUPPORTED, "%s: width %d not supported (2, 3, 4)", op, width);
+  if (flags & ~EMA_CONV_SILU) return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
+  if (state && (rc = check_slots(op, slots, n_slots, batch))) return rc;
+  if (n_rows == 0) return EMA_OK;
+  if (!x || !w || !y) return set_error(EMA_ERR_INVALID_ARG, "%s: null x/w/y", op);
+  if (ldx < channels || ldy < channels)
+    return set_error(EMA_ERR_SHAPE, "%s: row strides %lld and %lld are below %d channels", op, (long long)ldx,
+                     (long long)ldy, channels);
+  if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)state | (uintptr_t)y) & el_mask(dtype))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: misaligned buffer", op);
+  if (x == y) return set_error(EMA_ERR_INVALID_ARG, "%s: y must not be x", op);
+  if (channels > (1 << 21)) return set_error(EMA_ERR_UNSUPPORTED, "%s: %d channels exceed 2^21", op, channels);
+  const CausalConvArgs a{x,   w,   bias,           starts, offsets, slots,    state, y,
+                   ldx, ldy, n_rows / batch, batch,  n_rows,  channels, width, n_slots, (int)(flags & EMA_CONV_SILU)};
+  return launch_causal_conv((hipStream_t)stream, a, dtype);
+}
+
+static int32_t check_ssm_shape(const char* op, int32_t n_heads, int32_t head_dim, int32_t d_state, int32_t n_groups) {
+  if (n_heads <= 0 || head_dim <= 0 || d_state <= 0 || n_groups <= 0)
+    return set_error(EMA_ERR_SHAPE, "%s: dims must be positive (n_heads=%d head_dim=%d d_state=%d n_groups=%d)", op,
+                     n_heads, head_dim, d_state, n_groups);
+  if (n_heads % n_groups)
+    return set_error(EMA_ERR_SHAPE, "%s: n_heads %d is not a multiple of n_groups %d", op, n_heads, n_groups);
+  if (d_state % 4 || d_state > 256)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: d_state %d is not a multiple of 4 up to 256", op, d_state);
+  if (n_heads > 65535 || head_dim > 4096)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %d heads of %d (at most 65535 of 4096)", op, n_heads, head_dim);
+  return EMA_OK;
+}
+
+extern "C" int32_t ema_ssm_workspace_size(int32_t batch, int32_t n_rows, int32_t max_rows, int32_t n_heads,
+                                          int32_t head_dim, int32_t d_state, int32_t n_groups, int32_t dtype,
+                                          uint64_t* bytes) {
+  const char* op = "ema_ssm_workspace_size";
+  if (!bytes) return set_error(EMA_ERR_INVALID_ARG, "%s: output is null", op);
+  *bytes = 0;
+  int32_t rc = check_mixer_dtype(op, dtype);
+  if (rc) return rc;
+  if ((rc = check_packed(op, batch, n_rows, max_rows, false))) return rc;
+  if ((rc = check_ssm_shape(op, n_heads, head_dim, d_state, n_groups))) return rc;
+  for (int vectors = 0; vectors < 2; ++vectors) {
+    const uint64_t need = plan_ssm(batch, n_rows, max_rows < n_rows ? max_rows : n_rows, n_heads, head_dim, d_state,
+                                   n_groups, dtype, vectors != 0, UINT64_MAX).bytes;
+    if (need > *bytes) *bytes = need;
+  }
+  return EMA_OK;
+}
+
+extern "C" int32_t ema_ssm_scan(ema_stream_t stream, const void* x, int64_t ldx, const void* dt, int64_t ld_dt,
+                                const void* b, int64_t ldb, const void* c, int64_t ldc, const float* a, const float* d,
+                                const float* dt_bias, float dt_min, float dt_max, const int32_t* starts,
+                                const int32_t* offsets, const int32_t* slots, int32_t batch, int32_t n_rows,
+                                int32_t max_rows, int32_t n_heads, int32_t head_dim, int32_t n_groups, int32_t d_state,
+                                uint32_t flags, float* state, int32_t n_slots, void* y, int64_t ldy, int32_t dtype,
+                                void* workspace, uint64_t workspace_bytes) {
+  const char* op = "ema_ssm_scan";
+  int32_t rc = check_mixer_dtype(op, dtype);
+  if (rc) return rc;
+  if ((rc = check_packed(op, batch, n_rows, max_rows, !starts))) return rc;
+  if ((rc = check_ssm_shape(op, n_heads, head_dim, d_state, n_groups))) return rc;
+  if (flags & ~EMA_SSM_SOFTPLUS) return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
+  if ((rc = check_slots(op, slots, n_slots, batch))) return rc;
+  if (!(dt_min <= dt_max)) return set_error(EMA_ERR_INVALID_ARG, "%s: dt_min must be at most dt_max", op);
+  if (n_rows == 0) return EMA_OK;
+  if (!x || !dt || !b || !c || !a || !state || !y)
+    return set_error(EMA_ERR_INVALID_ARG, "%s: null x/dt/b/c/a/state/y", op);
+  const int64_t wide = (int64_t)n_heads * head_dim, bc = (int64_t)n_groups * d_state;
+  if (ldx < wide || ldy < wide || ld_dt < n_heads || ldb < bc || ldc < bc)
+    return set_error(EMA_ERR_SHAPE, "%s: a row stride is below its row (x %lld, y %lld, dt %lld, b %lld, c %lld)", op,
+                     (long long)ldx, (long long)ldy, (long long)ld_dt, (long long)ldb, (long long)ldc);
+  const uintptr_t four = dtype == EMA_DTYPE_F32 ? 15u : 7u;
+  if ((((uintptr_t)x | (uintptr_t)dt | (uintptr_t)y) & el_mask(dtype)) ||
+      (((uintptr_t)a | (uintptr_t)d | (uintptr_t)dt_bias) & 3u) || (((uintptr_t)b | (uintptr_t)c) & four) || (ldb & 3) ||
+      (ldc & 3) || !aligned16(state))
+    return set_error(EMA_ERR_INVALID_ARG,
+                     "%s: misaligned buffer (state 16-byte; b and c and their strides to 4 elements)", op);
+  if (x == y) return set_error(EMA_ERR_INVALID_ARG, "%s: y must not be x", op);
+  if (workspace && !aligned16(workspace))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", op);
+  if (!starts) max_rows = n_rows / batch;
+  if (max_rows > n_rows) max_rows = n_rows;
+  const bool vectors = dtype == EMA_DTYPE_BF16 && aligned16(x) && aligned16(b) && aligned16(c) && aligned16(y) &&
+                       !(ldx & 7) && !(ldb & 7) && !(ldc & 7) && !(ldy & 7);
+  const SsmPlan plan = plan_ssm(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype, vectors,
+                                workspace ? workspace_bytes : 0);
+  if (plan.pieces * n_heads * ((head_dim + 3) / 4) >= INT32_MAX)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %lld pieces of %d heads of %d are too many", op, (long long)plan.pieces,
+                     n_heads, head_dim);
+  SsmArgs p{};
+  p.x = x;
+  p.dt = dt;
+  p.b = b;
+  p.c = c;
+  p.a = a;
+  p.d = d;
+  p.dt_bias = dt_bias;
+  p.starts = starts;
+  p.offsets = offsets;
+  p.slots = slots;
+  p.state = state;
+  p.y = y;
+  p.ldx = ldx;
+  p.lddt = ld_dt;
+  p.ldb = ldb;
+  p.ldc = ldc;
+  p.ldy = ldy;
+  p.dt_min = dt_min;
+  p.dt_max = dt_max;
+  p.T = n_rows / batch;
+  p.batch = batch;
+  p.n_rows = n_rows;
+  p.heads = n_heads;
+  p.head_dim = head_dim;
+  p.groups = n_groups;
+  p.d_state = d_state;
+  p.n_slots = n_slots;
+  p.softplus = flags & EMA_SSM_SOFTPLUS;
+  return launch_ssm((hipStream_t)stream, p, plan, workspace, dtype);
+}
+
+static int32_t check_norm_rows(const char* op, int32_t n_rows, int32_t dim, float eps) {
+  if (n_rows < 0 || dim <= 0) return set_error(EMA_ERR_SHAPE, "%s: n_rows=%d dim=%d", op, n_rows, dim);
+  if (!(eps >= 0.f)) return set_error(EMA_ERR_INVALID_ARG, "%s: eps must be >= 0", op);
+  return EMA_OK;
+}
+constexpr int32_t kNormMaxDim = 16384;  // values that a workgroup's registers hold
+
+extern "C" int32_t ema_gated_norm(ema_stream_t stream, const void* x, int64_t ldx, const void* gate, int64_t ldg,
+                                  const void* w, float eps, int32_t n_rows, int32_t dim, int32_t group, uint32_t flags,
+                                  void* y, int64_t ldy, int32_t dtype) {
+  const char* op = "ema_gated_norm";
+  int32_t rc = check_mixer_dtype(op, dtype);
+  if (rc) return rc;
+  if ((rc = check_norm_rows(op, n_rows, dim, eps))) return rc;
+  if (group <= 0 || dim % group) return set_error(EMA_ERR_SHAPE, "%s: dim %d is not a multiple of group %d", op, dim, group);
+  if (group > kNormMaxDim) return set_error(EMA_ERR_UNSUPPORTED, "%s: group %d exceeds %d", op, group, kNormMaxDim);
+  if (flags & ~(EMA_NORM_GATE_FIRST | EMA_NORM_GATE_SIGMOID | EMA_NORM_SHARED_WEIGHT | EMA_NORM_UNIT_OFFSET))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
+  if (n_rows == 0) return EMA_OK;
+  if (!x || !y) return set_error(EMA_ERR_INVALID_ARG, "%s: null x/y", op);
+  if (ldx < dim || ldy < dim || (gate && ldg < dim))
+    return set_error(EMA_ERR_SHAPE, "%s: a row stride is below dim %d (x %lld, gate %lld, y %lld)", op, dim,
+                     (long long)ldx, (long long)ldg, (long long)ldy);
+  if (((uintptr_t)x | (uintptr_t)gate | (uintptr_t)w | (uintptr_t)y) & el_mask(dtype))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: misaligned buffer", op);
+  if ((y == x && ldy != ldx) || (y == gate && ldy != ldg))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: y in its input's place needs its row stride", op);
+  if ((int64_t)n_rows * (dim / group) >= INT32_MAX)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %d rows of %d groups are too many", op, n_rows, dim / group);
+  const GatedNormArgs a{x, gate, w, y, ldx, gate ? ldg : 0, ldy, eps, n_rows, group, dim / group, flags};
+  return launch_gated_norm((hipStream_t)stream, a, dtype);
+}
+
+extern "C" int32_t ema_residual_norm(ema_stream_t stream, const void* branch, int64_t ldx, const void* post_w,
+                                     const void* gate, int64_t ldg, float scale, void* residual, int64_t ldr,
+                                     int32_t residual_dtype, const void* pre_w, float eps, int32_t n_rows, int32_t dim,
+                                     uint32_t flags, void* out, int64_t ldo, int32_t dtype) {
+  const char* op = "ema_residual_norm";
+  int32_t rc = check_mixer_dtype(op, dtype);
+  if (rc) return rc;
+  if (residual_dtype != dtype && residual_dtype != EMA_DTYPE_F32)
+    return set_error(EMA_ERR_INVALID_ARG, "%s: residual dtype %d is neither the activations' nor f32", op, residual_dtype);
+  if ((rc = check_norm_rows(op, n_rows, dim, eps))) return rc;
+  if (dim > kNormMaxDim) return set_error(EMA_ERR_UNSUPPORTED, "%s: dim %d exceeds %d", op, dim, kNormMaxDim);
+  if (flags & ~EMA_NORM_UNIT_OFFSET) return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
+  if (!out != !pre_w) return set_error(EMA_ERR_INVALID_ARG, "%s: out and pre_w go together", op);
+  if (n_rows == 0) return EMA_OK;
+  if (!branch || !residual) return set_error(EMA_ERR_INVALID_ARG, "%s: null branch/residual", op);
+  if (ldx < dim || ldr < dim || (out && ldo < dim) || (gate && ldg != 0 && ldg < dim))
+    return set_error(EMA_ERR_SHAPE, "%s: a row stride is below dim %d (branch %lld, residual %lld, gate %lld, out %lld)",
+                     op, dim, (long long)ldx, (long long)ldr, (long long)ldg, (long long)ldo);
+  if ((((uintptr_t)branch | (uintptr_t)post_w | (uintptr_t)gate | (uintptr_t)pre_w | (uintptr_t)out) & el_mask(dtype)) ||
+      ((uintptr_t)residual & el_mask(residual_dtype)))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: misaligned buffer", op);
+  if (branch == residual || out == residual || gate == residual || (gate && out == gate) || (out == branch && ldo != ldx))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: the residual stream and the gate have places of their own; out in the "
+                     "branch's place needs its row stride", op);
+  const ResidualNormArgs a{branch, post_w, gate,  pre_w, residual, out, ldx, gate ? ldg : 0,
+                           ldr,    out ? ldo : 0, scale, eps,      n_rows, dim, flags};
+  return launch_residual_norm((hipStream_t)stream, a, dtype, residual_dtype);
 }
 
 int32_t ema_quantized_matmul(ema_stream_t stream, const void* x, int64_t ldx, const uint32_t* w, const void* scales,

@@ -287,6 +287,75 @@ uint64_t gdn_wy_chunk_bytes(int B, int hk, int hv, int dk, int dv);
 int32_t launch_gdn_wy(hipStream_t s, const void* q, const void* k, const void* v, const float* g, const float* beta,
                       float* state, void* y, int B, int T, int hk, int hv, int dk, int dv, void* ws,
                       uint64_t ws_bytes);
+// The mixer calls (arguments validated by the caller).
+struct CausalConvArgs {
+  const void* x;
+  const void* w;
+  const void* bias;         // null: none
+  const int32_t* starts;    // null: T rows per sequence
+  const int32_t* offsets;   // null: every sequence continues
+  const int32_t* slots;     // null: slot b
+  void* state;              // null: none
+  void* y;
+  int64_t ldx, ldy;
+  int T, batch, n_rows, channels, width, n_slots, silu;
+};
+int32_t launch_causal_conv(hipStream_t s, const CausalConvArgs& a, int dtype);
+struct GatedNormArgs {
+  const void* x;
+  const void* gate;  // null: none
+  const void* w;     // null: none
+  void* y;
+  int64_t ldx, ldg, ldy;
+  float eps;
+  int n_rows, group, groups;  // groups of a row
+  uint32_t flags;
+};
+int32_t launch_gated_norm(hipStream_t s, const GatedNormArgs& a, int dtype);
+struct ResidualNormArgs {
+  const void* branch;
+  const void* post_w;  // null: none
+  const void* gate;    // null: none
+  const void* pre_w;
+  void* residual;
+  void* out;           // null: the residual stream alone
+  int64_t ldx, ldg, ldr, ldo;
+  float scale, eps;
+  int n_rows, dim;
+  uint32_t flags;
+};
+int32_t launch_residual_norm(hipStream_t s, const ResidualNormArgs& a, int dtype, int residual_dtype);
+struct SsmArgs {
+  const void* x;
+  const void* dt;
+  const void* b;
+  const void* c;
+  const float* a;
+  const float* d;        // null: 0
+  const float* dt_bias;  // null: 0
+  const int32_t* starts;
+  const int32_t* offsets;
+  const int32_t* slots;
+  float* state;
+  void* y;
+  float* carry;        // workspace: state of each (piece, head), then its decay; null: no cut
+  float* carry_decay;
+  int64_t ldx, lddt, ldb, ldc, ldy;
+  float dt_min, dt_max;
+  int T, batch, n_rows, heads, head_dim, groups, d_state, n_slots, softplus;
+  int piece;  // rows of a piece (2^30: a sequence is one)
+};
+// How a call runs: pieces of how many rows, on which kernels.
+struct SsmPlan {
+  int piece;        // rows of a piece, 0: no cut
+  int64_t pieces;   // piece numbers
+  bool chunks;      // on the matrix cores
+  uint64_t bytes;   // of the workspace
+};
+// ws_bytes: the workspace that there is; vectors: rows allow 16-byte accesses.
+SsmPlan plan_ssm(int batch, int n_rows, int max_rows, int heads, int head_dim, int d_state, int groups, int dtype,
+                 bool vectors, uint64_t ws_bytes);
+int32_t launch_ssm(hipStream_t s, SsmArgs& a, const SsmPlan& plan, void* ws, int dtype);
 // Affine-quantised matmul y = x W^T over MLX-packed W (arguments validated by the caller).
 int32_t launch_qmatmul(hipStream_t s, const void* x, int64_t ldx, const void* w, const void* scales,
                        const void* biases, void* y, int64_t ldy, int M, int N, int K, int gs, int bits,

@@ -1,0 +1,35 @@
+// Shared by the token-by-token and the chunked state space scans (ssm.hip, ssm_chunk.hip).
+//
+// The state space recurrence of head h (S is [head_dim, d_state], f32) is
+//   S = exp(d_t A) S + d_t x_t B_t^T,   y_t = S C_t + D x_t
+// so a piece of rows t0 .. t1 maps its start state S to decay S + E, with
+//   decay = exp(A sum d_t)   and   E = sum_t exp(A sum_{u > t} d_u) d_t x_t B_t^T
+// both independent of S. A long sequence is cut into pieces that run at once: one launch forms every
+// piece's E and decay (all pieces but a sequence's last), one joins them in order into the pieces'
+// start states, one runs the pieces from those.
+#pragma once
+
+#include "packed.hpp"
+
+namespace ema {
+
+enum SsmPhase {
+  kSsmWhole = 0,   // a piece is a sequence: start from the pool, write y and the pool
+  kSsmEnds = 1,    // E and decay of each piece that is not its sequence's last
+  kSsmPieces = 2,  // from the joined start states: y, and the pool from the last piece
+};
+
+#if defined(__HIPCC__)
+// The step of raw value r (dt + bias): softplus (r itself above 20, where they differ by less than
+// 2^-28 of it), then the limits.
+__device__ __forceinline__ float ssm_step(float r, const SsmArgs& a) {
+  if (a.softplus) r = r > 20.0f ? r : log1pf(__expf(r));
+  return fminf(fmaxf(r, a.dt_min), a.dt_max);
+}
+#endif
+
+// Chunked scan on the matrix cores, bf16.
+bool ssm_chunk_shape(int head_dim, int d_state, int heads, int groups);
+hipError_t launch_ssm_chunk(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhase phase);
+
+}  // namespace ema

@@ -41,6 +41,12 @@ EMA_KV_ROTATING = 1
 EMA_PREFILL_CAUSAL = 1
 EMA_PREFILL_CHUNK_ONLY = 2
 EMA_PREFILL_ROWS_DECODED = 4
+EMA_CONV_SILU = 1
+EMA_SSM_SOFTPLUS = 1
+EMA_NORM_GATE_FIRST = 1
+EMA_NORM_GATE_SIGMOID = 2
+EMA_NORM_SHARED_WEIGHT = 4
+EMA_NORM_UNIT_OFFSET = 8
 
 EXPORTED = (
     "ema_last_error", "ema_version", "ema_kvcache_init", "ema_kvcache_alloc", "ema_kvcache_free",
@@ -50,7 +56,8 @@ EXPORTED = (
     "ema_decode_attention", "ema_decode_step", "ema_decode_step_noalloc", "ema_prefill_attention", "ema_prefill_workspace_size",
     "ema_prefill_attention_ws", "ema_gdn_scan", "ema_gdn_scan_workspace_size", "ema_gdn_scan_ws",
     "ema_quantized_matmul", "ema_paged_append", "ema_paged_workspace_size", "ema_paged_attention",
-    "ema_prefix_attention",
+    "ema_prefix_attention", "ema_causal_conv", "ema_ssm_workspace_size", "ema_ssm_scan", "ema_gated_norm",
+    "ema_residual_norm",
 )
 
 
@@ -120,6 +127,12 @@ def lib() -> ctypes.CDLL:
             "ema_paged_attention": (i32, [vp, vp, D, vp, i32, vp, vp, i32, i32, i32, i32, i32, f32, u32, vp, vp, u64]),
             "ema_prefix_attention": (i32, [vp, vp, D, vp, i32, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, f32,
                                            vp, vp, u64]),
+            "ema_causal_conv": (i32, [vp, vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, u32, vp, i32, vp, i64, i32]),
+            "ema_ssm_workspace_size": (i32, [i32] * 8 + [ctypes.POINTER(u64)]),
+            "ema_ssm_scan": (i32, [vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, f32, f32, vp, vp, vp, i32, i32, i32,
+                                   i32, i32, i32, i32, u32, vp, i32, vp, i64, i32, vp, u64]),
+            "ema_gated_norm": (i32, [vp, vp, i64, vp, i64, vp, f32, i32, i32, i32, u32, vp, i64, i32]),
+            "ema_residual_norm": (i32, [vp, vp, i64, vp, vp, i64, f32, vp, i64, i32, vp, f32, i32, i32, u32, vp, i64, i32]),
             "ema_quantized_matmul": (i32, [vp, vp, i64, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32]),
         }
         for name, (res, args) in sig.items():
@@ -733,4 +746,251 @@ def prefix_attention(q, cache: PagedCache, prefix_table, prefix_len, max_prefix,
                 prefix_table.numel(), prefix_len.data_ptr(), max_prefix, table.data_ptr(), cols, _ptr(q_starts),
                 lengths.data_ptr(), B, n, max_q, max_len, Hq, scale, out.data_ptr(), workspace.data_ptr(),
                 workspace.numel())
+    return out
+
+
+# ---- around the recurrent scans: convolution, state space scan, norms
+
+
+_act_codes: dict = {}
+
+
+def _act_code(op: str, t):
+    """EMA_DTYPE_* of an activation tensor."""
+    import torch
+
+    if not _act_codes:
+        _act_codes.update({torch.bfloat16: EMA_DTYPE_BF16, torch.float16: EMA_DTYPE_F16, torch.float32: EMA_DTYPE_F32})
+    code = _act_codes.get(t.dtype)
+    if code is None:
+        raise EmaError(EMA_ERR_INVALID_ARG, op, f"unsupported activation dtype {t.dtype}")
+    return code
+
+
+def _rows_of(op: str, name: str, t, dtype, shape, device: int) -> int:
+    """Row stride of a [n, ...] tensor of the given dtype and shape whose rows are contiguous."""
+    if t.shape != shape or t.dtype is not dtype:
+        raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be a {dtype} tensor {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != device:
+        raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} is on {t.device}, not on device {device}")
+    width = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if stride != width and size != 1:
+            raise EmaError(EMA_ERR_SHAPE, op, f"a row of {name} must be contiguous, not strided {t.stride()}")
+        width *= size
+    # (the stride of a single row, or of none, means nothing: a view may give any)
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+def _batch_of(op: str, n: int, dev: int, starts, offsets, slots, batch):
+    """The number of sequences; checks the int32 tensors that describe them."""
+    import torch
+
+    if batch is None:
+        batch = (starts.shape[0] - 1 if starts is not None else offsets.shape[0] if offsets is not None
+                 else slots.shape[0] if slots is not None else None)
+        if batch is None:
+            raise EmaError(EMA_ERR_INVALID_ARG, op, "batch is needed without starts, offsets and slots")
+    for name, t, size in (("starts", starts, batch + 1), ("offsets", offsets, batch), ("slots", slots, batch)):
+        if t is not None and not (t.dtype is torch.int32 and t.shape == (size,) and t.is_contiguous()
+                                  and t.get_device() == dev):
+            _want(op, name, t, torch.int32, (size,), dev)
+    return batch
+
+
+def _mixer_call(op: str, dev: int, stream, *args) -> None:
+    """The library's call on `dev`'s current stream, or the given one, with `dev` current."""
+    import torch
+
+    if dev < 0:
+        raise EmaError(EMA_ERR_INVALID_ARG, op, "the tensors are not on a GPU")
+    raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    call = getattr(lib(), op)
+    rc = call(raw, *args) if torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, raw, *args)
+    if rc:
+        _check(rc, op)
+
+
+def causal_conv(x, weight, bias=None, state=None, starts=None, offsets=None, slots=None, batch=None, max_rows=None,
+                silu=True, out=None, stream=None):
+    """Short causal convolution of each channel over its sequence's time (ema_causal_conv): x [n, C] (rows may
+    be pieces of wider ones) in bf16, f16 or f32, weight [C, W] and bias [C] in the same type, W 2 to 4; state
+    [n_slots, W-1, C], the inputs kept between calls, updated in place (None: start from zeros, keep nothing).
+    starts int32 [B+1] (None: n / B rows each), offsets int32 [B] (position of the first row: at 0 a sequence
+    starts from zeros), slots int32 [B] (None: slot b). Returns out [n, C]."""
+    import torch
+
+    op = "ema_causal_conv"
+    try:
+        code, dev, dtype = _act_code(op, x), x.get_device(), x.dtype
+        if x.dim() != 2 or weight.dim() != 2:
+            raise EmaError(EMA_ERR_SHAPE, op, f"x must be [n, C] and weight [C, W], not {tuple(x.shape)}, {tuple(weight.shape)}")
+        n, C = x.shape
+        W = weight.shape[1]
+        if batch is None and starts is None and offsets is None and slots is None:
+            batch = state.shape[0] if state is not None else 1
+        batch = _batch_of(op, n, dev, starts, offsets, slots, batch)
+        if out is None:
+            with _on(stream):
+                out = torch.empty((n, C), dtype=dtype, device=x.device)
+        ldx, ldy = _rows_of(op, "x", x, dtype, (n, C), dev), _rows_of(op, "out", out, dtype, (n, C), dev)
+        _want(op, "weight", weight, dtype, (C, W), dev)
+        if bias is not None:
+            _want(op, "bias", bias, dtype, (C,), dev)
+        if state is not None:
+            _want(op, "state", state, dtype, (state.shape[0], W - 1, C), dev)
+    except AttributeError:
+        _no_tensor(op, dict(x=x, weight=weight),
+                   dict(bias=bias, state=state, starts=starts, offsets=offsets, slots=slots, out=out))
+        raise
+    _mixer_call(op, dev, stream, x.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(starts), _ptr(offsets),
+                _ptr(slots), batch, n, n if max_rows is None else max_rows, C, W, EMA_CONV_SILU if silu else 0,
+                _ptr(state), 0 if state is None else state.shape[0], out.data_ptr(), ldy, code)
+    return out
+
+
+def ssm_workspace_size(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype=None) -> int:
+    """Bytes with which ssm_scan splits such a call in time as it likes best (0: it does not); dtype a torch
+    type, bf16 by default."""
+    import torch
+
+    out = ctypes.c_uint64()
+    code = {None: EMA_DTYPE_BF16, torch.bfloat16: EMA_DTYPE_BF16, torch.float16: EMA_DTYPE_F16,
+            torch.float32: EMA_DTYPE_F32}.get(dtype, 0)
+    _check(lib().ema_ssm_workspace_size(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, code,
+                                        ctypes.byref(out)), "ema_ssm_workspace_size")
+    return out.value
+
+
+def ssm_workspace(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype=None, device="cuda"):
+    """A workspace for ssm_scan (no initialisation needed), reusable on one stream."""
+    import torch
+
+    return torch.empty(ssm_workspace_size(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype),
+                       dtype=torch.uint8, device=device)
+
+
+def ssm_scan(x, dt, B, C, A, state, D=None, dt_bias=None, starts=None, offsets=None, slots=None, batch=None,
+             max_rows=None, softplus=True, dt_limit=(0.0, math.inf), out=None, workspace=None, stream=None):
+    """Selective state space scan, one decay per head (ema_ssm_scan): x [n, H, P], dt [n, H], B and C [n, G, N]
+    in bf16, f16 or f32 (rows may be pieces of wider ones); A (at most 0), D, dt_bias f32 [H]; state f32
+    [n_slots, H, P, N], updated in place; starts, offsets, slots as in causal_conv; max_rows a host bound of a
+    sequence's rows. workspace: a uint8 tensor (ssm_workspace) that long sequences are split over; None
+    allocates one. Returns out [n, H, P]."""
+    import torch
+
+    op = "ema_ssm_scan"
+    try:
+        code, dev, dtype = _act_code(op, x), x.get_device(), x.dtype
+        if x.dim() != 3 or B.dim() != 3 or state.dim() != 4:
+            raise EmaError(EMA_ERR_SHAPE, op, f"x [n, H, P], B [n, G, N] and state [n_slots, H, P, N] are wanted, not "
+                                              f"{tuple(x.shape)}, {tuple(B.shape)}, {tuple(state.shape)}")
+        n, H, P = x.shape
+        G, N = B.shape[1:]
+        if batch is None and starts is None and offsets is None and slots is None:
+            batch = state.shape[0]
+        batch = _batch_of(op, n, dev, starts, offsets, slots, batch)
+        if max_rows is None:
+            max_rows = n
+        if out is None:
+            with _on(stream):
+                out = torch.empty((n, H, P), dtype=dtype, device=x.device)
+        ldx, ldy = _rows_of(op, "x", x, dtype, (n, H, P), dev), _rows_of(op, "out", out, dtype, (n, H, P), dev)
+        ldb, ldc = _rows_of(op, "B", B, dtype, (n, G, N), dev), _rows_of(op, "C", C, dtype, (n, G, N), dev)
+        lddt = _rows_of(op, "dt", dt, dtype, (n, H), dev)
+        f32 = torch.float32
+        for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
+            if (t is not None or name == "A") and not (t.dtype is f32 and t.shape == (H,) and t.is_contiguous()
+                                                       and t.get_device() == dev):
+                _want(op, name, t, f32, (H,), dev)
+        _want(op, "state", state, f32, (state.shape[0], H, P, N), dev)
+        if workspace is not None:
+            _want(op, "workspace", workspace, torch.uint8, workspace.shape, dev)
+    except AttributeError:
+        _no_tensor(op, dict(x=x, dt=dt, B=B, C=C, A=A, state=state),
+                   dict(D=D, dt_bias=dt_bias, starts=starts, offsets=offsets, slots=slots, out=out, workspace=workspace))
+        raise
+    if workspace is None and dev >= 0 and n:
+        with _on(stream):
+            workspace = ssm_workspace(batch, n, max_rows, H, P, N, G, dtype, device=x.device)
+    _mixer_call(op, dev, stream, x.data_ptr(), ldx, dt.data_ptr(), lddt, B.data_ptr(), ldb, C.data_ptr(), ldc,
+                A.data_ptr(), _ptr(D), _ptr(dt_bias), dt_limit[0], dt_limit[1], _ptr(starts), _ptr(offsets), _ptr(slots),
+                batch, n, max_rows, H, P, G, N, EMA_SSM_SOFTPLUS if softplus else 0, state.data_ptr(), state.shape[0],
+                out.data_ptr(), ldy, code, _ptr(workspace) or None, 0 if workspace is None else workspace.numel())
+    return out
+
+
+def gated_norm(x, gate, weight, eps, group=None, gate_first=False, sigmoid=False, unit_offset=False, out=None,
+               stream=None):
+    """RMSNorm of each `group` values (default: all) of the rows x [n, dim], gated (ema_gated_norm): norm(x) * w *
+    act(gate), or norm(x * act(gate)) * w with gate_first; act is silu, or sigmoid. gate [n, dim] or None;
+    weight [dim], [group] (one for all groups) or None; unit_offset: 1 + w multiplies. Rows of x, gate and out
+    may be pieces of wider ones; out may be x or gate. Returns out [n, dim]."""
+    import torch
+
+    op = "ema_gated_norm"
+    try:
+        code, dev, dtype = _act_code(op, x), x.get_device(), x.dtype
+        if x.dim() != 2:
+            raise EmaError(EMA_ERR_SHAPE, op, f"x must be [n, dim], not {tuple(x.shape)}")
+        n, dim = x.shape
+        if group is None:
+            group = dim
+        if out is None:
+            with _on(stream):
+                out = torch.empty((n, dim), dtype=dtype, device=x.device)
+        ldx, ldy = _rows_of(op, "x", x, dtype, (n, dim), dev), _rows_of(op, "out", out, dtype, (n, dim), dev)
+        ldg = 0 if gate is None else _rows_of(op, "gate", gate, dtype, (n, dim), dev)
+        flags = ((EMA_NORM_GATE_FIRST if gate_first else 0) | (EMA_NORM_GATE_SIGMOID if sigmoid else 0)
+                 | (EMA_NORM_UNIT_OFFSET if unit_offset else 0))
+        if weight is not None:
+            if weight.shape == (group,) and group != dim:
+                flags |= EMA_NORM_SHARED_WEIGHT
+            _want(op, "weight", weight, dtype, (group,) if flags & EMA_NORM_SHARED_WEIGHT else (dim,), dev)
+    except AttributeError:
+        _no_tensor(op, dict(x=x), dict(gate=gate, weight=weight, out=out))
+        raise
+    _mixer_call(op, dev, stream, x.data_ptr(), ldx, _ptr(gate), ldg, _ptr(weight), eps, n, dim, group, flags,
+                out.data_ptr(), ldy, code)
+    return out
+
+
+def residual_norm(branch, residual, pre_weight, eps, post_weight=None, gate=None, scale=1.0, unit_offset=False,
+                  out=None, stream=None):
+    """The norm after one block and the one before the next (ema_residual_norm): residual += scale * gate *
+    norm(branch) * post_weight in place (post_weight None: the branch as it is), then returns out =
+    norm(residual) * pre_weight (of the sum before it is rounded). branch [n, dim] in bf16, f16 or f32, residual
+    [n, dim] in the same type or f32; gate [n, dim], [dim] (one for all rows) or None; pre_weight None: the
+    residual stream alone (returns None). Rows may be pieces of wider ones; out may be branch."""
+    import torch
+
+    op = "ema_residual_norm"
+    try:
+        code, dev, dtype = _act_code(op, branch), branch.get_device(), branch.dtype
+        if branch.dim() != 2:
+            raise EmaError(EMA_ERR_SHAPE, op, f"branch must be [n, dim], not {tuple(branch.shape)}")
+        n, dim = branch.shape
+        if out is None and pre_weight is not None:
+            with _on(stream):
+                out = torch.empty((n, dim), dtype=dtype, device=branch.device)
+        stream_code = EMA_DTYPE_F32 if residual.dtype is torch.float32 else code
+        ldx = _rows_of(op, "branch", branch, dtype, (n, dim), dev)
+        ldr = _rows_of(op, "residual", residual, torch.float32 if stream_code == EMA_DTYPE_F32 else dtype, (n, dim), dev)
+        ldo = 0 if out is None else _rows_of(op, "out", out, dtype, (n, dim), dev)
+        ldg = 0
+        if gate is not None:
+            if gate.dim() == 1:
+                _want(op, "gate", gate, dtype, (dim,), dev)
+            else:
+                ldg = _rows_of(op, "gate", gate, dtype, (n, dim), dev)
+        for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
+            if w is not None:
+                _want(op, name, w, dtype, (dim,), dev)
+    except AttributeError:
+        _no_tensor(op, dict(branch=branch, residual=residual),
+                   dict(pre_weight=pre_weight, post_weight=post_weight, gate=gate, out=out))
+        raise
+    _mixer_call(op, dev, stream, branch.data_ptr(), ldx, _ptr(post_weight), _ptr(gate), ldg, scale, residual.data_ptr(),
+                ldr, stream_code, _ptr(pre_weight), eps, n, dim, EMA_NORM_UNIT_OFFSET if unit_offset else 0, _ptr(out),
+                ldo, code)
     return out

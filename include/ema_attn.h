@@ -91,7 +91,7 @@ extern "C" {
  * rotating (EMA_KV_ROTATING) caches; decode only (prefill attends bf16 keys, as the
  * reference's does). */
 #define EMA_DTYPE_INT4_AFFINE 5
-/* activation types of ema_gdn_scan (besides EMA_DTYPE_BF16) */
+/* activation types of ema_gdn_scan and the mixer calls (besides EMA_DTYPE_BF16) */
 #define EMA_DTYPE_F16 3
 #define EMA_DTYPE_F32 4
 
@@ -513,6 +513,110 @@ EMA_API int32_t ema_gdn_scan_ws(ema_stream_t stream, const void* q, const void* 
                                 const float* g, const float* beta, float* state, void* y,
                                 int32_t batch, int32_t n_tokens, int32_t hk, int32_t hv, int32_t dk,
                                 int32_t dv, int32_t dtype, void* workspace, uint64_t workspace_bytes);
+
+/* ---- Around the recurrent scans: convolution, state space scan, norms --------------------
+ * The other pieces of a recurrent layer, for one token, a chunk or a prompt of every sequence of
+ * a ragged batch: in projection (ema_quantized_matmul) -> ema_causal_conv -> ema_gdn_scan or
+ * ema_ssm_scan -> ema_gated_norm -> out projection -> ema_residual_norm. dtype is the type of the
+ * activations and of the weights that multiply them: EMA_DTYPE_BF16, _F16 or _F32; arithmetic and
+ * the scan's state are in 32 bits, and every output value is rounded once. Tensors are packed rows
+ * [n_rows, ...] whose row stride ld* (elements) may be wider than a row: a piece of a projection's
+ * row is read where it lies. Outputs must not overlap inputs unless a call says that they may.
+ *   starts   device int32 [batch + 1], ascending: sequence b's rows are [starts[b], starts[b + 1]);
+ *            rows from starts[batch] on are neither read nor written. NULL: n_rows / batch rows for
+ *            every sequence. A sequence of no rows keeps its state as it is.
+ *   offsets  device int32 [batch]: position of each sequence's first row, or NULL. A sequence at
+ *            position 0 (or below) starts from a zero state, whatever its slot holds; others, and
+ *            all with NULL, from what their slot holds.
+ *   slots    device int32 [batch], or NULL (sequence b has slot b): which state of the pool
+ *            [n_slots, ...] is the sequence's. An entry outside [0, n_slots) is never followed: the
+ *            sequence starts from zeros and its state is not stored. No two sequences of a call may
+ *            have the same slot.
+ *   max_rows host bound of a sequence's rows; it chooses between kernels, and true values beyond it
+ *            still give the result.
+ * At most 4096 sequences a call. A call of no rows does nothing. The reference runs its convolution,
+ * norms and gates as separate MLX operators (crates/ops/src/gdn_forward.rs) and has no state space
+ * scan. */
+
+/* ema_causal_conv flags */
+#define EMA_CONV_SILU 1u /* y = v * sigmoid(v) of the convolved value v */
+/* ema_ssm_scan flags */
+#define EMA_SSM_SOFTPLUS 1u /* the step is softplus(dt + dt_bias), else dt + dt_bias */
+/* ema_gated_norm and ema_residual_norm flags */
+#define EMA_NORM_GATE_FIRST 1u    /* (gated) norm of x * act(gate), else norm of x times act(gate) */
+#define EMA_NORM_GATE_SIGMOID 2u  /* (gated) act is sigmoid, else silu                        */
+#define EMA_NORM_SHARED_WEIGHT 4u /* (gated) one weight [group] for all groups, else [dim]        */
+#define EMA_NORM_UNIT_OFFSET 8u   /* (both) the norm weights are stored less one: 1 + w multiplies */
+
+/* Short causal convolution of every channel over its sequence's time:
+ *   v[t, c] = bias[c] + sum_j w[c, j] * x[t - width + 1 + j, c],   y = v or silu(v)
+ * where rows before the sequence's first are the last width - 1 inputs of the call before (zeros at
+ * position 0).
+ *   x      [n_rows, ldx]: the first `channels` values of each row
+ *   w      [channels, width], width 2, 3 or 4; bias [channels] or NULL
+ *   state  [n_slots, width - 1, channels]: the last inputs, oldest first, as they came; updated in
+ *          place. NULL: all sequences start from zeros and nothing is kept (n_slots, offsets and
+ *          slots are not looked at)
+ *   y      [n_rows, ldy]: the first `channels` values of each row are written */
+EMA_API int32_t ema_causal_conv(ema_stream_t stream, const void* x, int64_t ldx, const void* w, const void* bias,
+                                const int32_t* starts, const int32_t* offsets, const int32_t* slots, int32_t batch,
+                                int32_t n_rows, int32_t max_rows, int32_t channels, int32_t width, uint32_t flags,
+                                void* state, int32_t n_slots, void* y, int64_t ldy, int32_t dtype);
+
+/* Workspace (bytes) with which ema_ssm_scan splits these bounds' rows in time as it likes best; 0
+ * where it does not split. */
+EMA_API int32_t ema_ssm_workspace_size(int32_t batch, int32_t n_rows, int32_t max_rows, int32_t n_heads,
+                                       int32_t head_dim, int32_t d_state, int32_t n_groups, int32_t dtype,
+                                       uint64_t* bytes);
+/* Selective state space scan with one decay per head: for each row t of a sequence and head h, with
+ * B and C of group h / (n_heads / n_groups),
+ *   d = clamp(softplus(dt[t, h] + dt_bias[h]), dt_min, dt_max)
+ *   S = exp(d A[h]) S + d x[t, h] B[t]^T;   y[t, h] = S C[t] + D[h] x[t, h]
+ * where S = state[slot, h] is [head_dim, d_state] f32.
+ *   x      [n_rows, ldx]: n_heads * head_dim values a row;  dt [n_rows, ld_dt]: n_heads a row
+ *   b, c   [n_rows, ldb], [n_rows, ldc]: n_groups * d_state values a row, aligned to 4 of them
+ *          (bf16, f16: 8 bytes; ldb and ldc multiples of 4)
+ *   a      [n_heads] f32, at most 0 (the decay is at most 1); d and dt_bias [n_heads] f32 or NULL
+ *   dt_min, dt_max  limits of the step (0 and infinity: none)
+ *   state  [n_slots, n_heads, head_dim, d_state] f32, 16-byte aligned, updated in place
+ *   y      [n_rows, ldy]: n_heads * head_dim values a row
+ * d_state a multiple of 4, at most 256. bf16 prompts (max_rows at least 32, d_state 64, 128 or 256,
+ * head_dim a multiple of 32, rows 16-byte aligned with strides of multiples of 8) run in chunks on
+ * the matrix cores; the others token by token. The workspace holds the states between the pieces that
+ * a long sequence is cut into, so that they run at once; a smaller one than
+ * ema_ssm_workspace_size's makes fewer, longer pieces, none (NULL, 0) no cut. It needs no
+ * initialisation and must be 16-byte aligned; calls that overlap need one each. */
+EMA_API int32_t ema_ssm_scan(ema_stream_t stream, const void* x, int64_t ldx, const void* dt, int64_t ld_dt,
+                             const void* b, int64_t ldb, const void* c, int64_t ldc, const float* a, const float* d,
+                             const float* dt_bias, float dt_min, float dt_max, const int32_t* starts,
+                             const int32_t* offsets, const int32_t* slots, int32_t batch, int32_t n_rows,
+                             int32_t max_rows, int32_t n_heads, int32_t head_dim, int32_t n_groups, int32_t d_state,
+                             uint32_t flags, float* state, int32_t n_slots, void* y, int64_t ldy, int32_t dtype,
+                             void* workspace, uint64_t workspace_bytes);
+
+/* RMSNorm of each `group` values of a row, with a gate:
+ *   y = norm(x) * w * act(gate)       or, with EMA_NORM_GATE_FIRST,   y = norm(x * act(gate)) * w
+ *   norm(u) = u / sqrt(mean u^2 + eps) over the group's values
+ *   x, gate, y  [n_rows, ld*]: the first `dim` values of each row; gate NULL: no gate. y may be x or
+ *               gate (the same address and stride)
+ *   w           [dim], or [group] with EMA_NORM_SHARED_WEIGHT; NULL: none
+ * dim a multiple of group, group at most 16384. */
+EMA_API int32_t ema_gated_norm(ema_stream_t stream, const void* x, int64_t ldx, const void* gate, int64_t ldg,
+                               const void* w, float eps, int32_t n_rows, int32_t dim, int32_t group, uint32_t flags,
+                               void* y, int64_t ldy, int32_t dtype);
+
+/* The norm after one block and the norm before the next, with the residual stream between them:
+ *   u = norm(branch) * post_w (post_w NULL: u = branch);   h = residual + scale * gate * u
+ *   residual = h;   out = norm(h) * pre_w   (of h before it is rounded to the stream's type)
+ *   branch, out  [n_rows, ld*] of `dim` values; out may be branch (the same address and stride);
+ *                out and pre_w NULL together: the residual stream alone
+ *   gate         [n_rows, ldg], or one row for all with ldg 0, or NULL: none
+ *   residual     [n_rows, ldr], updated in place, of type residual_dtype: dtype or EMA_DTYPE_F32
+ * dim at most 16384. */
+EMA_API int32_t ema_residual_norm(ema_stream_t stream, const void* branch, int64_t ldx, const void* post_w,
+                                  const void* gate, int64_t ldg, float scale, void* residual, int64_t ldr,
+                                  int32_t residual_dtype, const void* pre_w, float eps, int32_t n_rows, int32_t dim,
+                                  uint32_t flags, void* out, int64_t ldo, int32_t dtype);
 
 /* y = x W^T over an affine-quantised W in MLX's packing: MLX quantized_matmul(x, w,
  * scales, biases, transpose=true, group_size, bits, "affine"), the call behind the

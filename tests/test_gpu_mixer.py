@@ -1,0 +1,267 @@
+"""GPU tests of the mixer calls (ema_causal_conv, ema_ssm_scan, ema_gated_norm, ema_residual_norm) against their
+definitions in float64 (mixer_ref.py), at the sizes and layouts where they can go wrong."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+import mixer_ref as ref  # noqa: E402
+from mixer_ref import HALF, TINY, U  # noqa: E402
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = [BF, HF, F32]
+
+
+@pytest.fixture(scope="module")
+def ema():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need a ROCm GPU")
+    import ema_attn
+
+    ema_attn.lib()
+    return ema_attn
+
+
+def rand(seed, *shape, dtype=F32, scale=1.0, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).to(device)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def wide(t, before=8, after=8):
+    """The same values as a piece of wider rows."""
+    n, inner = t.shape[0], t[0].numel() if t.shape[0] else math.prod(t.shape[1:])
+    w = torch.full((n, before + inner + after), 77.0, dtype=t.dtype, device=t.device)
+    w[:, before:before + inner] = t.reshape(n, inner)
+    return w[:, before:before + inner].unflatten(1, t.shape[1:]) if t.dim() > 2 else w[:, before:before + inner]
+
+
+# ------------------------------------------------------------------ convolution
+def conv_case(ema, dtype, lens, C, W, seed, *, bias=True, silu=True, state=True, offsets=None, slots=None, n_slots=None,
+              tail=0, strided=False, batch=None, max_rows=None):
+    n, B = sum(lens) + tail, len(lens)
+    starts = ints([sum(lens[:i]) for i in range(B + 1)]) if len(set(lens)) > 1 or tail else None
+    x = rand(seed, n, C, dtype=dtype)
+    w = rand(seed + 1, C, W, dtype=dtype, scale=0.5)
+    b = rand(seed + 2, C, dtype=dtype, scale=0.2) if bias else None
+    pool = rand(seed + 3, n_slots or B, W - 1, C, dtype=dtype) if state else None
+    off, sl = (None if v is None else ints(v) for v in (offsets, slots))
+    want, want_pool, mag = ref.conv(x, w, b, pool, B, None if starts is None else starts.tolist(), offsets, slots, silu)
+    out = torch.full((n, C), 5.0, dtype=dtype, device="cuda")
+    xx, oo = (wide(x), wide(out)) if strided else (x, out)
+    ema.causal_conv(xx, w, bias=b, state=pool, starts=starts, offsets=off, slots=sl, batch=B, silu=silu, out=oo,
+                    max_rows=max_rows)
+    torch.cuda.synchronize()
+    used = sum(lens)
+    assert bool((oo[used:] == 5.0).all()), "rows behind the last sequence"
+    # W + 1 sums, the activation (its slope is at most 1.1) and one rounding
+    tol = HALF[dtype] * want.abs() + 1.1 * (W + 1) * U * mag + 2.0 ** -21 * want.abs() + TINY[dtype]
+    ref.check(oo[:used], want[:used], tol[:used], f"conv {dtype} {lens} C={C} W={W}")
+    if state:
+        assert torch.equal(pool.cpu().double(), want_pool), "the kept inputs are copies"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("W", [2, 3, 4])
+def test_conv_lengths(ema, dtype, W):
+    lens = [1, 2, 3, 4, 5, 0, 31, 32, 33, 64, 65, 97, 0]
+    conv_case(ema, dtype, lens, 520, W, 10, offsets=[5, 0, 7, 1, 0, 3, 1, 0, 1, 1, 0, 9, 0], n_slots=20,
+              slots=[19, 3, 4, 0, 1, 2, 8, 9, 10, 11, 12, 13, 14], tail=5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("C", [1, 7, 8, 512, 1031, 8192])
+def test_conv_channels_and_strides(ema, dtype, C):
+    conv_case(ema, dtype, [1, 40], C, 4, 20, bias=C != 8, silu=C != 7, strided=C != 1)
+    conv_case(ema, dtype, [1] * 9, C, 4, 21, strided=True)
+    conv_case(ema, dtype, [3], C, 2, 22, state=False)
+
+
+def test_conv_slots_that_are_not_there(ema):
+    """A slot outside the pool is not followed: zeros before the sequence, nothing kept."""
+    conv_case(ema, BF, [2, 5, 40, 1], 64, 4, 30, slots=[-1, 3, 1 << 30, 2], n_slots=5, offsets=[4, 4, 4, 4])
+
+
+def test_conv_many_sequences(ema):
+    lens = [(i * 7) % 5 for i in range(700)]
+    conv_case(ema, BF, lens, 16, 4, 40, offsets=[i % 3 for i in range(700)])
+    conv_case(ema, F32, [1] * 4096, 4, 3, 41)
+
+
+def test_conv_of_pieces_is_the_conv_of_the_whole(ema):
+    """A prompt in chunks and single tokens: the same bits as at once."""
+    C, W, n = 264, 4, 150
+    x, w, b = rand(50, n, C, dtype=BF), rand(51, C, W, dtype=BF), rand(52, C, dtype=BF)
+    pool = rand(53, 2, W - 1, C, dtype=BF)
+    whole = ema.causal_conv(x, w, bias=b, state=pool, offsets=ints([0]), slots=ints([1]))
+    kept = pool.clone()
+    pool2 = rand(53, 2, W - 1, C, dtype=BF)
+    at, got = 0, []
+    for n_i in [1, 1, 2, 60, 3, 1, 82]:
+        got.append(ema.causal_conv(x[at:at + n_i], w, bias=b, state=pool2, offsets=ints([at]), slots=ints([1])))
+        at += n_i
+    assert torch.equal(torch.cat(got), whole) and torch.equal(pool2, kept)
+
+
+def test_conv_values_that_are_not_finite_stay_in_their_channel(ema):
+    x, w = rand(60, 40, 64, dtype=BF), rand(61, 64, 4, dtype=BF)
+    clean = ema.causal_conv(x, w, batch=1)
+    x[7, 3], x[20, 10] = math.nan, math.inf
+    got = ema.causal_conv(x, w, batch=1)
+    touched = torch.zeros(40, 64, dtype=torch.bool, device="cuda")
+    touched[7:11, 3], touched[20:24, 10] = True, True
+    assert torch.equal(got[~touched], clean[~touched]) and bool(got[7:11, 3].isnan().all())
+
+
+# ------------------------------------------------------------------ scan
+def scan_case(ema, dtype, lens, H, P, N, G, seed, *, offsets=None, slots=None, n_slots=None, tail=0, strided=False,
+              D=True, bias=True, softplus=True, limit=(0.0, math.inf), max_rows=None, a_scale=16.0, workspace=None,
+              split_bits=0.0, dt_scale=1.0, read_bits=0.0):
+    n, B = sum(lens) + tail, len(lens)
+    starts = ints([sum(lens[:i]) for i in range(B + 1)]) if len(set(lens)) > 1 or tail else None
+    x = rand(seed, n, H, P, dtype=dtype)
+    bm, cm = rand(seed + 1, n, G, N, dtype=dtype), rand(seed + 2, n, G, N, dtype=dtype)
+    dt = rand(seed + 3, n, H, dtype=dtype, scale=dt_scale)
+    if not softplus:
+        dt = dt.abs() * 0.1
+    A = -(1 + (a_scale - 1) * torch.rand(H, generator=torch.Generator().manual_seed(seed + 4))).cuda()
+    Dw = rand(seed + 5, H) if D else None
+    db = (rand(seed + 6, H) - 3) if bias else None
+    state = rand(seed + 7, n_slots or B, H, P, N, scale=0.3)
+    off, sl = (None if v is None else ints(v) for v in (offsets, slots))
+    want, want_pool, mag, pool_mag = ref.scan(x, dt, bm, cm, A, state, B, Dw, db,
+                                              None if starts is None else starts.tolist(), offsets, slots, softplus, limit)
+    out = torch.full((n, H, P), 5.0, dtype=dtype, device="cuda")
+    xx, oo, bb, cc, tt = (wide(t, 8, 16) for t in (x, out, bm, cm, dt)) if strided else (x, out, bm, cm, dt)
+    untouched = state.clone()
+    ema.ssm_scan(xx, tt, bb, cc, A, state, D=Dw, dt_bias=db, starts=starts, offsets=off, slots=sl, batch=B,
+                 max_rows=max_rows, softplus=softplus, dt_limit=limit, out=oo, workspace=workspace)
+    torch.cuda.synchronize()
+    used = sum(lens)
+    assert bool((oo[used:] == 5.0).all()), "rows behind the last sequence"
+    # every row's step adds a few roundings of the state, the sums over rows and d_state theirs
+    rows = max(lens) if lens else 0
+    tol_y = HALF[dtype] * want.abs() + ((2 * rows + N + 16) * U + 2.0 ** -21 + read_bits) * mag + TINY[dtype]
+    tol_s = ((2 * rows + 16) * U + 2.0 ** -21 + split_bits) * pool_mag + 1e-37
+    ref.check(oo[:used], want[:used], tol_y[:used], f"scan {dtype} {lens[:12]} H={H} P={P} N={N} G={G}: y")
+    ref.check(state, want_pool, tol_s, "  state")
+    held = set(range(B)) if slots is None else {s for s, l in zip(slots, lens) if l}
+    for i in range(state.shape[0]):
+        if i not in held or (slots is None and lens[i] == 0):
+            assert torch.equal(state[i], untouched[i]), "a slot that no sequence has"
+
+
+SHAPES = [(4, 64, 128, 2), (3, 48, 80, 3), (8, 32, 64, 1), (2, 128, 256, 2), (5, 20, 36, 1), (2, 1, 4, 1), (1, 65, 16, 1)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scan_tokens(ema, dtype, shape):
+    scan_case(ema, dtype, [1] * 5, *shape, 100, slots=[6, 0, 3, -1, 5], n_slots=7, offsets=[3, 0, 1, 2, 8])
+    scan_case(ema, dtype, [1, 0, 3, 7, 2], *shape, 101, strided=shape[0] % 2 == 0, tail=3, max_rows=1)
+
+
+@pytest.mark.parametrize("dtype", [HF, F32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scan_prompts(ema, dtype, shape):
+    scan_case(ema, dtype, [1, 0, 33, 64, 130, 31], *shape, 110, slots=[6, 0, 3, 2, 5, 1], n_slots=7,
+              offsets=[3, 0, 1, 0, 8, 0], tail=2)
+
+
+def test_scan_options(ema):
+    for i, kw in enumerate([dict(D=False), dict(bias=False), dict(softplus=False), dict(limit=(0.05, 0.2)),
+                            dict(dt_scale=30.0), dict(a_scale=1.0)]):
+        scan_case(ema, F32, [40, 3], 4, 64, 128, 2, 120 + i, **kw)
+
+
+def test_scan_many_sequences(ema):
+    scan_case(ema, F32, [(i * 7) % 4 for i in range(300)], 2, 16, 16, 1, 130, offsets=[i % 3 for i in range(300)])
+
+
+# ------------------------------------------------------------------ gated norm
+def gated_case(ema, dtype, n, dim, group, seed, *, gate=True, first=False, sigmoid=False, unit=False, w="dim",
+               strided=False, scale=1.0, inplace=False):
+    x = rand(seed, n, dim, dtype=dtype, scale=scale)
+    z = rand(seed + 1, n, dim, dtype=dtype) if gate else None
+    wt = None if w is None else (rand(seed + 2, group if w == "group" else dim, scale=0.2) + (0 if unit else 1)).to(dtype)
+    want = ref.gated(x, z, wt, 1e-5, group, first, sigmoid, unit)
+    out = torch.empty_like(x)
+    if strided:
+        x, out = wide(x), wide(out)
+        z = None if z is None else wide(z, 16, 8)
+    got = ema.gated_norm(x, z, wt, 1e-5, group=group, gate_first=first, sigmoid=sigmoid, unit_offset=unit,
+                         out=x if inplace else out)
+    torch.cuda.synchronize()
+    # the sum of squares (at most group + 8 steps, half of which reaches the root) and the factors
+    tol = (HALF[dtype] + (group + 8) * U + 2.0 ** -20) * want.abs() + TINY[dtype]
+    ref.check(got, want, tol, f"gated {dtype} [{n}, {dim}/{group}]")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,group", [(128, 128), (1024, 64), (1000, 40), (1536, 192), (1024, 512), (99, 33), (520, 520),
+                                       (3000, 1500), (4096, 4096), (2049, 2049), (8192, 8192), (16384, 16384), (9001, 9001),
+                                       (7, 1), (5, 5)])
+def test_gated_sizes(ema, dtype, dim, group):
+    gated_case(ema, dtype, 3, dim, group, 200)
+    gated_case(ema, dtype, 5, dim, group, 201, first=True, w="group", strided=True)
+
+
+@pytest.mark.parametrize("kw", [dict(gate=False), dict(sigmoid=True), dict(first=True, sigmoid=True), dict(unit=True),
+                                dict(w=None), dict(w=None, gate=False), dict(unit=True, w="group"), dict(inplace=True),
+                                dict(inplace=True, strided=True), dict(scale=1e-3), dict(scale=1e3)])
+@pytest.mark.parametrize("group", [128, 640])
+def test_gated_options(ema, kw, group):
+    gated_case(ema, BF, 65, 640, group, 210, **kw)
+
+
+def test_gated_zero_rows_and_no_rows(ema):
+    x = torch.zeros(2, 256, dtype=BF, device="cuda")
+    z, w = rand(220, 2, 256, dtype=BF), rand(221, 256, dtype=BF)
+    assert bool((ema.gated_norm(x, z, w, 1e-6) == 0).all())
+    assert ema.gated_norm(x[:0], z[:0], w, 1e-6).shape == (0, 256)
+
+
+# ------------------------------------------------------------------ residual norm
+def residual_case(ema, dtype, n, dim, seed, *, stream=None, post=True, gate=None, scale=0.7, unit=False, pre=True,
+                  strided=False, inplace=False):
+    stream = stream or dtype
+    br, res = rand(seed, n, dim, dtype=dtype), rand(seed + 1, n, dim, dtype=stream)
+    pw = (rand(seed + 2, dim, scale=0.2) + (0 if unit else 1)).to(dtype) if pre else None
+    qw = (rand(seed + 3, dim, scale=0.2) + (0 if unit else 1)).to(dtype) if post else None
+    g = None if gate is None else rand(seed + 4, *((dim,) if gate == "one" else (n, dim)), dtype=dtype)
+    h, want, mag = ref.residual(br, res, pw, 1e-5, qw, g, scale, unit)
+    out = torch.empty_like(br) if pre else None
+    if strided:
+        br, res, out = wide(br), wide(res), wide(out) if pre else None
+        g = wide(g, 16, 8) if gate == "rows" else g
+    got = ema.residual_norm(br, res, pw, 1e-5, post_weight=qw, gate=g, scale=scale, unit_offset=unit,
+                            out=br if inplace else out)
+    torch.cuda.synchronize()
+    each = ((dim + 8) * U + 2.0 ** -20) * mag  # of h: the branch's norm, its factors, the sum
+    ref.check(res, h, HALF[stream] * h.abs() + each + TINY[stream], f"residual {dtype}/{stream} [{n}, {dim}]: h")
+    if pre:
+        root = torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-5)
+        w = ref.f64(pw).abs() if not unit else (1 + ref.f64(pw)).abs()
+        # what h is off by, in each value and in the root, beside the roundings of the norm itself
+        off = each / root * w + (each * h.abs()).mean(-1, keepdim=True) / root ** 2 * want.abs()
+        ref.check(got, want, (HALF[dtype] + (dim + 8) * U + 2.0 ** -20) * want.abs() + off + TINY[dtype], "  out")
+    else:
+        assert got is None
+
+
+@pytest.mark.parametrize("dtype,stream", [(BF, BF), (BF, F32), (HF, HF), (HF, F32), (F32, F32)])
+@pytest.mark.parametrize("dim", [1, 8, 100, 512, 1111, 2048, 4096, 5120, 8192, 9001, 16384])
+def test_residual_sizes(ema, dtype, stream, dim):
+    residual_case(ema, dtype, 3, dim, 300, stream=stream, gate="rows")
+    residual_case(ema, dtype, 2, dim, 301, stream=stream, post=False, strided=True, gate="one")
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(post=False), dict(unit=True), dict(pre=False), dict(gate="one"), dict(gate="rows"),
+                                dict(inplace=True), dict(inplace=True, strided=True), dict(scale=-2.0), dict(scale=0.0)])
+def test_residual_options(ema, kw):
+    residual_case(ema, BF, 33, 768, 310, **kw)
+    residual_case(ema, BF, 33, 768, 311, stream=F32, **kw)
