@@ -187,17 +187,17 @@ hipError_t launch_state(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhas
 SsmPlan plan_ssm(int batch, int n_rows, int max_rows, int heads, int head_dim, int d_state, int groups, int dtype,
                  bool vectors, uint64_t ws_bytes) {
   SsmPlan p{};
-  p.chunks = false;
-  p.piece = 0;
+  p.chunks = dtype == EMA_DTYPE_BF16 && vectors && max_rows >= 32 && ssm_chunk_shape(head_dim, d_state);
   p.pieces = batch;
-  p.bytes = 0;
-  // Cut where the sequences' heads leave most of the chip idle: into pieces that give every CU four
-  // workgroups, of at least 32 rows; the pieces' ends take about as long again as the pieces.
-  const int64_t wgs = (int64_t)batch * heads * ((head_dim + 63) / 64);
-  const int64_t want = 4 * (int64_t)device_cus() / wgs;
-  if (want < 4 || max_rows < 64) return p;
+  // Cut where the sequences' heads leave most of the chip idle: into pieces that give every CU two
+  // (chunks) or four workgroups; the pieces' ends take about half as long again (chunks) or as long.
+  const int64_t wgs = batch * (p.chunks ? (int64_t)ssm_chunk_workgroups(heads, head_dim, groups)
+                                        : heads * (int64_t)((head_dim + 63) / 64));
+  const int64_t want = (p.chunks ? 2 : 4) * (int64_t)device_cus() / wgs;
+  const int least = p.chunks ? 2 * kSsmChunk : 32, step = p.chunks ? kSsmChunk : 16;
+  if (want < 3 || max_rows < 2 * least) return p;
   int64_t piece = (max_rows + want - 1) / want;
-  piece = piece < 32 ? 32 : (piece + 15) / 16 * 16;
+  piece = piece < least ? least : (piece + step - 1) / step * step;
   for (; piece < max_rows; piece *= 2) {
     const int64_t pieces = packed_pieces(n_rows, batch, (int)piece);
     const uint64_t bytes = (uint64_t)pieces * heads * ((uint64_t)head_dim * d_state + 4) * 4;
@@ -212,7 +212,8 @@ SsmPlan plan_ssm(int batch, int n_rows, int max_rows, int heads, int head_dim, i
 
 int32_t launch_ssm(hipStream_t s, SsmArgs& a, const SsmPlan& plan, void* ws, int dtype) {
   auto phase = [&](SsmPhase ph) {
-    return dtype == EMA_DTYPE_BF16  ? launch_state<ActBf16>(s, a, plan.pieces, ph)
+    return plan.chunks              ? launch_ssm_chunk(s, a, plan.pieces, ph)
+           : dtype == EMA_DTYPE_BF16  ? launch_state<ActBf16>(s, a, plan.pieces, ph)
            : dtype == EMA_DTYPE_F16 ? launch_state<ActF16>(s, a, plan.pieces, ph)
                                     : launch_state<ActF32>(s, a, plan.pieces, ph);
   };

@@ -24,12 +24,15 @@ enum SsmPhase {
 // 2^-28 of it), then the limits.
 __device__ __forceinline__ float ssm_step(float r, const SsmArgs& a) {
   if (a.softplus) r = r > 20.0f ? r : log1pf(__expf(r));
-  return fminf(fmaxf(r, a.dt_min), a.dt_max);
+  r = r < a.dt_min ? a.dt_min : r;  // (NaN stays)
+  return r > a.dt_max ? a.dt_max : r;
 }
 #endif
 
-// Chunked scan on the matrix cores, bf16.
-bool ssm_chunk_shape(int head_dim, int d_state, int heads, int groups);
+// Chunked scan on the matrix cores (bf16): the shapes it takes, the workgroups of a piece, and a launch.
+constexpr int kSsmChunk = 64;  // rows of a chunk
+bool ssm_chunk_shape(int head_dim, int d_state);
+int ssm_chunk_workgroups(int heads, int head_dim, int groups);
 hipError_t launch_ssm_chunk(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhase phase);
 
 }  // namespace ema

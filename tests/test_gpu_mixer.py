@@ -172,6 +172,67 @@ def test_scan_prompts(ema, dtype, shape):
               offsets=[3, 0, 1, 0, 8, 0], tail=2)
 
 
+# in chunks on the matrix cores: H and M are rounded to bf16 where y reads them, the terms of the state to two
+CHUNKED = dict(read_bits=2.0 ** -8, split_bits=2.0 ** -16)
+CHUNK_SHAPES = [(4, 64, 128, 2), (3, 64, 64, 1), (4, 32, 64, 1), (5, 32, 128, 1), (2, 96, 128, 1), (2, 128, 256, 1),
+                (1, 160, 128, 1), (8, 64, 128, 8)]
+
+
+@pytest.mark.parametrize("shape", CHUNK_SHAPES)
+def test_scan_chunks(ema, shape):
+    scan_case(ema, BF, [1, 0, 33, 64, 130, 31], *shape, 140, slots=[6, 0, 3, 2, 5, 1], n_slots=7,
+              offsets=[3, 0, 1, 0, 8, 0], tail=2, **CHUNKED)
+    scan_case(ema, BF, [65, 65], *shape, 141, strided=True, slots=[-1, 1], n_slots=2, **CHUNKED)
+
+
+@pytest.mark.parametrize("dtype,extra", [(BF, CHUNKED), (F32, {})])
+def test_scan_in_pieces(ema, dtype, extra):
+    """Few heads and long sequences: cut in time, with as much workspace as they like, some, and none."""
+    lens = [700, 3, 0, 257]
+    need = ema.ssm_workspace_size(4, sum(lens), 700, 2, 64, 128, 1, dtype)
+    assert need > 0
+    for size in [need, need // 2, need // 4, 16, 0]:
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        scan_case(ema, dtype, lens, 2, 64, 128, 1, 150, offsets=[5, 0, 2, 0], workspace=ws, max_rows=700, a_scale=1.5,
+                  **extra)
+    # bounds below the true lengths: another way, the same result
+    scan_case(ema, dtype, lens, 2, 64, 128, 1, 150, offsets=[5, 0, 2, 0], max_rows=1, a_scale=1.5)
+    scan_case(ema, dtype, lens, 2, 64, 128, 1, 150, offsets=[5, 0, 2, 0], max_rows=130, a_scale=1.5, **extra)
+
+
+def test_scan_chunk_options(ema):
+    for i, kw in enumerate([dict(D=False), dict(bias=False), dict(softplus=False), dict(limit=(0.05, 0.2)),
+                            dict(dt_scale=30.0), dict(a_scale=1.0), dict(limit=(0.0, 0.0)), dict(limit=(5.0, math.inf))]):
+        scan_case(ema, BF, [100, 40], 4, 64, 128, 2, 160 + i, **CHUNKED, **kw)
+
+
+@pytest.mark.parametrize("what", ["x", "B", "C", "dt", "state"])
+@pytest.mark.parametrize("rows", [1, 100])
+def test_scan_values_that_are_not_finite(ema, what, rows):
+    """They reach what the recurrence says they reach: no earlier row, no other column, head or sequence."""
+    H, P, N, G = 4, 64, 128, 2
+    n = 2 * rows
+    a = dict(x=rand(170, n, H, P, dtype=BF), dt=rand(171, n, H, dtype=BF), B=rand(172, n, G, N, dtype=BF),
+             C=rand(173, n, G, N, dtype=BF), state=rand(174, 2, H, P, N))
+    A = -torch.rand(H, device="cuda") - 0.5
+    at = rows // 2
+    for bad in (math.nan, math.inf, -math.inf):
+        b = {k: v.clone() for k, v in a.items()}
+        if what == "state":
+            b["state"][0, 1, 5, 7] = bad
+        elif what == "x":
+            b["x"][at, 1, 5] = bad
+        elif what == "dt":
+            b["dt"][at, 1] = math.nan
+        else:
+            b[what][at, 1, 7] = bad
+        want, want_pool, _, _ = ref.scan(b["x"], b["dt"], b["B"], b["C"], A, b["state"], 2)
+        y = ema.ssm_scan(b["x"], b["dt"], b["B"], b["C"], A, b["state"], batch=2)
+        torch.cuda.synchronize()
+        same = [int((torch.isfinite(g).cpu() != torch.isfinite(w)).sum()) for g, w in ((y, want), (b["state"], want_pool))]
+        assert same == [0, 0], (what, bad, same)
+
+
 def test_scan_options(ema):
     for i, kw in enumerate([dict(D=False), dict(bias=False), dict(softplus=False), dict(limit=(0.05, 0.2)),
                             dict(dt_scale=30.0), dict(a_scale=1.0)]):
