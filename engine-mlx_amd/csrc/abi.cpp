@@ -1005,7 +1005,7 @@ extern "C" int32_t ema_ssm_scan(ema_stream_t stream, const void* x, int64_t ldx,
   if (max_rows > n_rows) max_rows = n_rows;
   const bool vectors = dtype == EMA_DTYPE_BF16 && aligned16(x) && aligned16(b) && aligned16(c) && aligned16(y) &&
                        !(ldx & 7) && !(ldb & 7) && !(ldc & 7) && !(ldy & 7) && ldx < (1 << 23) && ldb < (1 << 23) &&
-                       ldc < (1 << 23);
+                       ldc < (1 << 23) && ldy < (1 << 23);
   const SsmPlan plan = plan_ssm(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype, vectors,
                                 workspace ? workspace_bytes : 0);
   if (plan.pieces * n_heads * ((head_dim + 3) / 4) >= INT32_MAX)

@@ -194,7 +194,7 @@ SsmPlan plan_ssm(int batch, int n_rows, int max_rows, int heads, int head_dim, i
   const int64_t wgs = batch * (p.chunks ? (int64_t)ssm_chunk_workgroups(heads, head_dim, groups)
                                         : heads * (int64_t)((head_dim + 63) / 64));
   const int64_t want = (p.chunks ? 2 : 4) * (int64_t)device_cus() / wgs;
-  const int least = p.chunks ? 2 * kSsmChunk : 32, step = p.chunks ? kSsmChunk : 16;
+  const int least = p.chunks ? 4 * kSsmChunk : 32, step = p.chunks ? kSsmChunk : 16;
   if (want < 3 || max_rows < 2 * least) return p;
   int64_t piece = (max_rows + want - 1) / want;
   piece = piece < least ? least : (piece + step - 1) / step * step;

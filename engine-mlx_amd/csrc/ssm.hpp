@@ -20,17 +20,32 @@ enum SsmPhase {
 };
 
 #if defined(__HIPCC__)
-// The step of raw value r (dt + bias): softplus (r itself above 20, where they differ by less than
-// 2^-28 of it), then the limits.
+// softplus(r) = max(r, 0) + log(1 + u) with u = e^-|r| at most 1, and log(1 + u) = 2 atanh(u / (2 + u))
+// by the series of atanh: the argument is at most 1/3, so eight terms leave 2^-29 of it.
+__device__ __forceinline__ float softplus_(float r) {
+  const float u = expf(-fabsf(r));
+  const float s = u * __builtin_amdgcn_rcpf(2.0f + u), q = s * s;
+  float p = 1.0f / 15;
+  p = fmaf(p, q, 1.0f / 13);
+  p = fmaf(p, q, 1.0f / 11);
+  p = fmaf(p, q, 1.0f / 9);
+  p = fmaf(p, q, 1.0f / 7);
+  p = fmaf(p, q, 1.0f / 5);
+  p = fmaf(p, q, 1.0f / 3);
+  p = fmaf(p, q, 1.0f);
+  return fmaf(2.0f * s, p, r > 0.0f ? r : 0.0f);
+}
+// The step of raw value r (dt + bias): softplus, then the limits.
 __device__ __forceinline__ float ssm_step(float r, const SsmArgs& a) {
-  if (a.softplus) r = r > 20.0f ? r : log1pf(__expf(r));
+  const float sp = softplus_(r);
+  r = a.softplus ? sp : r;  // (no branch: the chunked kernel schedules this under its products)
   r = r < a.dt_min ? a.dt_min : r;  // (NaN stays)
   return r > a.dt_max ? a.dt_max : r;
 }
 #endif
 
 // Chunked scan on the matrix cores (bf16): the shapes it takes, the workgroups of a piece, and a launch.
-constexpr int kSsmChunk = 64;  // rows of a chunk
+constexpr int kSsmChunk = 32;  // rows of a chunk
 bool ssm_chunk_shape(int head_dim, int d_state);
 int ssm_chunk_workgroups(int heads, int head_dim, int groups);
 hipError_t launch_ssm_chunk(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhase phase);

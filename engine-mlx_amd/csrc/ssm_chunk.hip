@@ -1,10 +1,10 @@
-// Selective state space scan in chunks of 64 rows on the matrix cores, bf16 activations.
+// Selective state space scan in chunks of 32 rows on the matrix cores, bf16 activations.
 //
 // With a_t = d_t A and sums over rows of the chunk, a chunk that starts from the state H gives
 //   y_t = e^(a_0 + .. + a_t) H C_t + sum_{s <= t} M[t][s] x_s,
 //   M[t][s] = (C_t . B_s) e^(a_(s+1) + .. + a_t) d_s  (+ D for s = t),
-//   H'  = e^(a_0 + .. + a_63) H + sum_s (d_s e^(a_(s+1) + .. + a_63) x_s) B_s^T,
-// so C B^T is formed once for all heads of a group, and the rest is products with 64-row operands.
+//   H'  = e^(a_0 + .. + a_31) H + sum_s (d_s e^(a_(s+1) + .. + a_31) x_s) B_s^T,
+// so C B^T is formed once for all heads of a workgroup, and the rest is products with 32-row operands.
 //
 // A workgroup of four waves takes 128 columns of x (two heads of 64, one of 128, ...) of one group,
 // a wave 32 of them: its H^T [d_state, 32] stays in 32-bit accumulators over the rows of the piece.
@@ -12,11 +12,12 @@
 //   C B^T as [s, t]          A = B rows,       B = C rows (columns t)
 //   y^T [p, t]              A = H (the accumulators, rounded to bf16) and x^T, B = C and M
 //   H^T [n, p]              A = B^T,           B = x^T scaled
-// An accumulator pair holds k slots in the order 4 c + (0..3), 16 + 4 c + (0..3) of lane group c;
-// operands from LDS are read in the same order (C and B rows in two 8-byte reads; x^T and B^T by
-// the transposing read). The decays of M are products of factors at most 1 (A <= 0): from s to the
-// end of its 16-row tile and the tiles between (g), and from t's tile's start to t (f); differences
-// of sums only inside the tiles on the diagonal.
+// A pair of 16x16 accumulator tiles holds, in lane group c, rows 4 c + (0..3) of both tiles. The rows of
+// the state's tiles are numbered so that these are d_state 8 c + (0..7) of a 32-wide step (B^T's columns
+// are read in that order): rows of C are then read whole. M's are rows 4 c + (0..3) and 16 + 4 c +
+// (0..3); x^T and B^T are read from LDS in the same order of rows, by the transposing read. The
+// decays of M are products of factors at most 1 (A <= 0): from s to the end of its 16-row tile (g), and
+// from t's tile's start to t (f); differences of sums only inside the tiles on the diagonal.
 //
 // Rounded to bf16: H and M where they are operands of y (as an attention's weights are; x, B and C
 // are exact), each by at most 2^-8 of the term. The state itself takes the scaled x as three bf16
@@ -25,6 +26,10 @@
 // A value of x that is not finite would reach rows before it through M's zeros (0 times infinity):
 // chunks with such values (a dot product with zeros finds them while they are staged) take those
 // columns' sums without them and put NaN into the rows from the value on.
+//
+// Chunks of 32 rows and not of 64: per row they cost a third more vector instructions for the state
+// (its decay and its rounding come twice as often), but 64 rows need more registers than two
+// workgroups a CU leave, and spilled the loads under way.
 #include <type_traits>
 
 #include "ssm.hpp"
@@ -32,26 +37,27 @@
 namespace ema {
 namespace {
 
-constexpr int kQ = 64;        // rows of a chunk
+constexpr int kQ = 32;        // rows of a chunk
 constexpr int kCols = 32;     // columns of x of a wave
+constexpr int kXW = 4 * kCols;
 constexpr int kThreads = 256;
 
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// Per-head values of a chunk (floats), written by one wave: index by row unless said otherwise.
+// Per-head values of a chunk (floats): index by row unless said otherwise.
 struct Dec {
   static constexpr int kCum = 0;     // sum of log2 decays from the row's 16-row tile's start, the row included
-  static constexpr int kStep = 64;   // d
-  static constexpr int kF = 128;     // decay from the tile's start: 2^kCum
-  static constexpr int kE = 192;     // decay from the chunk's start
-  static constexpr int kW = 256;     // d times the decay from behind the row to the chunk's end
-  static constexpr int kG = 320;     // [3][64]: d times the decay from behind row s to the start of tile 1, 2, 3
-  static constexpr int kAll = 512;   // decay over the chunk; its log2 at 513
-  static constexpr int kD = 514;     // D
-  static constexpr int kFloats = 516;
+  static constexpr int kStep = 32;   // d
+  static constexpr int kF = 64;      // decay from the tile's start: 2^kCum
+  static constexpr int kE = 96;      // decay from the chunk's start
+  static constexpr int kW = 128;     // d times the decay from behind the row to the chunk's end
+  static constexpr int kG = 160;     // d times the decay from behind the row to its tile's end
+  static constexpr int kAll = 192;   // decay over the chunk; its log2 at 193
+  static constexpr int kD = 194;     // D
+  static constexpr int kFloats = 196;
 };
 
-// Row pitch and swizzle of the LDS tiles of N-wide rows: 16-byte piece q of row r lies at piece
+// Row pitch and swizzle of the LDS tiles of W-wide rows: 16-byte piece q of row r lies at piece
 // q ^ x(r), so that 16 rows at one piece, and 8 rows at two neighbouring ones, are in distinct banks.
 template <int W>
 __device__ __forceinline__ int swizzle(int r) {
@@ -63,7 +69,6 @@ __device__ __forceinline__ int tile_at(int r, int q) {  // bytes
 }
 
 __device__ __forceinline__ bf16x8 join(u32x2 lo, u32x2 hi) { return as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]}); }
-__device__ __forceinline__ u32x2 read8(const uint8_t* p) { return *(const u32x2*)p; }
 __device__ __forceinline__ u32x2 read_tr(const uint8_t* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
 }
@@ -76,11 +81,12 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
 }
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 
-// Decays of one head's 64 rows, a row a lane; `raw` is dt + bias, rows from n on take no step.
+// Decays of two heads' 32 rows, a row a lane (lanes 32..63: the second head; dec is the lane's
+// head's). `raw` is dt + bias; rows from n on take no step.
 template <bool kOutputs>
 __device__ __forceinline__ void chunk_decays(float raw, int n, float A2, float D, const SsmArgs& a, float* dec) {
-  const int lane = threadIdx.x & 63;
-  const float d = lane < n ? ssm_step(raw, a) : 0.f;
+  const int lane = threadIdx.x & 63, row = lane & 31;
+  const float d = row < n ? ssm_step(raw, a) : 0.f;
   // log2 of the row's decay; below 2^-150 it is 0 either way, and sums stay finite
   const float l = fmaxf(d * A2, -150.f);
   float up = l, down = l;  // sums over the 16-row tile: up to the row, from the row on
@@ -93,37 +99,30 @@ __device__ __forceinline__ void chunk_decays(float raw, int n, float A2, float D
   up += dpp_shift<0x118>(up);
   down += dpp_shift<0x108>(down);
   const float behind = dpp_shift<0x101>(down);  // from behind the row to its tile's end
-  const float t0 = lane_value(up, 15), t1 = lane_value(up, 31), t2 = lane_value(up, 47), t3 = lane_value(up, 63);
-  const int tile = lane >> 4;
-  const float later = tile == 0 ? t1 + t2 + t3 : tile == 1 ? t2 + t3 : tile == 2 ? t3 : 0.f;
-  dec[Dec::kW + lane] = d * exp2_(behind + later);
-  if (lane == 0) {
-    const float all = (t0 + t1) + (t2 + t3);
-    dec[Dec::kAll] = exp2_(all);
-    dec[Dec::kAll + 1] = all;
-    dec[Dec::kD] = D;
-  }
+  const bool second = lane >= 32, tile1 = row >= 16;
+  const float t0 = second ? lane_value(up, 47) : lane_value(up, 15), t1 = second ? lane_value(up, 63) : lane_value(up, 31);
+  dec[Dec::kW + row] = d * exp2_(behind + (tile1 ? 0.f : t1));
+  dec[Dec::kAll] = exp2_(t0 + t1);  // (every lane the same)
+  dec[Dec::kAll + 1] = t0 + t1;
   if constexpr (kOutputs) {
-    const float before = tile == 0 ? 0.f : tile == 1 ? t0 : tile == 2 ? t0 + t1 : t0 + t1 + t2;
-    dec[Dec::kCum + lane] = up;
-    dec[Dec::kStep + lane] = d;
-    dec[Dec::kF + lane] = exp2_(up);
-    dec[Dec::kE + lane] = exp2_(up + before);
-    dec[Dec::kG + lane] = d * exp2_(behind);  // tile 0 to the start of tile 1
-    dec[Dec::kG + 64 + lane] = d * exp2_(behind + (tile == 0 ? t1 : 0.f));
-    dec[Dec::kG + 128 + lane] = d * exp2_(behind + (tile == 0 ? t1 + t2 : tile == 1 ? t2 : 0.f));
+    dec[Dec::kD] = D;
+    dec[Dec::kCum + row] = up;
+    dec[Dec::kStep + row] = d;
+    dec[Dec::kF + row] = exp2_(up);
+    dec[Dec::kE + row] = exp2_(up + (tile1 ? t0 : 0.f));
+    dec[Dec::kG + row] = d * exp2_(behind);
   }
 }
 
-// LDS (bytes): B, x, then for outputs C, M of every head of the workgroup; the heads' decays, twice;
-// the flags of chunks with values that are not finite, twice.
+// LDS (bytes): B, x and (for outputs) C, twice; M of every head of the workgroup; the heads' decays,
+// twice; the flags of chunks with values that are not finite, twice.
 template <int N, bool kOutputs>
 struct Lds {
-  static constexpr int kB = 0;
-  static constexpr int kX = kB + kQ * N * 2;
-  static constexpr int kC = kX + kQ * 4 * kCols * 2;
-  static constexpr int kM = kC + (kOutputs ? kQ * N * 2 : 0);
-  static constexpr int kMHead = 6 * 1024;  // (row tile, 32-row step): (0,0) (1,0) (2,0) (2,1) (3,0) (3,1)
+  static constexpr int kX = kQ * N * 2;
+  static constexpr int kC = kX + kQ * kXW * 2;
+  static constexpr int kBuf = kC + (kOutputs ? kQ * N * 2 : 0);
+  static constexpr int kM = 2 * kBuf;
+  static constexpr int kMHead = 2 * 1024;  // one operand for each 16-row tile of t
   static constexpr __host__ __device__ int dec(int heads) { return kM + (kOutputs ? heads * kMHead : 0); }
   static constexpr __host__ __device__ int flag(int heads) { return dec(heads) + 2 * heads * Dec::kFloats * 4; }
   static constexpr __host__ __device__ int bytes(int heads) { return flag(heads) + 16; }
@@ -149,7 +148,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   const int wg = (int)(k8 % (uint32_t)gr.wgs);
   const int64_t pair = xcd + 8 * (int64_t)(k8 / (uint32_t)gr.wgs);
   if (pair >= gr.pairs) return;
-  const int grp = (int)(pair % a.groups), index = (int)(pair / a.groups);
+  const int grp = (int)((uint32_t)pair % (uint32_t)a.groups), index = (int)((uint32_t)pair / (uint32_t)a.groups);
   const Piece pc = packed_piece(a.starts, a.batch, a.n_rows, a.T, a.piece, index);
   if (pc.n == 0) return;
   const bool last = pc.row + pc.n == pc.begin + pc.all;
@@ -172,16 +171,13 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   const int slot = packed_slot(a.slots, pc.b, a.n_slots);
   float* const pool = a.state + ((int64_t)slot * a.heads + head) * P * N;
   float* const carry = a.carry + ((int64_t)index * a.heads + head) * P * N;
-  const int64_t st_at = (int64_t)(p0 + l16) * N + 4 * c4;
+  const int st_at = (p0 + l16) * N + 8 * c4;
 
-  uint8_t* const Bs = lds + L::kB;
-  uint8_t* const Xs = lds + L::kX;
-  uint8_t* const Cs = lds + L::kC;
   uint8_t* const Ms = lds + L::kM;
   float* const decs = (float*)(lds + L::dec(HEADS));
   int* const flags = (int*)(lds + L::flag(HEADS));
 
-  // ---- state: h[ct][T] holds n = 16 T + 4 c4 + i of column p0 + 16 ct + l16
+  // ---- state: h[ct][T] holds n = 32 (T / 2) + 8 c4 + 4 (T % 2) + i of column p0 + 16 ct + l16
   f32x4 h[2][NT];
   {
     const float* from = nullptr;
@@ -192,32 +188,28 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
-      for (int T = 0; T < NT; ++T) {
-        h[ct][T] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (from) h[ct][T] = *(const f32x4*)(from + st_at + (int64_t)16 * ct * N + 16 * T);
-      }
+      for (int T = 0; T < NT; ++T) h[ct][T] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (from)
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+        for (int T = 0; T < NT; ++T) h[ct][T] = *(const f32x4*)(from + (st_at + 16 * ct * N + 32 * (T >> 1) + 4 * (T & 1)));
   }
 
-  // ---- staging: 16-byte pieces of rows, a chunk ahead in registers
+  // ---- staging: 16-byte pieces of rows, in registers from one chunk to the next
   constexpr int kRowB = N / 8;                     // pieces of a B or C row
   constexpr int kIn = kQ * kRowB / kThreads;       // pieces of B (or C) a thread
   constexpr int kInX = kQ * 16 / kThreads;
-  u32x4 rb[kIn], rc[kOutputs ? kIn : 1], rx[kInX];
-  float rdt = 0.f;
-  // rows within a chunk are 32-bit offsets from a uniform base (64 rows of ld* < 2^23: plan_ssm)
+  u32x4 rb[kIn], rc[kIn], rx[kInX];
+  // rows within a chunk are 32-bit offsets from a uniform base (ld* < 2^23)
   const uint8_t* const bp = (const uint8_t*)((const uint16_t*)a.b + (int64_t)pc.row * a.ldb + grp * N);
   const uint8_t* const cp = (const uint8_t*)((const uint16_t*)a.c + (int64_t)pc.row * a.ldc + grp * N);
   const uint8_t* const xp = (const uint8_t*)((const uint16_t*)a.x + (int64_t)pc.row * a.ldx + (int64_t)head0 * P + unit0 * kCols);
   const uint32_t ldb2 = (uint32_t)a.ldb * 2, ldc2 = (uint32_t)a.ldc * 2, ldx2 = (uint32_t)a.ldx * 2;
   const int x_pieces = (last_unit - unit0 + 1) * (kCols / 8);
-  const bool scalars = wave < n_heads;             // this wave forms a head's decays
-  const int s_head = head0 + first_head + (scalars ? wave : 0);
-  const uint16_t* const dp = (const uint16_t*)a.dt + (int64_t)pc.row * a.lddt + s_head;
-  const float A2 = a.a[s_head] * kLog2e, bias = a.dt_bias ? a.dt_bias[s_head] : 0.f;
-  const float D = a.d ? a.d[s_head] : 0.f;
-
-  // rows behind the piece are its last row again: what they would add has step 0
-  auto fetch = [&](int t0) __attribute__((always_inline)) {
+  // rows behind the piece are its last row again: what they would add has step 0 (and columns of no
+  // unit the last one's again: their wave is idle)
+  auto load = [&](int t0) __attribute__((always_inline)) {
     const uint32_t end = (uint32_t)(pc.n - t0 - 1);
     const uint8_t* const b0 = bp + (int64_t)t0 * ldb2;
     const uint8_t* const c0 = cp + (int64_t)t0 * ldc2;
@@ -232,124 +224,127 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
     for (int i = 0; i < kInX; ++i) {
       const uint32_t id = i * kThreads + tid, r = id >> 4, q = id & 15;
-      const uint32_t row = r < end ? r : end;
-      rx[i] = (int)q < x_pieces ? *(const u32x4*)(x0 + (row * ldx2 + 16 * q)) : u32x4{0u, 0u, 0u, 0u};
+      rx[i] = *(const u32x4*)(x0 + ((r < end ? r : end) * ldx2 + 16 * ((int)q < x_pieces ? q : x_pieces - 1)));
     }
-    if (scalars) rdt = bf16_to_f32(dp[(int64_t)(t0 + (int)((uint32_t)lane < end ? (uint32_t)lane : end)) * a.lddt]);
   };
-  auto stage = [&](int t0, int par) __attribute__((always_inline)) {
+  auto store = [&](int par) __attribute__((always_inline)) {
+    uint8_t* const buf = lds + par * L::kBuf;
 #pragma unroll
     for (int i = 0; i < kIn; ++i) {
-      const int id = i * kThreads + tid, r = id / kRowB, q = id % kRowB;
-      *(u32x4*)(Bs + tile_at<N>(r, q)) = rb[i];
-      if constexpr (kOutputs) *(u32x4*)(Cs + tile_at<N>(r, q)) = rc[i];
+      const int id = i * kThreads + tid, at = tile_at<N>(id / kRowB, id % kRowB);
+      *(u32x4*)(buf + at) = rb[i];
+      if constexpr (kOutputs) *(u32x4*)(buf + L::kC + at) = rc[i];
     }
     float zero = 0.f;
 #pragma unroll
     for (int i = 0; i < kInX; ++i) {
-      const int id = i * kThreads + tid, r = id >> 4, q = id & 15;
-      *(u32x4*)(Xs + tile_at<4 * kCols>(r, q)) = rx[i];
+      const int id = i * kThreads + tid;
+      *(u32x4*)(buf + L::kX + tile_at<kXW>(id >> 4, id & 15)) = rx[i];
       if constexpr (kOutputs)
 #pragma unroll
         for (int e = 0; e < 4; ++e) zero = dot2_bf16(rx[i][e], 0u, zero);
     }
     if constexpr (kOutputs)
       if (zero != zero) flags[par] = 1;
-    if (scalars) chunk_decays<kOutputs>(rdt + bias, pc.n - t0, A2, D, a, decs + (par * HEADS + wave) * Dec::kFloats);
+  };
+  // every wave forms the decays of its head and its neighbour (waves of one head write the same
+  // values): no wave waits for another's
+  const int d_head = (hh & ~1) + (lane >> 5) < n_heads ? (hh & ~1) + (lane >> 5) : hh & ~1;
+  const uint16_t* const dp = (const uint16_t*)a.dt + (int64_t)pc.row * a.lddt + head0 + first_head + d_head;
+  const float A2 = a.a[head0 + first_head + d_head] * kLog2e;
+  const float bias = a.dt_bias ? a.dt_bias[head0 + first_head + d_head] : 0.f;
+  const float D = a.d ? a.d[head0 + first_head + d_head] : 0.f;
+  uint16_t rdt = 0;
+  auto load_dt = [&](int t0) __attribute__((always_inline)) {
+    const int end = pc.n - t0 - 1, r = lane & 31;
+    rdt = dp[(int64_t)(t0 + (r < end ? r : end)) * a.lddt];
+  };
+  auto decays = [&](int t0, int par) __attribute__((always_inline)) {
+    chunk_decays<kOutputs>(bf16_to_f32(rdt) + bias, pc.n - t0, A2, D, a, decs + (par * HEADS + d_head) * Dec::kFloats);
   };
 
   if constexpr (kOutputs) {
-    // the upper halves of the steps (0, 0) and (2, 1) are tiles above the diagonal: zero for good
-    for (int i = tid; i < n_heads * 64; i += kThreads) {
-      uint8_t* const m = Ms + (i >> 6) * L::kMHead + (i & 63) * 16 + 8;
-      *(u32x2*)m = u32x2{0u, 0u};
-      *(u32x2*)(m + 3 * 1024) = u32x2{0u, 0u};
-    }
+    // M above the diagonal tile of rows 0..15 is zero for good
+    if (tid < 64)
+#pragma unroll
+      for (int j = 0; j < HEADS; ++j) *(u32x2*)(Ms + j * L::kMHead + tid * 16 + 8) = u32x2{0u, 0u};
     if (tid < 2) flags[tid] = 0;
+    __syncthreads();  // the flags are set after they are cleared
   }
-  __syncthreads();  // the flags are set after they are cleared
 
   // lane parts of the operand addresses
   const int x_of_row = swizzle<N>(l16);
-  const int row_b = l16 * (N * 2) + 8 * (c4 & 1);                  // rows of B and C at a tile's start
-  const int tr_row = 4 * c4 + (l16 >> 2);                          // transposed reads: row, and 16 more
-  const int tr_half = 8 * (l16 & 1), tr_q = (l16 & 3) >> 1;
-  // 8 values (slots of step ks) of row 16 tile + l16 of B or C
+  const int tr_row = 4 * c4 + (l16 >> 2);  // transposed reads: row, and 16 more (of the same swizzle)
+  // the 8 values of step ks of row 16 tile + l16 of B or C
   auto row_operand = [&](const uint8_t* base, int tile, int ks) __attribute__((always_inline)) {
-    const uint8_t* const r = base + tile * 16 * (N * 2) + row_b;
-    return join(read8(r + (((4 * ks + (c4 >> 1)) ^ x_of_row) << 4)), read8(r + (((4 * ks + 2 + (c4 >> 1)) ^ x_of_row) << 4)));
+    return as_bf16x8(*(const u32x4*)(base + tile * 16 * (N * 2) + (l16 * (N * 2) + (((4 * ks + c4) ^ x_of_row) << 4))));
   };
-  // 8 rows (slots of step kt) of column 16 tile + l16
-  auto col_operand = [&](auto width, const uint8_t* base, int tile, int kt) __attribute__((always_inline)) {
-    constexpr int W = decltype(width)::value;
-    const uint8_t* const r = base + (32 * kt) * (W * 2) + tr_half;
-    const int q = 2 * tile + tr_q;
-    const int sw = swizzle<W>(tr_row);  // (rows 16 apart have the same)
-    const uint8_t* const at = r + tr_row * (W * 2) + ((q ^ sw) << 4);
-    return join(read_tr(at), read_tr(at + 16 * (W * 2)));
+  // the chunk's rows of column 16 tile + l16 of x
+  auto x_operand = [&](const uint8_t* xs, int tile) __attribute__((always_inline)) {
+    const uint8_t* const at =
+        xs + (tr_row * (2 * kXW) + 8 * (l16 & 1) + (((2 * tile + ((l16 & 3) >> 1)) ^ swizzle<kXW>(tr_row)) << 4));
+    return join(read_tr(at), read_tr(at + 16 * (2 * kXW)));
   };
-  typedef std::integral_constant<int, 4 * kCols> XW;
-  typedef std::integral_constant<int, N> BW;
+  // the chunk's rows of the columns of state tile T of B
+  auto b_operand = [&](const uint8_t* bs, int T) __attribute__((always_inline)) {
+    const uint8_t* const at =
+        bs + (tr_row * (N * 2) + 8 * (T & 1) + (((4 * (T >> 1) + (l16 & 3)) ^ swizzle<N>(tr_row)) << 4));
+    return join(read_tr(at), read_tr(at + 16 * (N * 2)));
+  };
 
   float total = 0.f;  // log2 of the decay over the piece
-  uint16_t* const yp = (uint16_t*)a.y + (int64_t)pc.row * a.ldy + (int64_t)head * P + p0 + 4 * c4;
-  fetch(0);
-  stage(0, 0);
+  uint8_t* const yp = (uint8_t*)((uint16_t*)a.y + (int64_t)pc.row * a.ldy + (int64_t)head * P + p0);
+  const uint32_t ldy2 = (uint32_t)a.ldy * 2, y_at = l16 * ldy2 + 8 * c4;
+  load_dt(0);
+  load(0);
+  decays(0, 0);
+  store(0);
+  if (pc.n > kQ) {
+    load_dt(kQ);
+    load(kQ);
+  }
   for (int t0 = 0, par = 0; t0 < pc.n; t0 += kQ, par ^= 1) {
-    __syncthreads();  // the chunk is staged
+    __syncthreads();  // the chunk is staged, the buffers of the one before are free
     const bool more = t0 + kQ < pc.n;
-    if (more) fetch(t0 + kQ);
+    const uint8_t* const buf = lds + par * L::kBuf;
     const float* const dec = decs + (par * HEADS + hh) * Dec::kFloats;
-    bf16x8 xt[2][2];  // x^T: [column tile][32-row step]
-    if constexpr (kOutputs) {
-      // ---- C B^T tiles, and M of every head from them: a wave takes the diagonal tile (w, w) and two
-      // below it, (3, 0) (3, 1) | (2, 0) (3, 2) | (2, 1) twice | (1, 0) twice
-      f32x4 s[3];
-      int tt[3], st[3];
-      tt[0] = st[0] = wave;
-      tt[1] = wave == 0 ? 3 : wave == 3 ? 1 : 2;
-      st[1] = wave == 2 ? 1 : 0;
-      tt[2] = wave < 2 ? 3 : tt[1];
-      st[2] = wave == 0 ? 1 : wave == 1 ? 2 : st[1];
+    const float all = dec[Dec::kAll];
+    total += dec[Dec::kAll + 1];
+    bf16x8 xt[2];  // x^T of the column tiles
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) xt[ct] = x_operand(buf + L::kX, 2 * wave + ct);
+    // x scaled, in three bf16 parts: two neighbouring rows of one column a call
+    u32x4 part[3][2];
+    const f32x4 wt[2] = {*(const f32x4*)&dec[Dec::kW + 4 * c4], *(const f32x4*)&dec[Dec::kW + 16 + 4 * c4]};
+    auto scaled = [&](int ct, int e) __attribute__((always_inline)) {
+      const uint32_t xw = __builtin_bit_cast(u32x4, xt[ct])[e];
+      const f32x4 w = wt[e >> 1];
+      float v0 = bf16_lo(xw) * w[2 * (e & 1)], v1 = bf16_hi(xw) * w[2 * (e & 1) + 1];
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
-        s[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[k] = mfma16(row_operand(Bs, st[k], ks), row_operand(Cs, tt[k], ks), s[k]);
-      }
-#pragma unroll
-      for (int j = 0; j < HEADS; ++j) {
-        if (j > 0 && j >= n_heads) break;
-        const float* const dj = decs + (par * HEADS + j) * Dec::kFloats;
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const int t = 16 * tt[k] + l16, s0 = 16 * st[k] + 4 * c4;
-          f32x4 v;
-          if (k == 0) {
-            const f32x4 cum = *(const f32x4*)&dj[Dec::kCum + s0], step = *(const f32x4*)&dj[Dec::kStep + s0];
-            const float ct = dj[Dec::kCum + t];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              v[i] = s0 + i <= t ? s[k][i] * (exp2_(ct - cum[i]) * step[i]) : 0.f;
-              if (s0 + i == t) v[i] += dj[Dec::kD];
-            }
-          } else {
-            const f32x4 g = *(const f32x4*)&dj[Dec::kG + 64 * (tt[k] - 1) + s0];
-            const float f = dj[Dec::kF + t];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = s[k][i] * g[i] * f;
-          }
-          const int slot_m = tt[k] < 2 ? tt[k] : 2 * tt[k] - 2 + (st[k] >> 1);
-          *(u32x2*)(Ms + j * L::kMHead + slot_m * 1024 + lane * 16 + 8 * (st[k] & 1)) =
-              u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        const uint32_t u = pack_bf16x2(v0, v1);
+        part[k][ct][e] = u;
+        if (k < 2) {
+          v0 -= bf16_lo(u);
+          v1 -= bf16_hi(u);
         }
       }
-      // ---- H C_t for the wave's columns
-      f32x4 acc[4][2];
+    };
+    if constexpr (kOutputs) {
+      if (tid == 0) flags[par ^ 1] = 0;
+      // ---- a tile of C B^T: waves 0 and 1 the diagonal ones, 2 and 3 the one below (for every other head)
+      const uint8_t* const Bs = buf;
+      const uint8_t* const Cs = buf + L::kC;
+      const int tt = wave == 0 ? 0 : 1, st = wave == 1 ? 1 : 0;
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
+      for (int ks = 0; ks < KS; ++ks) s = mfma16(row_operand(Bs, st, ks), row_operand(Cs, tt, ks), s);
+      // ---- H C_t for the wave's columns; the state's decay
+      f32x4 acc[2][2];
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) acc[tt][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) acc[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         bf16x8 hb[2];
@@ -358,132 +353,132 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
           const f32x4 u = h[ct][2 * ks], v = h[ct][2 * ks + 1];
           hb[ct] = as_bf16x8(u32x4{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]),
                                    pack_bf16x2(v[2], v[3])});
+          h[ct][2 * ks] = u * all;
+          h[ct][2 * ks + 1] = v * all;
         }
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          const bf16x8 co = row_operand(Cs, tt, ks);
+        for (int t = 0; t < 2; ++t) {
+          const bf16x8 co = row_operand(Cs, t, ks);
 #pragma unroll
-          for (int ct = 0; ct < 2; ++ct) acc[tt][ct] = mfma16(hb[ct], co, acc[tt][ct]);
+          for (int ct = 0; ct < 2; ++ct) acc[t][ct] = mfma16(hb[ct], co, acc[t][ct]);
+        }
+#pragma unroll
+        for (int e = ks * 8 / KS; e < (ks + 1) * 8 / KS; ++e) scaled(e >> 2, e & 3);
+      }
+      // ---- M of the heads from the tile
+      uint8_t* const m = Ms + tt * 1024 + lane * 16 + 8 * st;
+      if (wave < 2) {
+        const int t = 16 * tt + l16, s0 = 16 * tt + 4 * c4;
+#pragma unroll
+        for (int j = 0; j < HEADS; ++j) {  // (a head that is not there: values that nothing reads)
+          const float* const dj = decs + (par * HEADS + j) * Dec::kFloats;
+          const f32x4 cum = *(const f32x4*)&dj[Dec::kCum + s0], step = *(const f32x4*)&dj[Dec::kStep + s0];
+          const float ct = dj[Dec::kCum + t], Dj = dj[Dec::kD];
+          f32x4 v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[i] = s0 + i <= t ? s[i] * (exp2_(ct - cum[i]) * step[i]) : 0.f;
+            v[i] = s0 + i == t ? v[i] + Dj : v[i];
+          }
+          *(u32x2*)(m + j * L::kMHead) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        }
+      } else {
+#pragma unroll
+        for (int jj = 0; jj < (HEADS + 1) / 2; ++jj) {
+          const int j = 2 * jj + (wave & 1);
+          if (j >= HEADS) break;
+          const float* const dj = decs + (par * HEADS + j) * Dec::kFloats;
+          const f32x4 g = *(const f32x4*)&dj[Dec::kG + 4 * c4];
+          const f32x4 v = s * g * dj[Dec::kF + 16 + l16];
+          *(u32x2*)(m + j * L::kMHead) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
         }
       }
-#pragma unroll
-      for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) xt[ct][kt] = col_operand(XW(), Xs, 2 * wave + ct, kt);
       __syncthreads();  // M is whole
       const bool bad = __builtin_amdgcn_readfirstlane(flags[par]) != 0;
-      int first[2] = {kQ, kQ};  // first row whose x is not finite, in column 16 ct + l16
-      if (bad) {
-#pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt) {
-            u32x4 v = __builtin_bit_cast(u32x4, xt[ct][kt]);
-#pragma unroll
-            for (int j = 7; j >= 0; --j) {
-              const uint32_t mask = j & 1 ? 0x7f800000u : 0x7f80u;
-              if ((v[j >> 1] & mask) == mask) {
-                const int r = 32 * kt + 4 * c4 + (j < 4 ? j : 12 + j);
-                first[ct] = r < first[ct] ? r : first[ct];
-                v[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;
-              }
-            }
-            xt[ct][kt] = as_bf16x8(v);
-          }
-          int other = __shfl_xor(first[ct], 16, 64);
-          first[ct] = other < first[ct] ? other : first[ct];
-          other = __shfl_xor(first[ct], 32, 64);
-          first[ct] = other < first[ct] ? other : first[ct];
-        }
+      if (more) {
+        store(par ^ 1);
+        if (t0 + 2 * kQ < pc.n) load(t0 + 2 * kQ);
       }
       const uint8_t* const mh = Ms + hh * L::kMHead + lane * 16;
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const float e = dec[Dec::kE + 16 * tt + l16];
-        const int base = tt < 2 ? tt : 2 * tt - 2;
+      for (int t = 0; t < 2; ++t) {
+        const float e = dec[Dec::kE + 16 * t + l16];
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) acc[tt][ct] *= e;
-#pragma unroll
-        for (int kt = 0; kt <= tt >> 1; ++kt) {
-          const bf16x8 mo = as_bf16x8(*(const u32x4*)(mh + (base + kt) * 1024));
-#pragma unroll
-          for (int ct = 0; ct < 2; ++ct) acc[tt][ct] = mfma16(xt[ct][kt], mo, acc[tt][ct]);
-        }
+        for (int ct = 0; ct < 2; ++ct) acc[t][ct] *= e;
       }
-      if (bad) {
+      if (!bad) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const bf16x8 mo = as_bf16x8(*(const u32x4*)(mh + t * 1024));
+#pragma unroll
+          for (int ct = 0; ct < 2; ++ct) acc[t][ct] = mfma16(xt[ct], mo, acc[t][ct]);
+        }
+      } else {
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) {
+          int first = kQ;  // first row that is not finite in column 16 ct + l16
+          u32x4 v = __builtin_bit_cast(u32x4, xt[ct]);
+#pragma unroll
+          for (int j = 7; j >= 0; --j) {
+            const uint32_t mask = j & 1 ? 0x7f800000u : 0x7f80u;
+            if ((v[j >> 1] & mask) == mask) {
+              const int r = 4 * c4 + (j < 4 ? j : 12 + j);
+              first = r < first ? r : first;
+              v[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;
+            }
+          }
+          int other = __shfl_xor(first, 16, 64);
+          first = other < first ? other : first;
+          other = __shfl_xor(first, 32, 64);
+          first = other < first ? other : first;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            acc[t][ct] = mfma16(as_bf16x8(v), as_bf16x8(*(const u32x4*)(mh + t * 1024)), acc[t][ct]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int from = __shfl(first[ct], 4 * c4 + i, 64);
+            const int from = __shfl(first, 4 * c4 + i, 64);
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt)
-              if (16 * tt + l16 >= from) acc[tt][ct][i] = __builtin_nanf("");
+            for (int t = 0; t < 2; ++t)
+              if (16 * t + l16 >= from) acc[t][ct][i] = __builtin_nanf("");
           }
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt) xt[ct][kt] = col_operand(XW(), Xs, 2 * wave + ct, kt);
         }
       }
       if (!idle)
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          const int t = t0 + 16 * tt + l16;
-          if (t < pc.n)
+        for (int t = 0; t < 2; ++t) {
+          uint8_t* const row = yp + (int64_t)(t0 + 16 * t) * ldy2;
+          if (16 * t + l16 < pc.n - t0)
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct) {
-              const f32x4 v = acc[tt][ct];
-              *(u32x2*)(yp + (int64_t)t * a.ldy + 16 * ct) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+              const f32x4 v = acc[t][ct];
+              *(u32x2*)(row + (y_at + 32 * ct)) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
             }
         }
     } else {
+      if (more) {
+        store(par ^ 1);
+        if (t0 + 2 * kQ < pc.n) load(t0 + 2 * kQ);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) scaled(e >> 2, e & 3);
 #pragma unroll
       for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) xt[ct][kt] = col_operand(XW(), Xs, 2 * wave + ct, kt);
+        for (int T = 0; T < NT; ++T) h[ct][T] *= all;
     }
-    // ---- the state
-    const float all = dec[Dec::kAll];
-    total += dec[Dec::kAll + 1];
+    // ---- the state, and the next chunk's decays (they have a place of their own)
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct)
+    for (int T = 0; T < NT; ++T) {
+      const bf16x8 bt = b_operand(buf, T);
 #pragma unroll
-      for (int T = 0; T < NT; ++T) h[ct][T] *= all;
+      for (int k = 2; k >= 0; --k)
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const f32x4 wl = *(const f32x4*)&dec[Dec::kW + 32 * kt + 4 * c4], wh = *(const f32x4*)&dec[Dec::kW + 32 * kt + 16 + 4 * c4];
-      bf16x8 part[3][2];
-#pragma unroll
-      for (int ct = 0; ct < 2; ++ct) {
-        const u32x4 xw = __builtin_bit_cast(u32x4, xt[ct][kt]);
-        u32x4 u[3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v0 = bf16_lo(xw[e]) * (e < 2 ? wl[2 * e] : wh[2 * e - 4]);
-          float v1 = bf16_hi(xw[e]) * (e < 2 ? wl[2 * e + 1] : wh[2 * e - 3]);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            u[k][e] = pack_bf16x2(v0, v1);
-            if (k < 2) {
-              v0 -= bf16_lo(u[k][e]);
-              v1 -= bf16_hi(u[k][e]);
-            }
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 3; ++k) part[k][ct] = as_bf16x8(u[k]);
-      }
-#pragma unroll
-      for (int T = 0; T < NT; ++T) {
-        const bf16x8 bt = col_operand(BW(), Bs, T, kt);
-#pragma unroll
-        for (int k = 2; k >= 0; --k)
-#pragma unroll
-          for (int ct = 0; ct < 2; ++ct) h[ct][T] = mfma16(bt, part[k][ct], h[ct][T]);
-      }
+        for (int ct = 0; ct < 2; ++ct) h[ct][T] = mfma16(bt, as_bf16x8(part[k][ct]), h[ct][T]);
     }
-    __syncthreads();  // the chunk's tiles are free
-    if (kOutputs && tid == 0) flags[par] = 0;
-    if (more) stage(t0 + kQ, par ^ 1);
+    if (more) {
+      decays(t0 + kQ, par ^ 1);
+      if (t0 + 2 * kQ < pc.n) load_dt(t0 + 2 * kQ);
+    }
   }
 
   float* const to = PHASE == kSsmEnds ? carry : (last && slot >= 0 ? pool : nullptr);
@@ -491,7 +486,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
-      for (int T = 0; T < NT; ++T) *(f32x4*)(to + st_at + (int64_t)16 * ct * N + 16 * T) = h[ct][T];
+      for (int T = 0; T < NT; ++T) *(f32x4*)(to + (st_at + 16 * ct * N + 32 * (T >> 1) + 4 * (T & 1))) = h[ct][T];
   if (PHASE == kSsmEnds && !idle && p0 == 0 && lane == 0) a.carry_decay[(int64_t)index * a.heads + head] = exp2_(total);
 }
 
