@@ -752,61 +752,69 @@ def prefix_attention(q, cache: PagedCache, prefix_table, prefix_len, max_prefix,
 # ---- around the recurrent scans: convolution, state space scan, norms
 
 
+# Each call decides in one expression whether its tensors are right (2 us for the eight tensors of a
+# convolution: the smallest calls are bound by the host), and looks for the one to name only when they
+# are not.
+_torch = None
 _act_codes: dict = {}
+
+
+def _load_torch():
+    global _torch
+    import torch
+
+    _act_codes.update({torch.bfloat16: EMA_DTYPE_BF16, torch.float16: EMA_DTYPE_F16, torch.float32: EMA_DTYPE_F32})
+    _torch = torch
+    lib()
+    return torch
 
 
 def _act_code(op: str, t):
     """EMA_DTYPE_* of an activation tensor."""
-    import torch
-
-    if not _act_codes:
-        _act_codes.update({torch.bfloat16: EMA_DTYPE_BF16, torch.float16: EMA_DTYPE_F16, torch.float32: EMA_DTYPE_F32})
+    _torch or _load_torch()
     code = _act_codes.get(t.dtype)
     if code is None:
         raise EmaError(EMA_ERR_INVALID_ARG, op, f"unsupported activation dtype {t.dtype}")
     return code
 
 
-def _rows_of(op: str, name: str, t, dtype, shape, device: int) -> int:
-    """Row stride of a [n, ...] tensor of the given dtype and shape whose rows are contiguous."""
+def _want_rows(op: str, name: str, t, dtype, shape, device: int) -> None:
+    """A [n, ...] tensor of the given dtype and shape whose rows are contiguous."""
     if t.shape != shape or t.dtype is not dtype:
         raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be a {dtype} tensor {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
     if t.get_device() != device:
         raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} is on {t.device}, not on device {device}")
+    if not _rows_whole(t):
+        raise EmaError(EMA_ERR_SHAPE, op, f"a row of {name} must be contiguous, not strided {t.stride()}")
+
+
+def _rows_whole(t) -> bool:
     width = 1
     for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
         if stride != width and size != 1:
-            raise EmaError(EMA_ERR_SHAPE, op, f"a row of {name} must be contiguous, not strided {t.stride()}")
+            return False
         width *= size
-    # (the stride of a single row, or of none, means nothing: a view may give any)
-    return t.stride(0) if t.shape[0] > 1 else width
+    return True
 
 
-def _batch_of(op: str, n: int, dev: int, starts, offsets, slots, batch):
-    """The number of sequences; checks the int32 tensors that describe them."""
-    import torch
-
-    if batch is None:
-        batch = (starts.shape[0] - 1 if starts is not None else offsets.shape[0] if offsets is not None
-                 else slots.shape[0] if slots is not None else None)
-        if batch is None:
-            raise EmaError(EMA_ERR_INVALID_ARG, op, "batch is needed without starts, offsets and slots")
+def _name_batch(op: str, dev: int, batch, starts, offsets, slots) -> None:
+    """Raises for the first of the int32 tensors that describe the sequences that is not right."""
     for name, t, size in (("starts", starts, batch + 1), ("offsets", offsets, batch), ("slots", slots, batch)):
-        if t is not None and not (t.dtype is torch.int32 and t.shape == (size,) and t.is_contiguous()
-                                  and t.get_device() == dev):
-            _want(op, name, t, torch.int32, (size,), dev)
-    return batch
+        if t is not None:
+            _want(op, name, t, _torch.int32, (size,), dev)
 
 
-def _mixer_call(op: str, dev: int, stream, *args) -> None:
+def _empty(stream, shape, dtype, device):
+    with _on(stream):
+        return _torch.empty(shape, dtype=dtype, device=device)
+
+
+def _mixer_call(op: str, dev: int, call, stream, *args) -> None:
     """The library's call on `dev`'s current stream, or the given one, with `dev` current."""
-    import torch
-
     if dev < 0:
         raise EmaError(EMA_ERR_INVALID_ARG, op, "the tensors are not on a GPU")
-    raw = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
-    call = getattr(lib(), op)
-    rc = call(raw, *args) if torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, raw, *args)
+    raw = _torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    rc = call(raw, *args) if _torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, raw, *args)
     if rc:
         _check(rc, op)
 
@@ -818,45 +826,61 @@ def causal_conv(x, weight, bias=None, state=None, starts=None, offsets=None, slo
     [n_slots, W-1, C], the inputs kept between calls, updated in place (None: start from zeros, keep nothing).
     starts int32 [B+1] (None: n / B rows each), offsets int32 [B] (position of the first row: at 0 a sequence
     starts from zeros), slots int32 [B] (None: slot b). Returns out [n, C]."""
-    import torch
-
     op = "ema_causal_conv"
+    i32 = (_torch or _load_torch()).int32
     try:
-        code, dev, dtype = _act_code(op, x), x.get_device(), x.dtype
-        if x.dim() != 2 or weight.dim() != 2:
-            raise EmaError(EMA_ERR_SHAPE, op, f"x must be [n, C] and weight [C, W], not {tuple(x.shape)}, {tuple(weight.shape)}")
-        n, C = x.shape
+        dtype, dev = x.dtype, x.get_device()
+        (n, C), (ldx, sx) = x.shape, x.stride()
         W = weight.shape[1]
-        if batch is None and starts is None and offsets is None and slots is None:
-            batch = state.shape[0] if state is not None else 1
-        batch = _batch_of(op, n, dev, starts, offsets, slots, batch)
+        if batch is None:
+            batch = (starts.shape[0] - 1 if starts is not None else offsets.shape[0] if offsets is not None
+                     else slots.shape[0] if slots is not None else state.shape[0] if state is not None else 1)
         if out is None:
-            with _on(stream):
-                out = torch.empty((n, C), dtype=dtype, device=x.device)
-        ldx, ldy = _rows_of(op, "x", x, dtype, (n, C), dev), _rows_of(op, "out", out, dtype, (n, C), dev)
-        _want(op, "weight", weight, dtype, (C, W), dev)
-        if bias is not None:
-            _want(op, "bias", bias, dtype, (C,), dev)
-        if state is not None:
-            _want(op, "state", state, dtype, (state.shape[0], W - 1, C), dev)
-    except AttributeError:
+            out = _empty(stream, (n, C), dtype, x.device)
+        ldy, sy = out.stride()
+        n_slots = 0 if state is None else state.shape[0]
+        if not (dtype in _act_codes and (sx == 1 or C == 1) and (sy == 1 or C == 1)
+                and out.dtype is dtype and out.shape == (n, C) and out.get_device() == dev
+                and weight.dtype is dtype and weight.shape == (C, W) and weight.is_contiguous() and weight.get_device() == dev
+                and (bias is None or (bias.dtype is dtype and bias.shape == (C,) and bias.is_contiguous()
+                                      and bias.get_device() == dev))
+                and (state is None or (state.dtype is dtype and state.shape == (n_slots, W - 1, C)
+                                       and state.is_contiguous() and state.get_device() == dev))
+                and (starts is None or (starts.dtype is i32 and starts.shape == (batch + 1,) and starts.is_contiguous()
+                                        and starts.get_device() == dev))
+                and (offsets is None or (offsets.dtype is i32 and offsets.shape == (batch,) and offsets.is_contiguous()
+                                         and offsets.get_device() == dev))
+                and (slots is None or (slots.dtype is i32 and slots.shape == (batch,) and slots.is_contiguous()
+                                       and slots.get_device() == dev))):
+            _act_code(op, x)
+            _want_rows(op, "x", x, dtype, (n, C), dev)
+            _want_rows(op, "out", out, dtype, (n, C), dev)
+            _want(op, "weight", weight, dtype, (C, W), dev)
+            for name, t, shape in (("bias", bias, (C,)), ("state", state, (n_slots, W - 1, C))):
+                if t is not None:
+                    _want(op, name, t, dtype, shape, dev)
+            _name_batch(op, dev, batch, starts, offsets, slots)
+    except (AttributeError, ValueError, IndexError):
         _no_tensor(op, dict(x=x, weight=weight),
                    dict(bias=bias, state=state, starts=starts, offsets=offsets, slots=slots, out=out))
+        if x.dim() != 2 or weight.dim() != 2 or (out is not None and out.dim() != 2):
+            raise EmaError(EMA_ERR_SHAPE, op, f"x must be [n, C] and weight [C, W], not {tuple(x.shape)}, {tuple(weight.shape)}")
         raise
-    _mixer_call(op, dev, stream, x.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), _ptr(starts), _ptr(offsets),
-                _ptr(slots), batch, n, n if max_rows is None else max_rows, C, W, EMA_CONV_SILU if silu else 0,
-                _ptr(state), 0 if state is None else state.shape[0], out.data_ptr(), ldy, code)
+    _mixer_call(op, dev, _lib.ema_causal_conv, stream, x.data_ptr(), ldx if n > 1 else C, weight.data_ptr(),
+                None if bias is None else bias.data_ptr(), None if starts is None else starts.data_ptr(),
+                None if offsets is None else offsets.data_ptr(), None if slots is None else slots.data_ptr(), batch, n,
+                n if max_rows is None else max_rows, C, W, EMA_CONV_SILU if silu else 0,
+                None if state is None else state.data_ptr(), n_slots, out.data_ptr(), ldy if n > 1 else C,
+                _act_codes[dtype])
     return out
 
 
 def ssm_workspace_size(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype=None) -> int:
     """Bytes with which ssm_scan splits such a call in time as it likes best (0: it does not); dtype a torch
     type, bf16 by default."""
-    import torch
-
+    _torch or _load_torch()
     out = ctypes.c_uint64()
-    code = {None: EMA_DTYPE_BF16, torch.bfloat16: EMA_DTYPE_BF16, torch.float16: EMA_DTYPE_F16,
-            torch.float32: EMA_DTYPE_F32}.get(dtype, 0)
+    code = EMA_DTYPE_BF16 if dtype is None else _act_codes.get(dtype, 0)
     _check(lib().ema_ssm_workspace_size(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, code,
                                         ctypes.byref(out)), "ema_ssm_workspace_size")
     return out.value
@@ -864,10 +888,8 @@ def ssm_workspace_size(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_gr
 
 def ssm_workspace(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype=None, device="cuda"):
     """A workspace for ssm_scan (no initialisation needed), reusable on one stream."""
-    import torch
-
-    return torch.empty(ssm_workspace_size(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype),
-                       dtype=torch.uint8, device=device)
+    size = ssm_workspace_size(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype)
+    return _torch.empty(size, dtype=_torch.uint8, device=device)
 
 
 def ssm_scan(x, dt, B, C, A, state, D=None, dt_bias=None, starts=None, offsets=None, slots=None, batch=None,
@@ -877,46 +899,73 @@ def ssm_scan(x, dt, B, C, A, state, D=None, dt_bias=None, starts=None, offsets=N
     [n_slots, H, P, N], updated in place; starts, offsets, slots as in causal_conv; max_rows a host bound of a
     sequence's rows. workspace: a uint8 tensor (ssm_workspace) that long sequences are split over; None
     allocates one. Returns out [n, H, P]."""
-    import torch
-
     op = "ema_ssm_scan"
+    torch = _torch or _load_torch()
+    i32, f32 = torch.int32, torch.float32
     try:
-        code, dev, dtype = _act_code(op, x), x.get_device(), x.dtype
-        if x.dim() != 3 or B.dim() != 3 or state.dim() != 4:
-            raise EmaError(EMA_ERR_SHAPE, op, f"x [n, H, P], B [n, G, N] and state [n_slots, H, P, N] are wanted, not "
-                                              f"{tuple(x.shape)}, {tuple(B.shape)}, {tuple(state.shape)}")
-        n, H, P = x.shape
-        G, N = B.shape[1:]
-        if batch is None and starts is None and offsets is None and slots is None:
-            batch = state.shape[0]
-        batch = _batch_of(op, n, dev, starts, offsets, slots, batch)
+        dtype, dev = x.dtype, x.get_device()
+        (n, H, P), (ldx, sh, sp) = x.shape, x.stride()
+        _, G, N = B.shape
+        (ldb, sbg, sbn), (ldc, scg, scn), (lddt, sdt) = B.stride(), C.stride(), dt.stride()
+        n_slots = state.shape[0]
+        if batch is None:
+            batch = (starts.shape[0] - 1 if starts is not None else offsets.shape[0] if offsets is not None
+                     else slots.shape[0] if slots is not None else n_slots)
         if max_rows is None:
             max_rows = n
         if out is None:
-            with _on(stream):
-                out = torch.empty((n, H, P), dtype=dtype, device=x.device)
-        ldx, ldy = _rows_of(op, "x", x, dtype, (n, H, P), dev), _rows_of(op, "out", out, dtype, (n, H, P), dev)
-        ldb, ldc = _rows_of(op, "B", B, dtype, (n, G, N), dev), _rows_of(op, "C", C, dtype, (n, G, N), dev)
-        lddt = _rows_of(op, "dt", dt, dtype, (n, H), dev)
-        f32 = torch.float32
-        for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
-            if (t is not None or name == "A") and not (t.dtype is f32 and t.shape == (H,) and t.is_contiguous()
-                                                       and t.get_device() == dev):
-                _want(op, name, t, f32, (H,), dev)
-        _want(op, "state", state, f32, (state.shape[0], H, P, N), dev)
-        if workspace is not None:
-            _want(op, "workspace", workspace, torch.uint8, workspace.shape, dev)
-    except AttributeError:
+            out = _empty(stream, (n, H, P), dtype, x.device)
+        ldy, yh, yp = out.stride()
+        if not (dtype in _act_codes and (sp == 1 or P == 1) and (sh == P or H == 1) and (yp == 1 or P == 1)
+                and (yh == P or H == 1) and (sbn == 1 or N == 1) and (sbg == N or G == 1) and (scn == 1 or N == 1)
+                and (scg == N or G == 1) and (sdt == 1 or H == 1)
+                and out.dtype is dtype and out.shape == (n, H, P) and out.get_device() == dev
+                and B.dtype is dtype and B.shape == (n, G, N) and B.get_device() == dev
+                and C.dtype is dtype and C.shape == (n, G, N) and C.get_device() == dev
+                and dt.dtype is dtype and dt.shape == (n, H) and dt.get_device() == dev
+                and A.dtype is f32 and A.shape == (H,) and A.is_contiguous() and A.get_device() == dev
+                and state.dtype is f32 and state.shape == (n_slots, H, P, N) and state.is_contiguous()
+                and state.get_device() == dev
+                and (D is None or (D.dtype is f32 and D.shape == (H,) and D.is_contiguous() and D.get_device() == dev))
+                and (dt_bias is None or (dt_bias.dtype is f32 and dt_bias.shape == (H,) and dt_bias.is_contiguous()
+                                         and dt_bias.get_device() == dev))
+                and (starts is None or (starts.dtype is i32 and starts.shape == (batch + 1,) and starts.is_contiguous()
+                                        and starts.get_device() == dev))
+                and (offsets is None or (offsets.dtype is i32 and offsets.shape == (batch,) and offsets.is_contiguous()
+                                         and offsets.get_device() == dev))
+                and (slots is None or (slots.dtype is i32 and slots.shape == (batch,) and slots.is_contiguous()
+                                       and slots.get_device() == dev))
+                and (workspace is None or (workspace.dtype is torch.uint8 and workspace.is_contiguous()
+                                           and workspace.get_device() == dev))):
+            _act_code(op, x)
+            for name, t, shape in (("x", x, (n, H, P)), ("out", out, (n, H, P)), ("B", B, (n, G, N)), ("C", C, (n, G, N)),
+                                   ("dt", dt, (n, H))):
+                _want_rows(op, name, t, dtype, shape, dev)
+            for name, t, shape in (("A", A, (H,)), ("D", D, (H,)), ("dt_bias", dt_bias, (H,)),
+                                   ("state", state, (n_slots, H, P, N))):
+                if t is not None or name == "A":
+                    _want(op, name, t, f32, shape, dev)
+            if workspace is not None:
+                _want(op, "workspace", workspace, torch.uint8, workspace.shape, dev)
+            _name_batch(op, dev, batch, starts, offsets, slots)
+    except (AttributeError, ValueError, IndexError):
         _no_tensor(op, dict(x=x, dt=dt, B=B, C=C, A=A, state=state),
                    dict(D=D, dt_bias=dt_bias, starts=starts, offsets=offsets, slots=slots, out=out, workspace=workspace))
+        for name, t, dims in (("x", x, 3), ("dt", dt, 2), ("B", B, 3), ("C", C, 3), ("out", out, 3)):
+            if t is not None and t.dim() != dims:
+                raise EmaError(EMA_ERR_SHAPE, op, f"{name} must have {dims} dimensions, not {tuple(t.shape)}")
         raise
     if workspace is None and dev >= 0 and n:
-        with _on(stream):
-            workspace = ssm_workspace(batch, n, max_rows, H, P, N, G, dtype, device=x.device)
-    _mixer_call(op, dev, stream, x.data_ptr(), ldx, dt.data_ptr(), lddt, B.data_ptr(), ldb, C.data_ptr(), ldc,
-                A.data_ptr(), _ptr(D), _ptr(dt_bias), dt_limit[0], dt_limit[1], _ptr(starts), _ptr(offsets), _ptr(slots),
-                batch, n, max_rows, H, P, G, N, EMA_SSM_SOFTPLUS if softplus else 0, state.data_ptr(), state.shape[0],
-                out.data_ptr(), ldy, code, _ptr(workspace) or None, 0 if workspace is None else workspace.numel())
+        size = ssm_workspace_size(batch, n, max_rows, H, P, N, G, dtype)
+        workspace = _empty(stream, (size,), torch.uint8, x.device)
+    size = 0 if workspace is None else workspace.numel()
+    _mixer_call(op, dev, _lib.ema_ssm_scan, stream, x.data_ptr(), ldx if n > 1 else H * P, dt.data_ptr(),
+                lddt if n > 1 else H, B.data_ptr(), ldb if n > 1 else G * N, C.data_ptr(), ldc if n > 1 else G * N,
+                A.data_ptr(), None if D is None else D.data_ptr(), None if dt_bias is None else dt_bias.data_ptr(),
+                dt_limit[0], dt_limit[1], None if starts is None else starts.data_ptr(),
+                None if offsets is None else offsets.data_ptr(), None if slots is None else slots.data_ptr(), batch, n,
+                max_rows, H, P, G, N, EMA_SSM_SOFTPLUS if softplus else 0, state.data_ptr(), n_slots, out.data_ptr(),
+                ldy if n > 1 else H * P, _act_codes[dtype], workspace.data_ptr() if size else None, size)
     return out
 
 
@@ -926,32 +975,44 @@ def gated_norm(x, gate, weight, eps, group=None, gate_first=False, sigmoid=False
     act(gate), or norm(x * act(gate)) * w with gate_first; act is silu, or sigmoid. gate [n, dim] or None;
     weight [dim], [group] (one for all groups) or None; unit_offset: 1 + w multiplies. Rows of x, gate and out
     may be pieces of wider ones; out may be x or gate. Returns out [n, dim]."""
-    import torch
-
     op = "ema_gated_norm"
+    _torch or _load_torch()
     try:
-        code, dev, dtype = _act_code(op, x), x.get_device(), x.dtype
-        if x.dim() != 2:
-            raise EmaError(EMA_ERR_SHAPE, op, f"x must be [n, dim], not {tuple(x.shape)}")
-        n, dim = x.shape
+        dtype, dev = x.dtype, x.get_device()
+        (n, dim), (ldx, sx) = x.shape, x.stride()
         if group is None:
             group = dim
         if out is None:
-            with _on(stream):
-                out = torch.empty((n, dim), dtype=dtype, device=x.device)
-        ldx, ldy = _rows_of(op, "x", x, dtype, (n, dim), dev), _rows_of(op, "out", out, dtype, (n, dim), dev)
-        ldg = 0 if gate is None else _rows_of(op, "gate", gate, dtype, (n, dim), dev)
+            out = _empty(stream, (n, dim), dtype, x.device)
+        ldy, sy = out.stride()
+        ldg, sg = (0, 1) if gate is None else gate.stride()
         flags = ((EMA_NORM_GATE_FIRST if gate_first else 0) | (EMA_NORM_GATE_SIGMOID if sigmoid else 0)
                  | (EMA_NORM_UNIT_OFFSET if unit_offset else 0))
-        if weight is not None:
-            if weight.shape == (group,) and group != dim:
-                flags |= EMA_NORM_SHARED_WEIGHT
-            _want(op, "weight", weight, dtype, (group,) if flags & EMA_NORM_SHARED_WEIGHT else (dim,), dev)
-    except AttributeError:
+        width = dim
+        if weight is not None and group != dim and weight.shape == (group,):
+            flags |= EMA_NORM_SHARED_WEIGHT
+            width = group
+        if not (dtype in _act_codes and (sx == 1 or dim == 1) and (sy == 1 or dim == 1) and (sg == 1 or dim == 1)
+                and out.dtype is dtype and out.shape == (n, dim) and out.get_device() == dev
+                and (gate is None or (gate.dtype is dtype and gate.shape == (n, dim) and gate.get_device() == dev))
+                and (weight is None or (weight.dtype is dtype and weight.shape == (width,) and weight.is_contiguous()
+                                        and weight.get_device() == dev))):
+            _act_code(op, x)
+            for name, t in (("x", x), ("out", out), ("gate", gate)):
+                if t is not None:
+                    _want_rows(op, name, t, dtype, (n, dim), dev)
+            if weight is not None:
+                _want(op, "weight", weight, dtype, (width,), dev)
+    except (AttributeError, ValueError):
         _no_tensor(op, dict(x=x), dict(gate=gate, weight=weight, out=out))
+        for name, t in (("x", x), ("gate", gate), ("out", out)):
+            if t is not None and t.dim() != 2:
+                raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be [n, dim], not {tuple(t.shape)}")
         raise
-    _mixer_call(op, dev, stream, x.data_ptr(), ldx, _ptr(gate), ldg, _ptr(weight), eps, n, dim, group, flags,
-                out.data_ptr(), ldy, code)
+    _mixer_call(op, dev, _lib.ema_gated_norm, stream, x.data_ptr(), ldx if n > 1 else dim,
+                None if gate is None else gate.data_ptr(), ldg if n > 1 else dim,
+                None if weight is None else weight.data_ptr(), eps, n, dim, group, flags, out.data_ptr(),
+                ldy if n > 1 else dim, _act_codes[dtype])
     return out
 
 
@@ -962,35 +1023,50 @@ def residual_norm(branch, residual, pre_weight, eps, post_weight=None, gate=None
     norm(residual) * pre_weight (of the sum before it is rounded). branch [n, dim] in bf16, f16 or f32, residual
     [n, dim] in the same type or f32; gate [n, dim], [dim] (one for all rows) or None; pre_weight None: the
     residual stream alone (returns None). Rows may be pieces of wider ones; out may be branch."""
-    import torch
-
     op = "ema_residual_norm"
+    f32 = (_torch or _load_torch()).float32
     try:
-        code, dev, dtype = _act_code(op, branch), branch.get_device(), branch.dtype
-        if branch.dim() != 2:
-            raise EmaError(EMA_ERR_SHAPE, op, f"branch must be [n, dim], not {tuple(branch.shape)}")
-        n, dim = branch.shape
+        dtype, dev, rtype = branch.dtype, branch.get_device(), residual.dtype
+        (n, dim), (ldx, sx), (ldr, sr) = branch.shape, branch.stride(), residual.stride()
         if out is None and pre_weight is not None:
-            with _on(stream):
-                out = torch.empty((n, dim), dtype=dtype, device=branch.device)
-        stream_code = EMA_DTYPE_F32 if residual.dtype is torch.float32 else code
-        ldx = _rows_of(op, "branch", branch, dtype, (n, dim), dev)
-        ldr = _rows_of(op, "residual", residual, torch.float32 if stream_code == EMA_DTYPE_F32 else dtype, (n, dim), dev)
-        ldo = 0 if out is None else _rows_of(op, "out", out, dtype, (n, dim), dev)
-        ldg = 0
-        if gate is not None:
-            if gate.dim() == 1:
-                _want(op, "gate", gate, dtype, (dim,), dev)
-            else:
-                ldg = _rows_of(op, "gate", gate, dtype, (n, dim), dev)
-        for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
-            if w is not None:
-                _want(op, name, w, dtype, (dim,), dev)
-    except AttributeError:
+            out = _empty(stream, (n, dim), dtype, branch.device)
+        ldo, so = (0, 1) if out is None else out.stride()
+        one = gate is not None and gate.dim() == 1  # a row for all
+        ldg, sg = (0, 1) if gate is None or one else gate.stride()
+        if not (dtype in _act_codes and (rtype is dtype or rtype is f32) and (sx == 1 or dim == 1)
+                and (sr == 1 or dim == 1) and (so == 1 or dim == 1) and (sg == 1 or dim == 1)
+                and residual.shape == (n, dim) and residual.get_device() == dev
+                and (out is None or (out.dtype is dtype and out.shape == (n, dim) and out.get_device() == dev))
+                and (gate is None or (gate.dtype is dtype and gate.shape == ((dim,) if one else (n, dim))
+                                      and (not one or gate.is_contiguous()) and gate.get_device() == dev))
+                and (pre_weight is None or (pre_weight.dtype is dtype and pre_weight.shape == (dim,)
+                                            and pre_weight.is_contiguous() and pre_weight.get_device() == dev))
+                and (post_weight is None or (post_weight.dtype is dtype and post_weight.shape == (dim,)
+                                             and post_weight.is_contiguous() and post_weight.get_device() == dev))):
+            _act_code(op, branch)
+            _want_rows(op, "branch", branch, dtype, (n, dim), dev)
+            _want_rows(op, "residual", residual, f32 if rtype is f32 else dtype, (n, dim), dev)
+            if out is not None:
+                _want_rows(op, "out", out, dtype, (n, dim), dev)
+            if gate is not None:
+                (_want if one else _want_rows)(op, "gate", gate, dtype, (dim,) if one else (n, dim), dev)
+            for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
+                if w is not None:
+                    _want(op, name, w, dtype, (dim,), dev)
+    except (AttributeError, ValueError):
         _no_tensor(op, dict(branch=branch, residual=residual),
                    dict(pre_weight=pre_weight, post_weight=post_weight, gate=gate, out=out))
+        for name, t in (("branch", branch), ("residual", residual), ("gate", gate), ("out", out)):
+            if t is not None and t.dim() != 2 and not (name == "gate" and t.dim() == 1):
+                raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be [n, dim], not {tuple(t.shape)}")
         raise
-    _mixer_call(op, dev, stream, branch.data_ptr(), ldx, _ptr(post_weight), _ptr(gate), ldg, scale, residual.data_ptr(),
-                ldr, stream_code, _ptr(pre_weight), eps, n, dim, EMA_NORM_UNIT_OFFSET if unit_offset else 0, _ptr(out),
-                ldo, code)
+    if n <= 1:
+        ldx = ldr = ldo = dim
+        ldg = 0
+    _mixer_call(op, dev, _lib.ema_residual_norm, stream, branch.data_ptr(), ldx,
+                None if post_weight is None else post_weight.data_ptr(), None if gate is None else gate.data_ptr(), ldg,
+                scale, residual.data_ptr(), ldr, EMA_DTYPE_F32 if rtype is f32 else _act_codes[dtype],
+                None if pre_weight is None else pre_weight.data_ptr(), eps, n, dim,
+                EMA_NORM_UNIT_OFFSET if unit_offset else 0, None if out is None else out.data_ptr(), ldo,
+                _act_codes[dtype])
     return out
