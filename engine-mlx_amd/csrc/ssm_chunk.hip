@@ -21,7 +21,9 @@
 //
 // Rounded to bf16: H and M where they are operands of y (as an attention's weights are; x, B and C
 // are exact), each by at most 2^-8 of the term. The state itself takes the scaled x as three bf16
-// parts, 24 bits together (two left it 1.5e-6 off, three 5e-8), products and sums in 32 bits.
+// parts, 24 bits together (two left it 1.5e-6 off, three 5e-8), products and sums in 32 bits. The ends of
+// pieces take two parts, 16 bits: what they hand on decays over at least a piece more, and is rounded
+// to 8 bits where y reads it.
 //
 // A value of x that is not finite would reach rows before it through M's zeros (0 times infinity):
 // chunks with such values (a dot product with zeros finds them while they are staged) take those
@@ -46,14 +48,15 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // Per-head values of a chunk (floats): index by row unless said otherwise.
 struct Dec {
-  static constexpr int kCum = 0;     // sum of log2 decays from the row's 16-row tile's start, the row included
-  static constexpr int kStep = 32;   // d
-  static constexpr int kF = 64;      // decay from the tile's start: 2^kCum
-  static constexpr int kE = 96;      // decay from the chunk's start
-  static constexpr int kW = 128;     // d times the decay from behind the row to the chunk's end
-  static constexpr int kG = 160;     // d times the decay from behind the row to its tile's end
-  static constexpr int kAll = 192;   // decay over the chunk; its log2 at 193
-  static constexpr int kD = 194;     // D
+  static constexpr int kW = 0;       // d times the decay from behind the row to the chunk's end
+  static constexpr int kAll = 32;    // decay over the chunk; its log2 at 33
+  static constexpr int kEnds = 36;   // (that is all that the pieces' ends need)
+  static constexpr int kD = 34;      // D
+  static constexpr int kCum = 36;    // sum of log2 decays from the row's 16-row tile's start, the row included
+  static constexpr int kStep = 68;   // d
+  static constexpr int kF = 100;     // decay from the tile's start: 2^kCum
+  static constexpr int kE = 132;     // decay from the chunk's start
+  static constexpr int kG = 164;     // d times the decay from behind the row to its tile's end
   static constexpr int kFloats = 196;
 };
 
@@ -89,22 +92,23 @@ __device__ __forceinline__ void chunk_decays(float raw, int n, float A2, float D
   const float d = row < n ? ssm_step(raw, a) : 0.f;
   // log2 of the row's decay; below 2^-150 it is 0 either way, and sums stay finite
   const float l = fmaxf(d * A2, -150.f);
-  float up = l, down = l;  // sums over the 16-row tile: up to the row, from the row on
-  up += dpp_shift<0x111>(up);
+  float down = l;  // sum over the 16-row tile from the row on
   down += dpp_shift<0x101>(down);
-  up += dpp_shift<0x112>(up);
   down += dpp_shift<0x102>(down);
-  up += dpp_shift<0x114>(up);
   down += dpp_shift<0x104>(down);
-  up += dpp_shift<0x118>(up);
   down += dpp_shift<0x108>(down);
   const float behind = dpp_shift<0x101>(down);  // from behind the row to its tile's end
   const bool second = lane >= 32, tile1 = row >= 16;
-  const float t0 = second ? lane_value(up, 47) : lane_value(up, 15), t1 = second ? lane_value(up, 63) : lane_value(up, 31);
+  const float t0 = second ? lane_value(down, 32) : lane_value(down, 0), t1 = second ? lane_value(down, 48) : lane_value(down, 16);
   dec[Dec::kW + row] = d * exp2_(behind + (tile1 ? 0.f : t1));
   dec[Dec::kAll] = exp2_(t0 + t1);  // (every lane the same)
   dec[Dec::kAll + 1] = t0 + t1;
   if constexpr (kOutputs) {
+    float up = l;  // up to the row
+    up += dpp_shift<0x111>(up);
+    up += dpp_shift<0x112>(up);
+    up += dpp_shift<0x114>(up);
+    up += dpp_shift<0x118>(up);
     dec[Dec::kD] = D;
     dec[Dec::kCum + row] = up;
     dec[Dec::kStep + row] = d;
@@ -114,18 +118,21 @@ __device__ __forceinline__ void chunk_decays(float raw, int n, float A2, float D
   }
 }
 
-// LDS (bytes): B, x and (for outputs) C, twice; M of every head of the workgroup; the heads' decays,
-// twice; the flags of chunks with values that are not finite, twice.
-template <int N, bool kOutputs>
+// LDS (bytes): B, x and (for outputs) C, twice; M of every head of the workgroup; the heads' decays of
+// two groups of chunks; the flags of chunks with values that are not finite, twice.
+template <int N, int HEADS, bool kOutputs>
 struct Lds {
+  // chunks whose decays are formed at once, by a wave each (two heads a wave)
+  static constexpr int kGroup = HEADS == 4 ? 2 : 4;
   static constexpr int kX = kQ * N * 2;
   static constexpr int kC = kX + kQ * kXW * 2;
   static constexpr int kBuf = kC + (kOutputs ? kQ * N * 2 : 0);
   static constexpr int kM = 2 * kBuf;
   static constexpr int kMHead = 2 * 1024;  // one operand for each 16-row tile of t
-  static constexpr __host__ __device__ int dec(int heads) { return kM + (kOutputs ? heads * kMHead : 0); }
-  static constexpr __host__ __device__ int flag(int heads) { return dec(heads) + 2 * heads * Dec::kFloats * 4; }
-  static constexpr __host__ __device__ int bytes(int heads) { return flag(heads) + 16; }
+  static constexpr int kDec = kM + (kOutputs ? HEADS * kMHead : 0);
+  static constexpr int kDecHead = kOutputs ? Dec::kFloats : Dec::kEnds;
+  static constexpr int kFlag = kDec + 2 * kGroup * HEADS * kDecHead * 4;
+  static constexpr int kBytes = kFlag + 16;
 };
 
 struct ChunkGrid {
@@ -138,9 +145,10 @@ struct ChunkGrid {
 template <int N, int HEADS, int PHASE>
 __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(SsmArgs a, ChunkGrid gr) {
   constexpr bool kOutputs = PHASE != kSsmEnds;
-  typedef Lds<N, kOutputs> L;
+  typedef Lds<N, HEADS, kOutputs> L;
   constexpr int KS = N / 32;   // 32-wide steps over d_state
   constexpr int NT = N / 16;   // 16-row tiles of it
+  constexpr int kParts = kOutputs ? 3 : 2;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 
   // the workgroups of a (piece, group) read the same B and C: on one XCD (blocks go to the XCDs in turn)
@@ -174,8 +182,8 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   const int st_at = (p0 + l16) * N + 8 * c4;
 
   uint8_t* const Ms = lds + L::kM;
-  float* const decs = (float*)(lds + L::dec(HEADS));
-  int* const flags = (int*)(lds + L::flag(HEADS));
+  float* const decs = (float*)(lds + L::kDec);
+  int* const flags = (int*)(lds + L::kFlag);
 
   // ---- state: h[ct][T] holds n = 32 (T / 2) + 8 c4 + 4 (T % 2) + i of column p0 + 16 ct + l16
   f32x4 h[2][NT];
@@ -247,20 +255,31 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
     if constexpr (kOutputs)
       if (zero != zero) flags[par] = 1;
   };
-  // every wave forms the decays of its head and its neighbour (waves of one head write the same
-  // values): no wave waits for another's
-  const int d_head = (hh & ~1) + (lane >> 5) < n_heads ? (hh & ~1) + (lane >> 5) : hh & ~1;
+  // the decays of a group of chunks: each wave one chunk's of two heads
+  constexpr int kGroup = L::kGroup;
+  const int d_chunk = wave % kGroup, d_pair = 2 * (wave / kGroup);
+  const int d_head = d_pair + (lane >> 5) < n_heads ? d_pair + (lane >> 5) : (d_pair < n_heads ? d_pair : 0);
   const uint16_t* const dp = (const uint16_t*)a.dt + (int64_t)pc.row * a.lddt + head0 + first_head + d_head;
   const float A2 = a.a[head0 + first_head + d_head] * kLog2e;
   const float bias = a.dt_bias ? a.dt_bias[head0 + first_head + d_head] : 0.f;
   const float D = a.d ? a.d[head0 + first_head + d_head] : 0.f;
+  // The chunks in the order in which they are taken: their number `step` begins at row row_of(step). The
+  // ends of a piece (whole chunks) are taken from its last rows on: the decay from behind a chunk to the
+  // piece's end then goes into the chunk's factors, and the sums are never scaled.
+  const int n_steps = (pc.n + kQ - 1) / kQ;
+  auto row_of = [&](int step) __attribute__((always_inline)) { return kOutputs ? step * kQ : (n_steps - 1 - step) * kQ; };
   uint16_t rdt = 0;
-  auto load_dt = [&](int t0) __attribute__((always_inline)) {
-    const int end = pc.n - t0 - 1, r = lane & 31;
-    rdt = dp[(int64_t)(t0 + (r < end ? r : end)) * a.lddt];
+  auto load_dt = [&](int step) __attribute__((always_inline)) {  // of the wave's chunk in the group of `step`
+    const int s = step + d_chunk < n_steps ? step + d_chunk : n_steps - 1;
+    const int r = row_of(s) + (lane & 31);
+    rdt = dp[(int64_t)(r < pc.n ? r : pc.n - 1) * a.lddt];
   };
-  auto decays = [&](int t0, int par) __attribute__((always_inline)) {
-    chunk_decays<kOutputs>(bf16_to_f32(rdt) + bias, pc.n - t0, A2, D, a, decs + (par * HEADS + d_head) * Dec::kFloats);
+  auto dec_of = [&](int step, int head) __attribute__((always_inline)) {
+    return decs + (step % (2 * kGroup) * HEADS + head) * L::kDecHead;
+  };
+  auto decays = [&](int step) __attribute__((always_inline)) {
+    const int s = step + d_chunk < n_steps ? step + d_chunk : n_steps - 1;  // (a chunk that is not there: not read)
+    chunk_decays<kOutputs>(bf16_to_f32(rdt) + bias, pc.n - row_of(s), A2, D, a, dec_of(step + d_chunk, d_head));
   };
 
   if constexpr (kOutputs) {
@@ -296,35 +315,38 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   uint8_t* const yp = (uint8_t*)((uint16_t*)a.y + (int64_t)pc.row * a.ldy + (int64_t)head * P + p0);
   const uint32_t ldy2 = (uint32_t)a.ldy * 2, y_at = l16 * ldy2 + 8 * c4;
   load_dt(0);
-  load(0);
-  decays(0, 0);
+  load(row_of(0));
+  decays(0);
   store(0);
-  if (pc.n > kQ) {
-    load_dt(kQ);
-    load(kQ);
-  }
-  for (int t0 = 0, par = 0; t0 < pc.n; t0 += kQ, par ^= 1) {
+  if (n_steps > kGroup) load_dt(kGroup);
+  if (n_steps > 1) load(row_of(1));
+  for (int step = 0, par = 0; step < n_steps; ++step, par ^= 1) {
     __syncthreads();  // the chunk is staged, the buffers of the one before are free
-    const bool more = t0 + kQ < pc.n;
+    const int t0 = row_of(step);
+    const bool more = step + 1 < n_steps;
     const uint8_t* const buf = lds + par * L::kBuf;
-    const float* const dec = decs + (par * HEADS + hh) * Dec::kFloats;
-    const float all = dec[Dec::kAll];
+    const float* const dec = dec_of(step, hh);
+    const float all = dec[Dec::kAll], behind = kOutputs ? 1.f : exp2_(total);
     total += dec[Dec::kAll + 1];
     bf16x8 xt[2];  // x^T of the column tiles
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) xt[ct] = x_operand(buf + L::kX, 2 * wave + ct);
     // x scaled, in three bf16 parts: two neighbouring rows of one column a call
-    u32x4 part[3][2];
-    const f32x4 wt[2] = {*(const f32x4*)&dec[Dec::kW + 4 * c4], *(const f32x4*)&dec[Dec::kW + 16 + 4 * c4]};
+    u32x4 part[kParts][2];
+    f32x4 wt[2] = {*(const f32x4*)&dec[Dec::kW + 4 * c4], *(const f32x4*)&dec[Dec::kW + 16 + 4 * c4]};
+    if constexpr (!kOutputs) {
+      wt[0] *= behind;
+      wt[1] *= behind;
+    }
     auto scaled = [&](int ct, int e) __attribute__((always_inline)) {
       const uint32_t xw = __builtin_bit_cast(u32x4, xt[ct])[e];
       const f32x4 w = wt[e >> 1];
       float v0 = bf16_lo(xw) * w[2 * (e & 1)], v1 = bf16_hi(xw) * w[2 * (e & 1) + 1];
 #pragma unroll
-      for (int k = 0; k < 3; ++k) {
+      for (int k = 0; k < kParts; ++k) {
         const uint32_t u = pack_bf16x2(v0, v1);
         part[k][ct][e] = u;
-        if (k < 2) {
+        if (k < kParts - 1) {
           v0 -= bf16_lo(u);
           v1 -= bf16_hi(u);
         }
@@ -365,13 +387,16 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
         for (int e = ks * 8 / KS; e < (ks + 1) * 8 / KS; ++e) scaled(e >> 2, e & 3);
       }
+#pragma unroll
+      for (int k = 0; k < kParts; ++k)  // (formed here, under the products, not where they are used)
+        asm volatile("" : "+v"(part[k][0]), "+v"(part[k][1]));
       // ---- M of the heads from the tile
       uint8_t* const m = Ms + tt * 1024 + lane * 16 + 8 * st;
       if (wave < 2) {
         const int t = 16 * tt + l16, s0 = 16 * tt + 4 * c4;
 #pragma unroll
         for (int j = 0; j < HEADS; ++j) {  // (a head that is not there: values that nothing reads)
-          const float* const dj = decs + (par * HEADS + j) * Dec::kFloats;
+          const float* const dj = dec_of(step, j);
           const f32x4 cum = *(const f32x4*)&dj[Dec::kCum + s0], step = *(const f32x4*)&dj[Dec::kStep + s0];
           const float ct = dj[Dec::kCum + t], Dj = dj[Dec::kD];
           f32x4 v;
@@ -387,7 +412,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
         for (int jj = 0; jj < (HEADS + 1) / 2; ++jj) {
           const int j = 2 * jj + (wave & 1);
           if (j >= HEADS) break;
-          const float* const dj = decs + (par * HEADS + j) * Dec::kFloats;
+          const float* const dj = dec_of(step, j);
           const f32x4 g = *(const f32x4*)&dj[Dec::kG + 4 * c4];
           const f32x4 v = s * g * dj[Dec::kF + 16 + l16];
           *(u32x2*)(m + j * L::kMHead) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
@@ -397,7 +422,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
       const bool bad = __builtin_amdgcn_readfirstlane(flags[par]) != 0;
       if (more) {
         store(par ^ 1);
-        if (t0 + 2 * kQ < pc.n) load(t0 + 2 * kQ);
+        if (step + 2 < n_steps) load(row_of(step + 2));
       }
       const uint8_t* const mh = Ms + hh * L::kMHead + lane * 16;
 #pragma unroll
@@ -457,27 +482,23 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
     } else {
       if (more) {
         store(par ^ 1);
-        if (t0 + 2 * kQ < pc.n) load(t0 + 2 * kQ);
+        if (step + 2 < n_steps) load(row_of(step + 2));
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) scaled(e >> 2, e & 3);
-#pragma unroll
-      for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-        for (int T = 0; T < NT; ++T) h[ct][T] *= all;
     }
-    // ---- the state, and the next chunk's decays (they have a place of their own)
+    // ---- the state, and the next group's decays (they have a place of their own)
 #pragma unroll
     for (int T = 0; T < NT; ++T) {
       const bf16x8 bt = b_operand(buf, T);
 #pragma unroll
-      for (int k = 2; k >= 0; --k)
+      for (int k = kParts - 1; k >= 0; --k)
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) h[ct][T] = mfma16(bt, as_bf16x8(part[k][ct]), h[ct][T]);
     }
-    if (more) {
-      decays(t0 + kQ, par ^ 1);
-      if (t0 + 2 * kQ < pc.n) load_dt(t0 + 2 * kQ);
+    if (more && (step + 1) % kGroup == 0) {
+      decays(step + 1);
+      if (step + 1 + kGroup < n_steps) load_dt(step + 1 + kGroup);
     }
   }
 
@@ -492,7 +513,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 
 template <int N, int HEADS, int PHASE>
 hipError_t launch_phase(hipStream_t s, const SsmArgs& a, const ChunkGrid& g) {
-  constexpr int bytes = Lds<N, PHASE != kSsmEnds>::bytes(HEADS);
+  constexpr int bytes = Lds<N, HEADS, PHASE != kSsmEnds>::kBytes;
   static std::atomic<uint64_t> done{0};
   const void* fn = (const void*)ssm_chunk_kernel<N, HEADS, PHASE>;
   if (allow_lds_once(fn, bytes, &done, "ema_ssm_scan LDS") != EMA_OK) return hipErrorInvalidValue;
