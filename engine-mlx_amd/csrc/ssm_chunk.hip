@@ -118,8 +118,8 @@ __device__ __forceinline__ void chunk_decays(float raw, int n, float A2, float D
   }
 }
 
-// LDS (bytes): B, x and (for outputs) C, twice; M of every head of the workgroup; the heads' decays of
-// two groups of chunks; the flags of chunks with values that are not finite, twice.
+// LDS (bytes): B, x and (for outputs) C, twice; the heads' decays of two groups of chunks; the flags of
+// three chunks, whether they have values that are not finite.
 template <int N, int HEADS, bool kOutputs>
 struct Lds {
   // chunks whose decays are formed at once, by a wave each (two heads a wave)
@@ -127,9 +127,7 @@ struct Lds {
   static constexpr int kX = kQ * N * 2;
   static constexpr int kC = kX + kQ * kXW * 2;
   static constexpr int kBuf = kC + (kOutputs ? kQ * N * 2 : 0);
-  static constexpr int kM = 2 * kBuf;
-  static constexpr int kMHead = 2 * 1024;  // one operand for each 16-row tile of t
-  static constexpr int kDec = kM + (kOutputs ? HEADS * kMHead : 0);
+  static constexpr int kDec = 2 * kBuf;
   static constexpr int kDecHead = kOutputs ? Dec::kFloats : Dec::kEnds;
   static constexpr int kFlag = kDec + 2 * kGroup * HEADS * kDecHead * 4;
   static constexpr int kBytes = kFlag + 16;
@@ -181,7 +179,6 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   float* const carry = a.carry + ((int64_t)index * a.heads + head) * P * N;
   const int st_at = (p0 + l16) * N + 8 * c4;
 
-  uint8_t* const Ms = lds + L::kM;
   float* const decs = (float*)(lds + L::kDec);
   int* const flags = (int*)(lds + L::kFlag);
 
@@ -235,8 +232,8 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
       rx[i] = *(const u32x4*)(x0 + ((r < end ? r : end) * ldx2 + 16 * ((int)q < x_pieces ? q : x_pieces - 1)));
     }
   };
-  auto store = [&](int par) __attribute__((always_inline)) {
-    uint8_t* const buf = lds + par * L::kBuf;
+  auto store = [&](int step) __attribute__((always_inline)) {
+    uint8_t* const buf = lds + (step & 1) * L::kBuf;
 #pragma unroll
     for (int i = 0; i < kIn; ++i) {
       const int id = i * kThreads + tid, at = tile_at<N>(id / kRowB, id % kRowB);
@@ -253,7 +250,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
         for (int e = 0; e < 4; ++e) zero = dot2_bf16(rx[i][e], 0u, zero);
     }
     if constexpr (kOutputs)
-      if (zero != zero) flags[par] = 1;
+      if (zero != zero) flags[step % 3] = 1;
   };
   // the decays of a group of chunks: each wave one chunk's of two heads
   constexpr int kGroup = L::kGroup;
@@ -283,11 +280,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   };
 
   if constexpr (kOutputs) {
-    // M above the diagonal tile of rows 0..15 is zero for good
-    if (tid < 64)
-#pragma unroll
-      for (int j = 0; j < HEADS; ++j) *(u32x2*)(Ms + j * L::kMHead + tid * 16 + 8) = u32x2{0u, 0u};
-    if (tid < 2) flags[tid] = 0;
+    if (tid < 3) flags[tid] = 0;
     __syncthreads();  // the flags are set after they are cleared
   }
 
@@ -320,11 +313,11 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   store(0);
   if (n_steps > kGroup) load_dt(kGroup);
   if (n_steps > 1) load(row_of(1));
-  for (int step = 0, par = 0; step < n_steps; ++step, par ^= 1) {
+  for (int step = 0; step < n_steps; ++step) {
     __syncthreads();  // the chunk is staged, the buffers of the one before are free
     const int t0 = row_of(step);
     const bool more = step + 1 < n_steps;
-    const uint8_t* const buf = lds + par * L::kBuf;
+    const uint8_t* const buf = lds + (step & 1) * L::kBuf;
     const float* const dec = dec_of(step, hh);
     const float all = dec[Dec::kAll], behind = kOutputs ? 1.f : exp2_(total);
     total += dec[Dec::kAll + 1];
@@ -352,16 +345,21 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
         }
       }
     };
+    // ---- the next chunk to LDS, the one behind it on its way
+    if (more) {
+      store(step + 1);
+      if (step + 2 < n_steps) load(row_of(step + 2));
+    }
     if constexpr (kOutputs) {
-      if (tid == 0) flags[par ^ 1] = 0;
-      // ---- a tile of C B^T: waves 0 and 1 the diagonal ones, 2 and 3 the one below (for every other head)
+      // (the chunk before this one has been read, the one after the next is not stored yet)
+      if (tid == 0) flags[(step + 2) % 3] = 0;
+      const bool bad = __builtin_amdgcn_readfirstlane(flags[step % 3]) != 0;
+      // ---- C B^T, its tiles (0, 0), (0, 1) and (1, 1) of [s, t]; H C_t for the wave's columns; the state's
+      // decay. Each wave forms C B^T for itself: sharing the tiles through LDS took a barrier more
+      // (69.6 against 61 us a piece launch) than it saved
       const uint8_t* const Bs = buf;
       const uint8_t* const Cs = buf + L::kC;
-      const int tt = wave == 0 ? 0 : 1, st = wave == 1 ? 1 : 0;
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = mfma16(row_operand(Bs, st, ks), row_operand(Cs, tt, ks), s);
-      // ---- H C_t for the wave's columns; the state's decay
+      f32x4 s00 = {0.f, 0.f, 0.f, 0.f}, s01 = s00, s11 = s00;
       f32x4 acc[2][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -369,62 +367,38 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
         for (int ct = 0; ct < 2; ++ct) acc[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        bf16x8 hb[2];
+        const bf16x8 c0 = row_operand(Cs, 0, ks), c1 = row_operand(Cs, 1, ks);
+        const bf16x8 b0 = row_operand(Bs, 0, ks), b1 = row_operand(Bs, 1, ks);
+        s00 = mfma16(b0, c0, s00);
+        s01 = mfma16(b0, c1, s01);
+        s11 = mfma16(b1, c1, s11);
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) {
           const f32x4 u = h[ct][2 * ks], v = h[ct][2 * ks + 1];
-          hb[ct] = as_bf16x8(u32x4{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]),
-                                   pack_bf16x2(v[2], v[3])});
+          const bf16x8 hb = as_bf16x8(u32x4{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]),
+                                            pack_bf16x2(v[2], v[3])});
           h[ct][2 * ks] = u * all;
           h[ct][2 * ks + 1] = v * all;
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const bf16x8 co = row_operand(Cs, t, ks);
-#pragma unroll
-          for (int ct = 0; ct < 2; ++ct) acc[t][ct] = mfma16(hb[ct], co, acc[t][ct]);
-        }
-#pragma unroll
-        for (int e = ks * 8 / KS; e < (ks + 1) * 8 / KS; ++e) scaled(e >> 2, e & 3);
-      }
-#pragma unroll
-      for (int k = 0; k < kParts; ++k)  // (formed here, under the products, not where they are used)
-        asm volatile("" : "+v"(part[k][0]), "+v"(part[k][1]));
-      // ---- M of the heads from the tile
-      uint8_t* const m = Ms + tt * 1024 + lane * 16 + 8 * st;
-      if (wave < 2) {
-        const int t = 16 * tt + l16, s0 = 16 * tt + 4 * c4;
-#pragma unroll
-        for (int j = 0; j < HEADS; ++j) {  // (a head that is not there: values that nothing reads)
-          const float* const dj = dec_of(step, j);
-          const f32x4 cum = *(const f32x4*)&dj[Dec::kCum + s0], step = *(const f32x4*)&dj[Dec::kStep + s0];
-          const float ct = dj[Dec::kCum + t], Dj = dj[Dec::kD];
-          f32x4 v;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[i] = s0 + i <= t ? s[i] * (exp2_(ct - cum[i]) * step[i]) : 0.f;
-            v[i] = s0 + i == t ? v[i] + Dj : v[i];
-          }
-          *(u32x2*)(m + j * L::kMHead) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-        }
-      } else {
-#pragma unroll
-        for (int jj = 0; jj < (HEADS + 1) / 2; ++jj) {
-          const int j = 2 * jj + (wave & 1);
-          if (j >= HEADS) break;
-          const float* const dj = dec_of(step, j);
-          const f32x4 g = *(const f32x4*)&dj[Dec::kG + 4 * c4];
-          const f32x4 v = s * g * dj[Dec::kF + 16 + l16];
-          *(u32x2*)(m + j * L::kMHead) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+          acc[0][ct] = mfma16(hb, c0, acc[0][ct]);
+          acc[1][ct] = mfma16(hb, c1, acc[1][ct]);
         }
       }
-      __syncthreads();  // M is whole
-      const bool bad = __builtin_amdgcn_readfirstlane(flags[par]) != 0;
-      if (more) {
-        store(par ^ 1);
-        if (step + 2 < n_steps) load(row_of(step + 2));
-      }
-      const uint8_t* const mh = Ms + hh * L::kMHead + lane * 16;
+      // ---- M: lane (l16, c4) holds rows s = 4 c4 + i of its tiles in column t = l16
+      auto diagonal = [&](const f32x4 s, int tile) __attribute__((always_inline)) {
+        const f32x4 cum = *(const f32x4*)&dec[Dec::kCum + 16 * tile + 4 * c4];
+        const f32x4 step_s = *(const f32x4*)&dec[Dec::kStep + 16 * tile + 4 * c4];
+        const float ct = dec[Dec::kCum + 16 * tile + l16], D_h = dec[Dec::kD];
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = 4 * c4 + i <= l16 ? s[i] * (exp2_(ct - cum[i]) * step_s[i]) : 0.f;
+          v[i] = 4 * c4 + i == l16 ? v[i] + D_h : v[i];
+        }
+        return u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+      };
+      const f32x4 below = s01 * *(const f32x4*)&dec[Dec::kG + 4 * c4] * dec[Dec::kF + 16 + l16];
+      const bf16x8 m[2] = {join(diagonal(s00, 0), u32x2{0u, 0u}),
+                           join(u32x2{pack_bf16x2(below[0], below[1]), pack_bf16x2(below[2], below[3])}, diagonal(s11, 1))};
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const float e = dec[Dec::kE + 16 * t + l16];
@@ -433,11 +407,9 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
       }
       if (!bad) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const bf16x8 mo = as_bf16x8(*(const u32x4*)(mh + t * 1024));
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int ct = 0; ct < 2; ++ct) acc[t][ct] = mfma16(xt[ct], mo, acc[t][ct]);
-        }
+          for (int ct = 0; ct < 2; ++ct) acc[t][ct] = mfma16(xt[ct], m[t], acc[t][ct]);
       } else {
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) {
@@ -457,8 +429,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
           other = __shfl_xor(first, 32, 64);
           first = other < first ? other : first;
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            acc[t][ct] = mfma16(as_bf16x8(v), as_bf16x8(*(const u32x4*)(mh + t * 1024)), acc[t][ct]);
+          for (int t = 0; t < 2; ++t) acc[t][ct] = mfma16(as_bf16x8(v), m[t], acc[t][ct]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int from = __shfl(first, 4 * c4 + i, 64);
@@ -479,14 +450,9 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
               *(u32x2*)(row + (y_at + 32 * ct)) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
             }
         }
-    } else {
-      if (more) {
-        store(par ^ 1);
-        if (step + 2 < n_steps) load(row_of(step + 2));
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) scaled(e >> 2, e & 3);
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) scaled(e >> 2, e & 3);
     // ---- the state, and the next group's decays (they have a place of their own)
 #pragma unroll
     for (int T = 0; T < NT; ++T) {
