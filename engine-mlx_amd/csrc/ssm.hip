@@ -25,6 +25,10 @@ __device__ __forceinline__ float row_sum16(float v) {
   return dpp_add<0x140>(v);
 }
 
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
 template <typename A, int NI, int R, int PHASE>
 __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int row_blocks) {
   typedef typename A::T T;
@@ -76,10 +80,9 @@ __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int r
 
   struct Row {
     Vec<A, 4> b[NI], c[NI];
-    T x[R], dt;
+    T x[R];
   };
   auto fetch = [&](int t, Row& r) __attribute__((always_inline)) {
-    r.dt = dp[(int64_t)t * a.lddt];
 #pragma unroll
     for (int i = 0; i < R; ++i) r.x[i] = row0 + 4 * i < P ? xp[(int64_t)t * a.ldx + 4 * i] : T(0);
 #pragma unroll
@@ -92,15 +95,22 @@ __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int r
       }
     }
   };
-  float sum = 0.f;
+  // the steps of 64 rows, a row a lane
+  T raw = dp[(int64_t)(lane < pc.n ? lane : pc.n - 1) * a.lddt];
+  float steps = 0.f, decays = 0.f, sum = 0.f;
   Row now, next;
   fetch(0, now);
   for (int t = 0; t < pc.n; ++t) {
     if (t + 1 < pc.n) fetch(t + 1, next);
-    const float d = ssm_step(A::to(now.dt) + bias, a);
-    const float da = d * A_h;
-    const float decay = expf(da);
-    sum += da;
+    if ((t & 63) == 0) {
+      steps = ssm_step(A::to(raw) + bias, a);
+      decays = steps * A_h;
+      if (PHASE == kSsmEnds) sum += t + lane < pc.n ? decays : 0.f;
+      decays = expf(decays);
+      const int at = t + 64 + lane;
+      if (t + 64 < pc.n) raw = dp[(int64_t)(at < pc.n ? at : pc.n - 1) * a.lddt];
+    }
+    const float d = lane_value(steps, t & 63), decay = lane_value(decays, t & 63);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const float xv = A::to(now.x[i]);
@@ -127,7 +137,11 @@ __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int r
 #pragma unroll
       for (int k = 0; k < NI; ++k)
         if (row0 + 4 * i < P && on[k]) *(f32x4*)(to + (int64_t)(row0 + 4 * i) * N + 4 * p + 64 * k) = s[i][k];
-  if (PHASE == kSsmEnds && rb == 0 && threadIdx.x == 0) a.carry_decay[(int64_t)index * a.heads + h] = expf(sum);
+  if (PHASE == kSsmEnds && rb == 0 && wave == 0) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+    if (lane == 0) a.carry_decay[(int64_t)index * a.heads + h] = expf(sum);
+  }
 }
 
 // Joins a sequence's pieces in order: each piece's E in the workspace becomes its start state.
@@ -189,15 +203,18 @@ SsmPlan plan_ssm(int batch, int n_rows, int max_rows, int heads, int head_dim, i
   SsmPlan p{};
   p.chunks = dtype == EMA_DTYPE_BF16 && vectors && max_rows >= 32 && ssm_chunk_shape(head_dim, d_state);
   p.pieces = batch;
-  // Cut where the sequences' heads leave most of the chip idle: into pieces that give every CU two
-  // (chunks) or four workgroups; the pieces' ends take about half as long again (chunks) or as long.
-  const int64_t wgs = batch * (p.chunks ? (int64_t)ssm_chunk_workgroups(heads, head_dim, groups)
-                                        : heads * (int64_t)((head_dim + 63) / 64));
-  const int64_t want = (p.chunks ? 2 : 4) * (int64_t)device_cus() / wgs;
-  const int least = p.chunks ? 4 * kSsmChunk : 32, step = p.chunks ? kSsmChunk : 16;
-  if (want < 3 || max_rows < 2 * least) return p;
-  int64_t piece = (max_rows + want - 1) / want;
-  piece = piece < least ? least : (piece + step - 1) / step * step;
+  // Cut where the sequences' heads leave much of the chip idle: into pieces that give every CU two
+  // (chunks) or four workgroups. Chunks, 64 heads of 64, d_state 128: a whole sequence takes 0.065 us
+  // a row of the longest, cut ones 25 us and 0.0105 us a row of all (ends, joining, pieces), so that
+  // the longest has to be 384 rows and 2.6 pieces: 4 x 2048 rows 106 us cut, 133 whole, 5 x 1638
+  // 123 and 106, 512 rows 33 and 37, 256 the same. Token by token (f32): 8 x 300 rows of 24 heads
+  // 164 cut, 173 whole, 2048 rows 150 and 948.
+  const int per_cu = p.chunks ? 2 : 4, step = p.chunks ? kSsmChunk : 16, least = p.chunks ? 4 * kSsmChunk : 32;
+  const int64_t wgs = p.chunks ? (int64_t)ssm_chunk_workgroups(heads, head_dim, groups)
+                               : heads * (int64_t)((head_dim + 63) / 64);
+  const int64_t even = (n_rows * wgs + per_cu * device_cus() - 1) / (per_cu * device_cus());
+  if ((int64_t)max_rows * 5 < even * 13 + (p.chunks ? 1920 : 320)) return p;
+  int64_t piece = even < least ? least : (even + step - 1) / step * step;
   for (; piece < max_rows; piece *= 2) {
     const int64_t pieces = packed_pieces(n_rows, batch, (int)piece);
     const uint64_t bytes = (uint64_t)pieces * heads * ((uint64_t)head_dim * d_state + 4) * 4;
