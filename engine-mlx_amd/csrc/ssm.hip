@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int r
 
 // Joins a sequence's pieces in order: each piece's E in the workspace becomes its start state.
 // A lane per 4 elements of (head, state); the pieces' loads do not depend on the sums.
-__global__ __launch_bounds__(256) void ssm_join_kernel(SsmArgs a) {
+__global__ __launch_bounds__(256) void ssm_join_kernel(SsmArgs a, bool chunks) {
   const int b = blockIdx.y;
   const PackedRows r = packed_sequence(a.starts, b, a.n_rows, a.T);
   if (r.n <= a.piece) return;
@@ -160,7 +160,10 @@ __global__ __launch_bounds__(256) void ssm_join_kernel(SsmArgs a) {
   const float* const decay = a.carry_decay + (int64_t)first * a.heads + h;
   const int slot = packed_slot(a.slots, b, a.n_slots);
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0 && packed_continues(a.offsets, b)) s = ((const f32x4*)a.state)[slot * stride + v];
+  if (slot >= 0 && packed_continues(a.offsets, b)) {
+    const int e = v - h * per_head;
+    s = *(const f32x4*)(a.state + ((int64_t)slot * a.heads + h) * per_head * 4 + (chunks ? ssm_carry_element(e, a.d_state) : 4 * e));
+  }
   for (int i = 0; i < n - 1; ++i) {
     const f32x4 e = c[i * stride];
     c[i * stride] = s;
@@ -242,7 +245,8 @@ int32_t launch_ssm(hipStream_t s, SsmArgs& a, const SsmPlan& plan, void* ws, int
   hipError_t e = phase(kSsmEnds);
   if (e != hipSuccess) return check_hip(e, what);
   const int vecs = a.heads * (a.head_dim * a.d_state / 4);
-  hipLaunchKernelGGL(ssm_join_kernel, dim3((unsigned)((vecs + 255) / 256), (unsigned)a.batch), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(ssm_join_kernel, dim3((unsigned)((vecs + 255) / 256), (unsigned)a.batch), dim3(256), 0, s, a,
+                     plan.chunks);
   if ((e = hipGetLastError()) != hipSuccess) return check_hip(e, what);
   return check_hip(phase(kSsmPieces), what);
 }

@@ -176,7 +176,8 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   const int p0 = (unit % gr.per_head) * kCols;        // its first column of the head
   const int slot = packed_slot(a.slots, pc.b, a.n_slots);
   float* const pool = a.state + ((int64_t)slot * a.heads + head) * P * N;
-  float* const carry = a.carry + ((int64_t)index * a.heads + head) * P * N;
+  // (the workspace holds a wave's state in the order of its accumulators: ssm_carry_element)
+  float* const carry = a.carry + ((int64_t)index * a.heads + head) * P * N + p0 * N + 4 * lane;
   const int st_at = (p0 + l16) * N + 8 * c4;
 
   float* const decs = (float*)(lds + L::kDec);
@@ -185,11 +186,18 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   // ---- state: h[ct][T] holds n = 32 (T / 2) + 8 c4 + 4 (T % 2) + i of column p0 + 16 ct + l16
   f32x4 h[2][NT];
   {
+    // a sequence of one piece starts from the pool; pieces of a longer one never read what its last
+    // piece writes there
     const float* from = nullptr;
-    if (PHASE == kSsmPieces && pc.all > a.piece)
+    int step_ct = 16 * N, step_T = 32, step_u = 4;
+    if (PHASE == kSsmPieces && pc.all > a.piece) {
       from = carry;
-    else if (kOutputs && slot >= 0 && packed_continues(a.offsets, pc.b))
-      from = pool;
+      step_ct = NT * 256;
+      step_T = 512;
+      step_u = 256;
+    } else if (kOutputs && slot >= 0 && packed_continues(a.offsets, pc.b)) {
+      from = pool + st_at;
+    }
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
@@ -198,7 +206,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
       for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
-        for (int T = 0; T < NT; ++T) h[ct][T] = *(const f32x4*)(from + (st_at + 16 * ct * N + 32 * (T >> 1) + 4 * (T & 1)));
+        for (int T = 0; T < NT; ++T) h[ct][T] = *(const f32x4*)(from + (ct * step_ct + (T >> 1) * step_T + (T & 1) * step_u));
   }
 
   // ---- staging: 16-byte pieces of rows, in registers from one chunk to the next
@@ -468,12 +476,18 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
     }
   }
 
-  float* const to = PHASE == kSsmEnds ? carry : (last && slot >= 0 ? pool : nullptr);
-  if (to && !idle)
+  if (PHASE == kSsmEnds) {
+    if (!idle)
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+        for (int T = 0; T < NT; ++T) *(f32x4*)(carry + (ct * NT + T) * 256) = h[ct][T];
+  } else if (last && slot >= 0 && !idle) {
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
-      for (int T = 0; T < NT; ++T) *(f32x4*)(to + (st_at + 16 * ct * N + 32 * (T >> 1) + 4 * (T & 1))) = h[ct][T];
+      for (int T = 0; T < NT; ++T) *(f32x4*)(pool + (st_at + 16 * ct * N + 32 * (T >> 1) + 4 * (T & 1))) = h[ct][T];
+  }
   if (PHASE == kSsmEnds && !idle && p0 == 0 && lane == 0) a.carry_decay[(int64_t)index * a.heads + head] = exp2_(total);
 }
 
