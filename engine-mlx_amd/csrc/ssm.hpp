@@ -48,12 +48,13 @@ __device__ __forceinline__ float ssm_step(float r, const SsmArgs& a) {
 constexpr int kSsmChunk = 32;  // rows of a chunk
 bool ssm_chunk_shape(int head_dim, int d_state);
 int ssm_chunk_workgroups(int heads, int head_dim, int groups);
-// The workspace's order of a head's state: token by token [head_dim][d_state]; chunks: for each 32 columns
-// of head_dim, 16 of them and 16 of d_state after the other, the four neighbours that a lane holds
-// (lane l: column l % 16, d_state 8 (l / 16) + ..). Element 4 v of it lies at this place of the pool's.
+// The workspace's order of a head's state: token by token [head_dim][d_state]; chunks: accumulator tiles
+// of 16 columns (of head_dim) by 16 of d_state, the four values that a lane holds after each other.
+// Values 4 v .. of it are the pool's from this place on.
 EMA_HD int ssm_carry_element(int v, int d_state) {
-  const int lane = v & 63, T = (v >> 6) % (d_state / 16), col = (v >> 6) / (d_state / 16);  // 16-column tile
-  return (16 * col + (lane & 15)) * d_state + 32 * (T >> 1) + 8 * (lane >> 4) + 4 * (T & 1);
+  const int lane = v & 63, T = (v >> 6) % (d_state / 16), col = (v >> 6) / (d_state / 16);
+  const int p = 32 * (col >> 1) + 8 * ((lane & 15) >> 2) + 4 * (col & 1) + (lane & 3);
+  return p * d_state + 32 * (T >> 1) + 8 * (lane >> 4) + 4 * (T & 1);
 }
 hipError_t launch_ssm_chunk(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhase phase);
 

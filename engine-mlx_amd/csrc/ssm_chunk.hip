@@ -14,7 +14,8 @@
 //   H^T [n, p]              A = B^T,           B = x^T scaled
 // A pair of 16x16 accumulator tiles holds, in lane group c, rows 4 c + (0..3) of both tiles. The rows of
 // the state's tiles are numbered so that these are d_state 8 c + (0..7) of a 32-wide step (B^T's columns
-// are read in that order): rows of C are then read whole. M's are rows 4 c + (0..3) and 16 + 4 c +
+// are read in that order): rows of C are then read whole. Columns of x are numbered in the same way
+// over the wave's two tiles, so that a lane holds 8 neighbours of a row of y. M's are rows 4 c + (0..3) and 16 + 4 c +
 // (0..3); x^T and B^T are read from LDS in the same order of rows, by the transposing read. The
 // decays of M are products of factors at most 1 (A <= 0): from s to the end of its 16-row tile (g), and
 // from t's tile's start to t (f); differences of sums only inside the tiles on the diagonal.
@@ -178,18 +179,19 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   float* const pool = a.state + ((int64_t)slot * a.heads + head) * P * N;
   // (the workspace holds a wave's state in the order of its accumulators: ssm_carry_element)
   float* const carry = a.carry + ((int64_t)index * a.heads + head) * P * N + p0 * N + 4 * lane;
-  const int st_at = (p0 + l16) * N + 8 * c4;
+  const int st_at = (p0 + 8 * (l16 >> 2) + (l16 & 3)) * N + 8 * c4;
 
   float* const decs = (float*)(lds + L::kDec);
   int* const flags = (int*)(lds + L::kFlag);
 
-  // ---- state: h[ct][T] holds n = 32 (T / 2) + 8 c4 + 4 (T % 2) + i of column p0 + 16 ct + l16
+  // ---- state: h[ct][T] holds n = 32 (T / 2) + 8 c4 + 4 (T % 2) + i of column l16 of tile ct, which is
+  // p0 + 8 (l16 / 4) + 4 ct + l16 % 4
   f32x4 h[2][NT];
   {
     // a sequence of one piece starts from the pool; pieces of a longer one never read what its last
     // piece writes there
     const float* from = nullptr;
-    int step_ct = 16 * N, step_T = 32, step_u = 4;
+    int step_ct = 4 * N, step_T = 32, step_u = 4;
     if (PHASE == kSsmPieces && pc.all > a.piece) {
       from = carry;
       step_ct = NT * 256;
@@ -299,10 +301,10 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   auto row_operand = [&](const uint8_t* base, int tile, int ks) __attribute__((always_inline)) {
     return as_bf16x8(*(const u32x4*)(base + tile * 16 * (N * 2) + (l16 * (N * 2) + (((4 * ks + c4) ^ x_of_row) << 4))));
   };
-  // the chunk's rows of column 16 tile + l16 of x
-  auto x_operand = [&](const uint8_t* xs, int tile) __attribute__((always_inline)) {
+  // the chunk's rows of column l16 of the wave's column tile ct
+  auto x_operand = [&](const uint8_t* xs, int ct) __attribute__((always_inline)) {
     const uint8_t* const at =
-        xs + (tr_row * (2 * kXW) + 8 * (l16 & 1) + (((2 * tile + ((l16 & 3) >> 1)) ^ swizzle<kXW>(tr_row)) << 4));
+        xs + (tr_row * (2 * kXW) + 8 * ct + (((4 * wave + (l16 & 3)) ^ swizzle<kXW>(tr_row)) << 4));
     return join(read_tr(at), read_tr(at + 16 * (2 * kXW)));
   };
   // the chunk's rows of the columns of state tile T of B
@@ -314,7 +316,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 
   float total = 0.f;  // log2 of the decay over the piece
   uint8_t* const yp = (uint8_t*)((uint16_t*)a.y + (int64_t)pc.row * a.ldy + (int64_t)head * P + p0);
-  const uint32_t ldy2 = (uint32_t)a.ldy * 2, y_at = l16 * ldy2 + 8 * c4;
+  const uint32_t ldy2 = (uint32_t)a.ldy * 2, y_at = l16 * ldy2 + 16 * c4;
   load_dt(0);
   load(row_of(0));
   decays(0);
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
     total += dec[Dec::kAll + 1];
     bf16x8 xt[2];  // x^T of the column tiles
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct) xt[ct] = x_operand(buf + L::kX, 2 * wave + ct);
+    for (int ct = 0; ct < 2; ++ct) xt[ct] = x_operand(buf + L::kX, ct);
     // x scaled, in three bf16 parts: two neighbouring rows of one column a call
     u32x4 part[kParts][2];
     f32x4 wt[2] = {*(const f32x4*)&dec[Dec::kW + 4 * c4], *(const f32x4*)&dec[Dec::kW + 16 + 4 * c4]};
@@ -421,7 +423,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
       } else {
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) {
-          int first = kQ;  // first row that is not finite in column 16 ct + l16
+          int first = kQ;  // first row that is not finite in column l16 of tile ct
           u32x4 v = __builtin_bit_cast(u32x4, xt[ct]);
 #pragma unroll
           for (int j = 7; j >= 0; --j) {
@@ -451,12 +453,10 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           uint8_t* const row = yp + (int64_t)(t0 + 16 * t) * ldy2;
+          const f32x4 u = acc[t][0], v = acc[t][1];
           if (16 * t + l16 < pc.n - t0)
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-              const f32x4 v = acc[t][ct];
-              *(u32x2*)(row + (y_at + 32 * ct)) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-            }
+            *(u32x4*)(row + y_at) = u32x4{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]),
+                                          pack_bf16x2(v[2], v[3])};
         }
     }
 #pragma unroll
@@ -486,7 +486,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
-      for (int T = 0; T < NT; ++T) *(f32x4*)(pool + (st_at + 16 * ct * N + 32 * (T >> 1) + 4 * (T & 1))) = h[ct][T];
+      for (int T = 0; T < NT; ++T) *(f32x4*)(pool + (st_at + 4 * ct * N + 32 * (T >> 1) + 4 * (T & 1))) = h[ct][T];
   }
   if (PHASE == kSsmEnds && !idle && p0 == 0 && lane == 0) a.carry_decay[(int64_t)index * a.heads + head] = exp2_(total);
 }
