@@ -900,12 +900,14 @@ static int32_t check_packed(const char* op, int32_t batch, int32_t n_rows, int32
   if (batch <= 0 || n_rows < 0 || max_rows < 0)
     return set_error(EMA_ERR_SHAPE, "%s: batch=%d n_rows=%d max_rows=%d", op, batch, n_rows, max_rows);
   if (batch > kPackedMaxB) return set_error(EMA_ERR_UNSUPPORTED, "%s: batch %d exceeds %d", op, batch, kPackedMaxB);
-  if (n_rows > (1 << 30)) return set_error(EMA_ERR_UNSUPPORTED, "%s: %d rows exceed 2^30", op, n_rows);
+  if (n_rows > (1 << 30)) return set_error(EMA_ERR_UNSUPPORTED, "%s: %d rows exceed 2^30", op, n_rows);  // (a piece)
   if (uniform && n_rows % batch)
     return set_error(EMA_ERR_SHAPE, "%s: %d rows are not the same number for each of %d sequences (pass starts)", op,
                      n_rows, batch);
   return EMA_OK;
 }
+// Workgroups of 256 lanes that a launch can have (2^32 lanes); kernels of larger ones have fewer.
+constexpr int64_t kMixerMaxGroups = 1 << 24;
 static int32_t check_slots(const char* op, const int32_t* slots, int32_t n_slots, int32_t batch) {
   if (n_slots <= 0) return set_error(EMA_ERR_SHAPE, "%s: %d state slots", op, n_slots);
   if (!slots && n_slots < batch)
@@ -1008,9 +1010,9 @@ extern "C" int32_t ema_ssm_scan(ema_stream_t stream, const void* x, int64_t ldx,
                        ldc < (1 << 23) && ldy < (1 << 23);
   const SsmPlan plan = plan_ssm(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype, vectors,
                                 workspace ? workspace_bytes : 0);
-  if (plan.pieces * n_heads * ((head_dim + 3) / 4) >= INT32_MAX)
-    return set_error(EMA_ERR_UNSUPPORTED, "%s: %lld pieces of %d heads of %d are too many", op, (long long)plan.pieces,
-                     n_heads, head_dim);
+  if (plan.pieces * n_heads * ((head_dim + 15) / 16) >= kMixerMaxGroups)
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %lld sequences or pieces of %d heads of %d are too many", op,
+                     (long long)plan.pieces, n_heads, head_dim);
   SsmArgs p{};
   p.x = x;
   p.dt = dt;
@@ -1070,8 +1072,9 @@ extern "C" int32_t ema_gated_norm(ema_stream_t stream, const void* x, int64_t ld
     return set_error(EMA_ERR_INVALID_ARG, "%s: misaligned buffer", op);
   if ((y == x && ldy != ldx) || (y == gate && ldy != ldg))
     return set_error(EMA_ERR_INVALID_ARG, "%s: y in its input's place needs its row stride", op);
-  if ((int64_t)n_rows * (dim / group) >= INT32_MAX)
-    return set_error(EMA_ERR_UNSUPPORTED, "%s: %d rows of %d groups are too many", op, n_rows, dim / group);
+  // (a workgroup of up to 1024 lanes a norm, or 256 lanes for 4 norms and more)
+  if ((int64_t)n_rows * (dim / group) >= (group > 512 ? kMixerMaxGroups / 4 : 4 * kMixerMaxGroups))
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: %d rows of %d groups of %d are too many", op, n_rows, dim / group, group);
   const GatedNormArgs a{x, gate, w, y, ldx, gate ? ldg : 0, ldy, eps, n_rows, group, dim / group, flags};
   return launch_gated_norm((hipStream_t)stream, a, dtype);
 }
@@ -1087,6 +1090,7 @@ extern "C" int32_t ema_residual_norm(ema_stream_t stream, const void* branch, in
     return set_error(EMA_ERR_INVALID_ARG, "%s: residual dtype %d is neither the activations' nor f32", op, residual_dtype);
   if ((rc = check_norm_rows(op, n_rows, dim, eps))) return rc;
   if (dim > kNormMaxDim) return set_error(EMA_ERR_UNSUPPORTED, "%s: dim %d exceeds %d", op, dim, kNormMaxDim);
+  if (n_rows >= kMixerMaxGroups / 4) return set_error(EMA_ERR_UNSUPPORTED, "%s: %d rows are too many", op, n_rows);
   if (flags & ~EMA_NORM_UNIT_OFFSET) return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
   if (!out != !pre_w) return set_error(EMA_ERR_INVALID_ARG, "%s: out and pre_w go together", op);
   if (n_rows == 0) return EMA_OK;

@@ -534,7 +534,8 @@ EMA_API int32_t ema_gdn_scan_ws(ema_stream_t stream, const void* q, const void* 
  *            have the same slot.
  *   max_rows host bound of a sequence's rows; it chooses between kernels, and true values beyond it
  *            still give the result.
- * At most 4096 sequences a call. A call of no rows does nothing. The reference runs its convolution,
+ * At most 4096 sequences and 2^30 rows a call (norms: 2^22 of more than 512 values, 2^26 of fewer). A
+ * call of no rows does nothing. The reference runs its convolution,
  * norms and gates as separate MLX operators (crates/ops/src/gdn_forward.rs) and has no state space
  * scan. */
 

@@ -326,3 +326,161 @@ def test_residual_sizes(ema, dtype, stream, dim):
 def test_residual_options(ema, kw):
     residual_case(ema, BF, 33, 768, 310, **kw)
     residual_case(ema, BF, 33, 768, 311, stream=F32, **kw)
+
+
+# ------------------------------------------------------------------ together
+class Layer:
+    """A recurrent mixer layer between two norms, as a server runs it: the projections' outputs come in."""
+
+    def __init__(self, ema, seed, dtype=BF, n_slots=5, H=8, P=64, G=2, N=128):
+        self.ema, self.H, self.P, self.G, self.N, self.dtype = ema, H, P, G, N, dtype
+        self.inner, self.conv_dim = H * P, H * P + 2 * G * N
+        self.cw, self.cb = rand(seed, self.conv_dim, 4, dtype=dtype, scale=0.5), rand(seed + 1, self.conv_dim, dtype=dtype, scale=0.1)
+        self.A = -(0.5 + 4 * torch.rand(H, generator=torch.Generator().manual_seed(seed + 2))).cuda()
+        self.D, self.dt_bias = rand(seed + 3, H), rand(seed + 4, H) - 3
+        self.gw = (1 + rand(seed + 5, self.inner, scale=0.1)).to(dtype)
+        self.pre = (1 + rand(seed + 6, self.inner, scale=0.1)).to(dtype)
+        self.post = (1 + rand(seed + 7, self.inner, scale=0.1)).to(dtype)
+        # what a fresh slot holds does not matter
+        self.conv_state = torch.full((n_slots, 3, self.conv_dim), math.nan, dtype=dtype, device="cuda")
+        self.ssm_state = torch.full((n_slots, H, P, N), math.nan, device="cuda")
+
+    def __call__(self, proj, residual, starts=None, offsets=None, slots=None, max_rows=None, workspace=None, stream=None):
+        """proj: [z | x B C | dt] rows of the in projection. Returns the normed rows for the next block."""
+        e, H, P, G, N, I = self.ema, self.H, self.P, self.G, self.N, self.inner
+        seq = dict(starts=starts, offsets=offsets, slots=slots, max_rows=max_rows, stream=stream)
+        xbc = e.causal_conv(proj[:, I:I + self.conv_dim], self.cw, bias=self.cb, state=self.conv_state, **seq)
+        y = e.ssm_scan(xbc[:, :I].unflatten(1, (H, P)), proj[:, I + self.conv_dim:I + self.conv_dim + H],
+                       xbc[:, I:I + G * N].unflatten(1, (G, N)), xbc[:, I + G * N:].unflatten(1, (G, N)), self.A,
+                       self.ssm_state, D=self.D, dt_bias=self.dt_bias, workspace=workspace, **seq).flatten(1)
+        e.gated_norm(y, proj[:, :I], self.gw, 1e-5, group=I // G, gate_first=True, out=y, stream=stream)
+        return e.residual_norm(y, residual, self.pre, 1e-5, post_weight=self.post, scale=0.5, out=y, stream=stream)
+
+    def exact(self, proj, residual):
+        """The same for one sequence from its start, in float64."""
+        H, P, G, N, I, n = self.H, self.P, self.G, self.N, self.inner, proj.shape[0]
+        p = ref.f64(proj)
+        xbc, _, _ = ref.conv(p[:, I:I + self.conv_dim], self.cw, self.cb, None, 1)
+        y, _, _, _ = ref.scan(xbc[:, :I].view(n, H, P), p[:, I + self.conv_dim:I + self.conv_dim + H],
+                              xbc[:, I:I + G * N].view(n, G, N), xbc[:, I + G * N:].view(n, G, N), self.A,
+                              torch.zeros(1, H, P, N), 1, self.D, self.dt_bias)
+        y = ref.gated(y.flatten(1), p[:, :I], self.gw, 1e-5, I // G, first=True)
+        h, out, _ = ref.residual(y, residual, self.pre, 1e-5, self.post, None, 0.5)
+        return out, h
+
+    def inputs(self, seed, n):
+        width = self.inner + self.conv_dim + self.H
+        return rand(seed, n, width + (-width) % 8, dtype=self.dtype), rand(seed + 1, n, self.inner)
+
+
+# An intermediate tensor is rounded once where the definition in 64 bits has none: conv, scan, gated norm and out,
+# four half steps in a row, each of which a norm or the scan's sums hand on at about its own size.
+def close(got, want, dtype, what):
+    g = got.detach().cpu().double()
+    rel = float((g - want).norm() / want.norm())
+    print(f"  {what}: relative error {rel:.3e}", flush=True)
+    assert rel <= 4 * HALF[dtype], what
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_prompt_then_tokens(ema, dtype):
+    """Three users: prompts taken in together, in chunks, then tokens one by one, against each whole sequence."""
+    layer = Layer(ema, 500, dtype)
+    lens, new = [200, 33, 1], 6
+    data = [layer.inputs(510 + 10 * b, n + new) for b, n in enumerate(lens)]
+    outs = [[] for _ in lens]
+    at = [0, 0, 0]
+    slots = ints([3, 0, 4])
+    for step in [[150, 33, 1], [50, 0, 0]] + [[1, 1, 1]] * new:
+        rows = [(b, at[b], n) for b, n in enumerate(step)]
+        proj = torch.cat([data[b][0][a:a + n] for b, a, n in rows])
+        res = torch.cat([data[b][1][a:a + n] for b, a, n in rows])
+        starts = ints([sum(step[:i]) for i in range(len(step) + 1)])
+        out = layer(proj, res, starts=starts, offsets=ints(at), slots=slots, max_rows=max(step))
+        o = 0
+        for b, _, n in rows:
+            outs[b].append(out[o:o + n])
+            at[b] += n
+            o += n
+    for b in range(len(lens)):
+        want, _ = layer.exact(*data[b])
+        close(torch.cat(outs[b]), want, dtype, f"user {b}, {lens[b]} + {new} rows, {dtype}")
+
+
+@pytest.mark.parametrize("lens", [[1, 1, 1], [300, 40, 2]])
+def test_layer_captured(ema, lens):
+    """A layer's step in a HIP graph, replayed with eager work of the same buffers between: every replay is
+    what the eager calls give."""
+    layer, n = Layer(ema, 600), sum(lens)
+    starts, slots = ints([sum(lens[:i]) for i in range(len(lens) + 1)]), ints([2, 0, 4])
+    offsets = ints([0, 0, 0])
+    proj, res0 = layer.inputs(610, n)
+    res = res0.clone()
+    ws = ema.ssm_workspace(3, n, max(lens), layer.H, layer.P, layer.N, layer.G)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(proj, res, starts, offsets, slots, max(lens), ws)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(proj, res, starts, offsets, slots, max(lens), ws)
+    eager = Layer(ema, 600)
+    for k in range(4):
+        proj.copy_(layer.inputs(620 + 10 * k, n)[0])
+        res.copy_(res0)
+        offsets.fill_(0 if k == 0 else 100 * k)
+        graph.replay()
+        torch.cuda.synchronize()
+        want_res = res0.clone()
+        want = eager(proj, want_res, starts, offsets, slots, max(lens), ws)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(res, want_res), k
+        for a, b in ((layer.conv_state, eager.conv_state), (layer.ssm_state, eager.ssm_state)):
+            assert torch.equal(a[slots.long()], b[slots.long()]), k
+
+
+def test_layers_on_two_streams(ema):
+    """Two users' layers on streams of their own, a workspace each, at once: what one after the other gives."""
+    lens, layers = [900], [Layer(ema, 700), Layer(ema, 710)]
+    data = [l.inputs(720 + 10 * i, lens[0]) for i, l in enumerate(layers)]
+    want = []
+    for l, (p, r) in zip(layers, data):
+        want.append(l(p, r.clone(), offsets=ints([0]), slots=ints([1]), max_rows=900))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in layers]
+    spaces = [ema.ssm_workspace(1, 900, 900, 8, 64, 128, 2) for _ in layers]
+    zero, one = ints([0]), ints([1])
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        res = [r.clone() for _, r in data]
+        torch.cuda.synchronize()
+        for i, l in enumerate(layers):
+            got.append(l(data[i][0], res[i], offsets=zero, slots=one, max_rows=900, workspace=spaces[i], stream=streams[i]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_gdn_layer(ema):
+    """The pieces around the Gated DeltaNet scan: convolution of q|k|v, scan, norm of each value head, gate."""
+    Hk, Hv, Dk, Dv, T = 2, 4, 128, 128, 70
+    C = 2 * Hk * Dk + Hv * Dv
+    qkv, w = rand(800, T, C, dtype=BF), rand(801, C, 4, dtype=BF, scale=0.5)
+    z, gw = rand(802, T, Hv * Dv, dtype=BF), (1 + rand(803, Dv, scale=0.1)).to(BF)
+    conv = ema.causal_conv(qkv, w, batch=1)
+    q, k, v = conv.split([Hk * Dk, Hk * Dk, Hv * Dv], 1)
+    # queries and keys of each head to length 1: the gated norm without gate or weight, scaled
+    q = (ema.gated_norm(q, None, None, 1e-6, group=Dk).float() / Dk).to(BF)
+    k = (ema.gated_norm(k, None, None, 1e-6, group=Dk).float() / math.sqrt(Dk)).to(BF)
+    g = torch.sigmoid(rand(804, 1, T, Hv) + 3)
+    beta = torch.sigmoid(rand(805, 1, T, Hv))
+    state = torch.zeros(1, Hv, Dv, Dk, device="cuda")
+    y = ema.gdn_scan(q.view(1, T, Hk, Dk), k.view(1, T, Hk, Dk), v.reshape(1, T, Hv, Dv), g, beta, state)
+    out = ema.gated_norm(y.view(T, Hv * Dv), z, gw, 1e-6, group=Dv)
+    torch.cuda.synchronize()
+    # the definitions on the kernels' own intermediate tensors: each call within its bound
+    want, _, mag = ref.conv(qkv, w, None, None, 1)
+    ref.check(conv, want, HALF[BF] * want.abs() + 5.5 * U * mag + 2.0 ** -21 * want.abs() + TINY[BF], "q|k|v")
+    want = ref.gated(y.view(T, Hv * Dv), z, gw, 1e-6, Dv)
+    ref.check(out, want, (HALF[BF] + 136 * U + 2.0 ** -20) * want.abs() + TINY[BF], "gated heads")

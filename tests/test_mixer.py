@@ -63,20 +63,22 @@ REFUSED = [
                              dict(batch=-1), dict(n_slots=-1)]),
     ("ema_ssm_scan", UNSUPPORTED, [dict(d_state=18, ldb=64, ldc=64), dict(d_state=260, ldb=1024, ldc=1024),
                                    dict(head_dim=4097, ldx=1 << 20, ldy=1 << 20), dict(batch=4097),
-                                   dict(heads=65536, ldx=1 << 30, ldy=1 << 30, lddt=1 << 20)]),
+                                   dict(heads=65536, ldx=1 << 30, ldy=1 << 30, lddt=1 << 20),
+                                   dict(batch=4096, slots=0, n_slots=4096, heads=512, groups=1, head_dim=128, ldx=1 << 16,
+                                        ldy=1 << 16, lddt=512)]),
     ("ema_ssm_scan", CAPACITY, [dict(slots=0, n_slots=1)]),
     ("ema_gated_norm", INVALID, [dict(x=0), dict(y=0), dict(dtype=5), dict(flags=16), dict(eps=-1.0), dict(eps=NAN),
                                  dict(gate=P + 1), dict(y=P, ldy=72), dict(gate=3 * P, y=3 * P, ldy=72)]),
     ("ema_gated_norm", SHAPE, [dict(n_rows=-1), dict(dim=0), dict(group=0), dict(group=24), dict(ldx=63), dict(ldg=63),
                                dict(ldy=63)]),
     ("ema_gated_norm", UNSUPPORTED, [dict(dim=16392, group=16392, ldx=20000, ldg=20000, ldy=20000),
-                                     dict(n_rows=1 << 30)]),
+                                     dict(n_rows=1 << 30), dict(n_rows=1 << 22, dim=1024, group=1024, ldx=1024, ldg=1024, ldy=1024)]),
     ("ema_residual_norm", INVALID, [dict(branch=0), dict(residual=0), dict(out=0), dict(pre_w=0), dict(dtype=0),
                                     dict(rdtype=3), dict(dtype=4, rdtype=1), dict(flags=1), dict(eps=NAN),
                                     dict(residual=P), dict(out=2 * P), dict(out=P, ldo=72, gate=0), dict(gate=2 * P),
                                     dict(gate=3 * P), dict(residual=2 * P + 2), dict(branch=P + 1)]),
     ("ema_residual_norm", SHAPE, [dict(n_rows=-1), dict(dim=0), dict(ldx=63), dict(ldr=63), dict(ldo=63), dict(ldg=63)]),
-    ("ema_residual_norm", UNSUPPORTED, [dict(dim=16385, ldx=20000, ldg=20000, ldr=20000, ldo=20000)]),
+    ("ema_residual_norm", UNSUPPORTED, [dict(dim=16385, ldx=20000, ldg=20000, ldr=20000, ldo=20000), dict(n_rows=1 << 22)]),
 ]
 
 
