@@ -809,14 +809,8 @@ def _empty(stream, shape, dtype, device):
         return _torch.empty(shape, dtype=dtype, device=device)
 
 
-def _mixer_call(op: str, dev: int, call, stream, *args) -> None:
-    """The library's call on `dev`'s current stream, or the given one, with `dev` current."""
-    if dev < 0:
-        raise EmaError(EMA_ERR_INVALID_ARG, op, "the tensors are not on a GPU")
-    raw = _torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
-    rc = call(raw, *args) if _torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, raw, *args)
-    if rc:
-        _check(rc, op)
+def _not_on_gpu(op: str):
+    raise EmaError(EMA_ERR_INVALID_ARG, op, "the tensors are not on a GPU")
 
 
 def causal_conv(x, weight, bias=None, state=None, starts=None, offsets=None, slots=None, batch=None, max_rows=None,
@@ -827,7 +821,8 @@ def causal_conv(x, weight, bias=None, state=None, starts=None, offsets=None, slo
     starts int32 [B+1] (None: n / B rows each), offsets int32 [B] (position of the first row: at 0 a sequence
     starts from zeros), slots int32 [B] (None: slot b). Returns out [n, C]."""
     op = "ema_causal_conv"
-    i32 = (_torch or _load_torch()).int32
+    torch = _torch or _load_torch()
+    i32 = torch.int32
     try:
         dtype, dev = x.dtype, x.get_device()
         (n, C), (ldx, sx) = x.shape, x.stride()
@@ -866,12 +861,18 @@ def causal_conv(x, weight, bias=None, state=None, starts=None, offsets=None, slo
         if x.dim() != 2 or weight.dim() != 2 or (out is not None and out.dim() != 2):
             raise EmaError(EMA_ERR_SHAPE, op, f"x must be [n, C] and weight [C, W], not {tuple(x.shape)}, {tuple(weight.shape)}")
         raise
-    _mixer_call(op, dev, _lib.ema_causal_conv, stream, x.data_ptr(), ldx if n > 1 else C, weight.data_ptr(),
-                None if bias is None else bias.data_ptr(), None if starts is None else starts.data_ptr(),
-                None if offsets is None else offsets.data_ptr(), None if slots is None else slots.data_ptr(), batch, n,
-                n if max_rows is None else max_rows, C, W, EMA_CONV_SILU if silu else 0,
-                None if state is None else state.data_ptr(), n_slots, out.data_ptr(), ldy if n > 1 else C,
-                _act_codes[dtype])
+    if dev < 0:
+        _not_on_gpu(op)
+    args = (torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream, x.data_ptr(), ldx if n > 1 else C, weight.data_ptr(),
+            None if bias is None else bias.data_ptr(), None if starts is None else starts.data_ptr(),
+            None if offsets is None else offsets.data_ptr(), None if slots is None else slots.data_ptr(), batch, n,
+            n if max_rows is None else max_rows, C, W, EMA_CONV_SILU if silu else 0,
+            None if state is None else state.data_ptr(), n_slots, out.data_ptr(), ldy if n > 1 else C,
+            _act_codes[dtype])
+    call = _lib.ema_causal_conv
+    rc = call(*args) if torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, *args)
+    if rc:
+        _check(rc, op)
     return out
 
 
@@ -959,13 +960,19 @@ def ssm_scan(x, dt, B, C, A, state, D=None, dt_bias=None, starts=None, offsets=N
         size = ssm_workspace_size(batch, n, max_rows, H, P, N, G, dtype)
         workspace = _empty(stream, (size,), torch.uint8, x.device)
     size = 0 if workspace is None else workspace.numel()
-    _mixer_call(op, dev, _lib.ema_ssm_scan, stream, x.data_ptr(), ldx if n > 1 else H * P, dt.data_ptr(),
-                lddt if n > 1 else H, B.data_ptr(), ldb if n > 1 else G * N, C.data_ptr(), ldc if n > 1 else G * N,
-                A.data_ptr(), None if D is None else D.data_ptr(), None if dt_bias is None else dt_bias.data_ptr(),
-                dt_limit[0], dt_limit[1], None if starts is None else starts.data_ptr(),
-                None if offsets is None else offsets.data_ptr(), None if slots is None else slots.data_ptr(), batch, n,
-                max_rows, H, P, G, N, EMA_SSM_SOFTPLUS if softplus else 0, state.data_ptr(), n_slots, out.data_ptr(),
-                ldy if n > 1 else H * P, _act_codes[dtype], workspace.data_ptr() if size else None, size)
+    if dev < 0:
+        _not_on_gpu(op)
+    args = (torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream, x.data_ptr(), ldx if n > 1 else H * P, dt.data_ptr(),
+            lddt if n > 1 else H, B.data_ptr(), ldb if n > 1 else G * N, C.data_ptr(), ldc if n > 1 else G * N,
+            A.data_ptr(), None if D is None else D.data_ptr(), None if dt_bias is None else dt_bias.data_ptr(),
+            dt_limit[0], dt_limit[1], None if starts is None else starts.data_ptr(),
+            None if offsets is None else offsets.data_ptr(), None if slots is None else slots.data_ptr(), batch, n,
+            max_rows, H, P, G, N, EMA_SSM_SOFTPLUS if softplus else 0, state.data_ptr(), n_slots, out.data_ptr(),
+            ldy if n > 1 else H * P, _act_codes[dtype], workspace.data_ptr() if size else None, size)
+    call = _lib.ema_ssm_scan
+    rc = call(*args) if torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, *args)
+    if rc:
+        _check(rc, op)
     return out
 
 
@@ -976,7 +983,7 @@ def gated_norm(x, gate, weight, eps, group=None, gate_first=False, sigmoid=False
     weight [dim], [group] (one for all groups) or None; unit_offset: 1 + w multiplies. Rows of x, gate and out
     may be pieces of wider ones; out may be x or gate. Returns out [n, dim]."""
     op = "ema_gated_norm"
-    _torch or _load_torch()
+    torch = _torch or _load_torch()
     try:
         dtype, dev = x.dtype, x.get_device()
         (n, dim), (ldx, sx) = x.shape, x.stride()
@@ -1009,10 +1016,16 @@ def gated_norm(x, gate, weight, eps, group=None, gate_first=False, sigmoid=False
             if t is not None and t.dim() != 2:
                 raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be [n, dim], not {tuple(t.shape)}")
         raise
-    _mixer_call(op, dev, _lib.ema_gated_norm, stream, x.data_ptr(), ldx if n > 1 else dim,
-                None if gate is None else gate.data_ptr(), ldg if n > 1 else dim,
-                None if weight is None else weight.data_ptr(), eps, n, dim, group, flags, out.data_ptr(),
-                ldy if n > 1 else dim, _act_codes[dtype])
+    if dev < 0:
+        _not_on_gpu(op)
+    args = (torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream, x.data_ptr(), ldx if n > 1 else dim,
+            None if gate is None else gate.data_ptr(), ldg if n > 1 else dim,
+            None if weight is None else weight.data_ptr(), eps, n, dim, group, flags, out.data_ptr(),
+            ldy if n > 1 else dim, _act_codes[dtype])
+    call = _lib.ema_gated_norm
+    rc = call(*args) if torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, *args)
+    if rc:
+        _check(rc, op)
     return out
 
 
@@ -1024,7 +1037,8 @@ def residual_norm(branch, residual, pre_weight, eps, post_weight=None, gate=None
     [n, dim] in the same type or f32; gate [n, dim], [dim] (one for all rows) or None; pre_weight None: the
     residual stream alone (returns None). Rows may be pieces of wider ones; out may be branch."""
     op = "ema_residual_norm"
-    f32 = (_torch or _load_torch()).float32
+    torch = _torch or _load_torch()
+    f32 = torch.float32
     try:
         dtype, dev, rtype = branch.dtype, branch.get_device(), residual.dtype
         (n, dim), (ldx, sx), (ldr, sr) = branch.shape, branch.stride(), residual.stride()
@@ -1063,10 +1077,16 @@ def residual_norm(branch, residual, pre_weight, eps, post_weight=None, gate=None
     if n <= 1:
         ldx = ldr = ldo = dim
         ldg = 0
-    _mixer_call(op, dev, _lib.ema_residual_norm, stream, branch.data_ptr(), ldx,
-                None if post_weight is None else post_weight.data_ptr(), None if gate is None else gate.data_ptr(), ldg,
-                scale, residual.data_ptr(), ldr, EMA_DTYPE_F32 if rtype is f32 else _act_codes[dtype],
-                None if pre_weight is None else pre_weight.data_ptr(), eps, n, dim,
-                EMA_NORM_UNIT_OFFSET if unit_offset else 0, None if out is None else out.data_ptr(), ldo,
-                _act_codes[dtype])
+    if dev < 0:
+        _not_on_gpu(op)
+    args = (torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream, branch.data_ptr(), ldx,
+            None if post_weight is None else post_weight.data_ptr(), None if gate is None else gate.data_ptr(), ldg,
+            scale, residual.data_ptr(), ldr, EMA_DTYPE_F32 if rtype is f32 else _act_codes[dtype],
+            None if pre_weight is None else pre_weight.data_ptr(), eps, n, dim,
+            EMA_NORM_UNIT_OFFSET if unit_offset else 0, None if out is None else out.data_ptr(), ldo,
+            _act_codes[dtype])
+    call = _lib.ema_residual_norm
+    rc = call(*args) if torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, *args)
+    if rc:
+        _check(rc, op)
     return out
