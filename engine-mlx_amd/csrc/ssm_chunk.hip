@@ -32,7 +32,16 @@
 //
 // Chunks of 32 rows and not of 64: per row they cost a third more vector instructions for the state
 // (its decay and its rounding come twice as often), but 64 rows need more registers than two
-// workgroups a CU leave, and spilled the loads under way.
+// workgroups a CU leave, and spilled the loads under way (131 us against 74 at the time).
+//
+// Bound by issue: a product and a vector instruction of one SIMD do not overlap, not even of two waves
+// (48 products 388 ns, 144 fused multiply-adds 188 ns, side by side 568), so that a chunk is the sum of
+// both, here 80 products and about 330 vector instructions a wave: 1.1 us, 2.2 for the two waves of a
+// SIMD, of the 3.4 us that a chunk takes; the rest is waiting at two waves a SIMD. 8192 rows of 64
+// heads of 64, d_state 128, 8 groups: ends 30, joining 13, pieces 64 us, together 103 us, 1.7 TB/s of
+// what has to move, 0.2 PFLOP/s of the recurrence's operations. No gain: products interleaved with vector
+// instructions by scheduling groups, the state's decay kept as a factor (66), y stored a chunk later
+// (67), one column tile a wave in workgroups of eight waves (104, spilled).
 #include <type_traits>
 
 #include "ssm.hpp"
@@ -366,7 +375,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
       const bool bad = __builtin_amdgcn_readfirstlane(flags[step % 3]) != 0;
       // ---- C B^T, its tiles (0, 0), (0, 1) and (1, 1) of [s, t]; H C_t for the wave's columns; the state's
       // decay. Each wave forms C B^T for itself: sharing the tiles through LDS took a barrier more
-      // (69.6 against 61 us a piece launch) than it saved
+      // (69.6 against 64.6 us of pieces) than it saved
       const uint8_t* const Bs = buf;
       const uint8_t* const Cs = buf + L::kC;
       f32x4 s00 = {0.f, 0.f, 0.f, 0.f}, s01 = s00, s11 = s00;
