@@ -484,3 +484,107 @@ def test_gdn_layer(ema):
     ref.check(conv, want, HALF[BF] * want.abs() + 5.5 * U * mag + 2.0 ** -21 * want.abs() + TINY[BF], "q|k|v")
     want = ref.gated(y.view(T, Hv * Dv), z, gw, 1e-6, Dv)
     ref.check(out, want, (HALF[BF] + 136 * U + 2.0 ** -20) * want.abs() + TINY[BF], "gated heads")
+
+
+# ------------------------------------------------------------------ what the header allows beyond ordinary calls
+def far(t, ld):
+    """The same values in rows ld elements apart."""
+    n = t.shape[0]
+    buf = torch.empty((n - 1) * ld + t[0].numel(), dtype=t.dtype, device="cuda")
+    view = buf.as_strided((n, *t.shape[1:]), (ld, *t.stride()[1:]))
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rows_beyond_32_bit_offsets(ema, dtype):
+    """Row strides of 4 million elements: the last rows lie past 2^31 elements and 2^32 bytes."""
+    n, ld = 600, 4_000_000
+    C = 64
+    x, w = rand(900, n, C, dtype=dtype), rand(901, C, 4, dtype=dtype)
+    near, out = ema.causal_conv(x, w, batch=1), far(torch.zeros_like(x), ld)
+    ema.causal_conv(far(x, ld), w, batch=1, out=out)
+    assert torch.equal(out, near)
+    z, gw = rand(902, n, C, dtype=dtype), rand(903, C, dtype=dtype)
+    for group in (16, 64):
+        ema.gated_norm(far(x, ld), far(z, ld), gw, 1e-6, group=group, out=out)
+        assert torch.equal(out, ema.gated_norm(x, z, gw, 1e-6, group=group))
+    res, far_res = rand(904, n, C), far(rand(904, n, C), ld)
+    near = ema.residual_norm(x, res, gw, 1e-6, gate=z)
+    ema.residual_norm(far(x, ld), far_res, gw, 1e-6, gate=far(z, ld), out=out)
+    assert torch.equal(out, near) and torch.equal(far_res, res)
+    del out, far_res
+    H, P, N, G = 2, 64, 64, 1
+    x, b, c = rand(905, n, H, P, dtype=dtype), rand(906, n, G, N, dtype=dtype), rand(907, n, G, N, dtype=dtype)
+    dt, A = rand(908, n, H, dtype=dtype), -torch.rand(H, device="cuda") - 0.1
+    s1, s2 = torch.zeros(1, H, P, N, device="cuda"), torch.zeros(1, H, P, N, device="cuda")
+    near, out = ema.ssm_scan(x, dt, b, c, A, s1), far(torch.zeros_like(x), ld)
+    ema.ssm_scan(far(x, ld), far(dt, ld), far(b, ld), far(c, ld), A, s2, out=out)
+    assert torch.equal(out, near) and torch.equal(s1, s2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_at_any_element(ema, dtype):
+    """Rows that begin at odd elements (b and c of the scan at a multiple of four)."""
+    x, w, z = rand(910, 70, 64, dtype=dtype), rand(911, 64, 4, dtype=dtype), rand(912, 70, 64, dtype=dtype)
+    out = wide(torch.zeros_like(x), 3, 2)
+    ema.causal_conv(wide(x, 1, 2), w, batch=1, out=out)
+    assert torch.equal(out, ema.causal_conv(x, w, batch=1))
+    for group in (16, 64):
+        ema.gated_norm(wide(x, 1, 2), wide(z, 5, 1), None, 1e-6, group=group, out=out)
+        near = ema.gated_norm(x, z, None, 1e-6, group=group)
+        # (the sums of squares in another order)
+        ref.check(out, near.double().cpu(), (2 * HALF[dtype] + 64 * U) * near.double().cpu().abs() + TINY[dtype], "gated")
+    H, P, N, G = 2, 32, 64, 1
+    x, b, c = rand(913, 70, H, P, dtype=dtype), rand(914, 70, G, N, dtype=dtype), rand(915, 70, G, N, dtype=dtype)
+    dt, A = rand(916, 70, H, dtype=dtype), -torch.rand(H, device="cuda") - 0.1
+    state, out = torch.zeros(1, H, P, N, device="cuda"), wide(torch.zeros_like(x), 3, 2)
+    ema.ssm_scan(wide(x, 1, 2), wide(dt, 1, 2), wide(b, 4, 8), wide(c, 4, 8), A, state, out=out)
+    want, pool, mag, pool_mag = ref.scan(x, dt, b, c, A, torch.zeros(1, H, P, N), 1)
+    ref.check(out, want, HALF[dtype] * want.abs() + (2 * 70 + N + 32) * U * mag + TINY[dtype], "scan")
+    ref.check(state, pool, (2 * 70 + 32) * U * pool_mag + 1e-37, "  state")
+
+
+@pytest.mark.parametrize("starts", [[0, 50, 20, 80], [-7, 30, 30, 1000], [90, 10, 5, 0], [5, 5, 60, 70]])
+def test_row_starts_that_are_no_row_starts(ema, starts):
+    """They are taken as given only inside the rows: nothing outside the outputs and the slots is written."""
+    n, H, P, N, C = 100, 2, 32, 64, 64
+    pad = 4096
+
+    def guarded(*shape, dtype):
+        size = math.prod(shape)
+        buf = torch.full((size + 2 * pad,), 3.0, dtype=dtype, device="cuda")
+        return buf, buf[pad:pad + size].view(shape)
+
+    s = ints(starts)
+    ybuf, y = guarded(n, C, dtype=BF)
+    pbuf, pool = guarded(3, 3, C, dtype=BF)
+    ema.causal_conv(rand(920, n, C, dtype=BF), rand(921, C, 4, dtype=BF), state=pool, starts=s, out=y)
+    obuf, out = guarded(n, H, P, dtype=BF)
+    sbuf, state = guarded(3, H, P, N, dtype=F32)
+    for max_rows in (1, n):
+        ema.ssm_scan(rand(922, n, H, P, dtype=BF), rand(923, n, H, dtype=BF), rand(924, n, 1, N, dtype=BF),
+                     rand(925, n, 1, N, dtype=BF), -torch.ones(H, device="cuda"), state, starts=s, max_rows=max_rows, out=out)
+    torch.cuda.synchronize()
+    for buf in (ybuf, pbuf, obuf, sbuf):
+        assert bool((buf[:pad] == 3.0).all()) and bool((buf[-pad:] == 3.0).all())
+
+
+def test_workspace_holds_what_it_says(ema):
+    """The scan writes no byte behind the workspace it is told it has, whatever its size."""
+    lens, H, P, N = [500, 90], 2, 64, 128
+    n, pad = sum(lens), 4096
+    need = ema.ssm_workspace_size(2, n, 500, H, P, N, 1)
+    a = dict(x=rand(930, n, H, P, dtype=BF), dt=rand(931, n, H, dtype=BF), B=rand(932, n, 1, N, dtype=BF),
+             C=rand(933, n, 1, N, dtype=BF), A=-torch.ones(H, device="cuda"))
+    outs = []
+    for size in (need, need - 16, need // 2, 0):
+        buf = torch.full((size + pad,), 7, dtype=torch.uint8, device="cuda")
+        state = torch.zeros(2, H, P, N, device="cuda")
+        y = ema.ssm_scan(**a, state=state, starts=ints([0, 500, 590]), max_rows=500, workspace=buf[:size])
+        torch.cuda.synchronize()
+        assert bool((buf[size:] == 7).all()), size
+        outs.append((y.double(), state.double()))
+    for y, state in outs[1:]:
+        assert float((y - outs[0][0]).norm() / outs[0][0].norm()) < 2 * HALF[BF]
+        assert float((state - outs[0][1]).norm() / outs[0][1].norm()) < 1e-5
