@@ -951,6 +951,9 @@ static int32_t check_ssm_shape(const char* op, int32_t n_heads, int32_t head_dim
     return set_error(EMA_ERR_UNSUPPORTED, "%s: d_state %d is not a multiple of 4 up to 256", op, d_state);
   if (n_heads > 65535 || head_dim > 4096)
     return set_error(EMA_ERR_UNSUPPORTED, "%s: %d heads of %d (at most 65535 of 4096)", op, n_heads, head_dim);
+  if ((int64_t)n_heads * head_dim * d_state > (1 << 30))
+    return set_error(EMA_ERR_UNSUPPORTED, "%s: a state of %d heads of %d x %d exceeds 2^30 values", op, n_heads, head_dim,
+                     d_state);
   return EMA_OK;
 }
 
@@ -986,7 +989,8 @@ extern "C" int32_t ema_ssm_scan(ema_stream_t stream, const void* x, int64_t ldx,
   if ((rc = check_ssm_shape(op, n_heads, head_dim, d_state, n_groups))) return rc;
   if (flags & ~EMA_SSM_SOFTPLUS) return set_error(EMA_ERR_INVALID_ARG, "%s: unknown flags 0x%x", op, flags);
   if ((rc = check_slots(op, slots, n_slots, batch))) return rc;
-  if (!(dt_min <= dt_max)) return set_error(EMA_ERR_INVALID_ARG, "%s: dt_min must be at most dt_max", op);
+  if (!(dt_min >= 0.f && dt_min <= dt_max))
+    return set_error(EMA_ERR_INVALID_ARG, "%s: dt_min must be at least 0 and at most dt_max", op);
   if (n_rows == 0) return EMA_OK;
   if (!x || !dt || !b || !c || !a || !state || !y)
     return set_error(EMA_ERR_INVALID_ARG, "%s: null x/dt/b/c/a/state/y", op);

@@ -100,8 +100,9 @@ template <bool kOutputs>
 __device__ __forceinline__ void chunk_decays(float raw, int n, float A2, float D, const SsmArgs& a, float* dec) {
   const int lane = threadIdx.x & 63, row = lane & 31;
   const float d = row < n ? ssm_step(raw, a) : 0.f;
-  // log2 of the row's decay; below 2^-150 it is 0 either way, and sums stay finite
-  const float l = fmaxf(d * A2, -150.f);
+  // log2 of the row's decay; below 2^-150 it is 0 either way, and sums stay finite (NaN stays NaN)
+  float l = d * A2;
+  l = row >= n ? 0.f : (l < -150.f ? -150.f : l);
   float down = l;  // sum over the 16-row tile from the row on
   down += dpp_shift<0x101>(down);
   down += dpp_shift<0x102>(down);

@@ -578,12 +578,12 @@ EMA_API int32_t ema_ssm_workspace_size(int32_t batch, int32_t n_rows, int32_t ma
  *   b, c   [n_rows, ldb], [n_rows, ldc]: n_groups * d_state values a row, aligned to 4 of them
  *          (bf16, f16: 8 bytes; ldb and ldc multiples of 4)
  *   a      [n_heads] f32, at most 0 (the decay is at most 1); d and dt_bias [n_heads] f32 or NULL
- *   dt_min, dt_max  limits of the step (0 and infinity: none)
+ *   dt_min, dt_max  limits of the step, 0 <= dt_min <= dt_max (0 and infinity: a step is at least 0)
  *   state  [n_slots, n_heads, head_dim, d_state] f32, 16-byte aligned, updated in place
  *   y      [n_rows, ldy]: n_heads * head_dim values a row
- * d_state a multiple of 4, at most 256. bf16 prompts (max_rows at least 32, d_state 64, 128 or 256,
- * head_dim a multiple of 32, rows 16-byte aligned with strides of multiples of 8) run in chunks on
- * the matrix cores; the others token by token. The workspace holds the states between the pieces that
+ * d_state a multiple of 4, at most 256; a sequence's state at most 2^30 values. bf16 prompts
+ * (max_rows at least 32, d_state 64, 128 or 256, head_dim a multiple of 32, rows 16-byte aligned with
+ * strides of multiples of 8 below 2^23) run in chunks on the matrix cores; the others token by token. The workspace holds the states between the pieces that
  * a long sequence is cut into, so that they run at once; a smaller one than
  * ema_ssm_workspace_size's makes fewer, longer pieces, none (NULL, 0) no cut. It needs no
  * initialisation and must be 16-byte aligned; calls that overlap need one each. */

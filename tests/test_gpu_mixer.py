@@ -233,6 +233,22 @@ def test_scan_values_that_are_not_finite(ema, what, rows):
         assert same == [0, 0], (what, bad, same)
 
 
+@pytest.mark.parametrize("rows", [3, 100])
+def test_scan_decay_rates_not_finite(ema, rows):
+    """A head whose rate is NaN has no finite value; one of -inf forgets all but the row itself."""
+    H, P, N, n = 4, 32, 64, 2 * rows
+    x, b, c = rand(180, n, H, P, dtype=BF), rand(181, n, 1, N, dtype=BF), rand(182, n, 1, N, dtype=BF)
+    dt, state = rand(183, n, H, dtype=BF), rand(184, 2, H, P, N)
+    A = torch.tensor([-1.0, math.nan, -math.inf, 0.0], device="cuda")
+    want, pool, mag, pool_mag = ref.scan(x, dt, b, c, torch.where(A == -math.inf, -1e30, A), state, 2)
+    y = ema.ssm_scan(x, dt, b, c, A, state, batch=2)
+    for got, w, m, half in ((y, want, mag, HALF[BF]), (state, pool, pool_mag, 0.0)):
+        assert bool(torch.isnan(got[:, 1]).all())
+        keep = [0, 2, 3]
+        # (H and the weights of a chunk, rounded to bf16 as operands of y, and y itself)
+        ref.check(got[:, keep], w[:, keep], (3 * half + (2 * rows + N + 96) * U) * m[:, keep] + TINY[BF], "kept heads")
+
+
 def test_scan_options(ema):
     for i, kw in enumerate([dict(D=False), dict(bias=False), dict(softplus=False), dict(limit=(0.05, 0.2)),
                             dict(dt_scale=30.0), dict(a_scale=1.0)]):

@@ -82,6 +82,14 @@ REFUSED = [
 ]
 
 
+REFUSED += [
+    ("ema_ssm_scan", INVALID, [dict(dt_min=-0.5), dict(dt_min=-INF)]),
+    # a state of more than 2^30 values
+    ("ema_ssm_scan", UNSUPPORTED, [dict(heads=4096, head_dim=4096, d_state=256, groups=1, ldx=1 << 24, ldy=1 << 24, lddt=4096,
+                                        ldb=256, ldc=256)]),
+]
+
+
 @pytest.mark.parametrize("op,code,overs", REFUSED, ids=lambda v: str(v)[:24])
 def test_refused_on_the_host(ema, op, code, overs):
     for over in overs:
