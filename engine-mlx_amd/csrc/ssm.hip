@@ -4,11 +4,13 @@
 // n = 4 p + 64 i + j (i < NI, j < 4), so a 16-byte state access of a wave covers 256 contiguous
 // bytes of each of 4 rows, and y is a sum of 4 NI products and four DPP steps. A wave holds R
 // times 4 rows, which share the lane's B and C values. The state stays in registers over the rows of
-// the piece; the next row's inputs are loaded under this one's sums.
+// the piece.
 // One row (a decode step): HBM-bound, 8 bytes of state traffic per element against 6 flops: 32 users of
-// 64 heads of 64, d_state 128, 135 MB in 22 us (6.1 TB/s). Many rows: bound by the vector instructions
-// of a row, 0.44 us a row for one sequence of 24 heads in f32, and cut in time as long as that
-// fills the chip (2048 rows 137 us; whole 913).
+// 64 heads of 64, d_state 128, 135 MB in 21.4 us (6.3 TB/s). Many rows: bound by the vector instructions of
+// a row (R = 4: 128, of which 96 are the recurrence's) and, for smaller R, by the loads of B and C, which
+// each of a wave's four groups of 16 lanes makes: 8192 rows of 64 heads in f32 0.79 ms. Rows are loaded
+// kAhead before their sums from bases that are uniform; one ahead, with addresses formed in each lane,
+// 2048 rows of 24 heads took 913 us whole and 137 cut in time, now 414 and 112.
 #include "ssm.hpp"
 
 namespace ema {
@@ -32,7 +34,9 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-template <typename A, int NI, int R, int PHASE>
+// kEnds: E and the decay of the pieces that are not their sequence's last; else y, and the state.
+// kAhead: rows loaded ahead of their sums.
+template <typename A, int NI, int R, bool kWhole, bool kEnds, int kAhead>
 __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int row_blocks) {
   typedef typename A::T T;
   uint32_t id = blockIdx.x;
@@ -43,7 +47,8 @@ __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int r
   const Piece pc = packed_piece(a.starts, a.batch, a.n_rows, a.T, a.piece, index);
   if (pc.n == 0) return;
   const bool last = pc.row + pc.n == pc.begin + pc.all;
-  if (PHASE == kSsmEnds && last) return;
+  if (kEnds && last) return;
+  if ((rb * kWaves + (int)(threadIdx.x >> 6)) * 4 * R >= a.head_dim) return;  // (a whole wave; there are no barriers)
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int p = lane & 15;
@@ -54,93 +59,121 @@ __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int r
   float* const pool = a.state + ((int64_t)slot * a.heads + h) * P * N;
   float* const carry = a.carry + ((int64_t)index * a.heads + h) * P * N;
 
+  // Whole: every lane has its state rows and elements. Else the lanes behind the last take the last
+  // one's inputs; elements from d_state on are zeros, rows from head_dim on are not stored.
   bool on[NI];
+  uint32_t n_at[NI], x_at[R];
 #pragma unroll
-  for (int k = 0; k < NI; ++k) on[k] = 4 * p + 64 * k < N;
+  for (int k = 0; k < NI; ++k) {
+    on[k] = kWhole || 4 * p + 64 * k < N;
+    n_at[k] = on[k] ? 4 * p + 64 * k : N - 4;
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) x_at[i] = kWhole || row0 + 4 * i < P ? row0 + 4 * i : P - 1;
   f32x4 s[R][NI];
   {
     // a sequence of one piece starts from the pool; pieces of a longer one never read what its
     // last piece writes there
     const float* from = nullptr;
-    if (PHASE == kSsmPieces && pc.all > a.piece)
+    if (!kEnds && pc.all > a.piece)
       from = carry;
-    else if (PHASE != kSsmEnds && slot >= 0 && packed_continues(a.offsets, pc.b))
+    else if (!kEnds && slot >= 0 && packed_continues(a.offsets, pc.b))
       from = pool;
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int k = 0; k < NI; ++k) {
         s[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (from && row0 + 4 * i < P && on[k]) s[i][k] = *(const f32x4*)(from + (int64_t)(row0 + 4 * i) * N + 4 * p + 64 * k);
+        if (from && (kWhole || (row0 + 4 * i < P && on[k]))) s[i][k] = *(const f32x4*)(from + (int64_t)(row0 + 4 * i) * N + 4 * p + 64 * k);
       }
   }
   const float A_h = a.a[h], D_h = a.d ? a.d[h] : 0.f, bias = a.dt_bias ? a.dt_bias[h] : 0.f;
-  const T* const xp = (const T*)a.x + (int64_t)pc.row * a.ldx + h * P + row0;
-  const T* const bp = (const T*)a.b + (int64_t)pc.row * a.ldb + g * N + 4 * p;
-  const T* const cp = (const T*)a.c + (int64_t)pc.row * a.ldc + g * N + 4 * p;
   const T* const dp = (const T*)a.dt + (int64_t)pc.row * a.lddt + h;
-  T* const yp = (T*)a.y + (int64_t)pc.row * a.ldy + h * P + row0;
+  // the next row to load and to write: uniform, a lane's place in it a 32-bit offset
+  const T* xp = (const T*)a.x + (int64_t)pc.row * a.ldx + h * P;
+  const T* bp = (const T*)a.b + (int64_t)pc.row * a.ldb + g * N;
+  const T* cp = (const T*)a.c + (int64_t)pc.row * a.ldc + g * N;
+  T* yp = (T*)a.y + (int64_t)pc.row * a.ldy + h * P;
 
   struct Row {
     Vec<A, 4> b[NI], c[NI];
     T x[R];
   };
-  auto fetch = [&](int t, Row& r) __attribute__((always_inline)) {
+  int left = pc.n;  // rows not loaded (from the last on it is loaded again)
+  auto fetch = [&](Row& r) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) r.x[i] = row0 + 4 * i < P ? xp[(int64_t)t * a.ldx + 4 * i] : T(0);
+    for (int i = 0; i < R; ++i) r.x[i] = xp[x_at[i]];
 #pragma unroll
     for (int k = 0; k < NI; ++k) {
-      r.b[k].zero();
-      r.c[k].zero();
-      if (on[k]) {
-        r.b[k].load(bp + (int64_t)t * a.ldb + 64 * k);
-        if (PHASE != kSsmEnds) r.c[k].load(cp + (int64_t)t * a.ldc + 64 * k);
-      }
+      r.b[k].load(bp + n_at[k]);
+      if (!kEnds) r.c[k].load(cp + n_at[k]);
     }
+    const bool more = --left > 0;
+    xp += more ? a.ldx : 0;
+    bp += more ? a.ldb : 0;
+    if (!kEnds) cp += more ? a.ldc : 0;
   };
   // the steps of 64 rows, a row a lane
   T raw = dp[(int64_t)(lane < pc.n ? lane : pc.n - 1) * a.lddt];
   float steps = 0.f, decays = 0.f, sum = 0.f;
-  Row now, next;
-  fetch(0, now);
-  for (int t = 0; t < pc.n; ++t) {
-    if (t + 1 < pc.n) fetch(t + 1, next);
-    if ((t & 63) == 0) {
-      steps = ssm_step(A::to(raw) + bias, a);
-      decays = steps * A_h;
-      if (PHASE == kSsmEnds) sum += t + lane < pc.n ? decays : 0.f;
-      decays = expf(decays);
-      const int at = t + 64 + lane;
-      if (t + 64 < pc.n) raw = dp[(int64_t)(at < pc.n ? at : pc.n - 1) * a.lddt];
-    }
+  auto step64 = [&](int t) __attribute__((always_inline)) {
+    steps = ssm_step(A::to(raw) + bias, a);
+    decays = steps * A_h;
+    if (kEnds) sum += t + lane < pc.n ? decays : 0.f;
+    decays = expf(decays);
+    const int at = t + 64 + lane;
+    if (t + 64 < pc.n) raw = dp[(int64_t)(at < pc.n ? at : pc.n - 1) * a.lddt];
+  };
+  auto row = [&](int t, const Row& r) __attribute__((always_inline)) {
     const float d = lane_value(steps, t & 63), decay = lane_value(decays, t & 63);
+    T out[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const float xv = A::to(now.x[i]);
+      const float xv = A::to(r.x[i]);
       const float dx = d * xv;
       float y = 0.f;
 #pragma unroll
       for (int k = 0; k < NI; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[i][k][j] = fmaf(dx, now.b[k][j], decay * s[i][k][j]);
-          if (PHASE != kSsmEnds) y = fmaf(s[i][k][j], now.c[k][j], y);
+          s[i][k][j] = fmaf(dx, on[k] ? r.b[k][j] : 0.f, decay * s[i][k][j]);
+          if (!kEnds) y = fmaf(s[i][k][j], r.c[k][j], y);
         }
-      if (PHASE != kSsmEnds) {
-        y = fmaf(D_h, xv, row_sum16(y));
-        if (p == 0 && row0 + 4 * i < P) yp[(int64_t)t * a.ldy + 4 * i] = A::from(y);
-      }
+      if (!kEnds) out[i] = A::from(fmaf(D_h, xv, row_sum16(y)));
     }
-    now = next;
+    if (!kEnds) {
+      if (p == 0)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (kWhole || row0 + 4 * i < P) yp[x_at[i]] = out[i];
+      yp += a.ldy;
+    }
+  };
+  Row rows[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (i < pc.n) fetch(rows[i]);
+  int t = 0;
+  for (; t + kAhead <= pc.n; t += kAhead) {
+    if ((t & 63) == 0) step64(t);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      row(t + i, rows[i]);
+      fetch(rows[i]);
+    }
   }
-  float* const to = PHASE == kSsmEnds ? carry : (last && slot >= 0 ? pool : nullptr);
+  if (t < pc.n && (t & 63) == 0) step64(t);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (t + i < pc.n) row(t + i, rows[i]);
+  float* const to = kEnds ? carry : (last && slot >= 0 ? pool : nullptr);
   if (to)
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int k = 0; k < NI; ++k)
-        if (row0 + 4 * i < P && on[k]) *(f32x4*)(to + (int64_t)(row0 + 4 * i) * N + 4 * p + 64 * k) = s[i][k];
-  if (PHASE == kSsmEnds && rb == 0 && wave == 0) {
+        if (kWhole || (row0 + 4 * i < P && on[k])) *(f32x4*)(to + (int64_t)(row0 + 4 * i) * N + 4 * p + 64 * k) = s[i][k];
+  if (kEnds && rb == 0 && wave == 0) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
     if (lane == 0) a.carry_decay[(int64_t)index * a.heads + h] = expf(sum);
@@ -175,23 +208,39 @@ __global__ __launch_bounds__(256) void ssm_join_kernel(SsmArgs a, bool chunks) {
   c[(n - 1) * stride] = s;
 }
 
-template <typename A, int NI, int R>
+template <typename A, int NI, int R, bool kWhole>
 hipError_t launch_phase(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhase phase) {
+  // A call's pieces are long and their waves few: rows ahead; whole sequences of R = 4 may be tokens and come
+  // with many waves, which gain more from registers: one token of 32 users of 64 heads, d_state 128 21.2 us
+  // against 23.8 with four rows ahead, 31 tokens of 128 users of 24 heads of 48 x 80 111 and 137, 31 of 32
+  // users of 64 heads 83.0 and 82.3; pieces of 8192 rows of 64 heads (f32) 849 and 785.
+  constexpr int kAhead = NI == 4 ? 2 : 4, kWholeAhead = R == 4 && NI < 4 ? 1 : kAhead;
   const int rb = (a.head_dim + 4 * R * kWaves - 1) / (4 * R * kWaves);
   const dim3 grid((unsigned)(pieces * a.heads * rb)), block(64 * kWaves);
-  if (phase == kSsmWhole)
-    hipLaunchKernelGGL((ssm_token_kernel<A, NI, R, kSsmWhole>), grid, block, 0, s, a, rb);
-  else if (phase == kSsmEnds)
-    hipLaunchKernelGGL((ssm_token_kernel<A, NI, R, kSsmEnds>), grid, block, 0, s, a, rb);
+  if (phase == kSsmEnds)
+    hipLaunchKernelGGL((ssm_token_kernel<A, NI, R, kWhole, true, kAhead>), grid, block, 0, s, a, rb);
+  else if (phase == kSsmWhole)
+    hipLaunchKernelGGL((ssm_token_kernel<A, NI, R, kWhole, false, kWholeAhead>), grid, block, 0, s, a, rb);
   else
-    hipLaunchKernelGGL((ssm_token_kernel<A, NI, R, kSsmPieces>), grid, block, 0, s, a, rb);
+    hipLaunchKernelGGL((ssm_token_kernel<A, NI, R, kWhole, false, kAhead>), grid, block, 0, s, a, rb);
   return hipGetLastError();
 }
+template <typename A, int NI, int R>
+hipError_t launch_lanes(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhase phase) {
+  return a.d_state == 64 * NI && a.head_dim % (16 * R) == 0 ? launch_phase<A, NI, R, true>(s, a, pieces, phase)
+                                                            : launch_phase<A, NI, R, false>(s, a, pieces, phase);
+}
+// A wave's 4 R state rows share its loads of B and C, which bound the kernel once its waves fill the chip;
+// fewer rows a wave give more waves. 16 heads of 64, d_state 128, f32, 64 rows of 4 / 12 / 32 / 64
+// sequences: R = 1 14.8 / 33 / 75 / 144 us, R = 2 17.9 / 28.5 / 48 / 88, R = 4 26.7 / 30.0 / 44 / 75. So
+// R = 1 while its waves have a SIMD each, R = 4 from two waves of it a SIMD on.
 template <typename A, int NI>
 hipError_t launch_rows(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhase phase) {
-  // 64 state rows a workgroup where that gives the chip two of them per CU, else 16
-  const int64_t wgs = pieces * a.heads * ((a.head_dim + 63) / 64);
-  return wgs >= 2 * device_cus() ? launch_phase<A, NI, 4>(s, a, pieces, phase) : launch_phase<A, NI, 1>(s, a, pieces, phase);
+  const int64_t waves = pieces * a.heads * ((a.head_dim + 15) / 16);  // of R = 4
+  const int simds = 4 * device_cus();
+  return waves >= 2 * simds  ? launch_lanes<A, NI, 4>(s, a, pieces, phase)
+         : 4 * waves > simds ? launch_lanes<A, NI, 2>(s, a, pieces, phase)
+                             : launch_lanes<A, NI, 1>(s, a, pieces, phase);
 }
 template <typename A>
 hipError_t launch_state(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhase phase) {
@@ -210,16 +259,18 @@ SsmPlan plan_ssm(int batch, int n_rows, int max_rows, int heads, int head_dim, i
   p.chunks = dtype == EMA_DTYPE_BF16 && vectors && max_rows >= 32 && ssm_chunk_shape(head_dim, d_state);
   p.pieces = batch;
   // Cut where the sequences' heads leave much of the chip idle: into pieces that give every CU two
-  // (chunks) or four workgroups. Chunks, 64 heads of 64, d_state 128: a whole sequence takes 0.065 us
-  // a row of the longest, cut ones 25 us and 0.0105 us a row of all (ends, joining, pieces), so that
-  // the longest has to be 384 rows and 2.6 pieces: 4 x 2048 rows 106 us cut, 133 whole, 5 x 1638
-  // 123 and 106, 512 rows 33 and 37, 256 the same. Token by token (f32): 8 x 300 rows of 24 heads
-  // 164 cut, 173 whole, 2048 rows 150 and 948.
+  // (chunks) or four workgroups (token by token, of R = 4), of E rows if there are no shorter ones.
+  // Chunks, 64 heads of 64, d_state 128: a whole sequence takes 0.065 us a row of the longest, cut ones
+  // 25 us and 0.0105 us a row of all (ends, joining, pieces), so that the longest has to be 384 rows and
+  // 2.6 pieces: 4 x 2048 rows 106 us cut, 133 whole, 5 x 1638 123 and 106, 512 rows 33 and 37, 256 the
+  // same. Token by token (f32, d_state 128): whole 0.2 us a row of the longest and 0.72 E, cut 20 us and
+  // 1.66 E: 24 heads of 64, 2048 rows 112 us cut, 414 whole, 128 rows 24 and 25, 8 x 300 120 and 109; 64
+  // heads, 8192 rows 785 and 1994, 4 x 2048 800 and 765.
   const int per_cu = p.chunks ? 2 : 4, step = p.chunks ? kSsmChunk : 16, least = p.chunks ? 4 * kSsmChunk : 32;
   const int64_t wgs = p.chunks ? (int64_t)ssm_chunk_workgroups(heads, head_dim, groups)
                                : heads * (int64_t)((head_dim + 63) / 64);
   const int64_t even = (n_rows * wgs + per_cu * device_cus() - 1) / (per_cu * device_cus());
-  if ((int64_t)max_rows * 5 < even * 13 + (p.chunks ? 1920 : 320)) return p;
+  if ((int64_t)max_rows * 10 < (p.chunks ? even * 26 + 3840 : even * 47 + 1000)) return p;
   int64_t piece = even < least ? least : (even + step - 1) / step * step;
   for (; piece < max_rows; piece *= 2) {
     const int64_t pieces = packed_pieces(n_rows, batch, (int)piece);
