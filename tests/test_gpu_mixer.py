@@ -259,6 +259,24 @@ def test_scan_many_sequences(ema):
     scan_case(ema, F32, [(i * 7) % 4 for i in range(300)], 2, 16, 16, 1, 130, offsets=[i % 3 for i in range(300)])
 
 
+# How many state rows a lane holds goes by the waves that there are: sequences (whole) and long ones (cut in
+# time) that take two and four of them, of sizes that fill the lanes and that do not.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,shape", [(10, (8, 64, 64, 2)), (33, (16, 64, 64, 1)), (22, (8, 40, 36, 2)), (44, (16, 40, 36, 4)),
+                                         (9, (16, 64, 256, 1)), (33, (16, 64, 132, 2))])
+def test_scan_lanes_whole(ema, dtype, batch, shape):
+    scan_case(ema, dtype, [(3 * i) % 11 for i in range(batch)], *shape, 140, max_rows=31, strided=batch % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", [HF, F32])
+@pytest.mark.parametrize("rows,shape", [(300, (32, 64, 64, 2)), (300, (64, 64, 64, 1)), (250, (32, 40, 36, 2)),
+                                        (360, (64, 40, 36, 4))])
+def test_scan_lanes_cut(ema, dtype, rows, shape):
+    H, P, N, G = shape
+    assert ema.ssm_workspace_size(2, rows + 5, rows, H, P, N, G, dtype) > 0
+    scan_case(ema, dtype, [rows, 5], *shape, 150, offsets=[7, 0], tail=2)
+
+
 # ------------------------------------------------------------------ gated norm
 def gated_case(ema, dtype, n, dim, group, seed, *, gate=True, first=False, sigmoid=False, unit=False, w="dim",
                strided=False, scale=1.0, inplace=False):
