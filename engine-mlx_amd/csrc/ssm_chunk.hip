@@ -1,8 +1,8 @@
 // Selective state space scan in chunks of 32 rows on the matrix cores, bf16 activations.
 //
 // With a_t = d_t A and sums over rows of the chunk, a chunk that starts from the state H gives
-//   y_t = e^(a_0 + .. + a_t) H C_t + sum_{s <= t} M[t][s] x_s,
-//   M[t][s] = (C_t . B_s) e^(a_(s+1) + .. + a_t) d_s  (+ D for s = t),
+//   y_t = e^(a_0 + .. + a_t) H C_t + sum_{s <= t} M[t][s] x_s + D x_t,
+//   M[t][s] = (C_t . B_s) e^(a_(s+1) + .. + a_t) d_s,
 //   H'  = e^(a_0 + .. + a_31) H + sum_s (d_s e^(a_(s+1) + .. + a_31) x_s) B_s^T,
 // so C B^T is formed once for all heads of a workgroup, and the rest is products with 32-row operands.
 //
@@ -21,7 +21,7 @@
 // from t's tile's start to t (f); differences of sums only inside the tiles on the diagonal.
 //
 // Rounded to bf16: H and M where they are operands of y (as an attention's weights are; x, B and C
-// are exact), each by at most 2^-8 of the term. The state itself takes the scaled x as three bf16
+// are exact), each by at most 2^-8 of the term; D x is added in 32 bits. The state itself takes the scaled x as three bf16
 // parts, 24 bits together (two left it 1.5e-6 off, three 5e-8), products and sums in 32 bits. The ends of
 // pieces take two parts, 16 bits: what they hand on decays over at least a piece more, and is rounded
 // to 8 bits where y reads it.
@@ -61,7 +61,6 @@ struct Dec {
   static constexpr int kW = 0;       // d times the decay from behind the row to the chunk's end
   static constexpr int kAll = 32;    // decay over the chunk; its log2 at 33
   static constexpr int kEnds = 36;   // (that is all that the pieces' ends need)
-  static constexpr int kD = 34;      // D
   static constexpr int kCum = 36;    // sum of log2 decays from the row's 16-row tile's start, the row included
   static constexpr int kStep = 68;   // d
   static constexpr int kF = 100;     // decay from the tile's start: 2^kCum
@@ -97,7 +96,7 @@ __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(
 // Decays of two heads' 32 rows, a row a lane (lanes 32..63: the second head; dec is the lane's
 // head's). `raw` is dt + bias; rows from n on take no step.
 template <bool kOutputs>
-__device__ __forceinline__ void chunk_decays(float raw, int n, float A2, float D, const SsmArgs& a, float* dec) {
+__device__ __forceinline__ void chunk_decays(float raw, int n, float A2, const SsmArgs& a, float* dec) {
   const int lane = threadIdx.x & 63, row = lane & 31;
   const float d = row < n ? ssm_step(raw, a) : 0.f;
   // log2 of the row's decay; below 2^-150 it is 0 either way, and sums stay finite (NaN stays NaN)
@@ -120,7 +119,6 @@ __device__ __forceinline__ void chunk_decays(float raw, int n, float A2, float D
     up += dpp_shift<0x112>(up);
     up += dpp_shift<0x114>(up);
     up += dpp_shift<0x118>(up);
-    dec[Dec::kD] = D;
     dec[Dec::kCum + row] = up;
     dec[Dec::kStep + row] = d;
     dec[Dec::kF + row] = exp2_(up);
@@ -279,7 +277,6 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   const uint16_t* const dp = (const uint16_t*)a.dt + (int64_t)pc.row * a.lddt + head0 + first_head + d_head;
   const float A2 = a.a[head0 + first_head + d_head] * kLog2e;
   const float bias = a.dt_bias ? a.dt_bias[head0 + first_head + d_head] : 0.f;
-  const float D = a.d ? a.d[head0 + first_head + d_head] : 0.f;
   // The chunks in the order in which they are taken: their number `step` begins at row row_of(step). The
   // ends of a piece (whole chunks) are taken from its last rows on: the decay from behind a chunk to the
   // piece's end then goes into the chunk's factors, and the sums are never scaled.
@@ -296,7 +293,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   };
   auto decays = [&](int step) __attribute__((always_inline)) {
     const int s = step + d_chunk < n_steps ? step + d_chunk : n_steps - 1;  // (a chunk that is not there: not read)
-    chunk_decays<kOutputs>(bf16_to_f32(rdt) + bias, pc.n - row_of(s), A2, D, a, dec_of(step + d_chunk, d_head));
+    chunk_decays<kOutputs>(bf16_to_f32(rdt) + bias, pc.n - row_of(s), A2, a, dec_of(step + d_chunk, d_head));
   };
 
   if constexpr (kOutputs) {
@@ -324,6 +321,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
     return join(read_tr(at), read_tr(at + 16 * (N * 2)));
   };
 
+  const float D_h = kOutputs && a.d ? a.d[head] : 0.f;
   float total = 0.f;  // log2 of the decay over the piece
   uint8_t* const yp = (uint8_t*)((uint16_t*)a.y + (int64_t)pc.row * a.ldy + (int64_t)head * P + p0);
   const uint32_t ldy2 = (uint32_t)a.ldy * 2, y_at = l16 * ldy2 + 16 * c4;
@@ -407,13 +405,10 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
       auto diagonal = [&](const f32x4 s, int tile) __attribute__((always_inline)) {
         const f32x4 cum = *(const f32x4*)&dec[Dec::kCum + 16 * tile + 4 * c4];
         const f32x4 step_s = *(const f32x4*)&dec[Dec::kStep + 16 * tile + 4 * c4];
-        const float ct = dec[Dec::kCum + 16 * tile + l16], D_h = dec[Dec::kD];
+        const float ct = dec[Dec::kCum + 16 * tile + l16];
         f32x4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = 4 * c4 + i <= l16 ? s[i] * (exp2_(ct - cum[i]) * step_s[i]) : 0.f;
-          v[i] = 4 * c4 + i == l16 ? v[i] + D_h : v[i];
-        }
+        for (int i = 0; i < 4; ++i) v[i] = 4 * c4 + i <= l16 ? s[i] * (exp2_(ct - cum[i]) * step_s[i]) : 0.f;
         return u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
       };
       const f32x4 below = s01 * *(const f32x4*)&dec[Dec::kG + 4 * c4] * dec[Dec::kF + 16 + l16];
@@ -463,7 +458,16 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           uint8_t* const row = yp + (int64_t)(t0 + 16 * t) * ldy2;
-          const f32x4 u = acc[t][0], v = acc[t][1];
+          // the lane's 8 values of the row of x
+          const u32x4 xw = *(const u32x4*)(buf + L::kX + tile_at<kXW>(16 * t + l16, 4 * wave + c4));
+          f32x4 u = acc[t][0], v = acc[t][1];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            u[2 * e] = fmaf(D_h, bf16_lo(xw[e]), u[2 * e]);
+            u[2 * e + 1] = fmaf(D_h, bf16_hi(xw[e]), u[2 * e + 1]);
+            v[2 * e] = fmaf(D_h, bf16_lo(xw[2 + e]), v[2 * e]);
+            v[2 * e + 1] = fmaf(D_h, bf16_hi(xw[2 + e]), v[2 * e + 1]);
+          }
           if (16 * t + l16 < pc.n - t0)
             *(u32x4*)(row + y_at) = u32x4{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]),
                                           pack_bf16x2(v[2], v[3])};
