@@ -20,8 +20,9 @@
 // decays of M are products of factors at most 1 (A <= 0): from s to the end of its 16-row tile (g), and
 // from t's tile's start to t (f); differences of sums only inside the tiles on the diagonal.
 //
-// Rounded to bf16: H and M where they are operands of y (as an attention's weights are; x, B and C
-// are exact), each by at most 2^-8 of the term; D x is added in 32 bits. The state itself takes the scaled x as three bf16
+// Operands of the products: x, B and C are exact in bf16. H and M enter y in two bf16 parts, 16 bits
+// together (off by at most 2^-16 of the term; in one part y was 0.0022 off in place of its own rounding's
+// 0.0017, and a prompt's rows differed from the same rows token by token); D x is added in 32 bits. The state itself takes the scaled x as three bf16
 // parts, 24 bits together (two left it 1.5e-6 off, three 5e-8), products and sums in 32 bits. The ends of
 // pieces take two parts, 16 bits: what they hand on decays over at least a piece more, and is rounded
 // to 8 bits where y reads it.
@@ -80,6 +81,11 @@ __device__ __forceinline__ int tile_at(int r, int q) {  // bytes
   return r * (W * 2) + ((q ^ swizzle<W>(r)) << 4);
 }
 
+// Two values in two bf16 parts: their own bits, and those of what is left.
+__device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(a, b);
+  lo = pack_bf16x2(a - bf16_lo(hi), b - bf16_hi(hi));
+}
 __device__ __forceinline__ bf16x8 join(u32x2 lo, u32x2 hi) { return as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]}); }
 __device__ __forceinline__ u32x2 read_tr(const uint8_t* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p));
@@ -393,15 +399,28 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) {
           const f32x4 u = h[ct][2 * ks], v = h[ct][2 * ks + 1];
-          const bf16x8 hb = as_bf16x8(u32x4{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]),
-                                            pack_bf16x2(v[2], v[3])});
+          uint32_t hi[4], lo[4];
+          split(u[0], u[1], hi[0], lo[0]);
+          split(u[2], u[3], hi[1], lo[1]);
+          split(v[0], v[1], hi[2], lo[2]);
+          split(v[2], v[3], hi[3], lo[3]);
           h[ct][2 * ks] = u * all;
           h[ct][2 * ks + 1] = v * all;
+          const bf16x8 hl = as_bf16x8(u32x4{lo[0], lo[1], lo[2], lo[3]}), hb = as_bf16x8(u32x4{hi[0], hi[1], hi[2], hi[3]});
+          acc[0][ct] = mfma16(hl, c0, acc[0][ct]);
+          acc[1][ct] = mfma16(hl, c1, acc[1][ct]);
           acc[0][ct] = mfma16(hb, c0, acc[0][ct]);
           acc[1][ct] = mfma16(hb, c1, acc[1][ct]);
         }
       }
       // ---- M: lane (l16, c4) holds rows s = 4 c4 + i of its tiles in column t = l16
+      auto parts = [&](const f32x4 v, u32x2* m) __attribute__((always_inline)) {
+        uint32_t hi[2], lo[2];
+        split(v[0], v[1], hi[0], lo[0]);
+        split(v[2], v[3], hi[1], lo[1]);
+        m[0] = u32x2{hi[0], hi[1]};
+        m[1] = u32x2{lo[0], lo[1]};
+      };
       auto diagonal = [&](const f32x4 s, int tile) __attribute__((always_inline)) {
         const f32x4 cum = *(const f32x4*)&dec[Dec::kCum + 16 * tile + 4 * c4];
         const f32x4 step_s = *(const f32x4*)&dec[Dec::kStep + 16 * tile + 4 * c4];
@@ -409,22 +428,28 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
         f32x4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = 4 * c4 + i <= l16 ? s[i] * (exp2_(ct - cum[i]) * step_s[i]) : 0.f;
-        return u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        return v;
       };
       const f32x4 below = s01 * *(const f32x4*)&dec[Dec::kG + 4 * c4] * dec[Dec::kF + 16 + l16];
-      const bf16x8 m[2] = {join(diagonal(s00, 0), u32x2{0u, 0u}),
-                           join(u32x2{pack_bf16x2(below[0], below[1]), pack_bf16x2(below[2], below[3])}, diagonal(s11, 1))};
+      u32x2 m00[2], m01[2], m11[2];
+      parts(diagonal(s00, 0), m00);
+      parts(below, m01);
+      parts(diagonal(s11, 1), m11);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const float e = dec[Dec::kE + 16 * t + l16];
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) acc[t][ct] *= e;
       }
+      auto add = [&](f32x4& acc, const bf16x8 xv, int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 1; k >= 0; --k) acc = mfma16(xv, t ? join(m01[k], m11[k]) : join(m00[k], u32x2{0u, 0u}), acc);
+      };
       if (!bad) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int ct = 0; ct < 2; ++ct) acc[t][ct] = mfma16(xt[ct], m[t], acc[t][ct]);
+          for (int ct = 0; ct < 2; ++ct) add(acc[t][ct], xt[ct], t);
       } else {
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) {
@@ -444,7 +469,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
           other = __shfl_xor(first, 32, 64);
           first = other < first ? other : first;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) acc[t][ct] = mfma16(as_bf16x8(v), m[t], acc[t][ct]);
+          for (int t = 0; t < 2; ++t) add(acc[t][ct], as_bf16x8(v), t);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int from = __shfl(first, 4 * c4 + i, 64);

@@ -71,3 +71,22 @@ def test_skip_term_is_in_32_bits(ema, shape):
     got, _ = run(ema, a, D)
     # the scan's own terms are below 2^-7 of y's rounding whatever they are rounded to
     ref.check(got, want, HALF[BF] * want.abs() + 2.0 ** -7 * scan + 8 * U * mag + TINY[BF], f"skip {shape}")
+
+
+# H and M each in two bf16 parts: off by at most half a step of half a step, 2^-16 of the term
+PARTS = 2.0 ** -16
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_terms_of_a_prompt(ema, shape):
+    """The weights of the rows and the start state where y reads them, in rows all over a chunk."""
+    H = shape[0]
+    a = prompt(20, 70, *shape)
+    held(ema, a, [(7 * h + 3) % 70 for h in range(H)], PARTS, f"terms {shape}")
+    a["state"] = torch.zeros_like(a["state"])
+    held(ema, a, [(5 * h + 1) % 70 for h in range(H)], PARTS, f"rows' terms {shape}")
+
+
+def test_terms_of_a_prompt_cut_in_time(ema):
+    a = prompt(30, 600, 8, 64, 128, 2)
+    held(ema, a, [599, 511, 512, 300, 127, 128, 200, 64], PARTS, "cut")
