@@ -18,7 +18,9 @@
 // over the wave's two tiles, so that a lane holds 8 neighbours of a row of y. M's are rows 4 c + (0..3) and 16 + 4 c +
 // (0..3); x^T and B^T are read from LDS in the same order of rows, by the transposing read. The
 // decays of M are products of factors at most 1 (A <= 0): from s to the end of its 16-row tile (g), and
-// from t's tile's start to t (f); differences of sums only inside the tiles on the diagonal.
+// from t's tile's start to t (f); inside the tiles on the diagonal each is of a sum over its own rows,
+// s + 1 to t (a difference of two long sums keeps no more than their last bit: behind rows that decay
+// by 2^-100 each it was 2^-13 off).
 //
 // Operands of the products: x, B and C are exact in bf16. H and M enter y in two bf16 parts, 16 bits
 // together (off by at most 2^-16 of the term; in one part y was 0.0022 off in place of its own rounding's
@@ -62,12 +64,13 @@ struct Dec {
   static constexpr int kW = 0;       // d times the decay from behind the row to the chunk's end
   static constexpr int kAll = 32;    // decay over the chunk; its log2 at 33
   static constexpr int kEnds = 36;   // (that is all that the pieces' ends need)
-  static constexpr int kCum = 36;    // sum of log2 decays from the row's 16-row tile's start, the row included
+  static constexpr int kL = 36;      // log2 decay of the row
   static constexpr int kStep = 68;   // d
   static constexpr int kF = 100;     // decay from the tile's start: 2^kCum
   static constexpr int kE = 132;     // decay from the chunk's start
   static constexpr int kG = 164;     // d times the decay from behind the row to its tile's end
-  static constexpr int kFloats = 196;
+  static constexpr int kQ = 196;     // [tile][4][16]: sum of log2 decays from row 4 i + 4 of the tile to the row, included
+  static constexpr int kFloats = 324;
 };
 
 // Row pitch and swizzle of the LDS tiles of W-wide rows: 16-byte piece q of row r lies at piece
@@ -125,7 +128,20 @@ __device__ __forceinline__ void chunk_decays(float raw, int n, float A2, const S
     up += dpp_shift<0x112>(up);
     up += dpp_shift<0x114>(up);
     up += dpp_shift<0x118>(up);
-    dec[Dec::kCum + row] = up;
+    // from the second, third and fourth four rows of the tile on
+    const int r16 = row & 15;
+    float q[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      q[i] = r16 >= 4 * i + 4 ? l : 0.f;
+      q[i] += dpp_shift<0x111>(q[i]);
+      q[i] += dpp_shift<0x112>(q[i]);
+      if (i < 2) q[i] += dpp_shift<0x114>(q[i]);
+      if (i < 1) q[i] += dpp_shift<0x118>(q[i]);
+      dec[Dec::kQ + 64 * (row >> 4) + 16 * i + r16] = q[i];
+    }
+    dec[Dec::kQ + 64 * (row >> 4) + 48 + r16] = 0.f;
+    dec[Dec::kL + row] = l;
     dec[Dec::kStep + row] = d;
     dec[Dec::kF + row] = exp2_(up);
     dec[Dec::kE + row] = exp2_(up + (tile1 ? t0 : 0.f));
@@ -422,12 +438,15 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
         m[1] = u32x2{lo[0], lo[1]};
       };
       auto diagonal = [&](const f32x4 s, int tile) __attribute__((always_inline)) {
-        const f32x4 cum = *(const f32x4*)&dec[Dec::kCum + 16 * tile + 4 * c4];
+        const f32x4 l = *(const f32x4*)&dec[Dec::kL + 16 * tile + 4 * c4];
         const f32x4 step_s = *(const f32x4*)&dec[Dec::kStep + 16 * tile + 4 * c4];
-        const float ct = dec[Dec::kCum + 16 * tile + l16];
+        float sum = dec[Dec::kQ + 64 * tile + lane];  // of rows from 4 c4 + 4 to t, then from s + 1
         f32x4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = 4 * c4 + i <= l16 ? s[i] * (exp2_(ct - cum[i]) * step_s[i]) : 0.f;
+        for (int i = 3; i >= 0; --i) {
+          v[i] = 4 * c4 + i <= l16 ? s[i] * (exp2_(sum) * step_s[i]) : 0.f;
+          sum += 4 * c4 + i <= l16 ? l[i] : 0.f;
+        }
         return v;
       };
       const f32x4 below = s01 * *(const f32x4*)&dec[Dec::kG + 4 * c4] * dec[Dec::kF + 16 + l16];

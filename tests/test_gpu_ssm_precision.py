@@ -90,3 +90,14 @@ def test_terms_of_a_prompt(ema, shape):
 def test_terms_of_a_prompt_cut_in_time(ema):
     a = prompt(30, 600, 8, 64, 128, 2)
     held(ema, a, [599, 511, 512, 300, 127, 128, 200, 64], PARTS, "cut")
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_weak_decays_behind_strong_ones(ema, shape):
+    """14 rows that forget everything, then two that forget little, again and again: the little is not lost in
+    a sum with the other."""
+    H, n = shape[0], 64
+    weak = 2.0 ** -7 * (1 + torch.arange(H) / 64)
+    dt = torch.where(torch.arange(n)[:, None] % 16 < 14, torch.tensor(8.0), weak)
+    a = prompt(40, n, *shape, dt=dt, A=torch.full((H,), -16.0))
+    held(ema, a, [16 * (h % 4) + 15 for h in range(H)], PARTS, f"strong and weak {shape}", live=3)
