@@ -24,10 +24,9 @@
 //
 // Operands of the products: x, B and C are exact in bf16. H and M enter y in two bf16 parts, 16 bits
 // together (off by at most 2^-16 of the term; in one part y was 0.0022 off in place of its own rounding's
-// 0.0017, and a prompt's rows differed from the same rows token by token); D x is added in 32 bits. The state itself takes the scaled x as three bf16
-// parts, 24 bits together (two left it 1.5e-6 off, three 5e-8), products and sums in 32 bits. The ends of
-// pieces take two parts, 16 bits: what they hand on decays over at least a piece more, and is rounded
-// to 8 bits where y reads it.
+// 0.0017, and a prompt's rows differed from the same rows token by token); D x is added in 32 bits. The state itself takes
+// the scaled x as three bf16 parts, 24 bits together (two left it 1.5e-6 off, three 5e-8), products and sums in
+// 32 bits; the ends of pieces as well, since a head that hardly decays hands on all of them.
 //
 // A value of x that is not finite would reach rows before it through M's zeros (0 times infinity):
 // chunks with such values (a dot product with zeros finds them while they are staged) take those
@@ -177,7 +176,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   typedef Lds<N, HEADS, kOutputs> L;
   constexpr int KS = N / 32;   // 32-wide steps over d_state
   constexpr int NT = N / 16;   // 16-row tiles of it
-  constexpr int kParts = kOutputs ? 3 : 2;
+  constexpr int kParts = 3;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 
   // the workgroups of a (piece, group) read the same B and C: on one XCD (blocks go to the XCDs in turn)

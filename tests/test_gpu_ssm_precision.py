@@ -101,3 +101,31 @@ def test_weak_decays_behind_strong_ones(ema, shape):
     dt = torch.where(torch.arange(n)[:, None] % 16 < 14, torch.tensor(8.0), weak)
     a = prompt(40, n, *shape, dt=dt, A=torch.full((H,), -16.0))
     held(ema, a, [16 * (h % 4) + 15 for h in range(H)], PARTS, f"strong and weak {shape}", live=3)
+
+
+@pytest.mark.parametrize("rows,cut", [(100, False), (513, True), (640, True)])
+@pytest.mark.parametrize("shape", [(4, 32, 64, 1), (4, 64, 128, 2), (2, 128, 256, 1), (2, 160, 128, 1)])
+def test_state_of_a_prompt_keeps_32_bits(ema, rows, cut, shape):
+    """Rows that are added to a state that does not decay, each to a column of its own: a step of 16 bits times a
+    value of 8 is exact in 32, and stays so however a prompt is cut."""
+    H, P, N, G = shape
+    x = rand(50, rows, H, P, dtype=BF)
+    b = torch.zeros(rows, G, N, dtype=BF, device="cuda")
+    for t in range(N):
+        b[(t * 131) % rows if t < rows else 0, :, t] = 1.0  # (131 has no divisor in common with the row counts)
+    state = torch.zeros(1, H, P, N, device="cuda")
+    step = 43691 / 32768  # 16 bits, every other one set
+    bias = torch.full((H,), step, device="cuda")
+    need = ema.ssm_workspace_size(1, rows, rows, H, P, N, G)
+    ws = torch.full((need,), 85, dtype=torch.uint8, device="cuda")
+    ema.ssm_scan(x, torch.zeros(rows, H, dtype=BF, device="cuda"), b, torch.zeros_like(b), torch.zeros(H, device="cuda"), state,
+                 dt_bias=bias, softplus=False, batch=1, offsets=ints([0]), workspace=ws)
+    torch.cuda.synchronize()
+    assert bool((ws != 85).any()) == cut, "this test is of calls that are cut, or of calls that are not"
+    want = torch.zeros(1, H, P, N, dtype=torch.float64)
+    for t in range(min(N, rows)):
+        want[0, :, :, t] += ref.f64(x[(t * 131) % rows]) * step
+    if N > rows:  # the columns from `rows` on took row 0
+        want[0, :, :, rows:] += (ref.f64(x[0]) * step)[:, :, None]
+    # (step and product have at most 24 bits, each column one of them)
+    assert torch.equal(state.cpu().double(), want)
