@@ -898,8 +898,9 @@ def ssm_scan(x, dt, B, C, A, state, D=None, dt_bias=None, starts=None, offsets=N
     """Selective state space scan, one decay per head (ema_ssm_scan): x [n, H, P], dt [n, H], B and C [n, G, N]
     in bf16, f16 or f32 (rows may be pieces of wider ones); A (at most 0), D, dt_bias f32 [H]; state f32
     [n_slots, H, P, N], updated in place; starts, offsets, slots as in causal_conv; max_rows a host bound of a
-    sequence's rows. workspace: a uint8 tensor (ssm_workspace) that long sequences are split over; None
-    allocates one. Returns out [n, H, P]."""
+    sequence's rows, by which the kernels are chosen: without starts n / B, with them n unless given, so give it
+    for a ragged step of few rows each. workspace: a uint8 tensor (ssm_workspace) that long sequences are split over;
+    None allocates one. Returns out [n, H, P]."""
     op = "ema_ssm_scan"
     torch = _torch or _load_torch()
     i32, f32 = torch.int32, torch.float32
@@ -912,7 +913,9 @@ def ssm_scan(x, dt, B, C, A, state, D=None, dt_bias=None, starts=None, offsets=N
         if batch is None:
             batch = (starts.shape[0] - 1 if starts is not None else offsets.shape[0] if offsets is not None
                      else slots.shape[0] if slots is not None else n_slots)
-        if max_rows is None:
+        if starts is None and batch > 0:
+            max_rows = n // batch
+        elif max_rows is None:
             max_rows = n
         if out is None:
             out = _empty(stream, (n, H, P), dtype, x.device)

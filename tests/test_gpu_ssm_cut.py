@@ -105,3 +105,16 @@ def test_row_starts_that_are_no_row_starts_in_cut_calls(ema, starts):
     torch.cuda.synchronize()
     for b in bufs:
         assert bool((b[:pad] == 3).all()) and bool((b[-pad:] == 3).all())
+
+
+def test_a_uniform_step_allocates_no_workspace(ema, monkeypatch):
+    """Without starts the bound of a sequence's rows is known: one row of each of 512 sequences is not cut."""
+    sizes, size = [], ema.ssm_workspace_size
+    monkeypatch.setattr(ema, "ssm_workspace_size", lambda *a: sizes.append(size(*a)) or sizes[-1])
+    B, H, P, N = 512, 2, 64, 128
+    a = dict(x=rand(1050, B, H, P, dtype=BF), dt=rand(1051, B, H, dtype=BF), B=rand(1052, B, 1, N, dtype=BF),
+             C=rand(1053, B, 1, N, dtype=BF), A=-torch.ones(H, device="cuda"))
+    state = torch.zeros(B, H, P, N, device="cuda")
+    for max_rows in (None, B, 1):
+        ema.ssm_scan(**a, state=state, max_rows=max_rows)
+    assert sizes == [0, 0, 0]
