@@ -338,7 +338,7 @@ struct SsmArgs {
   const int32_t* slots;
   float* state;
   void* y;
-  float* carry;        // workspace: state of each (piece, head), then its decay; null: no cut
+  float* carry;        // workspace: state of each (place, head), then its decay; null: no cut
   float* carry_decay;
   int64_t ldx, lddt, ldb, ldc, ldy;
   float dt_min, dt_max;
@@ -349,6 +349,7 @@ struct SsmArgs {
 struct SsmPlan {
   int piece;        // rows of a piece, 0: no cut
   int64_t pieces;   // piece numbers
+  int64_t places;   // states in the workspace
   bool chunks;      // on the matrix cores
   uint64_t bytes;   // of the workspace
 };

@@ -35,6 +35,19 @@ EMA_HD int packed_uniform_sequence(int index, int T, int L, int batch) {
   return b < batch ? (int)b : batch - 1;
 }
 EMA_HD int64_t packed_pieces(int n_rows, int batch, int L) { return (int64_t)n_rows / L + batch; }
+// Places of what the pieces of longer sequences (more than L rows: two pieces and more) hand on to each
+// other: sequence b's are consecutive from q + min(b, q) on, with q = starts[b] / L, so that sequences
+// of one piece take none. They do not meet: from start s to end e of a sequence of k L + r rows (0 < r <= L)
+// q grows by k at least, and where by no more than k, the minimum by one (b does, and q), which
+// makes the k + 1 places that its pieces need; all lie below the same of n_rows and batch.
+EMA_HD int packed_first_place(int s0, int b, int L) {
+  const int q = (int)((uint32_t)s0 / (uint32_t)L);
+  return q + (b < q ? b : q);
+}
+EMA_HD int64_t packed_places(int n_rows, int batch, int L) {
+  const int64_t q = n_rows / L;
+  return q + (batch < q ? batch : q);
+}
 
 }  // namespace ema
 

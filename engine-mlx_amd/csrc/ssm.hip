@@ -57,7 +57,8 @@ __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int r
   const int g = h / (a.heads / a.groups);
   const int slot = packed_slot(a.slots, pc.b, a.n_slots);
   float* const pool = a.state + ((int64_t)slot * a.heads + h) * P * N;
-  float* const carry = a.carry + ((int64_t)index * a.heads + h) * P * N;
+  const int64_t place = packed_first_place(pc.begin, pc.b, a.piece) + pc.index - pc.first;  // (of a longer sequence)
+  float* const carry = a.carry + (place * a.heads + h) * P * N;
 
   // Whole: every lane has its state rows and elements. Else the lanes behind the last take the last
   // one's inputs; elements from d_state on are zeros, rows from head_dim on are not stored.
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(64 * kWaves) void ssm_token_kernel(SsmArgs a, int r
   if (kEnds && rb == 0 && wave == 0) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
-    if (lane == 0) a.carry_decay[(int64_t)index * a.heads + h] = expf(sum);
+    if (lane == 0) a.carry_decay[place * a.heads + h] = expf(sum);
   }
 }
 
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(256) void ssm_join_kernel(SsmArgs a, bool chunks) {
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= a.heads * per_head) return;
   const int h = v / per_head;
-  const int first = packed_first_piece(r.begin, b, a.piece), n = (r.n + a.piece - 1) / a.piece;
+  const int first = packed_first_place(r.begin, b, a.piece), n = (r.n + a.piece - 1) / a.piece;
   const int64_t stride = (int64_t)a.heads * per_head;
   f32x4* const c = (f32x4*)a.carry + first * stride + v;
   const float* const decay = a.carry_decay + (int64_t)first * a.heads + h;
@@ -273,11 +274,12 @@ SsmPlan plan_ssm(int batch, int n_rows, int max_rows, int heads, int head_dim, i
   if ((int64_t)max_rows * 10 < (p.chunks ? even * 26 + 3840 : even * 47 + 1000)) return p;
   int64_t piece = even < least ? least : (even + step - 1) / step * step;
   for (; piece < max_rows; piece *= 2) {
-    const int64_t pieces = packed_pieces(n_rows, batch, (int)piece);
-    const uint64_t bytes = (uint64_t)pieces * heads * ((uint64_t)head_dim * d_state + 4) * 4;
+    const int64_t pieces = packed_pieces(n_rows, batch, (int)piece), places = packed_places(n_rows, batch, (int)piece);
+    const uint64_t bytes = (uint64_t)places * heads * ((uint64_t)head_dim * d_state + 4) * 4;
     if (bytes > ws_bytes) continue;
     p.piece = (int)piece;
     p.pieces = pieces;
+    p.places = places;
     p.bytes = bytes;
     break;
   }
@@ -295,7 +297,7 @@ int32_t launch_ssm(hipStream_t s, SsmArgs& a, const SsmPlan& plan, void* ws, int
   a.piece = plan.piece ? plan.piece : 1 << 30;
   if (!plan.piece) return check_hip(phase(kSsmWhole), what);
   a.carry = (float*)ws;
-  a.carry_decay = a.carry + (uint64_t)plan.pieces * a.heads * a.head_dim * a.d_state;
+  a.carry_decay = a.carry + (uint64_t)plan.places * a.heads * a.head_dim * a.d_state;
   hipError_t e = phase(kSsmEnds);
   if (e != hipSuccess) return check_hip(e, what);
   const int vecs = a.heads * (a.head_dim * a.d_state / 4);

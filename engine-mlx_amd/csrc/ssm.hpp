@@ -6,7 +6,7 @@
 //   decay = exp(A sum d_t)   and   E = sum_t exp(A sum_{u > t} d_u) d_t x_t B_t^T
 // both independent of S. A long sequence is cut into pieces that run at once: one launch forms every
 // piece's E and decay (all pieces but a sequence's last), one joins them in order into the pieces'
-// start states, one runs the pieces from those.
+// start states, one runs the pieces from those. A sequence of one piece has no place in the workspace.
 #pragma once
 
 #include "packed.hpp"

@@ -207,7 +207,8 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
   const int slot = packed_slot(a.slots, pc.b, a.n_slots);
   float* const pool = a.state + ((int64_t)slot * a.heads + head) * P * N;
   // (the workspace holds a wave's state in the order of its accumulators: ssm_carry_element)
-  float* const carry = a.carry + ((int64_t)index * a.heads + head) * P * N + p0 * N + 4 * lane;
+  const int64_t place = packed_first_place(pc.begin, pc.b, a.piece) + pc.index - pc.first;  // (of a longer sequence)
+  float* const carry = a.carry + (place * a.heads + head) * P * N + p0 * N + 4 * lane;
   const int st_at = (p0 + 8 * (l16 >> 2) + (l16 & 3)) * N + 8 * c4;
 
   float* const decs = (float*)(lds + L::kDec);
@@ -545,7 +546,7 @@ __global__ __launch_bounds__(kThreads, N == 256 ? 1 : 2) void ssm_chunk_kernel(S
 #pragma unroll
       for (int T = 0; T < NT; ++T) *(f32x4*)(pool + (st_at + 4 * ct * N + 32 * (T >> 1) + 4 * (T & 1))) = h[ct][T];
   }
-  if (PHASE == kSsmEnds && !idle && p0 == 0 && lane == 0) a.carry_decay[(int64_t)index * a.heads + head] = exp2_(total);
+  if (PHASE == kSsmEnds && !idle && p0 == 0 && lane == 0) a.carry_decay[place * a.heads + head] = exp2_(total);
 }
 
 template <int N, int HEADS, int PHASE>

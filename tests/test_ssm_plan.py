@@ -1,0 +1,28 @@
+"""The state space scan's plan without a GPU: the places of its workspace (tests/cpp/test_ssm_plan.cpp) and the sizes
+that are told for it."""
+import os
+import subprocess
+
+import pytest
+
+CPP = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
+
+
+def test_integer_parts():
+    subprocess.run(["make", "-s", "-C", CPP, "test_ssm_plan"], check=True)
+    r = subprocess.run([os.path.join(CPP, "test_ssm_plan")], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "checks passed" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.fixture(scope="module")
+def size():
+    import ema_attn
+
+    ema_attn.lib()
+    return ema_attn.ssm_workspace_size
+
+
+def test_sequences_of_one_piece_take_no_state(size):
+    """63 users' tokens beside a prompt: at most twice what the prompt needs alone."""
+    alone = size(1, 8192, 8192, 64, 64, 128, 8)
+    assert alone <= size(64, 8192 + 63, 8192, 64, 64, 128, 8) <= 2 * alone
