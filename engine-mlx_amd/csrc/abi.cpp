@@ -15,6 +15,7 @@
 #include "ema_common.hpp"
 #include "packed.hpp"
 #include "paged.hpp"
+#include "ssm_plan.hpp"
 
 namespace ema {
 
@@ -967,11 +968,8 @@ extern "C" int32_t ema_ssm_workspace_size(int32_t batch, int32_t n_rows, int32_t
   if (rc) return rc;
   if ((rc = check_packed(op, batch, n_rows, max_rows, false))) return rc;
   if ((rc = check_ssm_shape(op, n_heads, head_dim, d_state, n_groups))) return rc;
-  for (int vectors = 0; vectors < 2; ++vectors) {
-    const uint64_t need = plan_ssm(batch, n_rows, max_rows < n_rows ? max_rows : n_rows, n_heads, head_dim, d_state,
-                                   n_groups, dtype, vectors != 0, UINT64_MAX).bytes;
-    if (need > *bytes) *bytes = need;
-  }
+  *bytes = ssm_workspace_bytes(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype == EMA_DTYPE_BF16,
+                               device_cus());
   return EMA_OK;
 }
 
@@ -1012,7 +1010,7 @@ extern "C" int32_t ema_ssm_scan(ema_stream_t stream, const void* x, int64_t ldx,
   const bool vectors = dtype == EMA_DTYPE_BF16 && aligned16(x) && aligned16(b) && aligned16(c) && aligned16(y) &&
                        !(ldx & 7) && !(ldb & 7) && !(ldc & 7) && !(ldy & 7) && ldx < (1 << 23) && ldb < (1 << 23) &&
                        ldc < (1 << 23) && ldy < (1 << 23);
-  const SsmPlan plan = plan_ssm(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype, vectors,
+  const SsmPlan plan = plan_ssm(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, vectors, device_cus(),
                                 workspace ? workspace_bytes : 0);
   if (plan.pieces * n_heads * ((head_dim + 15) / 16) >= kMixerMaxGroups)
     return set_error(EMA_ERR_UNSUPPORTED, "%s: %lld sequences or pieces of %d heads of %d are too many", op,

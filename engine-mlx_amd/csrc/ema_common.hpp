@@ -345,17 +345,7 @@ struct SsmArgs {
   int T, batch, n_rows, heads, head_dim, groups, d_state, n_slots, softplus;
   int piece;  // rows of a piece (2^30: a sequence is one)
 };
-// How a call runs: pieces of how many rows, on which kernels.
-struct SsmPlan {
-  int piece;        // rows of a piece, 0: no cut
-  int64_t pieces;   // piece numbers
-  int64_t places;   // states in the workspace
-  bool chunks;      // on the matrix cores
-  uint64_t bytes;   // of the workspace
-};
-// ws_bytes: the workspace that there is; vectors: rows allow 16-byte accesses.
-SsmPlan plan_ssm(int batch, int n_rows, int max_rows, int heads, int head_dim, int d_state, int groups, int dtype,
-                 bool vectors, uint64_t ws_bytes);
+struct SsmPlan;
 int32_t launch_ssm(hipStream_t s, SsmArgs& a, const SsmPlan& plan, void* ws, int dtype);
 // Affine-quantised matmul y = x W^T over MLX-packed W (arguments validated by the caller).
 int32_t launch_qmatmul(hipStream_t s, const void* x, int64_t ldx, const void* w, const void* scales,

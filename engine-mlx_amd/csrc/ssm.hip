@@ -1,4 +1,4 @@
-// Selective state space scan, one decay per head, token by token; the plan of all its kernels.
+// Selective state space scan, one decay per head, token by token; the launches of all its kernels.
 //
 // Lane layout: 16 lanes share a state row (one value of head_dim); lane p holds its elements
 // n = 4 p + 64 i + j (i < NI, j < 4), so a 16-byte state access of a wave covers 256 contiguous
@@ -253,38 +253,6 @@ hipError_t launch_state(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhas
 }
 
 }  // namespace
-
-SsmPlan plan_ssm(int batch, int n_rows, int max_rows, int heads, int head_dim, int d_state, int groups, int dtype,
-                 bool vectors, uint64_t ws_bytes) {
-  SsmPlan p{};
-  p.chunks = dtype == EMA_DTYPE_BF16 && vectors && max_rows >= 32 && ssm_chunk_shape(head_dim, d_state);
-  p.pieces = batch;
-  // Cut where the sequences' heads leave much of the chip idle: into pieces that give every CU two
-  // (chunks) or four workgroups (token by token, of R = 4), of E rows if there are no shorter ones.
-  // Chunks, 64 heads of 64, d_state 128: a whole sequence takes 0.065 us a row of the longest, cut ones
-  // 25 us and 0.0105 us a row of all (ends, joining, pieces), so that the longest has to be 384 rows and
-  // 2.6 pieces: 4 x 2048 rows 106 us cut, 133 whole, 5 x 1638 123 and 106, 512 rows 33 and 37, 256 the
-  // same. Token by token (f32, d_state 128): whole 0.2 us a row of the longest and 0.72 E, cut 20 us and
-  // 1.66 E: 24 heads of 64, 2048 rows 112 us cut, 414 whole, 128 rows 24 and 25, 8 x 300 120 and 109; 64
-  // heads, 8192 rows 785 and 1994, 4 x 2048 800 and 765.
-  const int per_cu = p.chunks ? 2 : 4, step = p.chunks ? kSsmChunk : 16, least = p.chunks ? 4 * kSsmChunk : 32;
-  const int64_t wgs = p.chunks ? (int64_t)ssm_chunk_workgroups(heads, head_dim, groups)
-                               : heads * (int64_t)((head_dim + 63) / 64);
-  const int64_t even = (n_rows * wgs + per_cu * device_cus() - 1) / (per_cu * device_cus());
-  if ((int64_t)max_rows * 10 < (p.chunks ? even * 26 + 3840 : even * 47 + 1000)) return p;
-  int64_t piece = even < least ? least : (even + step - 1) / step * step;
-  for (; piece < max_rows; piece *= 2) {
-    const int64_t pieces = packed_pieces(n_rows, batch, (int)piece), places = packed_places(n_rows, batch, (int)piece);
-    const uint64_t bytes = (uint64_t)places * heads * ((uint64_t)head_dim * d_state + 4) * 4;
-    if (bytes > ws_bytes) continue;
-    p.piece = (int)piece;
-    p.pieces = pieces;
-    p.places = places;
-    p.bytes = bytes;
-    break;
-  }
-  return p;
-}
 
 int32_t launch_ssm(hipStream_t s, SsmArgs& a, const SsmPlan& plan, void* ws, int dtype) {
   auto phase = [&](SsmPhase ph) {

@@ -10,6 +10,7 @@
 #pragma once
 
 #include "packed.hpp"
+#include "ssm_plan.hpp"
 
 namespace ema {
 
@@ -44,10 +45,6 @@ __device__ __forceinline__ float ssm_step(float r, const SsmArgs& a) {
 }
 #endif
 
-// Chunked scan on the matrix cores (bf16): the shapes it takes, the workgroups of a piece, and a launch.
-constexpr int kSsmChunk = 32;  // rows of a chunk
-bool ssm_chunk_shape(int head_dim, int d_state);
-int ssm_chunk_workgroups(int heads, int head_dim, int groups);
 // The workspace's order of a head's state: token by token [head_dim][d_state]; chunks: accumulator tiles
 // of 16 columns (of head_dim) by 16 of d_state, the four values that a lane holds after each other.
 // Values 4 v .. of it are the pool's from this place on.

@@ -51,8 +51,7 @@
 namespace ema {
 namespace {
 
-constexpr int kQ = 32;        // rows of a chunk
-constexpr int kCols = 32;     // columns of x of a wave
+constexpr int kQ = kSsmChunk, kCols = kSsmCols;
 constexpr int kXW = 4 * kCols;
 constexpr int kThreads = 256;
 
@@ -574,14 +573,6 @@ hipError_t launch_state(hipStream_t s, const SsmArgs& a, const ChunkGrid& g, Ssm
 }
 
 }  // namespace
-
-bool ssm_chunk_shape(int head_dim, int d_state) {
-  return head_dim % kCols == 0 && (d_state == 64 || d_state == 128 || d_state == 256);
-}
-
-int ssm_chunk_workgroups(int heads, int head_dim, int groups) {
-  return groups * ((heads / groups * (head_dim / kCols) + 3) / 4);
-}
 
 hipError_t launch_ssm_chunk(hipStream_t s, const SsmArgs& a, int64_t pieces, SsmPhase phase) {
   ChunkGrid g;

@@ -877,8 +877,8 @@ def causal_conv(x, weight, bias=None, state=None, starts=None, offsets=None, slo
 
 
 def ssm_workspace_size(batch, n_rows, max_rows, n_heads, head_dim, d_state, n_groups, dtype=None) -> int:
-    """Bytes with which ssm_scan splits such a call in time as it likes best (0: it does not); dtype a torch
-    type, bf16 by default."""
+    """Bytes with which ssm_scan splits every call of at most these bounds in time as it likes best (0: it splits
+    none); dtype a torch type, bf16 by default."""
     _torch or _load_torch()
     out = ctypes.c_uint64()
     code = EMA_DTYPE_BF16 if dtype is None else _act_codes.get(dtype, 0)

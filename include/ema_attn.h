@@ -564,8 +564,8 @@ EMA_API int32_t ema_causal_conv(ema_stream_t stream, const void* x, int64_t ldx,
                                 int32_t n_rows, int32_t max_rows, int32_t channels, int32_t width, uint32_t flags,
                                 void* state, int32_t n_slots, void* y, int64_t ldy, int32_t dtype);
 
-/* Workspace (bytes) with which ema_ssm_scan splits these bounds' rows in time as it likes best; 0
- * where it does not split. */
+/* Workspace (bytes) with which ema_ssm_scan splits every call of at most these sequences, rows and
+ * rows of a sequence in time as it likes best; 0 where it splits none. */
 EMA_API int32_t ema_ssm_workspace_size(int32_t batch, int32_t n_rows, int32_t max_rows, int32_t n_heads,
                                        int32_t head_dim, int32_t d_state, int32_t n_groups, int32_t dtype,
                                        uint64_t* bytes);

@@ -1,11 +1,14 @@
 // CPU checks of where the state space scan keeps what the pieces of a cut sequence hand on to each other
-// (engine-mlx_amd/csrc/packed.hpp).
+// (engine-mlx_amd/csrc/packed.hpp), and that a workspace of the size that is told for some bounds is as
+// good as any for every call within them (engine-mlx_amd/csrc/ssm_plan.hpp).
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <random>
 #include <vector>
 
 #include "packed.hpp"
+#include "ssm_plan.hpp"
 
 using namespace ema;
 
@@ -36,6 +39,29 @@ static void places(const std::vector<int>& lens, int tail, int L) {
   }
 }
 
+static int log_pick(std::mt19937& rng, int most) {  // 1 .. most, over its logarithm
+  return (int)std::exp(std::uniform_real_distribution<double>(0, std::log(most + 0.99))(rng));
+}
+
+static void within_bounds(std::mt19937& rng) {
+  const int G = 1 << (rng() % 4), heads = G * log_pick(rng, 24), P = rng() % 3 ? 32 * (1 + (int)(rng() % 5)) : log_pick(rng, 200);
+  const int N = rng() % 3 ? 64 << (rng() % 3) : 4 * (1 + (int)(rng() % 64)), cus = rng() % 4 ? 256 : 32;
+  const int batch = log_pick(rng, 4096), rows = log_pick(rng, 1 << 20), longest = log_pick(rng, rows);
+  const bool bf16 = rng() % 2;
+  const uint64_t told = ssm_workspace_bytes(batch, rows, longest, heads, P, N, G, bf16, cus);
+  for (int k = 0; k < 60; ++k) {
+    const int b = rng() % 3 ? log_pick(rng, batch) : batch, n = rng() % 3 ? log_pick(rng, rows) : rows;
+    int most = rng() % 3 ? log_pick(rng, longest) : longest;
+    if (most > n) most = n;
+    for (int vectors = 0; vectors <= (bf16 ? 1 : 0); ++vectors) {
+      const SsmPlan best = plan_ssm(b, n, most, heads, P, N, G, vectors, cus, UINT64_MAX);
+      const SsmPlan p = plan_ssm(b, n, most, heads, P, N, G, vectors, cus, told);
+      CHECK(best.bytes <= told);
+      CHECK(p.piece == best.piece && p.chunks == best.chunks && p.bytes == best.bytes);
+    }
+  }
+}
+
 int main() {
   std::mt19937 rng(11);
   auto pick = [&](int n) { return (int)(rng() % n); };
@@ -59,6 +85,7 @@ int main() {
       if (r.n > L) CHECK(packed_first_place(r.begin, b, L) + (r.n + L - 1) / L <= packed_places(rows, B, L));
     }
   }
+  for (int k = 0; k < 20000; ++k) within_bounds(rng);
   std::printf("%ld checks passed\n", checks);
   return 0;
 }

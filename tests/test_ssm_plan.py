@@ -26,3 +26,9 @@ def test_sequences_of_one_piece_take_no_state(size):
     """63 users' tokens beside a prompt: at most twice what the prompt needs alone."""
     alone = size(1, 8192, 8192, 64, 64, 128, 8)
     assert alone <= size(64, 8192 + 63, 8192, 64, 64, 128, 8) <= 2 * alone
+
+
+def test_a_size_holds_every_smaller_call(size):
+    """A server sizes its workspace once: many long prompts, of which none is cut, and one alone, which is."""
+    assert size(8, 65536, 8192, 64, 64, 128, 8) >= size(1, 8192, 8192, 64, 64, 128, 8) > 0
+    assert size(32, 32, 1, 64, 64, 128, 8) == 0 and size(512, 512, 1, 2, 64, 128, 1) == 0
