@@ -434,25 +434,50 @@ def gdn_workspace(B, T, Hk, Hv, Dk, Dv, device="cuda"):
 
 def gdn_scan(q, k, v, g, beta, state, y=None, stream=None, workspace=None):
     """Gated DeltaNet recurrent scan (ema_gdn_scan): q, k [B,T,Hk,Dk], v [B,T,Hv,Dv] in bf16,
-    f16 or f32; g, beta [B,T,Hv] f32; state [B,Hv,Dv,Dk] f32, updated in place. Returns
+    f16 or f32; g, beta [B,T,Hv] f32 (inputs that are not contiguous, such as pieces of a convolution's
+    rows, are copied first); state [B,Hv,Dv,Dk] f32, contiguous, updated in place. Returns
     y [B,T,Hv,Dv] in the activation dtype. With a workspace (a uint8 tensor, e.g. from
     gdn_workspace) bf16 scans of 32+ tokens run in WY form (ema_gdn_scan_ws)."""
-    import torch
-
-    dtypes = {torch.bfloat16: EMA_DTYPE_BF16, torch.float16: EMA_DTYPE_F16, torch.float32: EMA_DTYPE_F32}
-    if q.dtype not in dtypes:
-        raise EmaError(EMA_ERR_INVALID_ARG, "ema_gdn_scan", f"unsupported activation dtype {q.dtype}")
+    op = "ema_gdn_scan"
+    torch = _torch or _load_torch()
+    dtype, dev, f32 = q.dtype, q.get_device(), torch.float32
+    code = _act_code(op, q)
+    if q.dim() != 4 or v.dim() != 4:
+        raise EmaError(EMA_ERR_SHAPE, op, f"q must be [B,T,Hk,Dk] and v [B,T,Hv,Dv], not {tuple(q.shape)}, {tuple(v.shape)}")
     B, T, Hk, Dk = q.shape
-    Hv, Dv = v.shape[2], v.shape[3]
+    _, _, Hv, Dv = v.shape
+    values, gates = (B, T, Hv, Dv), (B, T, Hv)
     if y is None:
-        y = torch.empty((B, T, Hv, Dv), dtype=q.dtype, device=q.device)
-    if workspace is None:
-        _check(lib().ema_gdn_scan(_stream(stream), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state),
-                                  _ptr(y), B, T, Hk, Hv, Dk, Dv, dtypes[q.dtype]), "ema_gdn_scan")
-    else:
-        _check(lib().ema_gdn_scan_ws(_stream(stream), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state),
-                                     _ptr(y), B, T, Hk, Hv, Dk, Dv, dtypes[q.dtype], _ptr(workspace),
-                                     workspace.numel() * workspace.element_size()), "ema_gdn_scan_ws")
+        y = _empty(stream, values, dtype, q.device) if stream is not None else torch.empty(values, dtype=dtype, device=q.device)
+    if not (k.dtype is dtype and k.shape == q.shape and k.get_device() == dev and k.is_contiguous() and q.is_contiguous()
+            and v.dtype is dtype and v.shape == values and v.get_device() == dev and v.is_contiguous()
+            and g.dtype is f32 and g.shape == gates and g.get_device() == dev and g.is_contiguous()
+            and beta.dtype is f32 and beta.shape == gates and beta.get_device() == dev and beta.is_contiguous()
+            and y.dtype is dtype and y.shape == values and y.get_device() == dev and y.is_contiguous()
+            and state.dtype is f32 and state.shape == (B, Hv, Dv, Dk) and state.get_device() == dev and state.is_contiguous()
+            and (workspace is None or (workspace.get_device() == dev and workspace.is_contiguous()))):
+        for name, t, kind, shape in (("k", k, dtype, (B, T, Hk, Dk)), ("v", v, dtype, values), ("g", g, f32, gates),
+                                     ("beta", beta, f32, gates)):
+            if t.shape != shape or t.dtype is not kind or t.get_device() != dev:
+                raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be a {kind} tensor {shape} on {q.device}, not {t.dtype} "
+                                                  f"{tuple(t.shape)} on {t.device}")
+        _want(op, "y", y, dtype, values, dev)
+        _want(op, "state", state, f32, (B, Hv, Dv, Dk), dev)
+        if workspace is not None:
+            _want(op, "workspace", workspace, workspace.dtype, workspace.shape, dev)
+        with _on(stream):
+            q, k, v, g, beta = (t.contiguous() for t in (q, k, v, g, beta))
+    if dev < 0:
+        _not_on_gpu(op)
+    args = (torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream, q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(), y.data_ptr(), B, T, Hk, Hv, Dk, Dv, code)
+    call = _lib.ema_gdn_scan
+    if workspace is not None:
+        call, op = _lib.ema_gdn_scan_ws, "ema_gdn_scan_ws"
+        args += workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    rc = call(*args) if torch._C._cuda_getDevice() == dev else _elsewhere(dev, call, *args)
+    if rc:
+        _check(rc, op)
     return y
 
 
@@ -552,12 +577,12 @@ class PagedCache:
 
 
 def _want(op: str, name: str, t, dtype, shape, device: int) -> None:
-    """A contiguous tensor of the given dtype and shape on the pool's device (an index; -1: CPU)."""
+    """A contiguous tensor of the given dtype and shape on the given device (an index; -1: CPU)."""
     if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
         raise EmaError(EMA_ERR_SHAPE, op, f"{name} must be a contiguous {dtype} tensor {tuple(shape)}, not "
                                           f"{t.dtype} {tuple(t.shape)} with strides {t.stride()}")
     if t.get_device() != device:
-        raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} is on {t.device}, the pages on device {device}")
+        raise EmaError(EMA_ERR_INVALID_ARG, op, f"{name} is on {t.device}, not on device {device}")
 
 
 def _refuse(op: str, device: int, *wanted) -> None:
