@@ -516,10 +516,13 @@ EMA_API int32_t ema_gdn_scan_ws(ema_stream_t stream, const void* q, const void* 
 
 /* ---- Around the recurrent scans: convolution, state space scan, norms --------------------
  * The other pieces of a recurrent layer, for one token, a chunk or a prompt of every sequence of
- * a ragged batch: in projection (ema_quantized_matmul) -> ema_causal_conv -> ema_gdn_scan or
- * ema_ssm_scan -> ema_gated_norm -> out projection -> ema_residual_norm. dtype is the type of the
+ * a ragged batch: in projection (ema_quantized_matmul) -> ema_causal_conv -> ema_ssm_scan ->
+ * ema_gated_norm -> out projection -> ema_residual_norm. Around ema_gdn_scan they serve batches whose
+ * sequences have the same number of rows: it has no starts, offsets, slots or row strides, so that the
+ * convolution's q|k|v are copied apart for it and its states are the batch's. dtype is the type of the
  * activations and of the weights that multiply them: EMA_DTYPE_BF16, _F16 or _F32; arithmetic and
- * the scan's state are in 32 bits, and every output value is rounded once. Tensors are packed rows
+ * the scan's state are in 32 bits, and every output value is rounded once (the operands of bf16 prompts of
+ * ema_ssm_scan: see there). Tensors are packed rows
  * [n_rows, ...] whose row stride ld* (elements) may be wider than a row: a piece of a projection's
  * row is read where it lies. Outputs must not overlap inputs unless a call says that they may.
  *   starts   device int32 [batch + 1], ascending: sequence b's rows are [starts[b], starts[b + 1]);
@@ -532,10 +535,12 @@ EMA_API int32_t ema_gdn_scan_ws(ema_stream_t stream, const void* q, const void* 
  *            [n_slots, ...] is the sequence's. An entry outside [0, n_slots) is never followed: the
  *            sequence starts from zeros and its state is not stored. No two sequences of a call may
  *            have the same slot.
- *   max_rows host bound of a sequence's rows; it chooses between kernels, and true values beyond it
- *            still give the result.
- * At most 4096 sequences and 2^30 rows a call (norms: 2^22 of more than 512 values, 2^26 of fewer). A
- * call of no rows does nothing. The reference runs its convolution,
+ *   max_rows host bound of a sequence's rows; it chooses between the scan's kernels (the convolution has
+ *            one), and true values beyond it still give the result.
+ * At most 4096 sequences and 2^30 rows a call. Convolution: at most 2^21 channels. Scan: sequences (of a cut
+ * call its pieces: one a sequence and one for each `piece` rows more) * n_heads * ceil(head_dim / 16) below
+ * 2^24. Gated norm: n_rows * (dim / group) below 2^26, or 2^22 for groups of more than 512 values. Residual norm:
+ * n_rows below 2^22. A call of no rows does nothing. The reference runs its convolution,
  * norms and gates as separate MLX operators (crates/ops/src/gdn_forward.rs) and has no state space
  * scan. */
 
@@ -583,8 +588,11 @@ EMA_API int32_t ema_ssm_workspace_size(int32_t batch, int32_t n_rows, int32_t ma
  *   y      [n_rows, ldy]: n_heads * head_dim values a row
  * d_state a multiple of 4, at most 256; a sequence's state at most 2^30 values. bf16 prompts
  * (max_rows at least 32, d_state 64, 128 or 256, head_dim a multiple of 32, rows 16-byte aligned with
- * strides of multiples of 8 below 2^23) run in chunks on the matrix cores; the others token by token. The workspace holds the states between the pieces that
- * a long sequence is cut into, so that they run at once; a smaller one than
+ * strides of multiples of 8 below 2^23) run in chunks on the matrix cores, every sequence of the call; the others
+ * token by token. In chunks S and the weights of the rows enter the sums of y as two bf16 parts, each off by at
+ * most 2^-16 of its value, and the terms of S as three (2^-24); products and sums are in 32 bits. A row's y may so
+ * differ by a rounding between the two ways, which max_rows chooses for the whole call. The workspace holds
+ * the states between the pieces that a long sequence is cut into, so that they run at once; a smaller one than
  * ema_ssm_workspace_size's makes fewer, longer pieces, none (NULL, 0) no cut. It needs no
  * initialisation and must be 16-byte aligned; calls that overlap need one each. */
 EMA_API int32_t ema_ssm_scan(ema_stream_t stream, const void* x, int64_t ldx, const void* dt, int64_t ld_dt,
