@@ -84,7 +84,7 @@ inline uint64_t ssm_workspace_bytes(int batch, int n_rows, int max_rows, int hea
   for (int chunks = 0; chunks < 2; ++chunks) {
     if (chunks && !(bf16 && ssm_chunk_shape(head_dim, d_state))) continue;
     const SsmCut c = ssm_cut(chunks, heads, head_dim, groups, cus);
-    if (max_rows * 10 * c.fill < max_rows * c.wgs * c.by_even + c.by * c.fill) continue;
+    if ((int64_t)max_rows * 10 * c.fill < max_rows * c.wgs * c.by_even + c.by * c.fill) continue;
     const int64_t q = n_rows / c.least < c.fill / c.wgs ? n_rows / c.least : c.fill / c.wgs;
     const uint64_t bytes = ssm_places_bytes(q + (batch < q ? batch : q), heads, head_dim, d_state);
     if (bytes > most) most = bytes;

@@ -46,7 +46,7 @@ static int log_pick(std::mt19937& rng, int most) {  // 1 .. most, over its logar
 static void within_bounds(std::mt19937& rng) {
   const int G = 1 << (rng() % 4), heads = G * log_pick(rng, 24), P = rng() % 3 ? 32 * (1 + (int)(rng() % 5)) : log_pick(rng, 200);
   const int N = rng() % 3 ? 64 << (rng() % 3) : 4 * (1 + (int)(rng() % 64)), cus = rng() % 4 ? 256 : 32;
-  const int batch = log_pick(rng, 4096), rows = log_pick(rng, 1 << 20), longest = log_pick(rng, rows);
+  const int batch = log_pick(rng, 4096), rows = log_pick(rng, 1 << 30), longest = log_pick(rng, rows);
   const bool bf16 = rng() % 2;
   const uint64_t told = ssm_workspace_bytes(batch, rows, longest, heads, P, N, G, bf16, cus);
   for (int k = 0; k < 60; ++k) {
