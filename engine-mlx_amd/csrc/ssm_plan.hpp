@@ -36,14 +36,16 @@ struct SsmCut {
   int by_even, by;  // cut where the longest sequence has 0.1 (by_even E + by) rows and more, E = rows * wgs / fill
 };
 // Cut where the sequences' heads leave much of the chip idle: into pieces that fill it, of E rows if there are no
-// shorter ones. Chunks, 64 heads of 64, d_state 128: a whole sequence takes 0.065 us a row of the longest, cut ones
-// 25 us and 0.0105 us a row of all (ends, joining, pieces), so that the longest has to be 384 rows and
-// 2.6 pieces: 4 x 2048 rows 106 us cut, 133 whole, 5 x 1638 123 and 106, 512 rows 33 and 37, 256 the
-// same. Token by token (f32, d_state 128): whole 0.2 us a row of the longest and 0.72 E, cut 20 us and
-// 1.66 E: 24 heads of 64, 2048 rows 112 us cut, 414 whole, 128 rows 24 and 25, 8 x 300 120 and 109; 64
+// shorter ones. Chunks, 64 heads of 64, d_state 128: a whole sequence takes 6 us and 0.082 us a row of the longest,
+// cut ones 25 us and 0.0123 us a row of all (ends, joining, pieces; 0.197 E), so that the longest has to be 240 rows
+// and 2.5 E: 4 x 2048 rows 121 us cut, 173 whole, 4 x 1024 77 and 90, 6 x 1024 119 and 92, 5 x 1638 146 and 143, 512
+// rows 34 and 47, 320 29 and 32, 256 29 and 26. The state's size moves both sides: d_state 64, 32 heads 210 rows and
+// 3.7 E (384 rows 23 cut, 27 whole, 4096 45 and 234), d_state 256, 16 heads of 128 240 and 3.3 E (384 46 and 63,
+// 4 x 2048 146 and 300). Token by token (f32, d_state 128): whole 0.2 us a row of the longest and 0.72 E, cut 20 us
+// and 1.66 E: 24 heads of 64, 2048 rows 112 us cut, 414 whole, 128 rows 24 and 25, 8 x 300 120 and 109; 64
 // heads, 8192 rows 785 and 1994, 4 x 2048 800 and 765.
 inline SsmCut ssm_cut(bool chunks, int heads, int head_dim, int groups, int cus) {
-  if (chunks) return SsmCut{ssm_chunk_workgroups(heads, head_dim, groups), 2 * cus, kSsmChunk, 4 * kSsmChunk, 26, 3840};
+  if (chunks) return SsmCut{ssm_chunk_workgroups(heads, head_dim, groups), 2 * cus, kSsmChunk, 4 * kSsmChunk, 25, 2400};
   return SsmCut{heads * (int64_t)((head_dim + 63) / 64), 4 * cus, 16, 32, 47, 1000};
 }
 inline uint64_t ssm_places_bytes(int64_t places, int heads, int head_dim, int d_state) {
