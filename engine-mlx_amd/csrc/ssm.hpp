@@ -39,7 +39,7 @@ __device__ __forceinline__ float softplus_(float r) {
 // The step of raw value r (dt + bias): softplus, then the limits.
 __device__ __forceinline__ float ssm_step(float r, const SsmArgs& a) {
   const float sp = softplus_(r);
-  r = a.softplus ? sp : r;  // (no branch: the chunked kernel schedules this under its products)
+  r = a.softplus ? sp : r;  // (no branch)
   r = r < a.dt_min ? a.dt_min : r;  // (NaN stays)
   return r > a.dt_max ? a.dt_max : r;
 }

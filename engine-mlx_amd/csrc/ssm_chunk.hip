@@ -4,13 +4,13 @@
 //   y_t = e^(a_0 + .. + a_t) H C_t + sum_{s <= t} M[t][s] x_s + D x_t,
 //   M[t][s] = (C_t . B_s) e^(a_(s+1) + .. + a_t) d_s,
 //   H'  = e^(a_0 + .. + a_31) H + sum_s (d_s e^(a_(s+1) + .. + a_31) x_s) B_s^T,
-// so C B^T is formed once for all heads of a workgroup, and the rest is products with 32-row operands.
+// so C B^T is the same for all heads of a group, and the rest is products with 32-row operands.
 //
 // A workgroup of four waves takes 128 columns of x (two heads of 64, one of 128, ...) of one group,
 // a wave 32 of them: its H^T [d_state, 32] stays in 32-bit accumulators over the rows of the piece.
 // All products are 16x16x32 in forms that chain without moving data between lanes:
 //   C B^T as [s, t]          A = B rows,       B = C rows (columns t)
-//   y^T [p, t]              A = H (the accumulators, rounded to bf16) and x^T, B = C and M
+//   y^T [p, t]              A = H (the accumulators, in two bf16 parts) and x^T, B = C and M
 //   H^T [n, p]              A = B^T,           B = x^T scaled
 // A pair of 16x16 accumulator tiles holds, in lane group c, rows 4 c + (0..3) of both tiles. The rows of
 // the state's tiles are numbered so that these are d_state 8 c + (0..7) of a 32-wide step (B^T's columns
@@ -20,13 +20,13 @@
 // decays of M are products of factors at most 1 (A <= 0): from s to the end of its 16-row tile (g), and
 // from t's tile's start to t (f); inside the tiles on the diagonal each is of a sum over its own rows,
 // s + 1 to t (a difference of two long sums keeps no more than their last bit: behind rows that decay
-// by 2^-100 each it was 2^-13 off).
+// by 2^-100 each it was up to 2^-13 off).
 //
 // Operands of the products: x, B and C are exact in bf16. H and M enter y in two bf16 parts, 16 bits
-// together (off by at most 2^-16 of the term; in one part y was 0.0022 off in place of its own rounding's
-// 0.0017, and a prompt's rows differed from the same rows token by token); D x is added in 32 bits. The state itself takes
-// the scaled x as three bf16 parts, 24 bits together (two left it 1.5e-6 off, three 5e-8), products and sums in
-// 32 bits; the ends of pieces as well, since a head that hardly decays hands on all of them.
+// together: off by at most 2^-16 of the term, 2^-8 of what y's own rounding may take (in one part y was 0.0022
+// off in place of 0.0017, and 0.0027 from the same sums in 32 bits; now 0.00006). D x is added in 32 bits. The state
+// itself takes the scaled x as three bf16 parts, 24 bits together (two left it 1.5e-6 off, three 5e-8),
+// products and sums in 32 bits; the ends of pieces as well, since a head that hardly decays hands on all of them.
 //
 // A value of x that is not finite would reach rows before it through M's zeros (0 times infinity):
 // chunks with such values (a dot product with zeros finds them while they are staged) take those
@@ -36,14 +36,14 @@
 // (its decay and its rounding come twice as often), but 64 rows need more registers than two
 // workgroups a CU leave, and spilled the loads under way (131 us against 74 at the time).
 //
-// Bound by issue: a product and a vector instruction of one SIMD do not overlap, not even of two waves
-// (48 products 388 ns, 144 fused multiply-adds 188 ns, side by side 568), so that a chunk is the sum of
-// both, here 80 products and about 330 vector instructions a wave: 1.1 us, 2.2 for the two waves of a
-// SIMD, of the 3.4 us that a chunk takes; the rest is waiting at two waves a SIMD. 8192 rows of 64
-// heads of 64, d_state 128, 8 groups: ends 30, joining 13, pieces 64 us, together 103 us, 1.7 TB/s of
-// what has to move, 0.2 PFLOP/s of the recurrence's operations. No gain: products interleaved with vector
-// instructions by scheduling groups, the state's decay kept as a factor (66), y stored a chunk later
-// (67), one column tile a wave in workgroups of eight waves (104, spilled).
+// Bound by issue and waits: a chunk of a wave is 100 products (16 cycles each) and about 680 vector
+// instructions (by the counters; 48 and 190 in the ends), 4300 cycles a wave and 8600 for the two of a SIMD
+// if none overlap, of the 5.2 us that a chunk takes. 8192 rows of 64 heads of 64, d_state 128, 8 groups: ends
+// 33, joining 13, pieces 84 us, together 119 us, 1.5 TB/s of what has to move, 0.18 PFLOP/s of the recurrence's
+// operations. With H and M in one bf16 part, D among M and the ends in two parts it was 30, 13 and 64, at
+// y 0.0022 off and the state 16 bits. No gain at that time: products interleaved with vector instructions by
+// scheduling groups, the state's decay kept as a factor (66), y stored a chunk later (67), one column tile a
+// wave in workgroups of eight waves (104, spilled).
 #include <type_traits>
 
 #include "ssm.hpp"
